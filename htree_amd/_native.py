@@ -33,7 +33,8 @@ EXPORTS = (
     "htree_backward",
     "htree_train_scores_bytes", "htree_forward_train", "htree_backward_train",
     "htree_forward_trace", "htree_topk_rows", "htree_backward_noalloc_bytes",
-    "htree_backward_noalloc", "htree_select",
+    "htree_backward_noalloc", "htree_select", "htree_page_tables", "htree_cache_append",
+    "htree_draft_attention_workspace_bytes", "htree_draft_attention",
 )
 
 
@@ -41,6 +42,12 @@ class HtreeDims(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int32) for n in (
         "B", "T", "H", "H_kv", "D", "compression_rate", "top_k", "max_top_nodes", "dtype",
         "rope_rows", "kv_share", "grad_dtype", "group_pad")]
+
+
+class HtreeCache(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_int32) for n in ("dtype", "H_kv", "Dk", "Dv", "page_size", "num_pages")]
+                + [(n, ctypes.c_int64) for n in ("k_page", "k_token", "k_head",
+                                                 "v_page", "v_token", "v_head")])
 
 
 class HtreeError(RuntimeError):
@@ -102,6 +109,17 @@ def lib() -> ctypes.CDLL:
         L.htree_backward_train.restype = ctypes.c_int
         L.htree_backward_train.argtypes = [DP, F, P, P, P, P, P, P, P, I64, P, P, P, I64, P, P, P,
                                            P, I64, P]
+    CP = ctypes.POINTER(HtreeCache)
+    L.htree_page_tables.restype = ctypes.c_int
+    L.htree_page_tables.argtypes = [I32, I32, I32, I32, I32, I64, I32] + [P] * 11
+    L.htree_cache_append.restype = ctypes.c_int
+    L.htree_cache_append.argtypes = [CP, I32, I32, P, I64, I64, P, I64, I64, P, I64, I64, P, P, P, P,
+                                     I32, P, P, P, P]
+    L.htree_draft_attention_workspace_bytes.restype = ctypes.c_int
+    L.htree_draft_attention_workspace_bytes.argtypes = [CP, I32, I32, I32, I32, ctypes.POINTER(I64)]
+    L.htree_draft_attention.restype = ctypes.c_int
+    L.htree_draft_attention.argtypes = [CP, I32, I32, I32, I32, I64, F, P, I64, I64, P, P, P, P, P, P,
+                                        P, I64, I64, P, I64, P]
     _lib = L
     return L
 

@@ -19,7 +19,8 @@ ARCH = "gfx950"
 
 SOURCES = ["htree_tree.hip", "htree_fwd.hip", "htree_fwd_stream.hip", "htree_fwd_wide_d32.hip",
            "htree_fwd_wide_d64.hip", "htree_fwd_wide_d128.hip", "htree_fwd_wide_d256.hip",
-           "htree_bwd.hip", "htree_topk.hip", "htree_split.hip"]
+           "htree_bwd.hip", "htree_topk.hip", "htree_split.hip", "htree_cache.hip",
+           "htree_draft_bf16.hip", "htree_draft_f16.hip", "htree_draft_f32.hip"]
 
 # packed fp32 ops are disabled on purpose: some of their forms have given
 # silently wrong results on these machines.

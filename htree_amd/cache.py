@@ -1,0 +1,205 @@
+"""Serving from a paged key/value cache: block tables and slot maps from
+request lengths, and new keys and values (rotated by their positions) written
+to their slots.  The attention over the cache is draft.py's.
+
+The reference has no serving path (its entry points take whole sequences,
+/root/reference/src/parallel.py:874-885); this one carries on where its
+forward ends: up to max_top_nodes tokens a sequence's tree has one level and
+htree_forward is dense causal attention with RoPE at the token's position
+(src/parallel.py:941-945, 983-988), whose next rows come from the cache.
+
+The cache is two tensors that the caller keeps, k_cache
+[pages, page_size, H_kv, K] and v_cache [pages, page_size, H_kv, V] (any
+strides that are whole 16-byte pieces, the head dim contiguous: a permuted
+[pages, H_kv, page_size, K] tensor serves too).  Token p of request b is in
+page block_table[b, p // page_size] at offset p % page_size; a slot is
+page * page_size + offset.
+
+Lengths, tables, slots and positions stay on the GPU and are not checked by
+the host; whatever they hold, the kernels touch nothing outside the tensors.
+Nothing here synchronises, so a step can be captured into a graph.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import _native as N
+
+MAX_REQUESTS = 4096
+MAX_HEAD_DIM = 256
+PAGE_SIZES = (16, 4096)       # of the cache: powers of two in this range
+MAX_REQUEST_TOKENS = 1 << 30  # block table width * page_size
+
+
+class PageTables(NamedTuple):
+    """What page_tables returns, int32 but for the slots (int64)."""
+    starts: torch.Tensor      # [B + 1] first row of each request
+    slots: torch.Tensor       # [rows] slot of each new token, -1: none
+    positions: torch.Tensor   # [rows] its position (depth in a drafted tree)
+    lens: torch.Tensor        # [B] tokens in the cache, the new ones included
+    pages_used: torch.Tensor  # [1] pages taken from the front of free_pages
+
+
+def _ints(t: torch.Tensor, name: str, shape, device) -> None:
+    assert t.dtype == torch.int32 and tuple(t.shape) == tuple(shape) and t.is_contiguous(), \
+        f"{name} must be a contiguous int32 tensor {list(shape)}, got {t.dtype} {list(t.shape)}"
+    assert t.device == device, f"{name} must be on {device}"
+
+
+def check_table(block_table: torch.Tensor, B: int, device) -> None:
+    assert block_table.dtype == torch.int32 and block_table.dim() == 2, "block_table must be int32 [B, width]"
+    assert block_table.shape[0] == B, f"block_table must have a row for each of the {B} requests"
+    assert block_table.stride(1) == 1 or block_table.shape[1] <= 1 or B == 0, "block_table rows must be contiguous"
+    assert block_table.device == device, f"block_table must be on {device}"
+
+
+def aligned_rows(x: torch.Tensor) -> torch.Tensor:
+    """x [rows, heads, D] itself where the kernels can read it: the head dim
+    contiguous, rows and heads at 16-byte steps; else a contiguous copy."""
+    n, h, d = x.stride()
+    es = x.element_size()
+    if (d == 1 or x.shape[2] == 1) and (n | h) * es % 16 == 0 and x.data_ptr() % 16 == 0:
+        return x
+    return x.clone(memory_format=torch.contiguous_format)
+
+
+def native_cache(k_cache: torch.Tensor, v_cache: torch.Tensor) -> "N.HtreeCache":
+    """Checks the cache tensors and describes them for the C ABI."""
+    assert k_cache.dim() == 4 and v_cache.dim() == 4, "k_cache / v_cache must be [pages, page_size, H_kv, D]"
+    pages, page, heads, K = k_cache.shape
+    V = v_cache.shape[3]
+    assert v_cache.shape[:3] == k_cache.shape[:3], "k_cache and v_cache must have the same pages and heads"
+    assert k_cache.dtype == v_cache.dtype and k_cache.dtype in N.DTYPE_CODE, \
+        "k_cache and v_cache must share one dtype: float32, bfloat16 or float16"
+    assert k_cache.is_cuda, "htree_amd runs on the GPU (no CPU fallback)"
+    assert k_cache.device == v_cache.device, "k_cache and v_cache must be on one device"
+    assert pages > 0 and heads > 0, "the cache needs a page and a head"
+    assert PAGE_SIZES[0] <= page <= PAGE_SIZES[1] and page & (page - 1) == 0, \
+        f"page_size must be a power of two from {PAGE_SIZES[0]} to {PAGE_SIZES[1]}, got {page}"
+    es = k_cache.element_size()
+    assert 0 < K <= MAX_HEAD_DIM and 0 < V <= MAX_HEAD_DIM and K * es % 16 == 0 and V * es % 16 == 0, \
+        f"head dims must be whole 16-byte pieces and at most {MAX_HEAD_DIM}, got K={K}, V={V}"
+    ks, vs = k_cache.stride(), v_cache.stride()
+    assert ks[3] == 1 and vs[3] == 1, "the cache's head dim must be contiguous"
+    assert (ks[0] | ks[1] | ks[2] | vs[0] | vs[1] | vs[2]) * es % 16 == 0 \
+        and k_cache.data_ptr() % 16 == 0 and v_cache.data_ptr() % 16 == 0, \
+        "the cache's pages, tokens and heads must be at 16-byte steps"
+    return N.HtreeCache(N.DTYPE_CODE[k_cache.dtype], heads, K, V, page, pages,
+                        ks[0], ks[1], ks[2], vs[0], vs[1], vs[2])
+
+
+def page_tables(ctx_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor,
+                free_pages: torch.Tensor, page_size: int, num_pages: int, rows: int,
+                parents: Optional[torch.Tensor] = None, out: Optional[PageTables] = None) -> PageTables:
+    """Room for a step's new tokens, worked out on the GPU.
+
+    Request b has ctx_lens[b] tokens in the cache and gets new_lens[b] more
+    (int32 [B]).  The pages it lacks are taken from the front of free_pages
+    (int32 [F]), request after request, and entered in block_table
+    (int32 [B, width], in place: its other entries stay).  `rows` is the
+    number of new tokens there is room for, at least the sum of new_lens in
+    the common case; tokens past it are dropped.  parents (int32 [rows])
+    makes the new tokens of a request drafted trees: parents[row] is the
+    index, within the request, of the token drafted before it, a smaller one
+    (-1: none); positions are then those along each branch.
+
+    Returns PageTables (`out`: written there).  Rows behind the last request
+    have slot and position -1; so has the slot of a token past the table's
+    width, or whose page free_pages was too short for (pages_used says how
+    many are wanted).  page_size is a power of two."""
+    assert ctx_lens.is_cuda, "htree_amd runs on the GPU (no CPU fallback)"
+    dev = ctx_lens.device
+    assert ctx_lens.dim() == 1, "ctx_lens must be int32 [B]"
+    B = ctx_lens.shape[0]
+    assert B <= MAX_REQUESTS, f"at most {MAX_REQUESTS} requests, got {B}"
+    _ints(ctx_lens, "ctx_lens", (B,), dev)
+    _ints(new_lens, "new_lens", (B,), dev)
+    check_table(block_table, B, dev)
+    assert free_pages.dim() == 1, "free_pages must be int32 [F]"
+    _ints(free_pages, "free_pages", free_pages.shape, dev)
+    assert page_size > 0 and page_size & (page_size - 1) == 0, f"page_size must be a power of two, got {page_size}"
+    assert 0 <= rows < 2 ** 31 and num_pages >= 0, "rows and num_pages must not be negative"
+    if parents is not None:
+        _ints(parents, "parents", (rows,), dev)
+    if out is None:
+        i32 = torch.empty(2 * B + 2 + rows, dtype=torch.int32, device=dev)
+        starts, lens, used, positions = i32.split((B + 1, B, 1, rows))
+        out = PageTables(starts, torch.empty(rows, dtype=torch.int64, device=dev), positions, lens, used)
+    else:
+        for t, name, n in ((out.starts, "out.starts", B + 1), (out.positions, "out.positions", rows),
+                           (out.lens, "out.lens", B), (out.pages_used, "out.pages_used", 1)):
+            _ints(t, name, (n,), dev)
+        assert out.slots.dtype == torch.int64 and out.slots.shape == (rows,) and out.slots.is_contiguous() \
+            and out.slots.device == dev, f"out.slots must be a contiguous int64 tensor [{rows}] on {dev}"
+    if B == 0:
+        out.starts.zero_(), out.pages_used.zero_(), out.slots.fill_(-1), out.positions.fill_(-1)
+        return out
+    with torch.cuda.device(dev):
+        rc = N.lib().htree_page_tables(
+            B, rows, page_size, num_pages, block_table.shape[1], block_table.stride(0),
+            free_pages.shape[0], N.ptr(ctx_lens), N.ptr(new_lens), N.ptr(parents), N.ptr(block_table),
+            N.ptr(free_pages), N.ptr(out.starts), N.ptr(out.slots), N.ptr(out.positions),
+            N.ptr(out.lens), N.ptr(out.pages_used), N.stream_ptr(dev))
+    N.check(rc, "htree_page_tables")
+    return out
+
+
+def cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                 slots: torch.Tensor, q: Optional[torch.Tensor] = None,
+                 positions: Optional[torch.Tensor] = None, cos: Optional[torch.Tensor] = None,
+                 sin: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """Writes new tokens' keys k [rows, H_kv, K] and values v [rows, H_kv, V]
+    into the cache at slots (int64 [rows], as page_tables gives them).
+
+    With the tables cos / sin (fp32 [n, K/2], htree_amd.rope_cache) each key
+    is rotated by its row's position (int32 [rows]) first, pairs
+    (d, d + K/2) as in htree_forward, and the queries q [rows, H, K] with
+    them: the rotated queries are returned (None without q).  Products and
+    sums are fp32, rounded once.  Rows whose slot or position is out of range
+    are not written, and a query without a position is zero.  The slots of a
+    call are distinct; two rows with one slot leave either's values there,
+    or parts of both."""
+    assert k.dim() == 3 and v.dim() == 3, "k / v must be [rows, H_kv, D]"
+    c = native_cache(k_cache, v_cache)
+    rows, dev = k.shape[0], k_cache.device
+    assert k.shape == (rows, c.H_kv, c.Dk) and v.shape == (rows, c.H_kv, c.Dv), \
+        f"k / v must be [rows, {c.H_kv}, {c.Dk} / {c.Dv}], got {list(k.shape)} / {list(v.shape)}"
+    assert k.dtype == v.dtype == k_cache.dtype, "k, v and the cache must share one dtype"
+    assert k.device == v.device == dev, "k, v and the cache must be on one device"
+    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
+        assert all(s > 0 or n == 1 for n, s in zip(t.shape, t.stride())), f"{name} must not be expanded"
+    assert slots.dtype == torch.int64 and slots.shape == (rows,) and slots.is_contiguous() \
+        and slots.device == dev, f"slots must be a contiguous int64 tensor [{rows}] on {dev}"
+    assert not (torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or
+                                             (q is not None and q.requires_grad))), \
+        "cache_append has no backward"
+    assert (cos is None) == (sin is None) == (positions is None), "positions, cos and sin go together"
+    H, rope_rows, q_out = 0, 0, None
+    if cos is not None:
+        assert c.Dk % 2 == 0, "rotating needs an even head dim K"
+        for name, t in (("cos", cos), ("sin", sin)):
+            assert t.dtype == torch.float32 and t.dim() == 2 and t.shape[1] == c.Dk // 2 and t.shape[0] > 0 \
+                and t.is_contiguous() and t.device == dev, \
+                f"{name} must be a contiguous fp32 tensor [n, {c.Dk // 2}] on {dev}"
+        assert cos.shape == sin.shape, "cos and sin must have one shape"
+        _ints(positions, "positions", (rows,), dev)
+        rope_rows = cos.shape[0]
+    if q is not None:
+        assert cos is not None, "q is taken to be rotated: it needs positions, cos and sin"
+        assert q.dim() == 3 and q.shape[0] == rows and q.shape[2] == c.Dk and q.shape[1] > 0, \
+            f"q must be [{rows}, H, {c.Dk}], got {list(q.shape)}"
+        assert q.dtype == k.dtype and q.device == dev, "q must have k's dtype and device"
+        H = q.shape[1]
+        q = aligned_rows(q)
+        q_out = torch.empty(rows, H, c.Dk, dtype=q.dtype, device=dev)
+    k, v = aligned_rows(k), aligned_rows(v)
+    with torch.cuda.device(dev):
+        rc = N.lib().htree_cache_append(
+            c, rows, H, N.ptr(k), k.stride(0), k.stride(1), N.ptr(v), v.stride(0), v.stride(1),
+            N.ptr(q), q.stride(0) if H else 0, q.stride(1) if H else 0, N.ptr(slots), N.ptr(positions),
+            N.ptr(cos), N.ptr(sin), rope_rows, N.ptr(q_out), N.ptr(k_cache), N.ptr(v_cache),
+            N.stream_ptr(dev))
+    N.check(rc, "htree_cache_append")
+    return q_out

@@ -1,0 +1,117 @@
+// Index arithmetic of the paged cache's kernels (htree_cache.hip,
+// htree_draft.h): how an attention call is split into units, which rows,
+// tokens and pages a unit touches, and which pages and slots a request's new
+// tokens get.  Lengths, tables and lists are device data that no host checks,
+// so everything read from them goes through these functions, and the host
+// replay over damaged inputs (tests/cache_replay_check.cpp) runs the same ones.
+#ifndef HTREE_CACHE_INDEX_H_
+#define HTREE_CACHE_INDEX_H_
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace htree {
+
+// ------------------------------------------------------- attention's split
+// tokens of a tile: 8 KB of keys and 8 KB of values (16 KB each for fp32 at
+// D 256), the loads that a wave has in flight while it computes
+__host__ __device__ constexpr int draft_tile(int D, int es) {
+  return 8192 / (D * es) > 64 ? 64 : 8192 / (D * es) < 16 ? 16 : 8192 / (D * es);
+}
+
+// A call's split.  Units: blocks of the launch, R = 16 MT rows of a request
+// and KV head each.  Groups: groups of rows whose units a second launch joins.
+struct DraftPlan {
+  int D, MT, R;
+  int target;  // units to split into (0: one unit per group of rows)
+  int64_t units, groups, slots, bytes;  // at most
+};
+__host__ __device__ inline DraftPlan draft_plan(int Dk, int Dv, int B, int rows, int H, int Hkv,
+                                                int width, int page_size) {
+  DraftPlan p;
+  const int m = Dk > Dv ? Dk : Dv;
+  p.D = m <= 32 ? 32 : m <= 64 ? 64 : m <= 128 ? 128 : 256;
+  const int G = H / Hkv;
+  const int64_t per = ((int64_t)rows * G + B - 1) / B;  // rows of a request, on average
+  p.MT = per <= 16 ? 1 : per <= 32 || p.D == 256 ? 2 : 4;
+  p.R = 16 * p.MT;
+  const int64_t rts = ((int64_t)rows * G / p.R + B) * Hkv;
+  // blocks that fit the GPU at once
+  const int full = p.MT == 1 && p.D <= 128 ? 512 : 256;
+  p.target = (int64_t)width * page_size <= 1024 ? 0 : full;
+  p.units = rts + p.target;
+  p.groups = rts < p.target ? rts : p.target;
+  // a split request has at most twice the chunks its tokens fill
+  p.slots = 2 * (int64_t)p.target;
+  p.bytes = p.slots * p.R * (p.D + 2) * 4;
+  return p;
+}
+
+// A request's lengths, held to what the buffers have
+struct DraftReq {
+  int s0, n;  // first row, rows (new tokens)
+  int len;    // tokens
+  int ctx;    // tokens before the new ones; negative: the first rows see nothing
+};
+__host__ __device__ inline DraftReq draft_req(int start, int end, int len, int rows) {
+  DraftReq r;
+  r.s0 = start < 0 ? 0 : start > rows ? rows : start;
+  r.n = (end < r.s0 ? r.s0 : end > rows ? rows : end) - r.s0;
+  r.len = len < 0 ? 0 : len;
+  r.ctx = r.len - r.n;
+  return r;
+}
+
+// tiles of a request; cap: tokens its table holds (at most 2^30)
+__host__ __device__ inline int draft_tiles(const DraftReq& r, int cap, int KT) {
+  return ((r.len < cap ? r.len : cap) + KT - 1) / KT;
+}
+// groups of rows of a request (and KV head)
+__host__ __device__ inline int64_t draft_row_groups(const DraftReq& r, int G, int R) {
+  return (r.n * (int64_t)G + R - 1) / R;
+}
+// Tiles of a chunk, from the tiles of all groups of rows: the same for every
+// request, a multiple of the block's 4 waves, two tiles a wave at least.
+__host__ __device__ inline int draft_chunk(int64_t tiles, int target) {
+  if (target <= 0) return 1 << 30;
+  int64_t c = (tiles + target - 1) / target;
+  c = (c + 3) / 4 * 4;
+  return (int)(c < 8 ? 8 : c > (1 << 30) ? (1 << 30) : c);
+}
+__host__ __device__ inline int draft_chunks(int tiles, int chunk) {
+  const int n = (int)(((int64_t)tiles + chunk - 1) / chunk);
+  return n < 1 ? 1 : n;
+}
+
+// What a unit's rows see: tokens [0, kend), tiles [t0, t1) in its chunk
+struct DraftSpan {
+  int kend, t0, t1;
+};
+__host__ __device__ inline DraftSpan draft_span(const DraftReq& r, int64_t row0, int R, int G, int cap,
+                                                int KT, int ch, int chunk) {
+  const int64_t nrow = (int64_t)r.n * G, last = (row0 + R < nrow ? row0 + R : nrow) - 1;
+  DraftSpan s;
+  const int64_t k = (int64_t)r.ctx + last / G + 1;
+  s.kend = (int)(k < 0 ? 0 : k > cap ? cap : k);
+  const int64_t t0 = (int64_t)ch * chunk, tn = (s.kend + KT - 1) / KT;
+  s.t0 = (int)(t0 < tn ? t0 : tn);
+  s.t1 = (int)(t0 + chunk < tn ? t0 + chunk : tn);
+  return s;
+}
+
+// a table entry as a page of the cache, or -1
+__host__ __device__ inline int cache_page(int entry, int num_pages) {
+  return entry >= 0 && entry < num_pages ? entry : -1;
+}
+
+// the token drafted before token j of a request, -1: none
+__host__ __device__ inline int draft_parent(int p, int j) { return p >= 0 && p < j ? p : -1; }
+
+// ------------------------------------------------------------ page tables
+// pages of n tokens
+__host__ __device__ inline int64_t table_pages(int64_t tokens, int shift) {
+  return (tokens + (((int64_t)1 << shift) - 1)) >> shift;
+}
+
+}  // namespace htree
+#endif  // HTREE_CACHE_INDEX_H_

@@ -1,0 +1,80 @@
+"""Attention of new tokens over a paged key/value cache: one token of each
+request (decoding), drafted trees of tokens to verify, or chunks of prompts.
+The cache, block tables and slots are cache.py's."""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional
+
+import torch
+
+from . import _native as N
+from .cache import MAX_REQUEST_TOKENS, _ints, aligned_rows, check_table, native_cache
+
+
+def draft_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                    block_table: torch.Tensor, lens: torch.Tensor, starts: torch.Tensor,
+                    parents: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """softmax(scale q k^T) v over what each row sees of its request.
+
+    q [rows, H, K]: the new tokens of all requests, rows starts[b] ..
+    starts[b + 1] - 1 (int32 [B + 1]) those of request b.  Their keys and
+    values are in the cache already (cache_append), the last of the lens[b]
+    tokens (int32 [B]) of the request.  Row j of a request sees the tokens
+    before the new ones, its ancestors by parents (int32 [rows]: the index
+    within the request of the token drafted before it, a smaller one, -1:
+    none) and itself; without parents the new tokens up to itself.  scale
+    defaults to K^-0.5.  Queries and keys come rotated.
+
+    Returns [rows, H, V] in q's dtype (`out`: written there, contiguous, no
+    overlap with the inputs).  Rows that see nothing are zero; rows behind
+    the last request are not written.  Pages outside the cache hold no
+    tokens, neither does the request past its table.
+
+    Scores and the softmax are fp32 (fp32 products for fp32 inputs); for
+    16-bit types P is rounded to the type for the product with the values.
+    Results do not depend on the other requests' values, but a request's
+    split, and so the last bits, depends on all lengths."""
+    c = native_cache(k_cache, v_cache)
+    dev = k_cache.device
+    assert q.dim() == 3, "q must be [rows, H, K]"
+    rows, H, K = q.shape
+    assert K == c.Dk, f"q and the cache must share the head dim K ({K} vs {c.Dk})"
+    assert H > 0 and H % c.H_kv == 0, f"H ({H}) must be divisible by H_kv ({c.H_kv})"
+    assert q.dtype == k_cache.dtype, "q and the cache must share one dtype"
+    assert q.device == dev, "q and the cache must be on one device"
+    assert lens.dim() == 1, "lens must be int32 [B]"
+    B = lens.shape[0]
+    _ints(lens, "lens", (B,), dev)
+    _ints(starts, "starts", (B + 1,), dev)
+    check_table(block_table, B, dev)
+    width = block_table.shape[1]
+    assert width * c.page_size <= MAX_REQUEST_TOKENS, \
+        f"a request's table holds at most {MAX_REQUEST_TOKENS} tokens, got {width * c.page_size}"
+    if parents is not None:
+        _ints(parents, "parents", (rows,), dev)
+    assert not (torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad
+                                             or v_cache.requires_grad)), "draft_attention has no backward"
+    if out is None:
+        out = torch.empty(rows, H, c.Dv, dtype=q.dtype, device=dev)
+    else:
+        assert out.shape == (rows, H, c.Dv) and out.dtype == q.dtype and out.is_contiguous() \
+            and out.device == dev and out.data_ptr() % 16 == 0, \
+            f"out must be a contiguous {q.dtype} tensor [{rows}, {H}, {c.Dv}] on {dev}"
+    if B == 0 or rows == 0:
+        return out
+    q = aligned_rows(q)
+    L = N.lib()
+    nbytes = ctypes.c_int64()
+    N.check(L.htree_draft_attention_workspace_bytes(c, B, rows, H, width, nbytes),
+            "htree_draft_attention_workspace_bytes")
+    with torch.cuda.device(dev):
+        ws = torch.empty(nbytes.value, dtype=torch.uint8, device=dev) if nbytes.value else None
+        rc = L.htree_draft_attention(
+            c, B, rows, H, width, block_table.stride(0), K ** -0.5 if scale is None else float(scale),
+            N.ptr(q), q.stride(0), q.stride(1), N.ptr(k_cache), N.ptr(v_cache), N.ptr(block_table),
+            N.ptr(lens), N.ptr(starts), N.ptr(parents), N.ptr(out), out.stride(0), out.stride(1),
+            N.ptr(ws), nbytes.value, N.stream_ptr(dev))
+    N.check(rc, "htree_draft_attention")
+    return out

@@ -286,6 +286,87 @@ int htree_topk_rows(const float* values, int64_t rows, int32_t n, int32_t k,
                     const int32_t* payload, int32_t n_payload, float* out_values,
                     int32_t* out_index, int32_t* out_payload, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Serving from a paged key / value cache.
+ *
+ * The cache is a pool of pages of page_size tokens: token p of request b is
+ * in page block_table[b][p / page_size] at offset p % page_size; a slot is
+ * page * page_size + offset.  The new tokens of all requests are packed:
+ * rows starts[b] .. starts[b + 1] - 1 are those of request b.  parents[row]
+ * is the index, among its request's new tokens, of the token it was drafted
+ * after, a smaller one (anything else: a root, drafted after the last cached
+ * token); without parents (NULL) each token follows the one before it.
+ *
+ * Lengths, tables, slots and positions are device data and are not checked
+ * on the host: whatever they hold, nothing outside the buffers is touched.
+ * The limits of a call are: page_size a power of two (16 .. 4096 for the
+ * cache itself), Dk and Dv up to 256 in rows of whole 16-byte pieces, every
+ * stride and base 16-byte aligned, at most 4096 requests in
+ * htree_page_tables, table_width * page_size <= 2^30 tokens a request. */
+
+typedef struct htree_cache {
+  int32_t dtype;      /* enum htree_dtype of keys, values, queries, output   */
+  int32_t H_kv, Dk, Dv;
+  int32_t page_size, num_pages;
+  int64_t k_page, k_token, k_head; /* strides of the key cache, in elements  */
+  int64_t v_page, v_token, v_head; /* and of the value cache; the head dim is
+                                      contiguous                             */
+} htree_cache;
+
+/* Block tables, slots and positions of a step: request b, with ctx_lens[b]
+ * tokens in the cache, gets new_lens[b] more (negative lengths count as 0).
+ * Pages are taken from free_pages [n_free] from the front, request after
+ * request, and written to block_table [B][table_stride] (entries
+ * ceil(ctx/page_size) .. ceil((ctx+new)/page_size) - 1, no others).
+ *   starts     [B + 1] first row of each request; new tokens past `rows`
+ *              are dropped
+ *   slots      [rows] of each new token; -1 for rows behind the last
+ *              request, past the table's width, without a page
+ *   positions  [rows] ctx + depth in the drafted tree (without parents:
+ *              ctx + index); -1 behind the last request
+ *   lens       [B] ctx + new (these and positions end at 2^31 - 1)
+ *   pages_used [1] pages wanted; more than n_free: the last ones are missing
+ *              (their entries are -1) */
+int htree_page_tables(int32_t B, int32_t rows, int32_t page_size, int32_t num_pages,
+                      int32_t table_width, int64_t table_stride, int32_t n_free,
+                      const int32_t* ctx_lens, const int32_t* new_lens,
+                      const int32_t* parents, int32_t* block_table,
+                      const int32_t* free_pages, int32_t* starts, int64_t* slots,
+                      int32_t* positions, int32_t* lens, int32_t* pages_used, void* stream);
+
+/* Writes k [rows, H_kv, Dk] and v [rows, H_kv, Dv] (strides in elements) to
+ * their slots.  With cos / sin tables [rope_rows, Dk/2] keys are rotated by
+ * their row's position first, as htree_forward rotates them (pairs d,
+ * d + Dk/2), and so are the queries q [rows, H, Dk] (may be NULL) into q_out
+ * [rows, H, Dk], contiguous.  Rows whose slot or position is out of range
+ * are not written; without a position q_out is zero.  Two rows with one slot
+ * leave either's values there, or parts of both. */
+int htree_cache_append(const htree_cache* c, int32_t rows, int32_t H, const void* k,
+                       int64_t k_row, int64_t k_head, const void* v, int64_t v_row,
+                       int64_t v_head, const void* q, int64_t q_row, int64_t q_head,
+                       const int64_t* slots, const int32_t* positions,
+                       const float* cos_table, const float* sin_table, int32_t rope_rows,
+                       void* q_out, void* k_cache, void* v_cache, void* stream);
+
+/* Bytes of workspace htree_draft_attention needs (host). */
+int htree_draft_attention_workspace_bytes(const htree_cache* c, int32_t B, int32_t rows,
+                                          int32_t H, int32_t table_width, int64_t* bytes);
+
+/* Attention of the new tokens' queries q [rows, H, Dk] over the cache, which
+ * holds lens[b] tokens of request b, the new ones among them as the last:
+ * row j of request b sees the tokens before the new ones, its ancestors in
+ * the drafted tree (without parents: the new tokens before it) and itself.
+ * Tokens in pages outside the cache (-1 entries) or past the table are not
+ * there; a row that sees nothing gets zeros.  Rows of `out` [rows, H, Dv]
+ * behind the last request are left as they were. */
+int htree_draft_attention(const htree_cache* c, int32_t B, int32_t rows, int32_t H,
+                          int32_t table_width, int64_t table_stride, float scale,
+                          const void* q, int64_t q_row, int64_t q_head, const void* k_cache,
+                          const void* v_cache, const int32_t* block_table,
+                          const int32_t* lens, const int32_t* starts, const int32_t* parents,
+                          void* out, int64_t out_row, int64_t out_head, void* workspace,
+                          int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
