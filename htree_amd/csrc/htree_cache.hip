@@ -290,7 +290,7 @@ static bool off16(const void* p) { return ((uintptr_t)p & 15) != 0; }
 static int log2i(int x) { return __builtin_ctz((unsigned)x); }
 
 static DraftPlan draft_plan(const htree_cache* c, int B, int rows, int H, int width) {
-  return draft_plan(c->Dk, c->Dv, B, rows, H, c->H_kv, width, c->page_size);
+  return draft_plan(c->Dk, c->Dv, cache_es(c), B, rows, H, c->H_kv, width, c->page_size);
 }
 
 static int draft_check(const htree_cache* c, int32_t B, int32_t rows, int32_t H, int32_t width) {
@@ -428,9 +428,10 @@ extern "C" int htree_draft_attention(const htree_cache* c, int32_t B, int32_t ro
   a.B = B, a.rows = rows, a.H = H, a.Hkv = c->H_kv, a.G = H / c->H_kv, a.Dk = c->Dk, a.Dv = c->Dv;
   a.width = table_width, a.page_shift = log2i(c->page_size), a.num_pages = c->num_pages;
   a.target = p.target;
-  a.c = scale * kLog2e;
+  a.negate = scale < 0.f;
+  a.c = fmaxf(fabsf(scale) * kLog2e, 1e-38f);  // a scale of 0 still multiplies -inf
   hipStream_t s = (hipStream_t)stream;
-  if (c->dtype == HTREE_F32) return draft_launch_type<float>(a, p.D, p.MT, p.units, p.groups, s);
-  if (c->dtype == HTREE_BF16) return draft_launch_type<__bf16>(a, p.D, p.MT, p.units, p.groups, s);
-  return draft_launch_type<_Float16>(a, p.D, p.MT, p.units, p.groups, s);
+  if (c->dtype == HTREE_F32) return draft_launch_type<float>(a, p, s);
+  if (c->dtype == HTREE_BF16) return draft_launch_type<__bf16>(a, p, s);
+  return draft_launch_type<_Float16>(a, p, s);
 }

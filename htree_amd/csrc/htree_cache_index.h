@@ -13,20 +13,32 @@
 namespace htree {
 
 // ------------------------------------------------------- attention's split
-// tokens of a tile: 8 KB of keys and 8 KB of values (16 KB each for fp32 at
-// D 256), the loads that a wave has in flight while it computes
-__host__ __device__ constexpr int draft_tile(int D, int es) {
-  return 8192 / (D * es) > 64 ? 64 : 8192 / (D * es) < 16 ? 16 : 8192 / (D * es);
+// A block's form.  NW = 1: four waves with the same 16 MT rows and tiles of
+// their own (few rows); else NW waves with 16 MT rows each and common tiles.
+struct DraftForm {
+  int MT, NW;
+};
+// the form for many rows
+__host__ __device__ constexpr DraftForm draft_rows_form(int D, int es) {
+  return DraftForm{2, 4};
+}
+// tokens of a tile: of a wave's own, 8 KB of keys and 8 KB of values (16 KB
+// each for fp32 at D 256), the loads that it has in flight while it computes;
+// of a block's, twice that
+__host__ __device__ constexpr int draft_tile(int D, int es, int NW = 1) {
+  return (NW > 1 ? 16384 : 8192) / (D * es) > 64 ? 64
+         : (NW > 1 ? 16384 : 8192) / (D * es) < 16 ? 16
+                                                    : (NW > 1 ? 16384 : 8192) / (D * es);
 }
 
-// A call's split.  Units: blocks of the launch, R = 16 MT rows of a request
-// and KV head each.  Groups: groups of rows whose units a second launch joins.
+// A call's split.  Units: blocks of the launch, R rows of a request and KV
+// head each.  Groups: groups of rows whose units a second launch joins.
 struct DraftPlan {
-  int D, MT, R;
+  int D, MT, NW, R;
   int target;  // units to split into (0: one unit per group of rows)
   int64_t units, groups, slots, bytes;  // at most
 };
-__host__ __device__ inline DraftPlan draft_plan(int Dk, int Dv, int B, int rows, int H, int Hkv,
+__host__ __device__ inline DraftPlan draft_plan(int Dk, int Dv, int es, int B, int rows, int H, int Hkv,
                                                 int width, int page_size) {
   DraftPlan p;
   const int m = Dk > Dv ? Dk : Dv;
@@ -34,10 +46,15 @@ __host__ __device__ inline DraftPlan draft_plan(int Dk, int Dv, int B, int rows,
   const int G = H / Hkv;
   const int64_t per = ((int64_t)rows * G + B - 1) / B;  // rows of a request, on average
   p.MT = per <= 16 ? 1 : per <= 32 || p.D == 256 ? 2 : 4;
-  p.R = 16 * p.MT;
+  p.NW = 1;
+  if (per > 64) {
+    const DraftForm f = draft_rows_form(p.D, es);
+    p.MT = f.MT, p.NW = f.NW;
+  }
+  p.R = 16 * p.MT * p.NW;
   const int64_t rts = ((int64_t)rows * G / p.R + B) * Hkv;
   // blocks that fit the GPU at once
-  const int full = p.MT == 1 && p.D <= 128 ? 512 : 256;
+  const int full = (p.NW > 1 || p.MT == 1) && p.D <= 128 ? 512 : 256;
   p.target = (int64_t)width * page_size <= 1024 ? 0 : full;
   p.units = rts + p.target;
   p.groups = rts < p.target ? rts : p.target;

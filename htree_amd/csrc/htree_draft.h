@@ -32,7 +32,8 @@ struct DraftArgs {
   int64_t k_page, k_token, k_head, v_page, v_token, v_head;            // bytes
   int32_t B, rows, H, Hkv, G, Dk, Dv, width, page_shift, num_pages;
   int32_t target;  // units to split into (0: one unit per group of rows)
-  float c;         // scale * log2(e)
+  float c;         // |scale| * log2(e), not 0
+  int32_t negate;  // the scale is negative: the queries change sign
 };
 
 template <typename T>
@@ -59,29 +60,31 @@ struct DraftT<_Float16> {
 template <>
 struct DraftT<float> {};
 
-template <typename T, int D, int MT>
+template <typename T, int D>
 struct DraftShape {
   static constexpr int ES = (int)sizeof(T);
   static constexpr bool F32 = ES == 4;
   static constexpr int ROWB = D * ES;      // bytes of a staged row
   static constexpr int CPR = ROWB / 16;    // its 16-byte chunks
   static constexpr int RPI = 64 / CPR;     // rows of one load of a wave
-  static constexpr int KT = draft_tile(D, ES);
-  static constexpr int NI = KT / RPI;      // loads of a tile's keys
-  static constexpr int NG = KT / 16;       // groups of 16 tokens: each in one page
-  static constexpr int R = 16 * MT;
-  static constexpr int TILE = KT * ROWB;
-  static constexpr int WAVE_LDS = 2 * TILE;
-  static constexpr int NW = kWavesPerBlock;
   static constexpr int NQ = D / 16;        // groups of 4 dims that a lane holds of a row
   // fp32: dims of a lane's V operand read at once
   static constexpr int VW = D / 16 > 4 ? 4 : D / 16;
+  static constexpr int OC = D / 4;         // 16-byte chunks of an fp32 row
+  static constexpr int OS = OC < 16 ? 7 : 15;
 };
 
-// place of a row's chunk: rows that are read together fall on other banks
+// Places of a row's chunk: rows that are read together fall on other banks.
+// Keys (and fp32 values): 16 rows, one chunk of each at a time.
 template <int CPR>
 __device__ __forceinline__ int draft_swz(int row, int chunk) {
   return CPR >= 16 ? chunk ^ (row & 15) : CPR == 8 ? chunk ^ ((row >> 1) & 7) : chunk ^ ((row >> 2) & 3);
+}
+// 16-bit values: the transposing reads take two chunks of 8 rows at a time.
+template <int CPR, bool F32>
+__device__ __forceinline__ int draft_swz_v(int row, int chunk) {
+  if (F32) return draft_swz<CPR>(row, chunk);
+  return CPR >= 16 ? chunk ^ ((row & 7) << 1) : CPR == 8 ? chunk ^ (((row >> 1) & 3) << 1) : chunk ^ (((row >> 2) & 1) << 1);
 }
 
 __device__ __forceinline__ int64_t wave_sum64(int64_t x) {
@@ -162,9 +165,9 @@ __device__ __forceinline__ bool draft_unit(const DraftArgs& a, int64_t u, bool g
 
 // 4 consecutive dims of a lane's row: dims dim(q) .. dim(q) + 3, from the
 // accumulators of the products' layouts
-template <typename T, int D, int MT>
+template <typename T, int D>
 struct DraftQuad {
-  using S = DraftShape<T, D, MT>;
+  using S = DraftShape<T, D>;
   static __device__ __forceinline__ int dim(int q, int g) {
     if constexpr (!S::F32) return 16 * q + 4 * g;
     else if constexpr (S::VW == 4) return 64 * (q >> 2) + 16 * g + 4 * (q & 3);
@@ -186,163 +189,123 @@ struct DraftQuad {
   }
 };
 
-template <typename T, int D, int MT>
-__global__ __launch_bounds__(256, (MT == 1 && D <= 128) ? 2 : 1) void draft_kernel(DraftArgs a) {
-  using S = DraftShape<T, D, MT>;
-  using Quad = DraftQuad<T, D, MT>;
-  constexpr int KT = S::KT, NI = S::NI, NG = S::NG, CPR = S::CPR, RPI = S::RPI, R = S::R;
-  constexpr int ES = S::ES, ROWB = S::ROWB, NQ = S::NQ, NW = S::NW;
-  constexpr bool F32 = S::F32;
-  __shared__ __attribute__((aligned(16))) char lds[NW * S::WAVE_LDS];
-  __shared__ float ml[NW][R][2];
-
-  DraftUnit u;
-  if (!draft_unit<KT, R>(a, blockIdx.x, false, &u)) return;  // uniform over the block
-  const int lane = threadIdx.x & 63, wv = uniform(threadIdx.x >> 6);
-  const int n16 = lane & 15, g = lane >> 4;
-  const DraftReq rq = draft_request(a, u.b);
-  const int s0 = uniform(rq.s0), ctx = uniform(rq.ctx);
-  const int cap = a.width << a.page_shift;
-  const int64_t nrow = (int64_t)rq.n * a.G, row0 = (int64_t)u.rt * R;
-  const DraftSpan sp = draft_span(rq, row0, R, a.G, cap, KT, u.ch, u.chunk);
-  const int kend = uniform(sp.kend), t0 = uniform(sp.t0), t1 = uniform(sp.t1);
-
-  // ---- the rows' queries, as the product's second operand (column n16)
-  int tok[MT];  // the row's new token, -1 behind the last row
-  int64_t orow[MT];
-  f32x4 qf[MT][F32 ? D / 16 : 1];
-  typename std::conditional<F32, f32x4, bf16x8>::type qh[MT][F32 ? 1 : D / 32];
+// whether a 16-byte piece holds an infinite or NaN element (every exponent
+// bit set)
+template <typename T>
+__device__ __forceinline__ bool draft_odd(uint4 x) {
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+  bool bad = false;
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-    const int64_t r = row0 + mt * 16 + n16;
-    const bool on = r < nrow;
-    const int j = on ? (int)(r / a.G) : 0, hg = on ? (int)(r - (int64_t)j * a.G) : 0;
-    tok[mt] = on ? j : -1;
-    const char* p = a.q + (int64_t)(s0 + j) * a.q_row + (int64_t)(u.h * a.G + hg) * a.q_head;
-    if constexpr (F32) {
-#pragma unroll
-      for (int s = 0; s < D / 16; ++s) {
-        const int d = 16 * s + 4 * g;
-        qf[mt][s] = on && d < a.Dk ? *(const f32x4*)(p + d * 4) : f32x4{0.f, 0.f, 0.f, 0.f};
-      }
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      bad |= (w[i] & 0x7f800000u) == 0x7f800000u;
     } else {
-#pragma unroll
-      for (int s = 0; s < D / 32; ++s) {
-        const int d = 32 * s + 8 * g;
-        const uint4 x = on && d < a.Dk ? *(const uint4*)(p + d * 2) : make_uint4(0, 0, 0, 0);
-        qh[mt][s] = __builtin_bit_cast(bf16x8, x);
-      }
+      constexpr uint32_t E = std::is_same<T, __bf16>::value ? 0x7f80u : 0x7c00u;
+      bad |= (w[i] & E) == E || ((w[i] >> 16) & E) == E;
     }
   }
+  return bad;
+}
 
+// What a block knows of its unit
+struct DraftCtx {
+  int s0, ctx, kend, t0, t1, used, shift;
+  int full;  // tokens that every row sees, where their pages exist
+  int64_t nrow;
+  const char *kh, *vh;     // the KV head's keys and values
+  const int32_t* tab;      // the request's table
+  const int32_t* par;      // its new tokens' parents, or null
+  // page of the 16 tokens from `key`, -1: none (past the end, no page of the
+  // cache)
+  __device__ __forceinline__ int page(const DraftArgs& a, int key, bool on) const {
+    const int pi = key >> shift;
+    return cache_page(on && pi < used ? tab[pi] : -1, a.num_pages);
+  }
+};
+template <int KT, int R>
+__device__ __forceinline__ DraftCtx draft_ctx(const DraftArgs& a, const DraftUnit& u, const DraftReq& rq) {
+  DraftCtx c;
+  c.s0 = uniform(rq.s0), c.ctx = uniform(rq.ctx);
+  c.shift = a.page_shift;
+  c.nrow = (int64_t)rq.n * a.G;
+  const DraftSpan sp = draft_span(rq, (int64_t)u.rt * R, R, a.G, a.width << a.page_shift, KT, u.ch, u.chunk);
+  c.kend = uniform(sp.kend), c.t0 = uniform(sp.t0), c.t1 = uniform(sp.t1);
+  c.used = (c.kend + (1 << c.shift) - 1) >> c.shift;
+  // rows behind the request's last see nothing, but are not stored either
+  c.full = min(a.parents ? c.ctx : c.ctx + (int)((int64_t)u.rt * R / a.G) + 1, c.kend);
+  c.kh = a.k + u.h * a.k_head;
+  c.vh = a.v + u.h * a.v_head;
+  c.tab = a.table + u.b * a.table_stride;
+  c.par = a.parents ? a.parents + c.s0 : nullptr;
+  return c;
+}
+
+// A wave's rows and their running softmax: 16 MT rows, in the products'
+// layout of one row per lane of 16 (column n16), the lane's group g of 4
+// holding a quarter of the tokens (scores) or of the dims (output).
+template <typename T, int D, int MT, int KT>
+struct DraftWave {
+  using S = DraftShape<T, D>;
+  using Quad = DraftQuad<T, D>;
+  static constexpr int NG = KT / 16, CPR = S::CPR, ROWB = S::ROWB, NQ = S::NQ;
+  static constexpr bool F32 = S::F32;
+  int n16, g;
+  int tok[MT];  // the row's new token, -1 behind the last row
+  f32x4 qf[MT][F32 ? D / 16 : 1];
+  bf16x8 qh[MT][F32 ? 1 : D / 32];
   float m[MT], l[MT];
   f32x4 o[MT][NQ];
+
+  __device__ __forceinline__ void init(const DraftArgs& a, const DraftCtx& c, int h, int64_t row0) {
+    const int lane = threadIdx.x & 63;
+    n16 = lane & 15, g = lane >> 4;
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-    m[mt] = -INFINITY;
-    l[mt] = 0.f;
+    for (int mt = 0; mt < MT; ++mt) {
+      const int64_t r = row0 + mt * 16 + n16;
+      const bool on = r < c.nrow;
+      const int j = on ? (int)(r / a.G) : 0, hg = on ? (int)(r - (int64_t)j * a.G) : 0;
+      tok[mt] = on ? j : -1;
+      const char* p = a.q + (int64_t)(c.s0 + j) * a.q_row + (int64_t)(h * a.G + hg) * a.q_head;
+      if constexpr (F32) {
 #pragma unroll
-    for (int q = 0; q < NQ; ++q) o[mt][q] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int s = 0; s < D / 16; ++s) {
+          const int d = 16 * s + 4 * g;
+          const f32x4 x = on && d < a.Dk ? *(const f32x4*)(p + d * 4) : f32x4{0.f, 0.f, 0.f, 0.f};
+          qf[mt][s] = a.negate ? -x : x;
+        }
+      } else {
+#pragma unroll
+        for (int s = 0; s < D / 32; ++s) {
+          const int d = 32 * s + 8 * g;
+          uint4 x = on && d < a.Dk ? *(const uint4*)(p + d * 2) : make_uint4(0, 0, 0, 0);
+          const uint32_t f = a.negate ? 0x80008000u : 0u;
+          x.x ^= f, x.y ^= f, x.z ^= f, x.w ^= f;
+          qh[mt][s] = __builtin_bit_cast(bf16x8, x);
+        }
+      }
+      m[mt] = -INFINITY;
+      l[mt] = 0.f;
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) o[mt][q] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
   }
 
-  // ---- this wave's tiles
-  char* kb = lds + wv * S::WAVE_LDS;
-  char* vb = kb + S::TILE;
-  const int lr = lane / CPR, lc = lane % CPR;
-  // lanes past the head dim read the row's first chunk and write zeros
-  const bool kin = lc * 16 < a.Dk * ES, vin = lc * 16 < a.Dv * ES;
-  const int64_t koff = lr * a.k_token + (kin ? lc * 16 : 0);
-  const int64_t voff = lr * a.v_token + (vin ? lc * 16 : 0);
-  const char* kh = a.k + u.h * a.k_head;
-  const char* vh = a.v + u.h * a.v_head;
-  const int32_t* tab = a.table + u.b * a.table_stride;
-  const int used = (kend + (1 << a.page_shift) - 1) >> a.page_shift;  // <= width
+  // whether row mt's token sees the request's token `key` < kend
+  __device__ __forceinline__ bool sees(const DraftCtx& c, int mt, int key) const {
+    if (tok[mt] < 0) return false;
+    if (!c.par) return key <= c.ctx + tok[mt];
+    if (key < c.ctx) return true;
+    int j = tok[mt];
+    while (j >= 0 && c.ctx + j > key) j = draft_parent(c.par[j], j);
+    return j >= 0 && c.ctx + j == key;
+  }
 
-  // page of each group of 16 tokens, -1: none (past the end, or no page of the cache)
-  auto pages = [&](int t, int (&e)[NG]) {
-#pragma unroll
-    for (int i = 0; i < NG; ++i) {
-      const int pi = (t * KT + 16 * i) >> a.page_shift;
-      e[i] = cache_page(t < t1 && pi < used ? tab[pi] : -1, a.num_pages);
-    }
-  };
-  uint4 kr[NI], vr[NI];
-  auto load = [&](int t, const int (&e)[NG]) {
-#pragma unroll
-    for (int i = 0; i < NG; ++i) {
-      const int64_t pg = e[i] < 0 ? 0 : e[i];
-      const int at = (t * KT + 16 * i) & ((1 << a.page_shift) - 1);
-      const char* kp = kh + pg * a.k_page + at * a.k_token;
-      const char* vp = vh + pg * a.v_page + at * a.v_token;
-#pragma unroll
-      for (int x = 0; x < NI / NG; ++x) {
-        kr[i * (NI / NG) + x] = *(const uint4*)(kp + (koff + (int64_t)(x * RPI) * a.k_token));
-        vr[i * (NI / NG) + x] = *(const uint4*)(vp + (voff + (int64_t)(x * RPI) * a.v_token));
-      }
-    }
-  };
-
-  int ent[NG], nxt[NG];
-  int t = t0 + wv;
-  pages(t, ent);
-  pages(t + NW, nxt);
-  if (t < t1) load(t, ent);
-  for (; t < t1; t += NW) {
-    const int key0 = t * KT;
-    // tokens that every row sees need no mask: those before the new ones,
-    // in pages that exist
-    bool masked = key0 + KT > min(ctx, kend);
-#pragma unroll
-    for (int i = 0; i < NG; ++i) masked |= ent[i] < 0;
-    uint64_t odd = 0;  // tokens with an infinite or NaN value
-    if (masked) {
-      // Values that no row sees must not meet the product: 0 x NaN is NaN.
-#pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        const int row = i * RPI + lr;
-        if (key0 + row >= kend || ent[i * RPI / 16] < 0) vr[i] = make_uint4(0, 0, 0, 0);
-        // every exponent bit set in an element
-        bool bad;
-        if constexpr (F32) {
-          bad = false;
-          const uint32_t w[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
-#pragma unroll
-          for (int x = 0; x < 4; ++x) bad |= (w[x] & 0x7f800000u) == 0x7f800000u;
-        } else {
-          constexpr uint32_t E = std::is_same<T, __bf16>::value ? 0x7f80u : 0x7c00u;
-          bad = false;
-          const uint32_t w[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
-#pragma unroll
-          for (int x = 0; x < 4; ++x)
-            bad |= (w[x] & E) == E || ((w[x] >> 16) & E) == E;
-        }
-        uint64_t hit = __ballot(bad && vin);
-        if (hit) {
-#pragma unroll
-          for (int x = 0; x < RPI; ++x) {
-            const uint64_t lanes = (CPR == 64 ? ~0ull : ((1ull << (CPR & 63)) - 1)) << ((x * CPR) & 63);
-            if (hit & lanes) odd |= 1ull << (i * RPI + x);
-          }
-          if ((odd >> row) & 1) vr[i] = make_uint4(0, 0, 0, 0);
-        }
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      const int row = i * RPI + lr;
-      const int at = row * ROWB + draft_swz<CPR>(row, lc) * 16;
-      if (!kin) kr[i] = make_uint4(0, 0, 0, 0);
-      if (!vin) vr[i] = make_uint4(0, 0, 0, 0);
-      *(uint4*)(kb + at) = kr[i];
-      *(uint4*)(vb + at) = vr[i];
-    }
-    int cur[NG];
-#pragma unroll
-    for (int i = 0; i < NG; ++i) cur[i] = ent[i], ent[i] = nxt[i];
-    if (t + NW < t1) load(t + NW, ent);
-    pages(t + 2 * NW, nxt);
-    wave_sync();
-
+  // One tile of KT tokens from key0, staged at kb / vb.  MASKED: not every
+  // row sees every token; there: the tokens (bits) that exist; odd: those
+  // with an infinite or NaN value, whose staged values are zero.
+  template <bool MASKED>
+  __device__ __forceinline__ void tile(const DraftArgs& a, const DraftCtx& c, const char* kb, const char* vb,
+                                       int key0, uint64_t there, uint64_t odd) {
     // ---- scores, token x row: a lane holds tokens 4 g .. 4 g + 3 of each
     // group of 16, of row n16
     f32x4 sc[MT][NG];
@@ -374,31 +337,21 @@ __global__ __launch_bounds__(256, (MT == 1 && D <= 128) ? 2 : 1) void draft_kern
       }
     }
 
-    // ---- to log2 units; masks
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int i = 0; i < NG; ++i) sc[mt][i] *= a.c;
-    if (masked) {
-      uint64_t there = 0;  // tokens before the end, in pages that exist
-#pragma unroll
-      for (int i = 0; i < NG; ++i) {
-        const int left = min(max(kend - key0 - 16 * i, 0), 16);
-        if (cur[i] >= 0) there |= (uint64_t)((1u << left) - 1u) << (16 * i);
-      }
+    // ---- masks
+    if constexpr (MASKED) {
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
         uint64_t see = 0;
         if (tok[mt] >= 0) {
-          if (a.parents) {
-            const int c0 = min(max(ctx - key0, 0), 64);  // cached tokens of the tile
+          if (c.par) {
+            const int c0 = min(max(c.ctx - key0, 0), 64);  // cached tokens of the tile
             see = c0 == 64 ? ~0ull : (1ull << c0) - 1;
-            for (int j = tok[mt]; j >= 0 && ctx + j >= key0;) {
-              if (ctx + j - key0 < KT) see |= 1ull << (ctx + j - key0);
-              j = draft_parent(a.parents[s0 + j], j);
+            for (int j = tok[mt]; j >= 0 && c.ctx + j >= key0;) {
+              if (c.ctx + j - key0 < KT) see |= 1ull << (c.ctx + j - key0);
+              j = draft_parent(c.par[j], j);
             }
           } else {
-            const int c1 = min(max(ctx + tok[mt] + 1 - key0, 0), 64);
+            const int c1 = min(max(c.ctx + tok[mt] + 1 - key0, 0), 64);
             see = c1 == 64 ? ~0ull : (1ull << c1) - 1;
           }
         }
@@ -411,7 +364,9 @@ __global__ __launch_bounds__(256, (MT == 1 && D <= 128) ? 2 : 1) void draft_kern
       }
     }
 
-    // ---- running softmax
+    // ---- running softmax, in log2 units.  The max a row's weights are taken
+    // against only moves when a score passes it by 8: weights up to 2^8 lose
+    // nothing, and the output is seldom rescaled.
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       float mx = -INFINITY;
@@ -419,9 +374,9 @@ __global__ __launch_bounds__(256, (MT == 1 && D <= 128) ? 2 : 1) void draft_kern
       for (int i = 0; i < NG; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) mx = fmaxf(mx, sc[mt][i][e]);
-      mx = max_xor32(max_xor16(mx));
-      if (__any(mx > m[mt])) {
-        const float mn = fmaxf(m[mt], mx);
+      mx = max_xor32(max_xor16(mx)) * a.c;
+      if (__any(mx > m[mt] + 8.f)) {
+        const float mn = mx > m[mt] + 8.f ? mx : m[mt];
         const float al = m[mt] == mn ? 1.f : __builtin_amdgcn_exp2f(m[mt] - mn);
         m[mt] = mn;
         l[mt] *= al;
@@ -433,19 +388,18 @@ __global__ __launch_bounds__(256, (MT == 1 && D <= 128) ? 2 : 1) void draft_kern
       for (int i = 0; i < NG; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          sc[mt][i][e] = __builtin_amdgcn_exp2f(sc[mt][i][e] - ref);
+          sc[mt][i][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[mt][i][e], a.c, -ref));
           l[mt] += sc[mt][i][e];
         }
     }
 
-    // ---- tokens with infinite or NaN values (their staged rows are zero):
-    // only the rows that see them take them
-    if (odd) {
+    // ---- tokens with infinite or NaN values: only the rows that see them
+    // take them
+    if (MASKED && odd) {
       for (uint64_t left = odd; left; left &= left - 1) {
-        const int key = __builtin_ctzll(left);
-        const int pi = (key0 + key) >> a.page_shift, at = (key0 + key) & ((1 << a.page_shift) - 1);
-        const int64_t pg = tab[pi];  // a page of the cache: its values were read
-        const char* vp = vh + pg * a.v_page + at * a.v_token;
+        const int key = __builtin_ctzll(left), at = key0 + key;
+        const int64_t pg = c.tab[at >> c.shift];  // a page of the cache: its values were read
+        const T* vp = (const T*)(c.vh + pg * a.v_page + (at & ((1 << c.shift) - 1)) * a.v_token);
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
           float p = 0.f;
@@ -455,21 +409,13 @@ __global__ __launch_bounds__(256, (MT == 1 && D <= 128) ? 2 : 1) void draft_kern
             for (int e = 0; e < 4; ++e)
               if (key >> 4 == i && (key & 3) == e) p = sc[mt][i][e];
           p = __shfl(p, ((key >> 2) & 3) * 16 + n16);
-          // row n16 sees it: not masked (p may be 0 for a very low score)
-          bool see = tok[mt] >= 0;
-          if (see && a.parents) {
-            int j = tok[mt];
-            while (j >= 0 && ctx + j > key0 + key) j = draft_parent(a.parents[s0 + j], j);
-            see = key0 + key < ctx || (j >= 0 && ctx + j == key0 + key);
-          } else if (see) {
-            see = key0 + key <= ctx + tok[mt];
-          }
+          const bool see = sees(c, mt, at);
 #pragma unroll
           for (int q = 0; q < NQ; ++q)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int d = Quad::dim(q, g) + e;
-              if (see && d < a.Dv) Quad::add(o[mt], q, e, p * Io<T>::ld((const T*)vp + d));
+              if (see && d < a.Dv) Quad::add(o[mt], q, e, p * Io<T>::ld(vp + d));
             }
         }
       }
@@ -486,14 +432,14 @@ __global__ __launch_bounds__(256, (MT == 1 && D <= 128) ? 2 : 1) void draft_kern
 #pragma unroll
           for (int q = 0; q < NQ; q += S::VW) {
             if constexpr (S::VW == 4) {
-              const f32x4 x = *(const f32x4*)(vb + row * ROWB + draft_swz<CPR>(row, 4 * q + n16) * 16);
+              const f32x4 x = *(const f32x4*)(vb + row * ROWB + draft_swz_v<CPR, F32>(row, 4 * q + n16) * 16);
 #pragma unroll
               for (int w = 0; w < 4; ++w)
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
                   o[mt][q + w] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[w], sc[mt][i][e], o[mt][q + w], 0, 0, 0);
             } else {
-              const f32x2 x = *(const f32x2*)(vb + row * ROWB + draft_swz<CPR>(row, n16 >> 1) * 16 + (n16 & 1) * 8);
+              const f32x2 x = *(const f32x2*)(vb + row * ROWB + draft_swz_v<CPR, F32>(row, n16 >> 1) * 16 + (n16 & 1) * 8);
 #pragma unroll
               for (int w = 0; w < 2; ++w)
 #pragma unroll
@@ -518,7 +464,7 @@ __global__ __launch_bounds__(256, (MT == 1 && D <= 128) ? 2 : 1) void draft_kern
       // it addresses token 4 g + n16 / 4, dims 4 (n16 % 4) ..
       auto col = [&](int i, int q) {
         const int row = 16 * i + 4 * g + (n16 >> 2);
-        const char* p = vb + row * ROWB + draft_swz<CPR>(row, 2 * q + ((n16 & 3) >> 1)) * 16 + (n16 & 1) * 8;
+        const char* p = vb + row * ROWB + draft_swz_v<CPR, F32>(row, 2 * q + ((n16 & 3) >> 1)) * 16 + (n16 & 1) * 8;
         return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
             (__attribute__((address_space(3))) s16x4*)(const __attribute__((address_space(3))) void*)p);
       };
@@ -544,86 +490,354 @@ __global__ __launch_bounds__(256, (MT == 1 && D <= 128) ? 2 : 1) void draft_kern
         }
       }
     }
-    wave_sync();  // this tile's reads come before the next one's writes
+  }
+
+  // the lane's part of row n16 of group mt, times f, into 16 fp32 rows at dst
+  __device__ __forceinline__ void put(float* dst, int mt, float f) const {
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+      const int ch = Quad::dim(q, g) >> 2;
+      *(f32x4*)(dst + n16 * D + ((ch ^ (n16 & S::OS)) << 2)) = Quad::get(o[mt], q) * f;
+    }
+  }
+};
+
+// one chunk of 4 dims of a row, as put() left it
+template <typename T, int D>
+__device__ __forceinline__ f32x4 draft_got(const float* src, int row, int ch) {
+  return *(const f32x4*)(src + row * D + ((ch ^ (row & DraftShape<T, D>::OS)) << 2));
+}
+
+// stores chunk ch of the request's row r (x: weighted sum, sum: the weights')
+template <typename T>
+__device__ __forceinline__ void draft_store(const DraftArgs& a, int s0, int h, int64_t r, int ch, f32x4 x, float sum) {
+  if (ch * 4 >= a.Dv) return;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row that sees nothing is zero
+  const int j = (int)(r / a.G), hg = (int)(r - (int64_t)j * a.G);
+  typedef __attribute__((ext_vector_type(4))) T T4;
+  *(T4*)(a.out + (int64_t)(s0 + j) * a.o_row + (int64_t)(h * a.G + hg) * a.o_head + ch * 4 * sizeof(T)) =
+      __builtin_convertvector(x * inv, T4);
+}
+
+// Few rows: the four waves of a block have the same 16 MT rows and take the
+// chunk's tiles in turn, each through LDS of its own, so that there is no
+// barrier before their states meet.
+template <typename T, int D, int MT>
+__global__ __launch_bounds__(256, (MT == 1 && D <= 128) ? 2 : 1) void draft_kernel(DraftArgs a) {
+  using S = DraftShape<T, D>;
+  constexpr int KT = draft_tile(D, S::ES), NG = KT / 16, CPR = S::CPR, RPI = S::RPI, R = 16 * MT;
+  constexpr int NI = KT / RPI, ROWB = S::ROWB, NW = kWavesPerBlock;
+  constexpr int WAVE_LDS = 2 * KT * ROWB;
+  __shared__ __attribute__((aligned(16))) char lds[NW * WAVE_LDS];
+  __shared__ float ml[NW][R][2];
+
+  DraftUnit u;
+  if (!draft_unit<KT, R>(a, blockIdx.x, false, &u)) return;  // uniform over the block
+  const int lane = threadIdx.x & 63, wv = uniform(threadIdx.x >> 6);
+  const DraftReq rq = draft_request(a, u.b);
+  const DraftCtx c = draft_ctx<KT, R>(a, u, rq);
+  const int64_t row0 = (int64_t)u.rt * R;
+  DraftWave<T, D, MT, KT> w;
+  w.init(a, c, u.h, row0);
+
+  char* kb = lds + wv * WAVE_LDS;
+  char* vb = kb + KT * ROWB;
+  const int lr = lane / CPR, lc = lane % CPR;
+  // lanes past the head dim read the row's first chunk and write zeros
+  const bool kin = lc * 16 < a.Dk * S::ES, vin = lc * 16 < a.Dv * S::ES;
+  const int64_t koff = lr * a.k_token + (kin ? lc * 16 : 0);
+  const int64_t voff = lr * a.v_token + (vin ? lc * 16 : 0);
+
+  auto pages = [&](int t, int (&e)[NG]) {
+#pragma unroll
+    for (int i = 0; i < NG; ++i) e[i] = c.page(a, t * KT + 16 * i, t < c.t1);
+  };
+  uint4 kr[NI], vr[NI];
+  auto load = [&](int t, const int (&e)[NG]) {
+#pragma unroll
+    for (int i = 0; i < NG; ++i) {
+      const int64_t pg = e[i] < 0 ? 0 : e[i];
+      const int at = (t * KT + 16 * i) & ((1 << c.shift) - 1);
+      const char* kp = c.kh + pg * a.k_page + at * a.k_token;
+      const char* vp = c.vh + pg * a.v_page + at * a.v_token;
+#pragma unroll
+      for (int x = 0; x < NI / NG; ++x) {
+        kr[i * (NI / NG) + x] = *(const uint4*)(kp + (koff + (int64_t)(x * RPI) * a.k_token));
+        vr[i * (NI / NG) + x] = *(const uint4*)(vp + (voff + (int64_t)(x * RPI) * a.v_token));
+      }
+    }
+  };
+
+  // the staged tile into LDS; the loads of the wave's next one go out
+  int ent[NG], nxt[NG];
+  int t = c.t0 + wv;
+  auto stage = [&]() {
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int row = i * RPI + lr;
+      if (!kin) kr[i] = make_uint4(0, 0, 0, 0);
+      if (!vin) vr[i] = make_uint4(0, 0, 0, 0);
+      *(uint4*)(kb + row * ROWB + draft_swz<CPR>(row, lc) * 16) = kr[i];
+      *(uint4*)(vb + row * ROWB + draft_swz_v<CPR, S::F32>(row, lc) * 16) = vr[i];
+    }
+#pragma unroll
+    for (int i = 0; i < NG; ++i) ent[i] = nxt[i];
+    if (t + NW < c.t1) load(t + NW, ent);
+    pages(t + 2 * NW, nxt);
+    wave_sync();
+  };
+  // tiles that some row does not see all of: past `full`, or pages missing
+  auto masked = [&]() {
+    bool x = (t + 1) * KT > c.full;
+#pragma unroll
+    for (int i = 0; i < NG; ++i) x |= ent[i] < 0;
+    return x;
+  };
+  pages(t, ent);
+  pages(t + NW, nxt);
+  if (t < c.t1) load(t, ent);
+  while (t < c.t1) {
+    for (; t < c.t1 && !masked(); t += NW) {
+      stage();
+      w.template tile<false>(a, c, kb, vb, t * KT, 0, 0);
+      wave_sync();  // this tile's reads come before the next one's writes
+    }
+    for (; t < c.t1 && masked(); t += NW) {
+      const int key0 = t * KT;
+      uint64_t odd = 0, there = 0;
+#pragma unroll
+      for (int i = 0; i < NG; ++i) {
+        const int left = min(max(c.kend - key0 - 16 * i, 0), 16);
+        if (ent[i] >= 0) there |= (uint64_t)((1u << left) - 1u) << (16 * i);
+      }
+      // Values that no row sees must not meet the product: 0 x NaN is NaN.
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const int row = i * RPI + lr;
+        if (!((there >> row) & 1)) vr[i] = make_uint4(0, 0, 0, 0);
+        const uint64_t hit = __ballot(draft_odd<T>(vr[i]) && vin);
+        if (hit) {
+#pragma unroll
+          for (int x = 0; x < RPI; ++x) {
+            const uint64_t lanes = (CPR == 64 ? ~0ull : ((1ull << (CPR & 63)) - 1)) << ((x * CPR) & 63);
+            if (hit & lanes) odd |= 1ull << (i * RPI + x);
+          }
+          if ((odd >> row) & 1) vr[i] = make_uint4(0, 0, 0, 0);
+        }
+      }
+      stage();
+      w.template tile<true>(a, c, kb, vb, key0, there, odd);
+      wave_sync();
+    }
   }
 
   // ---- the four waves' states meet
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
-    l[mt] = add_xor32(add_xor16(l[mt]));
-    if (g == 0) {
-      ml[wv][mt * 16 + n16][0] = m[mt];
-      ml[wv][mt * 16 + n16][1] = l[mt];
+    w.l[mt] = add_xor32(add_xor16(w.l[mt]));
+    if (w.g == 0) {
+      ml[wv][mt * 16 + w.n16][0] = w.m[mt];
+      ml[wv][mt * 16 + w.n16][1] = w.l[mt];
     }
   }
   __syncthreads();
-  constexpr int OC = D / 4;           // 16-byte chunks of an fp32 row
-  constexpr int OS = OC < 16 ? 7 : 15;
-  const bool part = u.nch > 1;
-  const int64_t slot = part ? u.slot + (u.ch * draft_row_groups(rq, a.G, R) + u.rt) * a.Hkv + u.h : 0;
+  const int64_t slot = u.nch > 1 ? u.slot + (u.ch * draft_row_groups(rq, a.G, R) + u.rt) * a.Hkv + u.h : -1;
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
     float mm = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < NW; ++w) mm = fmaxf(mm, ml[w][mt * 16 + n16][0]);
-    const float f = m[mt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[mt] - mm);
-    // a wave that saw no token of the row adds nothing; NaN states stay NaN
-    float* mine = (float*)(lds + wv * S::WAVE_LDS);
-#pragma unroll
-    for (int q = 0; q < NQ; ++q) {
-      const f32x4 x = Quad::get(o[mt], q);
-      const int ch = Quad::dim(q, g) >> 2;
-      *(f32x4*)(mine + n16 * D + ((ch ^ (n16 & OS)) << 2)) = m[mt] == -INFINITY ? x : x * f;
-    }
+    for (int i = 0; i < NW; ++i) mm = fmaxf(mm, ml[i][mt * 16 + w.n16][0]);
+    // a wave that saw no token of the row adds nothing (NaN scores leave the
+    // max alone and make sums NaN, which stay)
+    w.put((float*)(lds + wv * WAVE_LDS), mt, w.m[mt] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(w.m[mt] - mm));
     __syncthreads();
-    for (int i = threadIdx.x; i < 16 * OC; i += 256) {
-      const int row = i / OC, ch = i % OC, rr = mt * 16 + row;
-      const int64_t r = row0 + rr;
-      if (r >= nrow) continue;
+    for (int i = threadIdx.x; i < 16 * S::OC; i += 256) {
+      const int row = i / S::OC, ch = i % S::OC, rr = mt * 16 + row;
+      if (row0 + rr >= c.nrow) continue;
       f32x4 x = {0.f, 0.f, 0.f, 0.f};
       float big = -INFINITY, sum = 0.f;
 #pragma unroll
-      for (int w = 0; w < NW; ++w) big = fmaxf(big, ml[w][rr][0]);
+      for (int j = 0; j < NW; ++j) big = fmaxf(big, ml[j][rr][0]);
 #pragma unroll
-      for (int w = 0; w < NW; ++w) {
-        x += *(const f32x4*)((const float*)(lds + w * S::WAVE_LDS) + row * D + ((ch ^ (row & OS)) << 2));
-        const float mw = ml[w][rr][0];
-        sum += mw == -INFINITY ? ml[w][rr][1] : ml[w][rr][1] * __builtin_amdgcn_exp2f(mw - big);
+      for (int j = 0; j < NW; ++j) {
+        x += draft_got<T, D>((const float*)(lds + j * WAVE_LDS), row, ch);
+        const float mj = ml[j][rr][0];
+        sum += mj == -INFINITY ? ml[j][rr][1] : ml[j][rr][1] * __builtin_amdgcn_exp2f(mj - big);
       }
-      if (part) {
+      if (slot >= 0) {
         *(f32x4*)(a.ws_o + (slot * R + rr) * D + ch * 4) = x;
         if (ch == 0) {
           a.ws_ml[(slot * R + rr) * 2] = big;
           a.ws_ml[(slot * R + rr) * 2 + 1] = sum;
         }
-      } else if (ch * 4 < a.Dv) {
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row that sees nothing is zero
-        const int j = (int)(r / a.G), hg = (int)(r - (int64_t)j * a.G);
-        char* p = a.out + (int64_t)(s0 + j) * a.o_row + (int64_t)(u.h * a.G + hg) * a.o_head + ch * 4 * ES;
-        typedef __attribute__((ext_vector_type(4))) T T4;
-        *(T4*)p = __builtin_convertvector(x * inv, T4);
+      } else {
+        draft_store<T>(a, c.s0, u.h, row0 + rr, ch, x, sum);
       }
     }
     __syncthreads();
   }
 }
 
+// Many rows: each wave of a block has 16 MT rows of its own, and all of them
+// take the same tiles, which the block stages together in one of two LDS
+// buffers while it works on the other: one barrier a tile.
+template <typename T, int D, int MT, int NW, int KT>
+__global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void draft_rows_kernel(DraftArgs a) {
+  using S = DraftShape<T, D>;
+  constexpr int NG = KT / 16, CPR = S::CPR, RPI = S::RPI, R = 16 * MT * NW, ROWB = S::ROWB;
+  constexpr int WR = KT / NW;       // rows that a wave stages, in one page
+  constexpr int NI = WR / RPI;
+  static_assert(WR <= 16 && NI >= 1 && KT <= 64, "a wave stages rows of one page");
+  constexpr int STAGE = 2 * KT * ROWB;
+  static_assert(2 * STAGE >= NW * 16 * D * 4, "the output passes through the staging buffers");
+  __shared__ __attribute__((aligned(16))) char lds[2 * STAGE];
+  __shared__ uint64_t odds[2][NW];
+
+  DraftUnit u;
+  if (!draft_unit<KT, R>(a, blockIdx.x, false, &u)) return;  // uniform over the block
+  const int lane = threadIdx.x & 63, wv = uniform(threadIdx.x >> 6);
+  const DraftReq rq = draft_request(a, u.b);
+  const DraftCtx c = draft_ctx<KT, R>(a, u, rq);
+  const int64_t row0 = (int64_t)u.rt * R + wv * 16 * MT;
+  DraftWave<T, D, MT, KT> w;
+  w.init(a, c, u.h, row0);
+
+  const int lr = lane / CPR, lc = lane % CPR;
+  const bool kin = lc * 16 < a.Dk * S::ES, vin = lc * 16 < a.Dv * S::ES;
+  const int64_t koff = lr * a.k_token + (kin ? lc * 16 : 0);
+  const int64_t voff = lr * a.v_token + (vin ? lc * 16 : 0);
+  const int r0 = wv * WR;  // first of the rows this wave stages
+
+  uint4 kr[NI], vr[NI];
+  auto load = [&](int t, int e) {
+    const int64_t pg = e < 0 ? 0 : e;
+    const int at = (t * KT + r0) & ((1 << c.shift) - 1);
+    const char* kp = c.kh + pg * a.k_page + at * a.k_token;
+    const char* vp = c.vh + pg * a.v_page + at * a.v_token;
+#pragma unroll
+    for (int x = 0; x < NI; ++x) {
+      kr[x] = *(const uint4*)(kp + (koff + (int64_t)(x * RPI) * a.k_token));
+      vr[x] = *(const uint4*)(vp + (voff + (int64_t)(x * RPI) * a.v_token));
+    }
+  };
+  // pages of the tile, and of the rows of the next that this wave stages
+  int ent[NG], nxt[NG];
+  auto pages = [&](int t, int (&e)[NG]) {
+#pragma unroll
+    for (int i = 0; i < NG; ++i) e[i] = c.page(a, t * KT + 16 * i, t < c.t1);
+  };
+  auto mine = [&](int t) { return c.page(a, t * KT + r0 / 16 * 16, t < c.t1); };
+  int t = c.t0, own = mine(t);
+  char *kb = lds, *vb = lds + KT * ROWB;
+  auto stage = [&]() {
+    kb = lds + ((t - c.t0) & 1) * STAGE;
+    vb = kb + KT * ROWB;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int row = r0 + i * RPI + lr;
+      if (!kin) kr[i] = make_uint4(0, 0, 0, 0);
+      if (!vin) vr[i] = make_uint4(0, 0, 0, 0);
+      *(uint4*)(kb + row * ROWB + draft_swz<CPR>(row, lc) * 16) = kr[i];
+      *(uint4*)(vb + row * ROWB + draft_swz_v<CPR, S::F32>(row, lc) * 16) = vr[i];
+    }
+#pragma unroll
+    for (int i = 0; i < NG; ++i) ent[i] = nxt[i];
+    if (t + 1 < c.t1) load(t + 1, own);
+    own = mine(t + 2);
+    pages(t + 2, nxt);
+    __syncthreads();
+  };
+  auto masked = [&]() {
+    bool x = (t + 1) * KT > c.full;
+#pragma unroll
+    for (int i = 0; i < NG; ++i) x |= ent[i] < 0;
+    return x;
+  };
+  const bool on = row0 < c.nrow;  // the wave has rows
+  pages(t, ent);
+  pages(t + 1, nxt);
+  if (t < c.t1) load(t, own);
+  own = mine(t + 1);
+  while (t < c.t1) {
+    for (; t < c.t1 && !masked(); ++t) {
+      stage();
+      if (on) w.template tile<false>(a, c, kb, vb, t * KT, 0, 0);
+    }
+    for (; t < c.t1 && masked(); ++t) {
+      const int key0 = t * KT, buf = (t - c.t0) & 1;
+      uint64_t odd = 0, there = 0;
+#pragma unroll
+      for (int i = 0; i < NG; ++i) {
+        const int left = min(max(c.kend - key0 - 16 * i, 0), 16);
+        if (ent[i] >= 0) there |= (uint64_t)((1u << left) - 1u) << (16 * i);
+      }
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const int row = r0 + i * RPI + lr;
+        if (!((there >> row) & 1)) vr[i] = make_uint4(0, 0, 0, 0);
+        const uint64_t hit = __ballot(draft_odd<T>(vr[i]) && vin);
+        if (hit) {
+#pragma unroll
+          for (int x = 0; x < RPI; ++x) {
+            const uint64_t lanes = (CPR == 64 ? ~0ull : ((1ull << (CPR & 63)) - 1)) << ((x * CPR) & 63);
+            if (hit & lanes) odd |= 1ull << (r0 + i * RPI + x);
+          }
+          if ((odd >> row) & 1) vr[i] = make_uint4(0, 0, 0, 0);
+        }
+      }
+      if (lane == 0) odds[buf][wv] = odd;
+      stage();
+      odd = 0;
+#pragma unroll
+      for (int i = 0; i < NW; ++i) odd |= odds[buf][i];
+      if (on) w.template tile<true>(a, c, kb, vb, key0, there, odd);
+    }
+  }
+  __syncthreads();
+
+  const int64_t slot = u.nch > 1 ? u.slot + (u.ch * draft_row_groups(rq, a.G, R) + u.rt) * a.Hkv + u.h : -1;
+  float* my = (float*)lds + wv * 16 * D;
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    const float l = add_xor32(add_xor16(w.l[mt])), m = w.m[mt];
+    w.put(my, mt, 1.f);
+    wave_sync();
+#pragma unroll
+    for (int i = lane; i < 16 * S::OC; i += 64) {
+      const int row = i / S::OC, ch = i % S::OC;
+      const int64_t r = row0 + mt * 16 + row;
+      const float big = __shfl(m, row), sum = __shfl(l, row);
+      const f32x4 x = draft_got<T, D>(my, row, ch);
+      if (r >= c.nrow) continue;
+      if (slot >= 0) {
+        const int64_t at = slot * R + wv * 16 * MT + mt * 16 + row;
+        *(f32x4*)(a.ws_o + at * D + ch * 4) = x;
+        if (ch == 0) {
+          a.ws_ml[at * 2] = big;
+          a.ws_ml[at * 2 + 1] = sum;
+        }
+      } else {
+        draft_store<T>(a, c.s0, u.h, r, ch, x, sum);
+      }
+    }
+    wave_sync();
+  }
+}
+
 // Joins the chunks of split requests: one block per row, the threads split
 // over the chunks and the row's dims.
-template <typename T, int D, int MT>
+template <typename T, int D, int KT, int R>
 __global__ __launch_bounds__(256) void draft_join_kernel(DraftArgs a) {
-  using S = DraftShape<T, D, MT>;
-  constexpr int R = S::R, OC = D / 4, NP = 256 / OC;  // chunks taken at a time
+  constexpr int OC = D / 4, NP = 256 / OC;  // chunks taken at a time
   __shared__ f32x4 acc[256];
   __shared__ float lsum[NP];
   DraftUnit u;
-  if (!draft_unit<S::KT, R>(a, blockIdx.x / R, true, &u)) return;
+  if (!draft_unit<KT, R>(a, blockIdx.x / R, true, &u)) return;
   const int rr = blockIdx.x % R;
   const DraftReq rq = draft_request(a, u.b);
-  const int64_t nrow = (int64_t)rq.n * a.G, r = (int64_t)u.rt * R + rr;
-  if (r >= nrow) return;
-  const int64_t nrt = draft_row_groups(rq, a.G, R);
-  const int64_t base = u.slot + (int64_t)u.rt * a.Hkv + u.h, step = nrt * a.Hkv;
+  const int64_t r = (int64_t)u.rt * R + rr;
+  if (r >= (int64_t)rq.n * a.G) return;
+  const int64_t base = u.slot + (int64_t)u.rt * a.Hkv + u.h, step = draft_row_groups(rq, a.G, R) * a.Hkv;
   const int tid = threadIdx.x, p = tid / OC, ch = tid % OC;
   float big = -INFINITY;
   for (int c = tid & 63; c < u.nch; c += 64) big = fmaxf(big, a.ws_ml[((base + c * step) * R + rr) * 2]);
@@ -636,7 +850,6 @@ __global__ __launch_bounds__(256) void draft_join_kernel(DraftArgs a) {
     const float mc = a.ws_ml[at * 2], lc = a.ws_ml[at * 2 + 1];
     const f32x4 oc = *(const f32x4*)(a.ws_o + at * D + ch * 4);
     // a chunk whose tokens the row does not see has max -inf and zeros
-    // (NaN scores leave the max alone and make the sum NaN)
     const float f = mc == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mc - big);
     x += oc * f;
     sum += lc * f;
@@ -644,52 +857,53 @@ __global__ __launch_bounds__(256) void draft_join_kernel(DraftArgs a) {
   acc[tid] = x;
   if (ch == 0) lsum[p] = sum;
   __syncthreads();
-  if (p == 0 && ch * 4 < a.Dv) {
+  if (p == 0) {
 #pragma unroll
     for (int i = 1; i < NP; ++i) {
       x += acc[i * OC + ch];
       sum += lsum[i];
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const int j = (int)(r / a.G), hg = (int)(r - (int64_t)j * a.G);
-    char* o = a.out + (int64_t)(rq.s0 + j) * a.o_row + (int64_t)(u.h * a.G + hg) * a.o_head + ch * 4 * S::ES;
-    typedef __attribute__((ext_vector_type(4))) T T4;
-    *(T4*)o = __builtin_convertvector(x * inv, T4);
+    draft_store<T>(a, rq.s0, u.h, r, ch, x, sum);
   }
 }
 
-template <typename T, int D, int MT>
+template <typename T, int D, int MT, int NW>
 int draft_launch(const DraftArgs& a, int64_t units, int64_t groups, hipStream_t st) {
-  hipLaunchKernelGGL((draft_kernel<T, D, MT>), dim3((unsigned)units), dim3(256), 0, st, a);
+  constexpr int KT = draft_tile(D, (int)sizeof(T), NW), R = 16 * MT * NW;
+  if constexpr (NW == 1)
+    hipLaunchKernelGGL((draft_kernel<T, D, MT>), dim3((unsigned)units), dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL((draft_rows_kernel<T, D, MT, NW, KT>), dim3((unsigned)units), dim3(64 * NW), 0, st, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return (int)e;
   if (groups > 0) {
-    hipLaunchKernelGGL((draft_join_kernel<T, D, MT>), dim3((unsigned)(groups * 16 * MT)), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((draft_join_kernel<T, D, KT, R>), dim3((unsigned)(groups * R)), dim3(256), 0, st, a);
     e = hipGetLastError();
   }
   return e == hipSuccess ? HTREE_OK : (int)e;
 }
 
 template <typename T>
-int draft_launch_type(const DraftArgs& a, int D, int MT, int64_t units, int64_t groups, hipStream_t st);
+int draft_launch_type(const DraftArgs& a, const DraftPlan& p, hipStream_t st);
 
-#define HTREE_DRAFT_TYPE(T)                                                                          \
-  template <>                                                                                        \
-  int draft_launch_type<T>(const DraftArgs& a, int D, int MT, int64_t units, int64_t groups,         \
-                           hipStream_t st) {                                                         \
-    switch (D * 8 + MT) {                                                                            \
-      case 32 * 8 + 1: return draft_launch<T, 32, 1>(a, units, groups, st);                          \
-      case 32 * 8 + 2: return draft_launch<T, 32, 2>(a, units, groups, st);                          \
-      case 32 * 8 + 4: return draft_launch<T, 32, 4>(a, units, groups, st);                          \
-      case 64 * 8 + 1: return draft_launch<T, 64, 1>(a, units, groups, st);                          \
-      case 64 * 8 + 2: return draft_launch<T, 64, 2>(a, units, groups, st);                          \
-      case 64 * 8 + 4: return draft_launch<T, 64, 4>(a, units, groups, st);                          \
-      case 128 * 8 + 1: return draft_launch<T, 128, 1>(a, units, groups, st);                        \
-      case 128 * 8 + 2: return draft_launch<T, 128, 2>(a, units, groups, st);                        \
-      case 128 * 8 + 4: return draft_launch<T, 128, 4>(a, units, groups, st);                        \
-      case 256 * 8 + 1: return draft_launch<T, 256, 1>(a, units, groups, st);                        \
-      default: return draft_launch<T, 256, 2>(a, units, groups, st);                                 \
-    }                                                                                                \
+template <typename T, int D>
+int draft_launch_dim(const DraftArgs& a, const DraftPlan& p, hipStream_t st) {
+  constexpr DraftForm f = draft_rows_form(D, (int)sizeof(T));
+  if (p.NW > 1) return draft_launch<T, D, f.MT, f.NW>(a, p.units, p.groups, st);
+  if (p.MT == 1) return draft_launch<T, D, 1, 1>(a, p.units, p.groups, st);
+  if constexpr (D <= 128) {
+    if (p.MT == 4) return draft_launch<T, D, 4, 1>(a, p.units, p.groups, st);
+  }
+  return draft_launch<T, D, 2, 1>(a, p.units, p.groups, st);
+}
+
+#define HTREE_DRAFT_TYPE(T)                                                        \
+  template <>                                                                      \
+  int draft_launch_type<T>(const DraftArgs& a, const DraftPlan& p, hipStream_t st) { \
+    if (p.D == 32) return draft_launch_dim<T, 32>(a, p, st);                       \
+    if (p.D == 64) return draft_launch_dim<T, 64>(a, p, st);                       \
+    if (p.D == 128) return draft_launch_dim<T, 128>(a, p, st);                     \
+    return draft_launch_dim<T, 256>(a, p, st);                                     \
   }
 
 }  // namespace htree

@@ -47,10 +47,10 @@ int main() {
     if (damaged && calls % 4 == 1)
       for (int& s : starts) if (upto(2) == 0) s = (int)g(), ascend = false;
     if (rows == 0) continue;
-    const DraftPlan p = draft_plan(Dk, Dv, B, rows, G * Hkv, Hkv, width, 1 << shift);
-    CHECK(p.D >= Dk && p.D >= Dv && p.R == 16 * p.MT);
+    const DraftPlan p = draft_plan(Dk, Dv, es, B, rows, G * Hkv, Hkv, width, 1 << shift);
+    CHECK(p.D >= Dk && p.D >= Dv && p.R == 16 * p.MT * p.NW);
     CHECK(p.bytes == p.slots * p.R * (p.D + 2) * 4);
-    const int KT = draft_tile(p.D, es);
+    const int KT = draft_tile(p.D, es, p.NW);
     CHECK(KT >= 16 && KT <= 64 && KT % 16 == 0);
     int64_t tiles = 0;
     std::vector<DraftReq> rq;
