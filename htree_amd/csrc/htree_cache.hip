@@ -284,6 +284,8 @@ static int cache_check(const htree_cache* c) {
   const int64_t st[6] = {c->k_page, c->k_token, c->k_head, c->v_page, c->v_token, c->v_head};
   for (int64_t s : st)
     if (s < 0 || s * es % 16) return HTREE_EUNSUPPORTED;
+  // lanes hold 32-bit offsets into 16 tokens
+  if (c->k_token * es > (1 << 26) || c->v_token * es > (1 << 26)) return HTREE_EUNSUPPORTED;
   return HTREE_OK;
 }
 static bool off16(const void* p) { return ((uintptr_t)p & 15) != 0; }

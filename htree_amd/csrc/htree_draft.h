@@ -87,6 +87,19 @@ __device__ __forceinline__ int draft_swz_v(int row, int chunk) {
   return CPR >= 16 ? chunk ^ ((row & 7) << 1) : CPR == 8 ? chunk ^ (((row >> 1) & 3) << 1) : chunk ^ (((row >> 2) & 1) << 1);
 }
 
+// LDS by its 32-bit address, for addresses made by exclusive or
+__device__ __forceinline__ uint32_t draft_lds(const char* p) {
+  return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)p;
+}
+template <typename V>
+__device__ __forceinline__ V draft_read(uint32_t at) {
+  return *(const __attribute__((address_space(3))) V*)(uintptr_t)at;
+}
+__device__ __forceinline__ uint2 draft_read_tr(uint32_t at) {
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                       (__attribute__((address_space(3))) s16x4*)(uintptr_t)at));
+}
+
 __device__ __forceinline__ int64_t wave_sum64(int64_t x) {
 #pragma unroll
   for (int m = 1; m < 64; m <<= 1) x += __shfl_xor((long long)x, m);
@@ -215,11 +228,31 @@ struct DraftCtx {
   const char *kh, *vh;     // the KV head's keys and values
   const int32_t* tab;      // the request's table
   const int32_t* par;      // its new tokens' parents, or null
-  // page of the 16 tokens from `key`, -1: none (past the end, no page of the
-  // cache)
-  __device__ __forceinline__ int page(const DraftArgs& a, int key, bool on) const {
+};
+// The pages of a request's tokens, asked for in ascending order: 64 entries
+// of the table in a register of the wave's lanes and the next 64 on their way.
+// (Read one by one through the scalar cache they held up the LDS reads, which
+// count on the same counter.)
+struct DraftPages {
+  const int32_t* tab;
+  int used, num_pages, shift, at, cur, nxt;
+  __device__ __forceinline__ int read(int b) const {
+    const int i = b * 64 + (int)__lane_id();
+    return cache_page(i < used ? tab[i] : -1, num_pages);
+  }
+  __device__ __forceinline__ DraftPages(const DraftArgs& a, const DraftCtx& c, int key)
+      : tab(c.tab), used(c.used), num_pages(a.num_pages), shift(c.shift), at((key >> c.shift) >> 6) {
+    cur = read(at);
+    nxt = read(at + 1);
+  }
+  // page of the 16 tokens from `key`, -1: none (past the end, no page of the cache)
+  __device__ __forceinline__ int page(int key) {
     const int pi = key >> shift;
-    return cache_page(on && pi < used ? tab[pi] : -1, a.num_pages);
+    if (pi >> 6 != at) {
+      cur = nxt;
+      nxt = read((at = pi >> 6) + 1);
+    }
+    return __builtin_amdgcn_readlane(cur, pi & 63);
   }
 };
 template <int KT, int R>
@@ -238,6 +271,14 @@ __device__ __forceinline__ DraftCtx draft_ctx(const DraftArgs& a, const DraftUni
   c.tab = a.table + u.b * a.table_stride;
   c.par = a.parents ? a.parents + c.s0 : nullptr;
   return c;
+}
+
+// The lane, not known to be the same each time: the LDS addresses worked out
+// from it are not kept in registers across the loop, which has none to spare.
+__device__ __forceinline__ int draft_lane_again() {
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));
+  return lane;
 }
 
 // A wave's rows and their running softmax: 16 MT rows, in the products'
@@ -300,45 +341,61 @@ struct DraftWave {
     return j >= 0 && c.ctx + j == key;
   }
 
-  // One tile of KT tokens from key0, staged at kb / vb.  MASKED: not every
-  // row sees every token; there: the tokens (bits) that exist; odd: those
-  // with an infinite or NaN value, whose staged values are zero.
-  template <bool MASKED>
-  __device__ __forceinline__ void tile(const DraftArgs& a, const DraftCtx& c, const char* kb, const char* vb,
-                                       int key0, uint64_t there, uint64_t odd) {
+  // The weights of a tile's tokens, as the second operand of the product with
+  // their values: of the values' type, fp32 for fp32.
+  struct Weights {
+    typename std::conditional<F32, f32x4, uint2>::type p[MT][NG];
+  };
+
+  // One tile of KT tokens from key0, its keys staged at kb.  masked: not every
+  // row sees every token; there: the tokens (bits) that exist.
+  __device__ __forceinline__ void scores(const DraftArgs& a, const DraftCtx& c, const char* kb, int key0,
+                                         bool masked, uint64_t there, Weights& wt) {
+    const int lane = draft_lane_again(), n16 = lane & 15, g = lane >> 4;
     // ---- scores, token x row: a lane holds tokens 4 g .. 4 g + 3 of each
-    // group of 16, of row n16
+    // group of 16, of row n16.  The operands come from LDS four products
+    // ahead (left to itself the compiler reads each where it is used, and the
+    // wave waits for every one).
     f32x4 sc[MT][NG];
 #pragma unroll
-    for (int i = 0; i < NG; ++i) {
+    for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) sc[mt][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-      const int row = 16 * i + n16;
-      const char* p = kb + row * ROWB;
-      if constexpr (F32) {
+      for (int i = 0; i < NG; ++i) sc[mt][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    {
+      constexpr int NS = NG * (F32 ? D / 16 : D / 32), AHEAD = NS < 4 ? NS : 4;
+      // (rows of 16 groups and buffers begin at multiples of 16 rows: the
+      // swizzle and the piece are bits of the address of their own)
+      const uint32_t k0 = draft_lds(kb) + n16 * ROWB + draft_swz<CPR>(n16, g) * 16;
+      auto key = [&](int x) {  // step x: 16-byte pieces of group x % NG
+        return draft_read<f32x4>((k0 ^ (x / NG * 64)) + x % NG * 16 * ROWB);
+      };
+      f32x4 f[AHEAD];
 #pragma unroll
-        for (int s = 0; s < D / 16; ++s) {
-          const f32x4 x = *(const f32x4*)(p + draft_swz<CPR>(row, 4 * s + g) * 16);
+      for (int x = 0; x < AHEAD; ++x) f[x] = key(x);
+#pragma unroll
+      for (int x = 0; x < NS; ++x) {
+        const int i = x % NG, s = x / NG;
+        if constexpr (F32) {
+          const f32x4 k4 = f[x % AHEAD];
 #pragma unroll
           for (int e = 0; e < 4; ++e)
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
-              sc[mt][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], qf[mt][s][e], sc[mt][i], 0, 0, 0);
-        }
-      } else {
-        using V8 = typename DraftT<T>::V8;
-#pragma unroll
-        for (int s = 0; s < D / 32; ++s) {
-          const V8 x = *(const V8*)(p + draft_swz<CPR>(row, 4 * s + g) * 16);
+              sc[mt][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(k4[e], qf[mt][s][e], sc[mt][i], 0, 0, 0);
+        } else {
+          using V8 = typename DraftT<T>::V8;
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt)
-            sc[mt][i] = DraftT<T>::mma(x, __builtin_bit_cast(V8, qh[mt][s]), sc[mt][i]);
+            sc[mt][i] = DraftT<T>::mma(__builtin_bit_cast(V8, f[x % AHEAD]), __builtin_bit_cast(V8, qh[mt][s]), sc[mt][i]);
         }
+        if (x + AHEAD < NS) f[x % AHEAD] = key(x + AHEAD);
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
 
     // ---- masks
-    if constexpr (MASKED) {
+    if (masked) {
+      const int g2 = draft_lane_again() >> 4;
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
         uint64_t see = 0;
@@ -360,7 +417,7 @@ struct DraftWave {
         for (int i = 0; i < NG; ++i)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (!((see >> (16 * i + 4 * g + e)) & 1)) sc[mt][i][e] = -INFINITY;
+            if (!((see >> (16 * i + 4 * g2 + e)) & 1)) sc[mt][i][e] = -INFINITY;
       }
     }
 
@@ -393,36 +450,27 @@ struct DraftWave {
         }
     }
 
-    // ---- tokens with infinite or NaN values: only the rows that see them
-    // take them
-    if (MASKED && odd) {
-      for (uint64_t left = odd; left; left &= left - 1) {
-        const int key = __builtin_ctzll(left), at = key0 + key;
-        const int64_t pg = c.tab[at >> c.shift];  // a page of the cache: its values were read
-        const T* vp = (const T*)(c.vh + pg * a.v_page + (at & ((1 << c.shift) - 1)) * a.v_token);
+    // P rounded to the values' type: a relative half step for each of many
+    // tokens, as large as the output's own rounding at most; the sum l is
+    // taken of the unrounded P
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          float p = 0.f;
+    for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-          for (int i = 0; i < NG; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (key >> 4 == i && (key & 3) == e) p = sc[mt][i][e];
-          p = __shfl(p, ((key >> 2) & 3) * 16 + n16);
-          const bool see = sees(c, mt, at);
-#pragma unroll
-          for (int q = 0; q < NQ; ++q)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int d = Quad::dim(q, g) + e;
-              if (see && d < a.Dv) Quad::add(o[mt], q, e, p * Io<T>::ld(vp + d));
-            }
+      for (int i = 0; i < NG; ++i) {
+        if constexpr (F32) {
+          wt.p[mt][i] = sc[mt][i];
+        } else {
+          typedef __attribute__((ext_vector_type(4))) T T4;
+          wt.p[mt][i] = __builtin_bit_cast(uint2, __builtin_convertvector(sc[mt][i], T4));
         }
       }
-    }
+  }
 
-    // ---- output, dim x row: the tokens of a product's k index are those a
-    // lane holds, so the scores' registers are its second operand as they are
+  // Adds the tile's values, staged at vb.  Output, dim x row: the tokens of a
+  // product's k index are those a lane holds, so the weights' registers are
+  // its second operand as they are.
+  __device__ __forceinline__ void values(const char* vb, const Weights& wt) {
+    const int lane = draft_lane_again(), n16 = lane & 15, g = lane >> 4;
     if constexpr (F32) {
 #pragma unroll
       for (int i = 0; i < NG; ++i)
@@ -432,64 +480,91 @@ struct DraftWave {
 #pragma unroll
           for (int q = 0; q < NQ; q += S::VW) {
             if constexpr (S::VW == 4) {
-              const f32x4 x = *(const f32x4*)(vb + row * ROWB + draft_swz_v<CPR, F32>(row, 4 * q + n16) * 16);
+              const f32x4 x = draft_read<f32x4>(draft_lds(vb) + row * ROWB + draft_swz_v<CPR, F32>(row, 4 * q + n16) * 16);
 #pragma unroll
               for (int w = 0; w < 4; ++w)
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
-                  o[mt][q + w] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[w], sc[mt][i][e], o[mt][q + w], 0, 0, 0);
+                  o[mt][q + w] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[w], wt.p[mt][i][e], o[mt][q + w], 0, 0, 0);
             } else {
-              const f32x2 x = *(const f32x2*)(vb + row * ROWB + draft_swz_v<CPR, F32>(row, n16 >> 1) * 16 + (n16 & 1) * 8);
+              const f32x2 x = draft_read<f32x2>(draft_lds(vb) + row * ROWB + draft_swz_v<CPR, F32>(row, n16 >> 1) * 16 + (n16 & 1) * 8);
 #pragma unroll
               for (int w = 0; w < 2; ++w)
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
-                  o[mt][q + w] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[w], sc[mt][i][e], o[mt][q + w], 0, 0, 0);
+                  o[mt][q + w] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[w], wt.p[mt][i][e], o[mt][q + w], 0, 0, 0);
             }
           }
         }
     } else {
-      // P rounded to the values' type: a relative half step for each of many
-      // tokens, as large as the output's own rounding at most; the sum l is
-      // taken of the unrounded P
-      uint2 ph[MT][NG];
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int i = 0; i < NG; ++i) {
-          typedef __attribute__((ext_vector_type(4))) T T4;
-          ph[mt][i] = __builtin_bit_cast(uint2, __builtin_convertvector(sc[mt][i], T4));
-        }
       // a transposing read gives lane n16 of group g four tokens of dim n16:
       // it addresses token 4 g + n16 / 4, dims 4 (n16 % 4) ..
-      auto col = [&](int i, int q) {
-        const int row = 16 * i + 4 * g + (n16 >> 2);
-        const char* p = vb + row * ROWB + draft_swz_v<CPR, F32>(row, 2 * q + ((n16 & 3) >> 1)) * 16 + (n16 & 1) * 8;
-        return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (__attribute__((address_space(3))) s16x4*)(const __attribute__((address_space(3))) void*)p);
+      const int row = 4 * g + (n16 >> 2);
+      const uint32_t v0 = draft_lds(vb) + row * ROWB + draft_swz_v<CPR, F32>(row, (n16 & 3) >> 1) * 16 + (n16 & 1) * 8;
+      auto col = [&](int i, int q) { return draft_read_tr((v0 ^ (q * 32)) + i * 16 * ROWB); };
+      constexpr int PG = NG == 1 ? 1 : 2, NS = NG / PG * NQ, AHEAD = NS < 4 ? NS : 4;  // groups of a product
+      uint2 f[AHEAD][PG];
+      auto value = [&](int x) {  // step x: dims x % NQ, groups from x / NQ
+#pragma unroll
+        for (int y = 0; y < PG; ++y) f[x % AHEAD][y] = col(x / NQ * PG + y, x % NQ);
       };
 #pragma unroll
-      for (int q = 0; q < NQ; ++q) {
-        if constexpr (NG == 1) {
-          const s16x4 x = col(0, q);
+      for (int x = 0; x < AHEAD; ++x) value(x);
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
-            o[mt][q] = DraftT<T>::mma_k16(x, __builtin_bit_cast(s16x4, ph[mt][0]), o[mt][q]);
-        } else {
-          using V8 = typename DraftT<T>::V8;
+      for (int x = 0; x < NS; ++x) {
+        const int q = x % NQ, i = x / NQ * PG;
 #pragma unroll
-          for (int i = 0; i < NG; i += 2) {
-            const uint2 x0 = __builtin_bit_cast(uint2, col(i, q)), x1 = __builtin_bit_cast(uint2, col(i + 1, q));
-            const V8 x = __builtin_bit_cast(V8, make_uint4(x0.x, x0.y, x1.x, x1.y));
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-              o[mt][q] = DraftT<T>::mma(
-                  x, __builtin_bit_cast(V8, make_uint4(ph[mt][i].x, ph[mt][i].y, ph[mt][i + 1].x, ph[mt][i + 1].y)),
-                  o[mt][q]);
+        for (int mt = 0; mt < MT; ++mt) {
+          if constexpr (PG == 1) {
+            o[mt][q] = DraftT<T>::mma_k16(__builtin_bit_cast(s16x4, f[x % AHEAD][0]),
+                                          __builtin_bit_cast(s16x4, wt.p[mt][i]), o[mt][q]);
+          } else {
+            using V8 = typename DraftT<T>::V8;
+            const uint2 y0 = f[x % AHEAD][0], y1 = f[x % AHEAD][PG - 1];
+            o[mt][q] = DraftT<T>::mma(
+                __builtin_bit_cast(V8, make_uint4(y0.x, y0.y, y1.x, y1.y)),
+                __builtin_bit_cast(V8, make_uint4(wt.p[mt][i].x, wt.p[mt][i].y, wt.p[mt][i + PG - 1].x, wt.p[mt][i + PG - 1].y)),
+                o[mt][q]);
           }
         }
+        if (x + AHEAD < NS) value(x + AHEAD);
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
+  }
+
+  // Adds what the rows that see token `key` take of it, where its values are
+  // infinite or NaN and were staged as zeros (l has its weight already).
+  __device__ __forceinline__ void odd_token(const DraftArgs& a, const DraftCtx& c, int key, int page) {
+    const int at = key & ((1 << c.shift) - 1);
+    const T* kp = (const T*)(c.kh + page * a.k_page + at * a.k_token);
+    const T* vp = (const T*)(c.vh + page * a.v_page + at * a.v_token);
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      if (!__any(sees(c, mt, key))) continue;
+      float x = 0.f;  // the row's score, a quarter of it in each lane
+#pragma unroll
+      for (int s = 0; s < (F32 ? D / 16 : D / 32); ++s)
+#pragma unroll
+        for (int e = 0; e < (F32 ? 4 : 8); ++e) {
+          const int d = F32 ? 16 * s + 4 * g + e : 32 * s + 8 * g + e;
+          if (d < a.Dk) x += q_at(mt, s, e) * Io<T>::ld(kp + d);
+        }
+      x = add_xor32(add_xor16(x)) * a.c;
+      const bool see = sees(c, mt, key);
+      const float p = __builtin_amdgcn_exp2f(x - (m[mt] == -INFINITY ? 0.f : m[mt]));
+#pragma unroll
+      for (int q = 0; q < NQ; ++q)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int d = Quad::dim(q, g) + e;
+          if (see && d < a.Dv) Quad::add(o[mt], q, e, p * Io<T>::ld(vp + d));
+        }
+    }
+  }
+  __device__ __forceinline__ float q_at(int mt, int s, int e) const {
+    if constexpr (F32) return qf[mt][s][e];
+    else return (float)__builtin_bit_cast(typename DraftT<T>::V8, qh[mt][s])[e];
   }
 
   // the lane's part of row n16 of group mt, times f, into 16 fp32 rows at dst
@@ -506,6 +581,14 @@ struct DraftWave {
 template <typename T, int D>
 __device__ __forceinline__ f32x4 draft_got(const float* src, int row, int ch) {
   return *(const f32x4*)(src + row * D + ((ch ^ (row & DraftShape<T, D>::OS)) << 2));
+}
+
+// Whether a token's values (row vp of Dv) hold an infinite or NaN one.
+template <typename T>
+__device__ __forceinline__ bool draft_odd_row(const DraftArgs& a, const char* vp) {
+  const int lane = threadIdx.x & 63;
+  const bool in = lane * 16 < a.Dv * (int)sizeof(T);
+  return __any(in && draft_odd<T>(*(const uint4*)(vp + (in ? lane * 16 : 0))));
 }
 
 // stores chunk ch of the request's row r (x: weighted sum, sum: the weights')
@@ -528,7 +611,7 @@ __global__ __launch_bounds__(256, (MT == 1 && D <= 128) ? 2 : 1) void draft_kern
   constexpr int KT = draft_tile(D, S::ES), NG = KT / 16, CPR = S::CPR, RPI = S::RPI, R = 16 * MT;
   constexpr int NI = KT / RPI, ROWB = S::ROWB, NW = kWavesPerBlock;
   constexpr int WAVE_LDS = 2 * KT * ROWB;
-  __shared__ __attribute__((aligned(16))) char lds[NW * WAVE_LDS];
+  __shared__ __attribute__((aligned(1024))) char lds[NW * WAVE_LDS];
   __shared__ float ml[NW][R][2];
 
   DraftUnit u;
@@ -545,26 +628,31 @@ __global__ __launch_bounds__(256, (MT == 1 && D <= 128) ? 2 : 1) void draft_kern
   const int lr = lane / CPR, lc = lane % CPR;
   // lanes past the head dim read the row's first chunk and write zeros
   const bool kin = lc * 16 < a.Dk * S::ES, vin = lc * 16 < a.Dv * S::ES;
-  const int64_t koff = lr * a.k_token + (kin ? lc * 16 : 0);
-  const int64_t voff = lr * a.v_token + (vin ? lc * 16 : 0);
+  const bool whole = a.Dk == D && a.Dv == D;
+  const uint32_t koff = lr * (uint32_t)a.k_token + (kin ? lc * 16 : 0);
+  const uint32_t voff = lr * (uint32_t)a.v_token + (vin ? lc * 16 : 0);
 
-  auto pages = [&](int t, int (&e)[NG]) {
+  DraftPages pg(a, c, (c.t0 + wv) * KT);
+  auto pages_of = [&](DraftPages& p, int t, int (&e)[NG]) {
 #pragma unroll
-    for (int i = 0; i < NG; ++i) e[i] = c.page(a, t * KT + 16 * i, t < c.t1);
+    for (int i = 0; i < NG; ++i) e[i] = p.page(t * KT + 16 * i);
   };
+  auto pages = [&](int t, int (&e)[NG]) { pages_of(pg, t, e); };
   uint4 kr[NI], vr[NI];
-  auto load = [&](int t, const int (&e)[NG]) {
+  auto load_k = [&](int t, const int (&e)[NG]) {
 #pragma unroll
     for (int i = 0; i < NG; ++i) {
-      const int64_t pg = e[i] < 0 ? 0 : e[i];
-      const int at = (t * KT + 16 * i) & ((1 << c.shift) - 1);
-      const char* kp = c.kh + pg * a.k_page + at * a.k_token;
-      const char* vp = c.vh + pg * a.v_page + at * a.v_token;
+      const char* p = c.kh + (int64_t)max(e[i], 0) * a.k_page + ((t * KT + 16 * i) & ((1 << c.shift) - 1)) * a.k_token;
 #pragma unroll
-      for (int x = 0; x < NI / NG; ++x) {
-        kr[i * (NI / NG) + x] = *(const uint4*)(kp + (koff + (int64_t)(x * RPI) * a.k_token));
-        vr[i * (NI / NG) + x] = *(const uint4*)(vp + (voff + (int64_t)(x * RPI) * a.v_token));
-      }
+      for (int x = 0; x < NI / NG; ++x) kr[i * (NI / NG) + x] = *(const uint4*)(p + x * RPI * a.k_token + koff);
+    }
+  };
+  auto load_v = [&](int t, const int (&e)[NG]) {
+#pragma unroll
+    for (int i = 0; i < NG; ++i) {
+      const char* p = c.vh + (int64_t)max(e[i], 0) * a.v_page + ((t * KT + 16 * i) & ((1 << c.shift) - 1)) * a.v_token;
+#pragma unroll
+      for (int x = 0; x < NI / NG; ++x) vr[i * (NI / NG) + x] = *(const uint4*)(p + x * RPI * a.v_token + voff);
     }
   };
 
@@ -572,17 +660,25 @@ __global__ __launch_bounds__(256, (MT == 1 && D <= 128) ? 2 : 1) void draft_kern
   int ent[NG], nxt[NG];
   int t = c.t0 + wv;
   auto stage = [&]() {
+    if (!whole) {
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        if (!kin) kr[i] = make_uint4(0, 0, 0, 0);
+        if (!vin) vr[i] = make_uint4(0, 0, 0, 0);
+      }
+    }
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       const int row = i * RPI + lr;
-      if (!kin) kr[i] = make_uint4(0, 0, 0, 0);
-      if (!vin) vr[i] = make_uint4(0, 0, 0, 0);
       *(uint4*)(kb + row * ROWB + draft_swz<CPR>(row, lc) * 16) = kr[i];
       *(uint4*)(vb + row * ROWB + draft_swz_v<CPR, S::F32>(row, lc) * 16) = vr[i];
     }
 #pragma unroll
     for (int i = 0; i < NG; ++i) ent[i] = nxt[i];
-    if (t + NW < c.t1) load(t + NW, ent);
+    if (t + NW < c.t1) {
+      load_k(t + NW, ent);
+      load_v(t + NW, ent);
+    }
     pages(t + 2 * NW, nxt);
     wave_sync();
   };
@@ -593,41 +689,56 @@ __global__ __launch_bounds__(256, (MT == 1 && D <= 128) ? 2 : 1) void draft_kern
     for (int i = 0; i < NG; ++i) x |= ent[i] < 0;
     return x;
   };
+  // tokens (bits) of tile t that exist
+  auto exist = [&]() {
+    uint64_t x = 0;
+#pragma unroll
+    for (int i = 0; i < NG; ++i) {
+      const int left = min(max(c.kend - t * KT - 16 * i, 0), 16);
+      if (ent[i] >= 0) x |= (uint64_t)((1u << left) - 1u) << (16 * i);
+    }
+    return x;
+  };
   pages(t, ent);
   pages(t + NW, nxt);
-  if (t < c.t1) load(t, ent);
-  while (t < c.t1) {
-    for (; t < c.t1 && !masked(); t += NW) {
-      stage();
-      w.template tile<false>(a, c, kb, vb, t * KT, 0, 0);
-      wave_sync();  // this tile's reads come before the next one's writes
-    }
-    for (; t < c.t1 && masked(); t += NW) {
-      const int key0 = t * KT;
-      uint64_t odd = 0, there = 0;
-#pragma unroll
-      for (int i = 0; i < NG; ++i) {
-        const int left = min(max(c.kend - key0 - 16 * i, 0), 16);
-        if (ent[i] >= 0) there |= (uint64_t)((1u << left) - 1u) << (16 * i);
-      }
-      // Values that no row sees must not meet the product: 0 x NaN is NaN.
+  if (t < c.t1) {
+    load_k(t, ent);
+    load_v(t, ent);
+  }
+  bool odd = false;  // a token with infinite or NaN values was met
+  for (; t < c.t1; t += NW) {
+    const bool part = masked();
+    uint64_t there = 0;
+    if (part) {
+      there = exist();
+      // Values that a row does not see must not meet the product: 0 x NaN is
+      // NaN.  Zeros take the place of those that no row sees, and of
+      // infinite or NaN ones, which join at the end.
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
         const int row = i * RPI + lr;
         if (!((there >> row) & 1)) vr[i] = make_uint4(0, 0, 0, 0);
         const uint64_t hit = __ballot(draft_odd<T>(vr[i]) && vin);
-        if (hit) {
-#pragma unroll
-          for (int x = 0; x < RPI; ++x) {
-            const uint64_t lanes = (CPR == 64 ? ~0ull : ((1ull << (CPR & 63)) - 1)) << ((x * CPR) & 63);
-            if (hit & lanes) odd |= 1ull << (i * RPI + x);
-          }
-          if ((odd >> row) & 1) vr[i] = make_uint4(0, 0, 0, 0);
-        }
+        odd |= hit != 0;
+        if ((hit >> (lr * CPR)) & (CPR == 64 ? ~0ull : (1ull << (CPR & 63)) - 1)) vr[i] = make_uint4(0, 0, 0, 0);
       }
-      stage();
-      w.template tile<true>(a, c, kb, vb, key0, there, odd);
-      wave_sync();
+    }
+    stage();
+    typename DraftWave<T, D, MT, KT>::Weights wt;
+    w.scores(a, c, kb, t * KT, part, there, wt);
+    w.values(vb, wt);
+    wave_sync();  // this tile's reads come before the next one's writes
+  }
+  if (odd) {
+    DraftPages again(a, c, (c.t0 + wv) * KT);
+    for (t = c.t0 + wv; t < c.t1; t += NW) {
+      pages_of(again, t, ent);
+      if (!masked()) continue;
+      for (uint64_t left = exist(); left; left &= left - 1) {
+        const int key = t * KT + __builtin_ctzll(left), p = again.page(key);
+        if (draft_odd_row<T>(a, c.vh + p * a.v_page + (key & ((1 << c.shift) - 1)) * a.v_token))
+          w.odd_token(a, c, key, p);
+      }
     }
   }
 
@@ -689,9 +800,9 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void draft_rows_kernel(D
   constexpr int NI = WR / RPI;
   static_assert(WR <= 16 && NI >= 1 && KT <= 64, "a wave stages rows of one page");
   constexpr int STAGE = 2 * KT * ROWB;
-  static_assert(2 * STAGE >= NW * 16 * D * 4, "the output passes through the staging buffers");
-  __shared__ __attribute__((aligned(16))) char lds[2 * STAGE];
-  __shared__ uint64_t odds[2][NW];
+  constexpr int PUT = NW * 16 * D * 4;  // the output passes through, 16 rows of each wave
+  __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE > PUT ? 2 * STAGE : PUT];
+  __shared__ int odds[NW];
 
   DraftUnit u;
   if (!draft_unit<KT, R>(a, blockIdx.x, false, &u)) return;  // uniform over the block
@@ -704,46 +815,52 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void draft_rows_kernel(D
 
   const int lr = lane / CPR, lc = lane % CPR;
   const bool kin = lc * 16 < a.Dk * S::ES, vin = lc * 16 < a.Dv * S::ES;
-  const int64_t koff = lr * a.k_token + (kin ? lc * 16 : 0);
-  const int64_t voff = lr * a.v_token + (vin ? lc * 16 : 0);
+  const bool whole = a.Dk == D && a.Dv == D;
+  const uint32_t koff = lr * (uint32_t)a.k_token + (kin ? lc * 16 : 0);
+  const uint32_t voff = lr * (uint32_t)a.v_token + (vin ? lc * 16 : 0);
   const int r0 = wv * WR;  // first of the rows this wave stages
 
   uint4 kr[NI], vr[NI];
-  auto load = [&](int t, int e) {
-    const int64_t pg = e < 0 ? 0 : e;
-    const int at = (t * KT + r0) & ((1 << c.shift) - 1);
-    const char* kp = c.kh + pg * a.k_page + at * a.k_token;
-    const char* vp = c.vh + pg * a.v_page + at * a.v_token;
+  auto load_k = [&](int t, int e) {
+    const char* p = c.kh + (int64_t)max(e, 0) * a.k_page + ((t * KT + r0) & ((1 << c.shift) - 1)) * a.k_token;
 #pragma unroll
-    for (int x = 0; x < NI; ++x) {
-      kr[x] = *(const uint4*)(kp + (koff + (int64_t)(x * RPI) * a.k_token));
-      vr[x] = *(const uint4*)(vp + (voff + (int64_t)(x * RPI) * a.v_token));
-    }
+    for (int x = 0; x < NI; ++x) kr[x] = *(const uint4*)(p + x * RPI * a.k_token + koff);
   };
-  // pages of the tile, and of the rows of the next that this wave stages
-  int ent[NG], nxt[NG];
-  auto pages = [&](int t, int (&e)[NG]) {
+  auto load_v = [&](int t, int e) {
+    const char* p = c.vh + (int64_t)max(e, 0) * a.v_page + ((t * KT + r0) & ((1 << c.shift) - 1)) * a.v_token;
 #pragma unroll
-    for (int i = 0; i < NG; ++i) e[i] = c.page(a, t * KT + 16 * i, t < c.t1);
+    for (int x = 0; x < NI; ++x) vr[x] = *(const uint4*)(p + x * RPI * a.v_token + voff);
   };
-  auto mine = [&](int t) { return c.page(a, t * KT + r0 / 16 * 16, t < c.t1); };
-  int t = c.t0, own = mine(t);
+  int ent[NG], nxt[NG], t = c.t0, own;
+  DraftPages pg(a, c, t * KT);
+  auto pages_of = [&](DraftPages& p, int t, int (&e)[NG]) {
+#pragma unroll
+    for (int i = 0; i < NG; ++i) e[i] = p.page(t * KT + 16 * i);
+  };
+  auto pages = [&](int t, int (&e)[NG]) { pages_of(pg, t, e); };
+  // the page of the rows that this wave stages (a tile's pages are in one
+  // batch of entries)
+  auto mine = [&](int t) { return pg.page(t * KT + r0 / 16 * 16); };
   char *kb = lds, *vb = lds + KT * ROWB;
   auto stage = [&]() {
     kb = lds + ((t - c.t0) & 1) * STAGE;
     vb = kb + KT * ROWB;
+    if (!whole) {
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        if (!kin) kr[i] = make_uint4(0, 0, 0, 0);
+        if (!vin) vr[i] = make_uint4(0, 0, 0, 0);
+      }
+    }
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       const int row = r0 + i * RPI + lr;
-      if (!kin) kr[i] = make_uint4(0, 0, 0, 0);
-      if (!vin) vr[i] = make_uint4(0, 0, 0, 0);
       *(uint4*)(kb + row * ROWB + draft_swz<CPR>(row, lc) * 16) = kr[i];
       *(uint4*)(vb + row * ROWB + draft_swz_v<CPR, S::F32>(row, lc) * 16) = vr[i];
     }
 #pragma unroll
     for (int i = 0; i < NG; ++i) ent[i] = nxt[i];
-    if (t + 1 < c.t1) load(t + 1, own);
-    own = mine(t + 2);
+    if (t + 1 < c.t1) load_k(t + 1, own);
     pages(t + 2, nxt);
     __syncthreads();
   };
@@ -753,44 +870,60 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void draft_rows_kernel(D
     for (int i = 0; i < NG; ++i) x |= ent[i] < 0;
     return x;
   };
+  auto exist = [&]() {
+    uint64_t x = 0;
+#pragma unroll
+    for (int i = 0; i < NG; ++i) {
+      const int left = min(max(c.kend - t * KT - 16 * i, 0), 16);
+      if (ent[i] >= 0) x |= (uint64_t)((1u << left) - 1u) << (16 * i);
+    }
+    return x;
+  };
   const bool on = row0 < c.nrow;  // the wave has rows
   pages(t, ent);
+  if (t < c.t1) {
+    load_k(t, mine(t));
+    load_v(t, mine(t));
+  }
   pages(t + 1, nxt);
-  if (t < c.t1) load(t, own);
   own = mine(t + 1);
-  while (t < c.t1) {
-    for (; t < c.t1 && !masked(); ++t) {
-      stage();
-      if (on) w.template tile<false>(a, c, kb, vb, t * KT, 0, 0);
-    }
-    for (; t < c.t1 && masked(); ++t) {
-      const int key0 = t * KT, buf = (t - c.t0) & 1;
-      uint64_t odd = 0, there = 0;
-#pragma unroll
-      for (int i = 0; i < NG; ++i) {
-        const int left = min(max(c.kend - key0 - 16 * i, 0), 16);
-        if (ent[i] >= 0) there |= (uint64_t)((1u << left) - 1u) << (16 * i);
-      }
+  bool odd = false;  // this wave staged a token with infinite or NaN values
+  for (; t < c.t1; ++t) {
+    const bool part = masked();
+    uint64_t there = 0;
+    if (part) {
+      there = exist();
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
         const int row = r0 + i * RPI + lr;
         if (!((there >> row) & 1)) vr[i] = make_uint4(0, 0, 0, 0);
         const uint64_t hit = __ballot(draft_odd<T>(vr[i]) && vin);
-        if (hit) {
-#pragma unroll
-          for (int x = 0; x < RPI; ++x) {
-            const uint64_t lanes = (CPR == 64 ? ~0ull : ((1ull << (CPR & 63)) - 1)) << ((x * CPR) & 63);
-            if (hit & lanes) odd |= 1ull << (r0 + i * RPI + x);
-          }
-          if ((odd >> row) & 1) vr[i] = make_uint4(0, 0, 0, 0);
-        }
+        odd |= hit != 0;
+        if ((hit >> (lr * CPR)) & (CPR == 64 ? ~0ull : (1ull << (CPR & 63)) - 1)) vr[i] = make_uint4(0, 0, 0, 0);
       }
-      if (lane == 0) odds[buf][wv] = odd;
-      stage();
-      odd = 0;
+    }
+    stage();
+    typename DraftWave<T, D, MT, KT>::Weights wt;
+    if (on) w.scores(a, c, kb, t * KT, part, there, wt);
+    // only now, when the scores' registers are free
+    if (t + 1 < c.t1) load_v(t + 1, own);
+    own = mine(t + 2);
+    if (on) w.values(vb, wt);
+  }
+  if (lane == 0) odds[wv] = odd;
+  __syncthreads();
 #pragma unroll
-      for (int i = 0; i < NW; ++i) odd |= odds[buf][i];
-      if (on) w.template tile<true>(a, c, kb, vb, key0, there, odd);
+  for (int i = 0; i < NW; ++i) odd |= odds[i] != 0;
+  if (odd && on) {
+    DraftPages again(a, c, c.t0 * KT);
+    for (t = c.t0; t < c.t1; ++t) {
+      pages_of(again, t, ent);
+      if (!masked()) continue;
+      for (uint64_t left = exist(); left; left &= left - 1) {
+        const int key = t * KT + __builtin_ctzll(left), p = again.page(key);
+        if (draft_odd_row<T>(a, c.vh + p * a.v_page + (key & ((1 << c.shift) - 1)) * a.v_token))
+          w.odd_token(a, c, key, p);
+      }
     }
   }
   __syncthreads();

@@ -30,7 +30,7 @@ BAD_CACHES = [
     (dict(page_size=8192), N.HTREE_EUNSUPPORTED),
     (dict(Dk=264), N.HTREE_EUNSUPPORTED), (dict(Dv=264), N.HTREE_EUNSUPPORTED),
     (dict(Dk=60), N.HTREE_EUNSUPPORTED), (dict(dtype=0, Dv=42), N.HTREE_EUNSUPPORTED),
-    (dict(k_token=250), N.HTREE_EUNSUPPORTED), (dict(v_page=-256), N.HTREE_EUNSUPPORTED),
+    (dict(k_token=250), N.HTREE_EUNSUPPORTED), (dict(k_token=1 << 26), N.HTREE_EUNSUPPORTED), (dict(v_page=-256), N.HTREE_EUNSUPPORTED),
 ]
 
 
@@ -76,7 +76,9 @@ def test_attention_workspace():
     one = ws_bytes(cache(), width=65)[1]
     assert one > 0
     assert ws_bytes(cache(), B=4000, rows=4000, width=8192)[1] == one
-    assert ws_bytes(cache(), B=1, rows=100000, width=8192)[1] <= 4 * one
+    assert ws_bytes(cache(), B=1, rows=100000, width=8192)[1] == ws_bytes(cache(), B=1, rows=64, width=8192)[1]
+    for d in (32, 64, 128, 256):
+        assert ws_bytes(cache(Dk=d, Dv=d), B=1, rows=1000, width=8192)[1] <= 160 << 20
     assert N.lib().htree_draft_attention_workspace_bytes(cache(), 1, 1, 32, 1, None) == N.HTREE_ENULL
 
 
