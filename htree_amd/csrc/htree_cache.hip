@@ -300,8 +300,10 @@ static int draft_check(const htree_cache* c, int32_t B, int32_t rows, int32_t H,
   if (rc) return rc;
   if (B < 0 || rows < 0 || H <= 0 || H % c->H_kv || width < 0) return HTREE_ESHAPE;
   if ((int64_t)width * c->page_size > (1 << 30)) return HTREE_EUNSUPPORTED;
-  // the grid: units of 16 rows at least, and a block for each row that is joined
-  if (((int64_t)rows * (H / c->H_kv) / 16 + B) * c->H_kv > (1 << 30)) return HTREE_EUNSUPPORTED;
+  // 32-bit rows (new tokens x heads of a group), and a grid of units of 16 at least
+  if ((int64_t)rows * (H / c->H_kv) >= 0x7fffff00ll ||
+      ((int64_t)rows * (H / c->H_kv) / 16 + B) * c->H_kv > (1 << 30))
+    return HTREE_EUNSUPPORTED;
   return HTREE_OK;
 }
 
@@ -431,7 +433,8 @@ extern "C" int htree_draft_attention(const htree_cache* c, int32_t B, int32_t ro
   a.width = table_width, a.page_shift = log2i(c->page_size), a.num_pages = c->num_pages;
   a.target = p.target;
   a.negate = scale < 0.f;
-  a.c = fmaxf(fabsf(scale) * kLog2e, 1e-38f);  // a scale of 0 still multiplies -inf
+  a.c = fmaxf(fabsf(scale) * kLog2e, 1e-37f);  // a scale of 0 still multiplies -inf
+  a.inv_c = 1.f / a.c;
   hipStream_t s = (hipStream_t)stream;
   if (c->dtype == HTREE_F32) return draft_launch_type<float>(a, p, s);
   if (c->dtype == HTREE_BF16) return draft_launch_type<__bf16>(a, p, s);

@@ -32,7 +32,7 @@ struct DraftArgs {
   int64_t k_page, k_token, k_head, v_page, v_token, v_head;            // bytes
   int32_t B, rows, H, Hkv, G, Dk, Dv, width, page_shift, num_pages;
   int32_t target;  // units to split into (0: one unit per group of rows)
-  float c;         // |scale| * log2(e), not 0
+  float c, inv_c;  // |scale| * log2(e), not 0
   int32_t negate;  // the scale is negative: the queries change sign
 };
 
@@ -224,7 +224,7 @@ __device__ __forceinline__ bool draft_odd(uint4 x) {
 struct DraftCtx {
   int s0, ctx, kend, t0, t1, used, shift;
   int full;  // tokens that every row sees, where their pages exist
-  int64_t nrow;
+  int nrow;                // rows: new tokens x heads of the group
   const char *kh, *vh;     // the KV head's keys and values
   const int32_t* tab;      // the request's table
   const int32_t* par;      // its new tokens' parents, or null
@@ -260,12 +260,12 @@ __device__ __forceinline__ DraftCtx draft_ctx(const DraftArgs& a, const DraftUni
   DraftCtx c;
   c.s0 = uniform(rq.s0), c.ctx = uniform(rq.ctx);
   c.shift = a.page_shift;
-  c.nrow = (int64_t)rq.n * a.G;
-  const DraftSpan sp = draft_span(rq, (int64_t)u.rt * R, R, a.G, a.width << a.page_shift, KT, u.ch, u.chunk);
+  c.nrow = uniform(rq.n * a.G);
+  const DraftSpan sp = draft_span(rq, u.rt * R, R, a.G, a.width << a.page_shift, KT, u.ch, u.chunk);
   c.kend = uniform(sp.kend), c.t0 = uniform(sp.t0), c.t1 = uniform(sp.t1);
   c.used = (c.kend + (1 << c.shift) - 1) >> c.shift;
   // rows behind the request's last see nothing, but are not stored either
-  c.full = min(a.parents ? c.ctx : c.ctx + (int)((int64_t)u.rt * R / a.G) + 1, c.kend);
+  c.full = min(a.parents ? c.ctx : c.ctx + u.rt * R / a.G + 1, c.kend);
   c.kh = a.k + u.h * a.k_head;
   c.vh = a.v + u.h * a.v_head;
   c.tab = a.table + u.b * a.table_stride;
@@ -290,22 +290,30 @@ struct DraftWave {
   using Quad = DraftQuad<T, D>;
   static constexpr int NG = KT / 16, CPR = S::CPR, ROWB = S::ROWB, NQ = S::NQ;
   static constexpr bool F32 = S::F32;
-  int n16, g;
-  int tok[MT];  // the row's new token, -1 behind the last row
+  int n16, g, row0;
   f32x4 qf[MT][F32 ? D / 16 : 1];
   bf16x8 qh[MT][F32 ? 1 : D / 32];
-  float m[MT], l[MT];
+  // The weights are exp2(score c + nm): nm is minus the max they are taken
+  // against (0 before there is one), in log2 units; a score past `top` moves it.
+  float nm[MT], top[MT];
+  // the weights' sum: whole for 16-bit types, which have it from a product
+  // with ones, a quarter of it in each lane for fp32
+  float l[MT];
   f32x4 o[MT][NQ];
 
-  __device__ __forceinline__ void init(const DraftArgs& a, const DraftCtx& c, int h, int64_t row0) {
+  // new token of lane n16's row of group mt, -1 behind the last row
+  __device__ __forceinline__ int token(const DraftArgs& a, const DraftCtx& c, int mt, int n16) const {
+    const int r = row0 + mt * 16 + n16;
+    return r < c.nrow ? r / a.G : -1;
+  }
+  __device__ __forceinline__ void init(const DraftArgs& a, const DraftCtx& c, int h, int row) {
     const int lane = threadIdx.x & 63;
-    n16 = lane & 15, g = lane >> 4;
+    n16 = lane & 15, g = lane >> 4, row0 = row;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-      const int64_t r = row0 + mt * 16 + n16;
+      const int r = row0 + mt * 16 + n16;
       const bool on = r < c.nrow;
-      const int j = on ? (int)(r / a.G) : 0, hg = on ? (int)(r - (int64_t)j * a.G) : 0;
-      tok[mt] = on ? j : -1;
+      const int j = on ? r / a.G : 0, hg = on ? r - j * a.G : 0;
       const char* p = a.q + (int64_t)(c.s0 + j) * a.q_row + (int64_t)(h * a.G + hg) * a.q_head;
       if constexpr (F32) {
 #pragma unroll
@@ -324,7 +332,8 @@ struct DraftWave {
           qh[mt][s] = __builtin_bit_cast(bf16x8, x);
         }
       }
-      m[mt] = -INFINITY;
+      nm[mt] = 0.f;
+      top[mt] = -INFINITY;
       l[mt] = 0.f;
 #pragma unroll
       for (int q = 0; q < NQ; ++q) o[mt][q] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -332,11 +341,11 @@ struct DraftWave {
   }
 
   // whether row mt's token sees the request's token `key` < kend
-  __device__ __forceinline__ bool sees(const DraftCtx& c, int mt, int key) const {
-    if (tok[mt] < 0) return false;
-    if (!c.par) return key <= c.ctx + tok[mt];
+  __device__ __forceinline__ bool sees(const DraftArgs& a, const DraftCtx& c, int mt, int key) const {
+    int j = token(a, c, mt, n16);
+    if (j < 0) return false;
+    if (!c.par) return key <= c.ctx + j;
     if (key < c.ctx) return true;
-    int j = tok[mt];
     while (j >= 0 && c.ctx + j > key) j = draft_parent(c.par[j], j);
     return j >= 0 && c.ctx + j == key;
   }
@@ -395,20 +404,20 @@ struct DraftWave {
 
     // ---- masks
     if (masked) {
-      const int g2 = draft_lane_again() >> 4;
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
         uint64_t see = 0;
-        if (tok[mt] >= 0) {
+        const int tok = token(a, c, mt, n16);
+        if (tok >= 0) {
           if (c.par) {
             const int c0 = min(max(c.ctx - key0, 0), 64);  // cached tokens of the tile
             see = c0 == 64 ? ~0ull : (1ull << c0) - 1;
-            for (int j = tok[mt]; j >= 0 && c.ctx + j >= key0;) {
+            for (int j = tok; j >= 0 && c.ctx + j >= key0;) {
               if (c.ctx + j - key0 < KT) see |= 1ull << (c.ctx + j - key0);
               j = draft_parent(c.par[j], j);
             }
           } else {
-            const int c1 = min(max(c.ctx + tok[mt] + 1 - key0, 0), 64);
+            const int c1 = min(max(c.ctx + tok + 1 - key0, 0), 64);
             see = c1 == 64 ? ~0ull : (1ull << c1) - 1;
           }
         }
@@ -417,13 +426,14 @@ struct DraftWave {
         for (int i = 0; i < NG; ++i)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (!((see >> (16 * i + 4 * g2 + e)) & 1)) sc[mt][i][e] = -INFINITY;
+            if (!((see >> (16 * i + 4 * g + e)) & 1)) sc[mt][i][e] = -INFINITY;
       }
     }
 
-    // ---- running softmax, in log2 units.  The max a row's weights are taken
-    // against only moves when a score passes it by 8: weights up to 2^8 lose
-    // nothing, and the output is seldom rescaled.
+    // ---- running softmax.  The max that a row's weights are taken against
+    // only moves when a score passes it by 8 log2 units: weights up to 2^8
+    // lose nothing, the output is seldom rescaled, and the lanes of a row
+    // seldom have to compare their scores.
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       float mx = -INFINITY;
@@ -431,28 +441,30 @@ struct DraftWave {
       for (int i = 0; i < NG; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) mx = fmaxf(mx, sc[mt][i][e]);
-      mx = max_xor32(max_xor16(mx)) * a.c;
-      if (__any(mx > m[mt] + 8.f)) {
-        const float mn = mx > m[mt] + 8.f ? mx : m[mt];
-        const float al = m[mt] == mn ? 1.f : __builtin_amdgcn_exp2f(m[mt] - mn);
-        m[mt] = mn;
-        l[mt] *= al;
+      if (__any(mx > top[mt])) {
+        mx = max_xor32(max_xor16(mx));
+        if (mx > top[mt]) {
+          const float mn = -mx * a.c, al = top[mt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mn - nm[mt]);
+          // (before the first score there is nothing to rescale, but NaN stays)
+          nm[mt] = mn;
+          top[mt] = mx + 8.f * a.inv_c;
+          l[mt] *= al;
 #pragma unroll
-        for (int q = 0; q < NQ; ++q) o[mt][q] *= al;
+          for (int q = 0; q < NQ; ++q) o[mt][q] *= al;
+        }
       }
-      const float ref = m[mt] == -INFINITY ? 0.f : m[mt];
 #pragma unroll
       for (int i = 0; i < NG; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          sc[mt][i][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[mt][i][e], a.c, -ref));
-          l[mt] += sc[mt][i][e];
+          sc[mt][i][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[mt][i][e], a.c, nm[mt]));
+          if constexpr (F32) l[mt] += sc[mt][i][e];
         }
     }
 
     // P rounded to the values' type: a relative half step for each of many
-    // tokens, as large as the output's own rounding at most; the sum l is
-    // taken of the unrounded P
+    // tokens, as large as the output's own rounding at most.  The sum is taken
+    // of the rounded P too, so that the weights still add up to one.
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -502,6 +514,24 @@ struct DraftWave {
       const int row = 4 * g + (n16 >> 2);
       const uint32_t v0 = draft_lds(vb) + row * ROWB + draft_swz_v<CPR, F32>(row, (n16 & 3) >> 1) * 16 + (n16 & 1) * 8;
       auto col = [&](int i, int q) { return draft_read_tr((v0 ^ (q * 32)) + i * 16 * ROWB); };
+      constexpr uint32_t one = std::is_same<T, __bf16>::value ? 0x3f803f80u : 0x3c003c00u;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+        if constexpr (NG == 1) {
+          sum = DraftT<T>::mma_k16(__builtin_bit_cast(s16x4, make_uint2(one, one)),
+                                   __builtin_bit_cast(s16x4, wt.p[mt][0]), sum);
+        } else {
+          using V8 = typename DraftT<T>::V8;
+#pragma unroll
+          for (int i = 0; i < NG; i += 2)
+            sum = DraftT<T>::mma(
+                __builtin_bit_cast(V8, make_uint4(one, one, one, one)),
+                __builtin_bit_cast(V8, make_uint4(wt.p[mt][i].x, wt.p[mt][i].y, wt.p[mt][i + 1].x, wt.p[mt][i + 1].y)),
+                sum);
+        }
+        l[mt] += sum[0];
+      }
       constexpr int PG = NG == 1 ? 1 : 2, NS = NG / PG * NQ, AHEAD = NS < 4 ? NS : 4;  // groups of a product
       uint2 f[AHEAD][PG];
       auto value = [&](int x) {  // step x: dims x % NQ, groups from x / NQ
@@ -541,7 +571,7 @@ struct DraftWave {
     const T* vp = (const T*)(c.vh + page * a.v_page + at * a.v_token);
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-      if (!__any(sees(c, mt, key))) continue;
+      if (!__any(sees(a, c, mt, key))) continue;
       float x = 0.f;  // the row's score, a quarter of it in each lane
 #pragma unroll
       for (int s = 0; s < (F32 ? D / 16 : D / 32); ++s)
@@ -551,8 +581,8 @@ struct DraftWave {
           if (d < a.Dk) x += q_at(mt, s, e) * Io<T>::ld(kp + d);
         }
       x = add_xor32(add_xor16(x)) * a.c;
-      const bool see = sees(c, mt, key);
-      const float p = __builtin_amdgcn_exp2f(x - (m[mt] == -INFINITY ? 0.f : m[mt]));
+      const bool see = sees(a, c, mt, key);
+      const float p = __builtin_amdgcn_exp2f(x + nm[mt]);
 #pragma unroll
       for (int q = 0; q < NQ; ++q)
 #pragma unroll
@@ -566,6 +596,12 @@ struct DraftWave {
     if constexpr (F32) return qf[mt][s][e];
     else return (float)__builtin_bit_cast(typename DraftT<T>::V8, qh[mt][s])[e];
   }
+
+  // the sum and max (log2 units, -inf: none) of row n16 of group mt
+  __device__ __forceinline__ float sum(int mt) const {
+    return F32 ? add_xor32(add_xor16(l[mt])) : l[mt];
+  }
+  __device__ __forceinline__ float peak(int mt) const { return top[mt] == -INFINITY ? -INFINITY : -nm[mt]; }
 
   // the lane's part of row n16 of group mt, times f, into 16 fp32 rows at dst
   __device__ __forceinline__ void put(float* dst, int mt, float f) const {
@@ -593,10 +629,10 @@ __device__ __forceinline__ bool draft_odd_row(const DraftArgs& a, const char* vp
 
 // stores chunk ch of the request's row r (x: weighted sum, sum: the weights')
 template <typename T>
-__device__ __forceinline__ void draft_store(const DraftArgs& a, int s0, int h, int64_t r, int ch, f32x4 x, float sum) {
+__device__ __forceinline__ void draft_store(const DraftArgs& a, int s0, int h, int r, int ch, f32x4 x, float sum) {
   if (ch * 4 >= a.Dv) return;
   const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row that sees nothing is zero
-  const int j = (int)(r / a.G), hg = (int)(r - (int64_t)j * a.G);
+  const int j = r / a.G, hg = r - j * a.G;
   typedef __attribute__((ext_vector_type(4))) T T4;
   *(T4*)(a.out + (int64_t)(s0 + j) * a.o_row + (int64_t)(h * a.G + hg) * a.o_head + ch * 4 * sizeof(T)) =
       __builtin_convertvector(x * inv, T4);
@@ -619,7 +655,7 @@ __global__ __launch_bounds__(256, (MT == 1 && D <= 128) ? 2 : 1) void draft_kern
   const int lane = threadIdx.x & 63, wv = uniform(threadIdx.x >> 6);
   const DraftReq rq = draft_request(a, u.b);
   const DraftCtx c = draft_ctx<KT, R>(a, u, rq);
-  const int64_t row0 = (int64_t)u.rt * R;
+  const int row0 = u.rt * R;
   DraftWave<T, D, MT, KT> w;
   w.init(a, c, u.h, row0);
 
@@ -745,10 +781,10 @@ __global__ __launch_bounds__(256, (MT == 1 && D <= 128) ? 2 : 1) void draft_kern
   // ---- the four waves' states meet
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
-    w.l[mt] = add_xor32(add_xor16(w.l[mt]));
+    const float sum = w.sum(mt);
     if (w.g == 0) {
-      ml[wv][mt * 16 + w.n16][0] = w.m[mt];
-      ml[wv][mt * 16 + w.n16][1] = w.l[mt];
+      ml[wv][mt * 16 + w.n16][0] = w.peak(mt);
+      ml[wv][mt * 16 + w.n16][1] = sum;
     }
   }
   __syncthreads();
@@ -760,7 +796,8 @@ __global__ __launch_bounds__(256, (MT == 1 && D <= 128) ? 2 : 1) void draft_kern
     for (int i = 0; i < NW; ++i) mm = fmaxf(mm, ml[i][mt * 16 + w.n16][0]);
     // a wave that saw no token of the row adds nothing (NaN scores leave the
     // max alone and make sums NaN, which stay)
-    w.put((float*)(lds + wv * WAVE_LDS), mt, w.m[mt] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(w.m[mt] - mm));
+    const float pk = w.peak(mt);
+    w.put((float*)(lds + wv * WAVE_LDS), mt, pk == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(pk - mm));
     __syncthreads();
     for (int i = threadIdx.x; i < 16 * S::OC; i += 256) {
       const int row = i / S::OC, ch = i % S::OC, rr = mt * 16 + row;
@@ -809,7 +846,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void draft_rows_kernel(D
   const int lane = threadIdx.x & 63, wv = uniform(threadIdx.x >> 6);
   const DraftReq rq = draft_request(a, u.b);
   const DraftCtx c = draft_ctx<KT, R>(a, u, rq);
-  const int64_t row0 = (int64_t)u.rt * R + wv * 16 * MT;
+  const int row0 = u.rt * R + wv * 16 * MT;
   DraftWave<T, D, MT, KT> w;
   w.init(a, c, u.h, row0);
 
@@ -932,13 +969,13 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void draft_rows_kernel(D
   float* my = (float*)lds + wv * 16 * D;
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
-    const float l = add_xor32(add_xor16(w.l[mt])), m = w.m[mt];
+    const float l = w.sum(mt), m = w.peak(mt);
     w.put(my, mt, 1.f);
     wave_sync();
 #pragma unroll
     for (int i = lane; i < 16 * S::OC; i += 64) {
       const int row = i / S::OC, ch = i % S::OC;
-      const int64_t r = row0 + mt * 16 + row;
+      const int r = row0 + mt * 16 + row;
       const float big = __shfl(m, row), sum = __shfl(l, row);
       const f32x4 x = draft_got<T, D>(my, row, ch);
       if (r >= c.nrow) continue;
@@ -968,8 +1005,8 @@ __global__ __launch_bounds__(256) void draft_join_kernel(DraftArgs a) {
   if (!draft_unit<KT, R>(a, blockIdx.x / R, true, &u)) return;
   const int rr = blockIdx.x % R;
   const DraftReq rq = draft_request(a, u.b);
-  const int64_t r = (int64_t)u.rt * R + rr;
-  if (r >= (int64_t)rq.n * a.G) return;
+  const int r = u.rt * R + rr;
+  if (r >= rq.n * a.G) return;
   const int64_t base = u.slot + (int64_t)u.rt * a.Hkv + u.h, step = draft_row_groups(rq, a.G, R) * a.Hkv;
   const int tid = threadIdx.x, p = tid / OC, ch = tid % OC;
   float big = -INFINITY;

@@ -49,8 +49,9 @@ def reference(q, k, v, see, scale, dtype):
     to 2^-22 relative, and the log2 form's product with log2 e to 3 x 2^-24 of
     |s| + |m|.  With e the largest of these, numerator and denominator are off
     by e each, relative to A = sum p |v| / sum p.  Sums of L terms in fp32, in
-    any order: L 2^-24 each.  16-bit types round P (half a step of A) and the
-    result (half a step of it)."""
+    any order: L 2^-24 each.  16-bit types round P, in the numerator and in the
+    sum alike: sum dp (v - o) / sum p is off by half a step of A + |o| at most;
+    and the result (half a step of it)."""
     n, H, K = q.shape
     L, Hkv, V = v.shape
     out, bar = np.zeros((n, H, V)), np.zeros((n, H, V))
@@ -72,7 +73,7 @@ def reference(q, k, v, see, scale, dtype):
         e = (K + 2 + 6) * u * mag + 2.0 ** -22
         b = A * (2 * e + (2 * L + 16) * u)[:, None]
         if dtype != "float32":
-            b = b + A * half
+            b = b + (A + np.abs(o)) * half
         out[:, h] = o
         bar[:, h] = b * 1.001 + (np.abs(o) + b) * (half if dtype != "float32" else 4 * u) + tiny
     return out, bar
