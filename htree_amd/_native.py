@@ -193,6 +193,20 @@ def stream_ptr(device) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+def address(t):
+    """Data pointer as ctypes takes it (None: NULL); ptr() without the object."""
+    return None if t is None else t.data_ptr()
+
+
+def launch(fn, dev, *args) -> int:
+    """fn(*args, stream) on dev's current stream, with dev the current device."""
+    index = dev.index
+    if torch.cuda.current_device() == index:  # the context manager costs as much as a call
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    with torch.cuda.device(index):
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
+
+
 def ptr_array(tensors):
     arr = (ctypes.c_void_p * MAX_LEVELS)()
     for i, t in enumerate(tensors):

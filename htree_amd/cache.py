@@ -21,6 +21,7 @@ Nothing here synchronises, so a step can be captured into a graph.
 """
 from __future__ import annotations
 
+from functools import lru_cache
 from typing import NamedTuple, Optional
 
 import torch
@@ -31,6 +32,7 @@ MAX_REQUESTS = 4096
 MAX_HEAD_DIM = 256
 PAGE_SIZES = (16, 4096)       # of the cache: powers of two in this range
 MAX_REQUEST_TOKENS = 1 << 30  # block table width * page_size
+MAX_TOKEN_BYTES = 1 << 26     # between a page's tokens
 
 
 class PageTables(NamedTuple):
@@ -42,14 +44,14 @@ class PageTables(NamedTuple):
     pages_used: torch.Tensor  # [1] pages taken from the front of free_pages
 
 
-def _ints(t: torch.Tensor, name: str, shape, device) -> None:
-    assert t.dtype == torch.int32 and tuple(t.shape) == tuple(shape) and t.is_contiguous(), \
-        f"{name} must be a contiguous int32 tensor {list(shape)}, got {t.dtype} {list(t.shape)}"
+def _ints(t: torch.Tensor, name: str, n: int, device) -> None:
+    assert t.dtype is torch.int32 and t.shape == (n,) and t.is_contiguous(), \
+        f"{name} must be a contiguous int32 tensor [{n}], got {t.dtype} {list(t.shape)}"
     assert t.device == device, f"{name} must be on {device}"
 
 
 def check_table(block_table: torch.Tensor, B: int, device) -> None:
-    assert block_table.dtype == torch.int32 and block_table.dim() == 2, "block_table must be int32 [B, width]"
+    assert block_table.dtype is torch.int32 and block_table.dim() == 2, "block_table must be int32 [B, width]"
     assert block_table.shape[0] == B, f"block_table must have a row for each of the {B} requests"
     assert block_table.stride(1) == 1 or block_table.shape[1] <= 1 or B == 0, "block_table rows must be contiguous"
     assert block_table.device == device, f"block_table must be on {device}"
@@ -59,35 +61,41 @@ def aligned_rows(x: torch.Tensor) -> torch.Tensor:
     """x [rows, heads, D] itself where the kernels can read it: the head dim
     contiguous, rows and heads at 16-byte steps; else a contiguous copy."""
     n, h, d = x.stride()
-    es = x.element_size()
-    if (d == 1 or x.shape[2] == 1) and (n | h) * es % 16 == 0 and x.data_ptr() % 16 == 0:
+    if (d == 1 or x.shape[2] == 1) and ((n | h) * x.element_size() | x.data_ptr()) % 16 == 0:
         return x
     return x.clone(memory_format=torch.contiguous_format)
 
 
-def native_cache(k_cache: torch.Tensor, v_cache: torch.Tensor) -> "N.HtreeCache":
-    """Checks the cache tensors and describes them for the C ABI."""
-    assert k_cache.dim() == 4 and v_cache.dim() == 4, "k_cache / v_cache must be [pages, page_size, H_kv, D]"
-    pages, page, heads, K = k_cache.shape
-    V = v_cache.shape[3]
-    assert v_cache.shape[:3] == k_cache.shape[:3], "k_cache and v_cache must have the same pages and heads"
-    assert k_cache.dtype == v_cache.dtype and k_cache.dtype in N.DTYPE_CODE, \
-        "k_cache and v_cache must share one dtype: float32, bfloat16 or float16"
-    assert k_cache.is_cuda, "htree_amd runs on the GPU (no CPU fallback)"
-    assert k_cache.device == v_cache.device, "k_cache and v_cache must be on one device"
+@lru_cache(maxsize=256)
+def _describe(kshape, kstride, vshape, vstride, dtype) -> "N.HtreeCache":
+    """The cache's sizes for the C ABI, checked (by sizes and strides alone)."""
+    assert len(kshape) == 4 and len(vshape) == 4, "k_cache / v_cache must be [pages, page_size, H_kv, D]"
+    pages, page, heads, K = kshape
+    V = vshape[3]
+    assert vshape[:3] == kshape[:3], "k_cache and v_cache must have the same pages and heads"
+    assert dtype in N.DTYPE_CODE, "the cache's dtype must be float32, bfloat16 or float16"
     assert pages > 0 and heads > 0, "the cache needs a page and a head"
     assert PAGE_SIZES[0] <= page <= PAGE_SIZES[1] and page & (page - 1) == 0, \
         f"page_size must be a power of two from {PAGE_SIZES[0]} to {PAGE_SIZES[1]}, got {page}"
-    es = k_cache.element_size()
+    es = dtype.itemsize
     assert 0 < K <= MAX_HEAD_DIM and 0 < V <= MAX_HEAD_DIM and K * es % 16 == 0 and V * es % 16 == 0, \
         f"head dims must be whole 16-byte pieces and at most {MAX_HEAD_DIM}, got K={K}, V={V}"
-    ks, vs = k_cache.stride(), v_cache.stride()
-    assert ks[3] == 1 and vs[3] == 1, "the cache's head dim must be contiguous"
-    assert (ks[0] | ks[1] | ks[2] | vs[0] | vs[1] | vs[2]) * es % 16 == 0 \
-        and k_cache.data_ptr() % 16 == 0 and v_cache.data_ptr() % 16 == 0, \
+    assert kstride[3] == 1 and vstride[3] == 1, "the cache's head dim must be contiguous"
+    assert all(n * es % 16 == 0 for n in kstride[:3] + vstride[:3]), \
         "the cache's pages, tokens and heads must be at 16-byte steps"
-    return N.HtreeCache(N.DTYPE_CODE[k_cache.dtype], heads, K, V, page, pages,
-                        ks[0], ks[1], ks[2], vs[0], vs[1], vs[2])
+    assert kstride[1] * es <= MAX_TOKEN_BYTES and vstride[1] * es <= MAX_TOKEN_BYTES, \
+        f"a page's tokens must be at most {MAX_TOKEN_BYTES} bytes apart"
+    return N.HtreeCache(N.DTYPE_CODE[dtype], heads, K, V, page, pages, *kstride[:3], *vstride[:3])
+
+
+def native_cache(k_cache: torch.Tensor, v_cache: torch.Tensor) -> "N.HtreeCache":
+    """Checks the cache tensors and describes them for the C ABI."""
+    dtype, dev = k_cache.dtype, k_cache.device
+    assert dev.type == "cuda", "htree_amd runs on the GPU (no CPU fallback)"
+    assert v_cache.dtype is dtype, "k_cache and v_cache must share one dtype"
+    assert v_cache.device == dev, "k_cache and v_cache must be on one device"
+    assert (k_cache.data_ptr() | v_cache.data_ptr()) % 16 == 0, "the cache must begin at a 16-byte step"
+    return _describe(k_cache.shape, k_cache.stride(), v_cache.shape, v_cache.stride(), dtype)
 
 
 def page_tables(ctx_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor,
@@ -109,40 +117,39 @@ def page_tables(ctx_lens: torch.Tensor, new_lens: torch.Tensor, block_table: tor
     have slot and position -1; so has the slot of a token past the table's
     width, or whose page free_pages was too short for (pages_used says how
     many are wanted).  page_size is a power of two."""
-    assert ctx_lens.is_cuda, "htree_amd runs on the GPU (no CPU fallback)"
     dev = ctx_lens.device
-    assert ctx_lens.dim() == 1, "ctx_lens must be int32 [B]"
-    B = ctx_lens.shape[0]
+    assert dev.type == "cuda", "htree_amd runs on the GPU (no CPU fallback)"
+    assert ctx_lens.dim() == 1 and free_pages.dim() == 1, "ctx_lens and free_pages must be int32 [B] and [F]"
+    B, F = ctx_lens.shape[0], free_pages.shape[0]
     assert B <= MAX_REQUESTS, f"at most {MAX_REQUESTS} requests, got {B}"
-    _ints(ctx_lens, "ctx_lens", (B,), dev)
-    _ints(new_lens, "new_lens", (B,), dev)
+    _ints(ctx_lens, "ctx_lens", B, dev)
+    _ints(new_lens, "new_lens", B, dev)
+    _ints(free_pages, "free_pages", F, dev)
     check_table(block_table, B, dev)
-    assert free_pages.dim() == 1, "free_pages must be int32 [F]"
-    _ints(free_pages, "free_pages", free_pages.shape, dev)
     assert page_size > 0 and page_size & (page_size - 1) == 0, f"page_size must be a power of two, got {page_size}"
     assert 0 <= rows < 2 ** 31 and num_pages >= 0, "rows and num_pages must not be negative"
     if parents is not None:
-        _ints(parents, "parents", (rows,), dev)
+        _ints(parents, "parents", rows, dev)
     if out is None:
-        i32 = torch.empty(2 * B + 2 + rows, dtype=torch.int32, device=dev)
-        starts, lens, used, positions = i32.split((B + 1, B, 1, rows))
+        starts, positions, lens, used = torch.empty(2 * B + 2 + rows, dtype=torch.int32, device=dev).split_with_sizes(
+            (B + 1, rows, B, 1))
         out = PageTables(starts, torch.empty(rows, dtype=torch.int64, device=dev), positions, lens, used)
     else:
-        for t, name, n in ((out.starts, "out.starts", B + 1), (out.positions, "out.positions", rows),
-                           (out.lens, "out.lens", B), (out.pages_used, "out.pages_used", 1)):
-            _ints(t, name, (n,), dev)
-        assert out.slots.dtype == torch.int64 and out.slots.shape == (rows,) and out.slots.is_contiguous() \
+        _ints(out.starts, "out.starts", B + 1, dev)
+        _ints(out.positions, "out.positions", rows, dev)
+        _ints(out.lens, "out.lens", B, dev)
+        _ints(out.pages_used, "out.pages_used", 1, dev)
+        assert out.slots.dtype is torch.int64 and out.slots.shape == (rows,) and out.slots.is_contiguous() \
             and out.slots.device == dev, f"out.slots must be a contiguous int64 tensor [{rows}] on {dev}"
     if B == 0:
         out.starts.zero_(), out.pages_used.zero_(), out.slots.fill_(-1), out.positions.fill_(-1)
         return out
-    with torch.cuda.device(dev):
-        rc = N.lib().htree_page_tables(
-            B, rows, page_size, num_pages, block_table.shape[1], block_table.stride(0),
-            free_pages.shape[0], N.ptr(ctx_lens), N.ptr(new_lens), N.ptr(parents), N.ptr(block_table),
-            N.ptr(free_pages), N.ptr(out.starts), N.ptr(out.slots), N.ptr(out.positions),
-            N.ptr(out.lens), N.ptr(out.pages_used), N.stream_ptr(dev))
-    N.check(rc, "htree_page_tables")
+    rc = N.launch(N.lib().htree_page_tables, dev, B, rows, page_size, num_pages, block_table.shape[1],
+                  block_table.stride(0), F, ctx_lens.data_ptr(), new_lens.data_ptr(), N.address(parents),
+                  block_table.data_ptr(), free_pages.data_ptr(), out.starts.data_ptr(), out.slots.data_ptr(),
+                  out.positions.data_ptr(), out.lens.data_ptr(), out.pages_used.data_ptr())
+    if rc:
+        N.check(rc, "htree_page_tables")
     return out
 
 
@@ -161,45 +168,46 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     are not written, and a query without a position is zero.  The slots of a
     call are distinct; two rows with one slot leave either's values there,
     or parts of both."""
-    assert k.dim() == 3 and v.dim() == 3, "k / v must be [rows, H_kv, D]"
     c = native_cache(k_cache, v_cache)
-    rows, dev = k.shape[0], k_cache.device
+    dtype, dev = k_cache.dtype, k_cache.device
+    assert k.dim() == 3 and v.dim() == 3, "k / v must be [rows, H_kv, D]"
+    rows = k.shape[0]
     assert k.shape == (rows, c.H_kv, c.Dk) and v.shape == (rows, c.H_kv, c.Dv), \
         f"k / v must be [rows, {c.H_kv}, {c.Dk} / {c.Dv}], got {list(k.shape)} / {list(v.shape)}"
-    assert k.dtype == v.dtype == k_cache.dtype, "k, v and the cache must share one dtype"
-    assert k.device == v.device == dev, "k, v and the cache must be on one device"
-    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
-        assert all(s > 0 or n == 1 for n, s in zip(t.shape, t.stride())), f"{name} must not be expanded"
-    assert slots.dtype == torch.int64 and slots.shape == (rows,) and slots.is_contiguous() \
+    assert k.dtype is dtype and v.dtype is dtype, "k, v and the cache must share one dtype"
+    assert k.device == dev and v.device == dev, "k, v and the cache must be on one device"
+    for n, x, y in zip(k_cache.shape, k_cache.stride(), v_cache.stride()):
+        assert n == 1 or (x > 0 and y > 0), "k_cache and v_cache must not be expanded"
+    assert slots.dtype is torch.int64 and slots.shape == (rows,) and slots.is_contiguous() \
         and slots.device == dev, f"slots must be a contiguous int64 tensor [{rows}] on {dev}"
-    assert not (torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or
-                                             (q is not None and q.requires_grad))), \
-        "cache_append has no backward"
+    if torch.is_grad_enabled():
+        assert not (k.requires_grad or v.requires_grad or (q is not None and q.requires_grad)), \
+            "cache_append has no backward"
     assert (cos is None) == (sin is None) == (positions is None), "positions, cos and sin go together"
-    H, rope_rows, q_out = 0, 0, None
+    H, rope_rows, q_out, q_row, q_head = 0, 0, None, 0, 0
     if cos is not None:
         assert c.Dk % 2 == 0, "rotating needs an even head dim K"
-        for name, t in (("cos", cos), ("sin", sin)):
-            assert t.dtype == torch.float32 and t.dim() == 2 and t.shape[1] == c.Dk // 2 and t.shape[0] > 0 \
-                and t.is_contiguous() and t.device == dev, \
-                f"{name} must be a contiguous fp32 tensor [n, {c.Dk // 2}] on {dev}"
-        assert cos.shape == sin.shape, "cos and sin must have one shape"
-        _ints(positions, "positions", (rows,), dev)
-        rope_rows = cos.shape[0]
+        rope_rows, half = cos.shape[0], c.Dk // 2
+        assert rope_rows > 0 and cos.shape == (rope_rows, half) and sin.shape == (rope_rows, half) \
+            and cos.dtype is torch.float32 and sin.dtype is torch.float32 \
+            and cos.is_contiguous() and sin.is_contiguous() and cos.device == dev and sin.device == dev, \
+            f"cos and sin must be contiguous fp32 tensors [n, {half}] on {dev}"
+        _ints(positions, "positions", rows, dev)
     if q is not None:
         assert cos is not None, "q is taken to be rotated: it needs positions, cos and sin"
         assert q.dim() == 3 and q.shape[0] == rows and q.shape[2] == c.Dk and q.shape[1] > 0, \
             f"q must be [{rows}, H, {c.Dk}], got {list(q.shape)}"
-        assert q.dtype == k.dtype and q.device == dev, "q must have k's dtype and device"
+        assert q.dtype is dtype and q.device == dev, "q must have k's dtype and device"
         H = q.shape[1]
         q = aligned_rows(q)
-        q_out = torch.empty(rows, H, c.Dk, dtype=q.dtype, device=dev)
+        q_row, q_head, _ = q.stride()
+        q_out = torch.empty((rows, H, c.Dk), dtype=dtype, device=dev)
     k, v = aligned_rows(k), aligned_rows(v)
-    with torch.cuda.device(dev):
-        rc = N.lib().htree_cache_append(
-            c, rows, H, N.ptr(k), k.stride(0), k.stride(1), N.ptr(v), v.stride(0), v.stride(1),
-            N.ptr(q), q.stride(0) if H else 0, q.stride(1) if H else 0, N.ptr(slots), N.ptr(positions),
-            N.ptr(cos), N.ptr(sin), rope_rows, N.ptr(q_out), N.ptr(k_cache), N.ptr(v_cache),
-            N.stream_ptr(dev))
-    N.check(rc, "htree_cache_append")
+    k_row, k_head, _ = k.stride()
+    v_row, v_head, _ = v.stride()
+    rc = N.launch(N.lib().htree_cache_append, dev, c, rows, H, k.data_ptr(), k_row, k_head, v.data_ptr(), v_row, v_head,
+                  N.address(q), q_row, q_head, slots.data_ptr(), N.address(positions), N.address(cos), N.address(sin),
+                  rope_rows, N.address(q_out), k_cache.data_ptr(), v_cache.data_ptr())
+    if rc:
+        N.check(rc, "htree_cache_append")
     return q_out

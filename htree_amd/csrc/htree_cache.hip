@@ -8,14 +8,14 @@ namespace htree {
 
 // ---------------------------------------------------------------- tables
 constexpr int kMaxRequests = 4096;  // the lengths' sums sit in one block's LDS
-constexpr int kTabRows = 1024;      // rows, or new pages, of a block
+constexpr int kTabTile = 256;       // rows, or new pages, that a block takes at a time
 
 struct TabArgs {
   const int32_t *ctx, *add, *parents, *free_pages;
   int32_t *table, *starts, *positions, *lens, *used;
   int64_t* slots;
   int64_t table_stride;
-  int32_t B, rows, page_shift, num_pages, width, n_free, page_blocks;
+  int32_t B, rows, page_shift, num_pages, width, n_free, page_blocks, tiles;
 };
 
 // Exclusive sums over the requests in `dst[0 .. B]`, of f(b), saturated at
@@ -62,13 +62,14 @@ __device__ __forceinline__ int tab_find(const int32_t* s, int B, int x) {
 }
 
 // Blocks 0 .. page_blocks - 1 write the new pages' table entries, the others
-// the rows' slots and positions.  Each block sums the lengths again (two
-// loads and two scans), which is less than a second launch; a row's slot comes
-// from the page list itself, not from the entry another block may be writing.
+// the rows' slots and positions, `tiles` times 256 each.  Each block sums the
+// lengths again (two loads and two scans), which is less than a second launch;
+// a row's slot comes from the page list itself, not from the entry another
+// block may be writing.
 __global__ __launch_bounds__(256) void page_tables_kernel(TabArgs a) {
   extern __shared__ int32_t tab_lds[];
   __shared__ int64_t red[4];
-  __shared__ int32_t par[kTabRows];
+  __shared__ int32_t par[kTabTile];
   int32_t* starts = tab_lds;          // [B + 1], rows at most
   int32_t* first = tab_lds + a.B + 1; // [B + 1], new pages of the requests before
   const int tid = threadIdx.x;
@@ -93,10 +94,9 @@ __global__ __launch_bounds__(256) void page_tables_kernel(TabArgs a) {
       if (tid == 0) a.used[0] = (int32_t)min(need, (int64_t)0x7fffffff);
     }
     const int64_t total = min(need, (int64_t)0x7fffffff);
-#pragma unroll
-    for (int x = 0; x < kTabRows / 256; ++x) {
-      const int64_t i = (int64_t)blockIdx.x * kTabRows + x * 256 + tid;
-      if (i >= total) break;
+    for (int x = 0; x < a.tiles; ++x) {
+      const int64_t i = ((int64_t)blockIdx.x * a.tiles + x) * kTabTile + tid;
+      if (i >= total) return;
       const int b = tab_find(first, a.B, (int)i);
       const int64_t j = had(b) + i - first[b];
       if (j < a.width) a.table[b * a.table_stride + j] = fresh(i);
@@ -104,20 +104,20 @@ __global__ __launch_bounds__(256) void page_tables_kernel(TabArgs a) {
     return;
   }
 
-  const int64_t row0 = (int64_t)(blockIdx.x - a.page_blocks) * kTabRows;
-  if (a.parents) {
-    for (int i = tid; i < kTabRows; i += 256) par[i] = row0 + i < a.rows ? a.parents[row0 + i] : -1;
-    __syncthreads();
-  }
-#pragma unroll
-  for (int x = 0; x < kTabRows / 256; ++x) {
-    const int64_t row = row0 + x * 256 + tid;
-    if (row >= a.rows) break;
+  for (int x = 0; x < a.tiles; ++x) {
+    const int64_t row0 = ((int64_t)(blockIdx.x - a.page_blocks) * a.tiles + x) * kTabTile, row = row0 + tid;
+    if (row0 >= a.rows) return;
+    if (a.parents) {
+      if (x) __syncthreads();  // the earlier tile's parents have been read
+      par[tid] = row < a.rows ? a.parents[row] : -1;
+      __syncthreads();
+    }
+    if (row >= a.rows) continue;
     int64_t slot = -1;
     int pos = -1;
     if (row < starts[a.B]) {
       const int b = tab_find(starts, a.B, (int)row);
-      const int ctx = max(a.ctx[b], 0), j = (int)row - starts[b];
+      const int ctx = max(a.ctx[b], 0), s0 = starts[b], j = (int)row - s0;
       const int64_t at = (int64_t)ctx + j;
       const int64_t pi = at >> a.page_shift, h = had(b);
       if (pi < a.width) {
@@ -129,12 +129,8 @@ __global__ __launch_bounds__(256) void page_tables_kernel(TabArgs a) {
       if (a.parents) {
         // up the tree; a parent comes before its children (else: a root)
         depth = 0;
-        for (int i = j;;) {
-          const int64_t r = starts[b] + i;
-          i = draft_parent(r >= row0 ? par[r - row0] : a.parents[r], i);
-          if (i < 0) break;
-          ++depth;
-        }
+        int i = j;
+        while ((i = draft_parent(s0 + i >= row0 ? par[s0 + i - row0] : a.parents[s0 + i], i)) >= 0) ++depth;
       }
       pos = (int)min(ctx + depth, (int64_t)0x7fffffff);
     }
@@ -300,9 +296,9 @@ static int draft_check(const htree_cache* c, int32_t B, int32_t rows, int32_t H,
   if (rc) return rc;
   if (B < 0 || rows < 0 || H <= 0 || H % c->H_kv || width < 0) return HTREE_ESHAPE;
   if ((int64_t)width * c->page_size > (1 << 30)) return HTREE_EUNSUPPORTED;
-  // 32-bit rows (new tokens x heads of a group), and a grid of units of 16 at least
+  // 32-bit rows (new tokens x heads of a group), and the units of 16 rows at least
   if ((int64_t)rows * (H / c->H_kv) >= 0x7fffff00ll ||
-      ((int64_t)rows * (H / c->H_kv) / 16 + B) * c->H_kv > (1 << 30))
+      ((int64_t)rows * (H / c->H_kv) / 16 + B + 512) * c->H_kv > kDraftMaxUnits)
     return HTREE_EUNSUPPORTED;
   return HTREE_OK;
 }
@@ -331,10 +327,14 @@ extern "C" int htree_page_tables(int32_t B, int32_t rows, int32_t page_size, int
   a.table_stride = table_stride;
   a.B = B, a.rows = rows, a.page_shift = log2i(page_size), a.num_pages = num_pages, a.width = table_width;
   a.n_free = n_free;
+  // few rows: a tile of 256 a block, for the latency; many: enough tiles that
+  // the sums of the lengths do not count
+  const int64_t row_tiles = ((int64_t)rows + kTabTile - 1) / kTabTile;
+  a.tiles = (int)(row_tiles <= 1024 ? 1 : row_tiles < 8192 ? (row_tiles + 1023) / 1024 : 8);
   // a request's new tokens begin at most one page more than they fill
-  const int64_t pages = (int64_t)rows / page_size + B;
-  a.page_blocks = (int)((pages + kTabRows - 1) / kTabRows);
-  const int64_t grid = a.page_blocks + ((int64_t)rows + kTabRows - 1) / kTabRows;
+  const int64_t pages = (int64_t)rows / page_size + B, step = (int64_t)kTabTile * a.tiles;
+  a.page_blocks = (int)((pages + step - 1) / step);
+  const int64_t grid = a.page_blocks + ((int64_t)rows + step - 1) / step;
   hipLaunchKernelGGL(page_tables_kernel, dim3((unsigned)grid), dim3(256), 2 * (B + 1) * 4, (hipStream_t)stream, a);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? HTREE_OK : (int)e;
@@ -432,6 +432,7 @@ extern "C" int htree_draft_attention(const htree_cache* c, int32_t B, int32_t ro
   a.B = B, a.rows = rows, a.H = H, a.Hkv = c->H_kv, a.G = H / c->H_kv, a.Dk = c->Dk, a.Dv = c->Dv;
   a.width = table_width, a.page_shift = log2i(c->page_size), a.num_pages = c->num_pages;
   a.target = p.target;
+  a.one_round = p.one_round;
   a.negate = scale < 0.f;
   a.c = fmaxf(fabsf(scale) * kLog2e, 1e-37f);  // a scale of 0 still multiplies -inf
   a.inv_c = 1.f / a.c;

@@ -32,11 +32,13 @@ __host__ __device__ constexpr int draft_tile(int D, int es, int NW = 1) {
 }
 
 // A call's split.  Units: blocks of the launch, R rows of a request and KV
-// head each.  Groups: groups of rows whose units a second launch joins.
+// head each.  Joins: blocks of the second launch, which joins the units of the
+// same rows and takes as many rounds as there are rows.
 struct DraftPlan {
   int D, MT, NW, R;
   int target;  // units to split into (0: one unit per group of rows)
-  int64_t units, groups, slots, bytes;  // at most
+  bool one_round;  // every piece of the join has a block of its own
+  int64_t units, joins, slots, bytes;  // at most
 };
 __host__ __device__ inline DraftPlan draft_plan(int Dk, int Dv, int es, int B, int rows, int H, int Hkv,
                                                 int width, int page_size) {
@@ -57,7 +59,9 @@ __host__ __device__ inline DraftPlan draft_plan(int Dk, int Dv, int es, int B, i
   const int full = (p.NW > 1 || p.MT == 1) && p.D <= 128 ? 512 : 256;
   p.target = (int64_t)width * page_size <= 1024 ? 0 : full;
   p.units = rts + p.target;
-  p.groups = rts < p.target ? rts : p.target;
+  // a group of rows makes R pieces of joining at most
+  p.one_round = rts * p.R <= 1024;
+  p.joins = p.target == 0 ? 0 : p.one_round ? rts * p.R : 1024;
   // a split request has at most twice the chunks its tokens fill
   p.slots = 2 * (int64_t)p.target;
   p.bytes = p.slots * p.R * (p.D + 2) * 4;
@@ -84,16 +88,25 @@ __host__ __device__ inline int draft_tiles(const DraftReq& r, int cap, int KT) {
   return ((r.len < cap ? r.len : cap) + KT - 1) / KT;
 }
 // groups of rows of a request (and KV head)
-__host__ __device__ inline int64_t draft_row_groups(const DraftReq& r, int G, int R) {
-  return (r.n * (int64_t)G + R - 1) / R;
+__host__ __device__ inline int draft_row_groups(const DraftReq& r, int G, int R) {
+  return (int)((r.n * (int64_t)G + R - 1) / R);
 }
-// Tiles of a chunk, from the tiles of all groups of rows: the same for every
-// request, a multiple of the block's 4 waves, two tiles a wave at least.
-__host__ __device__ inline int draft_chunk(int64_t tiles, int target) {
+// Pieces of work of a request: groups of rows times pieces of each.  A call
+// has at most 2^24 (kDraftMaxUnits); damaged lengths that claim more are cut
+// there, so that a wave's sums stay in 32 bits.
+constexpr int kDraftMaxUnits = 1 << 24;
+__host__ __device__ inline int draft_pieces(int each, int groups) {
+  const int64_t n = (int64_t)each * groups;
+  return n < kDraftMaxUnits ? (int)n : kDraftMaxUnits;
+}
+// Tiles of a chunk, from the tiles of all groups of rows (an fp32 sum, raised
+// by more than its rounding: the workspace is sized for the exact one): the
+// same for every request, a multiple of the block's 4 waves, two tiles a wave
+// at least.
+__host__ __device__ inline int draft_chunk(float tiles, int target) {
   if (target <= 0) return 1 << 30;
-  int64_t c = (tiles + target - 1) / target;
-  c = (c + 3) / 4 * 4;
-  return (int)(c < 8 ? 8 : c > (1 << 30) ? (1 << 30) : c);
+  const float c = tiles * 1.0001f / target;
+  return c > (float)(1 << 29) ? 1 << 30 : c <= 8.f ? 8 : ((int)c + 4) / 4 * 4;
 }
 __host__ __device__ inline int draft_chunks(int tiles, int chunk) {
   const int n = (int)(((int64_t)tiles + chunk - 1) / chunk);

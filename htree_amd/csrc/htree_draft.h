@@ -33,6 +33,7 @@ struct DraftArgs {
   int32_t B, rows, H, Hkv, G, Dk, Dv, width, page_shift, num_pages;
   int32_t target;  // units to split into (0: one unit per group of rows)
   float c, inv_c;  // |scale| * log2(e), not 0
+  int32_t one_round;  // the join's blocks take one piece of work each
   int32_t negate;  // the scale is negative: the queries change sign
 };
 
@@ -100,80 +101,84 @@ __device__ __forceinline__ uint2 draft_read_tr(uint32_t at) {
                                        (__attribute__((address_space(3))) s16x4*)(uintptr_t)at));
 }
 
-__device__ __forceinline__ int64_t wave_sum64(int64_t x) {
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) x += __shfl_xor((long long)x, m);
-  return x;
-}
-
 __device__ __forceinline__ DraftReq draft_request(const DraftArgs& a, int b) {
   return draft_req(a.starts[b], a.starts[b + 1], a.lens[b], a.rows);
 }
 
-// The unit of this block.  Every wave works it out from the lengths: with
+// Where a block's work is.  Every wave works it out from the lengths: with
 // `target` units wanted, a chunk is the same number of tiles everywhere, so a
 // long request gets more units than a short one.  The requests whose tokens
 // make more than one chunk get workspace slots, one per unit.
 struct DraftUnit {
-  int b, h, rt, ch, nch;
-  int chunk;     // tiles of a chunk
-  int64_t slot;  // of the request's first unit; -1 with one chunk
+  int b, nch;
+  int chunk;   // tiles of a chunk
+  int slot;    // of the request's first unit
+  int index;   // of the work within the request
+  int groups;  // of rows, of one KV head
 };
 
-template <int KT, int R>
-__device__ __forceinline__ bool draft_unit(const DraftArgs& a, int64_t u, bool groups, DraftUnit* o) {
+// The u-th piece of work where each group of rows of a request of `nch`
+// chunks makes per(nch) pieces; false past the last.
+template <int KT, int R, typename F>
+__device__ __forceinline__ bool draft_find(const DraftArgs& a, int64_t u, DraftUnit* o, F per) {
   const int lane = threadIdx.x & 63;
   const int cap = a.width << a.page_shift;
-  int64_t w = 0;
+  float w = 0.f;
   if (a.target > 0) {
     for (int b = lane; b < a.B; b += 64) {
       const DraftReq r = draft_request(a, b);
-      w += draft_tiles(r, cap, KT) * draft_row_groups(r, a.G, R);
+      w += (float)draft_tiles(r, cap, KT) * draft_row_groups(r, a.G, R);
     }
-    w = wave_sum64(w) * a.Hkv;
+    w = add_xor32(add_xor16(row_sum16(w))) * a.Hkv;
   }
   const int chunk = draft_chunk(w, a.target);
   int64_t first = 0, slot = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
     const int b = b0 + lane;
-    int nch = 0;
-    int64_t rt = 0;
+    int nch = 0, rt = 0;
     if (b < a.B) {
       const DraftReq r = draft_request(a, b);
       nch = draft_chunks(draft_tiles(r, cap, KT), chunk);
       rt = draft_row_groups(r, a.G, R) * a.Hkv;
     }
-    // units of a request; with `groups` set only those of split requests
-    // count, one for each group of rows
-    const int64_t mine = groups ? (nch > 1 ? rt : 0) : nch * rt;
-    const int64_t sl = nch > 1 ? nch * rt : 0;
-    int64_t pu = mine, ps = sl;
+    const int mine = draft_pieces(per(nch), rt), sl = draft_pieces(nch > 1 ? nch : 0, rt);
+    int pu = mine, ps = sl;
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) {
-      const int64_t x = __shfl_up((long long)pu, m), y = __shfl_up((long long)ps, m);
+      const int x = __shfl_up(pu, m), y = __shfl_up(ps, m);
       if (lane >= m) pu += x, ps += y;
     }
     const uint64_t hit = __ballot(first + pu > u);
     if (hit) {
       const int l = __builtin_ctzll(hit);
       o->b = b0 + l;
-      o->nch = uniform(__shfl(nch, l));
-      const int64_t before = first + __shfl((long long)(pu - mine), l);
-      const int64_t rts = __shfl((long long)rt, l);
-      o->slot = o->nch > 1 ? slot + __shfl((long long)(ps - sl), l) : -1;
+      o->nch = __builtin_amdgcn_readlane(nch, l);
       o->chunk = chunk;
-      // KV head fastest, then row group, then chunk
-      const int64_t i = u - before;
-      o->h = uniform((int)(i % a.Hkv));
-      const int64_t rest = i / a.Hkv, nrt = rts / a.Hkv;
-      o->rt = uniform((int)(rest % nrt));
-      o->ch = uniform((int)(rest / nrt));
+      o->slot = (int)slot + __builtin_amdgcn_readlane(ps - sl, l);
+      o->index = (int)(u - first) - __builtin_amdgcn_readlane(pu - mine, l);
+      o->groups = __builtin_amdgcn_readlane(rt, l) / a.Hkv;
       return true;
     }
-    first += __shfl((long long)pu, 63);
-    slot += __shfl((long long)ps, 63);
+    first += __builtin_amdgcn_readlane(pu, 63);
+    slot += __builtin_amdgcn_readlane(ps, 63);
   }
   return false;
+}
+
+// A unit: KV head h (fastest), group of rows rt, chunk ch of a request
+struct DraftPart {
+  int h, rt, ch;
+  int slot;  // -1: the request has one chunk
+};
+template <int KT, int R>
+__device__ __forceinline__ bool draft_unit(const DraftArgs& a, DraftUnit* u, DraftPart* p) {
+  if (!draft_find<KT, R>(a, blockIdx.x, u, [](int nch) { return nch; })) return false;
+  const uint32_t rest = (uint32_t)u->index / (uint32_t)a.Hkv;
+  p->h = uniform(u->index - rest * a.Hkv);
+  p->ch = uniform(rest / (uint32_t)u->groups);
+  p->rt = uniform(rest - p->ch * u->groups);
+  p->slot = u->nch > 1 ? u->slot + u->index : -1;
+  return true;
 }
 
 // 4 consecutive dims of a lane's row: dims dim(q) .. dim(q) + 3, from the
@@ -256,18 +261,18 @@ struct DraftPages {
   }
 };
 template <int KT, int R>
-__device__ __forceinline__ DraftCtx draft_ctx(const DraftArgs& a, const DraftUnit& u, const DraftReq& rq) {
+__device__ __forceinline__ DraftCtx draft_ctx(const DraftArgs& a, const DraftUnit& u, const DraftPart& p, const DraftReq& rq) {
   DraftCtx c;
   c.s0 = uniform(rq.s0), c.ctx = uniform(rq.ctx);
   c.shift = a.page_shift;
   c.nrow = uniform(rq.n * a.G);
-  const DraftSpan sp = draft_span(rq, u.rt * R, R, a.G, a.width << a.page_shift, KT, u.ch, u.chunk);
+  const DraftSpan sp = draft_span(rq, p.rt * R, R, a.G, a.width << a.page_shift, KT, p.ch, u.chunk);
   c.kend = uniform(sp.kend), c.t0 = uniform(sp.t0), c.t1 = uniform(sp.t1);
   c.used = (c.kend + (1 << c.shift) - 1) >> c.shift;
   // rows behind the request's last see nothing, but are not stored either
-  c.full = min(a.parents ? c.ctx : c.ctx + u.rt * R / a.G + 1, c.kend);
-  c.kh = a.k + u.h * a.k_head;
-  c.vh = a.v + u.h * a.v_head;
+  c.full = min(a.parents ? c.ctx : c.ctx + p.rt * R / a.G + 1, c.kend);
+  c.kh = a.k + p.h * a.k_head;
+  c.vh = a.v + p.h * a.v_head;
   c.tab = a.table + u.b * a.table_stride;
   c.par = a.parents ? a.parents + c.s0 : nullptr;
   return c;
@@ -651,13 +656,14 @@ __global__ __launch_bounds__(256, (MT == 1 && D <= 128) ? 2 : 1) void draft_kern
   __shared__ float ml[NW][R][2];
 
   DraftUnit u;
-  if (!draft_unit<KT, R>(a, blockIdx.x, false, &u)) return;  // uniform over the block
+  DraftPart part;
+  if (!draft_unit<KT, R>(a, &u, &part)) return;  // uniform over the block
   const int lane = threadIdx.x & 63, wv = uniform(threadIdx.x >> 6);
   const DraftReq rq = draft_request(a, u.b);
-  const DraftCtx c = draft_ctx<KT, R>(a, u, rq);
-  const int row0 = u.rt * R;
+  const DraftCtx c = draft_ctx<KT, R>(a, u, part, rq);
+  const int row0 = part.rt * R;
   DraftWave<T, D, MT, KT> w;
-  w.init(a, c, u.h, row0);
+  w.init(a, c, part.h, row0);
 
   char* kb = lds + wv * WAVE_LDS;
   char* vb = kb + KT * ROWB;
@@ -743,9 +749,9 @@ __global__ __launch_bounds__(256, (MT == 1 && D <= 128) ? 2 : 1) void draft_kern
   }
   bool odd = false;  // a token with infinite or NaN values was met
   for (; t < c.t1; t += NW) {
-    const bool part = masked();
+    const bool some = masked();
     uint64_t there = 0;
-    if (part) {
+    if (some) {
       there = exist();
       // Values that a row does not see must not meet the product: 0 x NaN is
       // NaN.  Zeros take the place of those that no row sees, and of
@@ -761,7 +767,7 @@ __global__ __launch_bounds__(256, (MT == 1 && D <= 128) ? 2 : 1) void draft_kern
     }
     stage();
     typename DraftWave<T, D, MT, KT>::Weights wt;
-    w.scores(a, c, kb, t * KT, part, there, wt);
+    w.scores(a, c, kb, t * KT, some, there, wt);
     w.values(vb, wt);
     wave_sync();  // this tile's reads come before the next one's writes
   }
@@ -788,7 +794,7 @@ __global__ __launch_bounds__(256, (MT == 1 && D <= 128) ? 2 : 1) void draft_kern
     }
   }
   __syncthreads();
-  const int64_t slot = u.nch > 1 ? u.slot + (u.ch * draft_row_groups(rq, a.G, R) + u.rt) * a.Hkv + u.h : -1;
+  const int64_t slot = part.slot;
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
     float mm = -INFINITY;
@@ -819,7 +825,7 @@ __global__ __launch_bounds__(256, (MT == 1 && D <= 128) ? 2 : 1) void draft_kern
           a.ws_ml[(slot * R + rr) * 2 + 1] = sum;
         }
       } else {
-        draft_store<T>(a, c.s0, u.h, row0 + rr, ch, x, sum);
+        draft_store<T>(a, c.s0, part.h, row0 + rr, ch, x, sum);
       }
     }
     __syncthreads();
@@ -842,13 +848,14 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void draft_rows_kernel(D
   __shared__ int odds[NW];
 
   DraftUnit u;
-  if (!draft_unit<KT, R>(a, blockIdx.x, false, &u)) return;  // uniform over the block
+  DraftPart part;
+  if (!draft_unit<KT, R>(a, &u, &part)) return;  // uniform over the block
   const int lane = threadIdx.x & 63, wv = uniform(threadIdx.x >> 6);
   const DraftReq rq = draft_request(a, u.b);
-  const DraftCtx c = draft_ctx<KT, R>(a, u, rq);
-  const int row0 = u.rt * R + wv * 16 * MT;
+  const DraftCtx c = draft_ctx<KT, R>(a, u, part, rq);
+  const int row0 = part.rt * R + wv * 16 * MT;
   DraftWave<T, D, MT, KT> w;
-  w.init(a, c, u.h, row0);
+  w.init(a, c, part.h, row0);
 
   const int lr = lane / CPR, lc = lane % CPR;
   const bool kin = lc * 16 < a.Dk * S::ES, vin = lc * 16 < a.Dv * S::ES;
@@ -926,9 +933,9 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void draft_rows_kernel(D
   own = mine(t + 1);
   bool odd = false;  // this wave staged a token with infinite or NaN values
   for (; t < c.t1; ++t) {
-    const bool part = masked();
+    const bool some = masked();
     uint64_t there = 0;
-    if (part) {
+    if (some) {
       there = exist();
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
@@ -941,7 +948,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void draft_rows_kernel(D
     }
     stage();
     typename DraftWave<T, D, MT, KT>::Weights wt;
-    if (on) w.scores(a, c, kb, t * KT, part, there, wt);
+    if (on) w.scores(a, c, kb, t * KT, some, there, wt);
     // only now, when the scores' registers are free
     if (t + 1 < c.t1) load_v(t + 1, own);
     own = mine(t + 2);
@@ -965,7 +972,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void draft_rows_kernel(D
   }
   __syncthreads();
 
-  const int64_t slot = u.nch > 1 ? u.slot + (u.ch * draft_row_groups(rq, a.G, R) + u.rt) * a.Hkv + u.h : -1;
+  const int64_t slot = part.slot;
   float* my = (float*)lds + wv * 16 * D;
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
@@ -987,58 +994,83 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void draft_rows_kernel(D
           a.ws_ml[at * 2 + 1] = sum;
         }
       } else {
-        draft_store<T>(a, c.s0, u.h, r, ch, x, sum);
+        draft_store<T>(a, c.s0, part.h, r, ch, x, sum);
       }
     }
     wave_sync();
   }
 }
 
-// Joins the chunks of split requests: one block per row, the threads split
-// over the chunks and the row's dims.
+// Joins the chunks of split requests.  The threads of a block are NP sets of
+// D / 4, a set holding a row.  Few chunks: each set takes a row and all its
+// chunks; many: the block takes a row and its sets share the chunks.
+constexpr int kJoinSerial = 16;
 template <typename T, int D, int KT, int R>
 __global__ __launch_bounds__(256) void draft_join_kernel(DraftArgs a) {
-  constexpr int OC = D / 4, NP = 256 / OC;  // chunks taken at a time
+  constexpr int OC = D / 4, NP = 256 / OC, RB = R / NP > 1 ? R / NP : 1;
   __shared__ f32x4 acc[256];
   __shared__ float lsum[NP];
-  DraftUnit u;
-  if (!draft_unit<KT, R>(a, blockIdx.x / R, true, &u)) return;
-  const int rr = blockIdx.x % R;
-  const DraftReq rq = draft_request(a, u.b);
-  const int r = u.rt * R + rr;
-  if (r >= rq.n * a.G) return;
-  const int64_t base = u.slot + (int64_t)u.rt * a.Hkv + u.h, step = draft_row_groups(rq, a.G, R) * a.Hkv;
   const int tid = threadIdx.x, p = tid / OC, ch = tid % OC;
-  float big = -INFINITY;
-  for (int c = tid & 63; c < u.nch; c += 64) big = fmaxf(big, a.ws_ml[((base + c * step) * R + rr) * 2]);
-  big = wave_max(big);
-  f32x4 x = {0.f, 0.f, 0.f, 0.f};
-  float sum = 0.f;
-#pragma unroll 4
-  for (int c = p; c < u.nch; c += NP) {
-    const int64_t at = (base + c * step) * R + rr;
-    const float mc = a.ws_ml[at * 2], lc = a.ws_ml[at * 2 + 1];
-    const f32x4 oc = *(const f32x4*)(a.ws_o + at * D + ch * 4);
-    // a chunk whose tokens the row does not see has max -inf and zeros
-    const float f = mc == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mc - big);
-    x += oc * f;
-    sum += lc * f;
-  }
-  acc[tid] = x;
-  if (ch == 0) lsum[p] = sum;
-  __syncthreads();
-  if (p == 0) {
-#pragma unroll
-    for (int i = 1; i < NP; ++i) {
-      x += acc[i * OC + ch];
-      sum += lsum[i];
+  for (int64_t at = blockIdx.x;; at += gridDim.x) {
+    DraftUnit u;
+    if (!draft_find<KT, R>(a, at, &u, [](int nch) { return nch <= 1 ? 0 : nch <= kJoinSerial ? RB : R; }))
+      return;  // uniform over the block
+    const DraftReq rq = draft_request(a, u.b);
+    const bool serial = u.nch <= kJoinSerial;
+    const int per = serial ? RB : R, sub = u.index % per;
+    const int group = u.index / per, h = group % a.Hkv, rt = group / a.Hkv;
+    const int rr = serial ? sub * NP + p : sub, r = rt * R + rr, nrow = rq.n * a.G;
+    // (rows of a block ascend: the first one behind the last ends it)
+    if (rt * R + (serial ? sub * NP : sub) >= nrow) {
+      if (a.one_round) return;
+      continue;
     }
-    draft_store<T>(a, rq.s0, u.h, r, ch, x, sum);
+    const bool on = rr < R && r < nrow;
+    const int64_t base = u.slot + (int64_t)rt * a.Hkv + h, step = (int64_t)u.groups * a.Hkv;
+    const int c0 = serial ? 0 : p, dc = serial ? 1 : NP;
+    float big = -INFINITY;
+    if (on) {
+      if (serial) {
+        for (int c = 0; c < u.nch; ++c) big = fmaxf(big, a.ws_ml[((base + c * step) * R + rr) * 2]);
+      } else {
+        for (int c = tid & 63; c < u.nch; c += 64) big = fmaxf(big, a.ws_ml[((base + c * step) * R + rr) * 2]);
+      }
+    }
+    if (!serial) big = wave_max(big);
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+    float sum = 0.f;
+    if (on) {
+#pragma unroll 4
+      for (int c = c0; c < u.nch; c += dc) {
+        const int64_t i = (base + c * step) * R + rr;
+        const float mc = a.ws_ml[i * 2], lc = a.ws_ml[i * 2 + 1];
+        const f32x4 oc = *(const f32x4*)(a.ws_o + i * D + ch * 4);
+        // a chunk whose tokens the row does not see has max -inf and zeros
+        const float f = mc == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mc - big);
+        x += oc * f;
+        sum += lc * f;
+      }
+    }
+    if (!serial) {
+      acc[tid] = x;
+      if (ch == 0) lsum[p] = sum;
+      __syncthreads();
+      if (p == 0) {
+#pragma unroll
+        for (int i = 1; i < NP; ++i) {
+          x += acc[i * OC + ch];
+          sum += lsum[i];
+        }
+      }
+      __syncthreads();
+    }
+    if (on && (serial || p == 0)) draft_store<T>(a, rq.s0, h, r, ch, x, sum);
+    if (a.one_round) return;
   }
 }
 
 template <typename T, int D, int MT, int NW>
-int draft_launch(const DraftArgs& a, int64_t units, int64_t groups, hipStream_t st) {
+int draft_launch(const DraftArgs& a, int64_t units, int64_t joins, hipStream_t st) {
   constexpr int KT = draft_tile(D, (int)sizeof(T), NW), R = 16 * MT * NW;
   if constexpr (NW == 1)
     hipLaunchKernelGGL((draft_kernel<T, D, MT>), dim3((unsigned)units), dim3(256), 0, st, a);
@@ -1046,8 +1078,8 @@ int draft_launch(const DraftArgs& a, int64_t units, int64_t groups, hipStream_t 
     hipLaunchKernelGGL((draft_rows_kernel<T, D, MT, NW, KT>), dim3((unsigned)units), dim3(64 * NW), 0, st, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return (int)e;
-  if (groups > 0) {
-    hipLaunchKernelGGL((draft_join_kernel<T, D, KT, R>), dim3((unsigned)(groups * R)), dim3(256), 0, st, a);
+  if (joins > 0) {
+    hipLaunchKernelGGL((draft_join_kernel<T, D, KT, R>), dim3((unsigned)joins), dim3(256), 0, st, a);
     e = hipGetLastError();
   }
   return e == hipSuccess ? HTREE_OK : (int)e;
@@ -1059,12 +1091,12 @@ int draft_launch_type(const DraftArgs& a, const DraftPlan& p, hipStream_t st);
 template <typename T, int D>
 int draft_launch_dim(const DraftArgs& a, const DraftPlan& p, hipStream_t st) {
   constexpr DraftForm f = draft_rows_form(D, (int)sizeof(T));
-  if (p.NW > 1) return draft_launch<T, D, f.MT, f.NW>(a, p.units, p.groups, st);
-  if (p.MT == 1) return draft_launch<T, D, 1, 1>(a, p.units, p.groups, st);
+  if (p.NW > 1) return draft_launch<T, D, f.MT, f.NW>(a, p.units, p.joins, st);
+  if (p.MT == 1) return draft_launch<T, D, 1, 1>(a, p.units, p.joins, st);
   if constexpr (D <= 128) {
-    if (p.MT == 4) return draft_launch<T, D, 4, 1>(a, p.units, p.groups, st);
+    if (p.MT == 4) return draft_launch<T, D, 4, 1>(a, p.units, p.joins, st);
   }
-  return draft_launch<T, D, 2, 1>(a, p.units, p.groups, st);
+  return draft_launch<T, D, 2, 1>(a, p.units, p.joins, st);
 }
 
 #define HTREE_DRAFT_TYPE(T)                                                        \

@@ -4,12 +4,21 @@ The cache, block tables and slots are cache.py's."""
 from __future__ import annotations
 
 import ctypes
+from functools import lru_cache
 from typing import Optional
 
 import torch
 
 from . import _native as N
 from .cache import MAX_REQUEST_TOKENS, _ints, aligned_rows, check_table, native_cache
+
+
+@lru_cache(maxsize=256)
+def _workspace_bytes(sizes, B: int, rows: int, H: int, width: int) -> int:
+    n = ctypes.c_int64()
+    N.check(N.lib().htree_draft_attention_workspace_bytes(N.HtreeCache(*sizes), B, rows, H, width, n),
+            "htree_draft_attention_workspace_bytes")
+    return n.value
 
 
 def draft_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -37,44 +46,43 @@ def draft_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     Results do not depend on the other requests' values, but a request's
     split, and so the last bits, depends on all lengths."""
     c = native_cache(k_cache, v_cache)
-    dev = k_cache.device
+    dtype, dev = k_cache.dtype, k_cache.device
     assert q.dim() == 3, "q must be [rows, H, K]"
     rows, H, K = q.shape
     assert K == c.Dk, f"q and the cache must share the head dim K ({K} vs {c.Dk})"
     assert H > 0 and H % c.H_kv == 0, f"H ({H}) must be divisible by H_kv ({c.H_kv})"
-    assert q.dtype == k_cache.dtype, "q and the cache must share one dtype"
+    assert q.dtype is dtype, "q and the cache must share one dtype"
     assert q.device == dev, "q and the cache must be on one device"
     assert lens.dim() == 1, "lens must be int32 [B]"
     B = lens.shape[0]
-    _ints(lens, "lens", (B,), dev)
-    _ints(starts, "starts", (B + 1,), dev)
+    _ints(lens, "lens", B, dev)
+    _ints(starts, "starts", B + 1, dev)
     check_table(block_table, B, dev)
     width = block_table.shape[1]
     assert width * c.page_size <= MAX_REQUEST_TOKENS, \
         f"a request's table holds at most {MAX_REQUEST_TOKENS} tokens, got {width * c.page_size}"
     if parents is not None:
-        _ints(parents, "parents", (rows,), dev)
-    assert not (torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad
-                                             or v_cache.requires_grad)), "draft_attention has no backward"
+        _ints(parents, "parents", rows, dev)
+    if torch.is_grad_enabled():
+        assert not (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad), \
+            "draft_attention has no backward"
     if out is None:
-        out = torch.empty(rows, H, c.Dv, dtype=q.dtype, device=dev)
+        out = torch.empty((rows, H, c.Dv), dtype=dtype, device=dev)
     else:
-        assert out.shape == (rows, H, c.Dv) and out.dtype == q.dtype and out.is_contiguous() \
+        assert out.shape == (rows, H, c.Dv) and out.dtype is dtype and out.is_contiguous() \
             and out.device == dev and out.data_ptr() % 16 == 0, \
-            f"out must be a contiguous {q.dtype} tensor [{rows}, {H}, {c.Dv}] on {dev}"
+            f"out must be a contiguous {dtype} tensor [{rows}, {H}, {c.Dv}] on {dev}"
     if B == 0 or rows == 0:
         return out
     q = aligned_rows(q)
-    L = N.lib()
-    nbytes = ctypes.c_int64()
-    N.check(L.htree_draft_attention_workspace_bytes(c, B, rows, H, width, nbytes),
-            "htree_draft_attention_workspace_bytes")
-    with torch.cuda.device(dev):
-        ws = torch.empty(nbytes.value, dtype=torch.uint8, device=dev) if nbytes.value else None
-        rc = L.htree_draft_attention(
-            c, B, rows, H, width, block_table.stride(0), K ** -0.5 if scale is None else float(scale),
-            N.ptr(q), q.stride(0), q.stride(1), N.ptr(k_cache), N.ptr(v_cache), N.ptr(block_table),
-            N.ptr(lens), N.ptr(starts), N.ptr(parents), N.ptr(out), out.stride(0), out.stride(1),
-            N.ptr(ws), nbytes.value, N.stream_ptr(dev))
-    N.check(rc, "htree_draft_attention")
+    q_row, q_head, _ = q.stride()
+    nbytes = _workspace_bytes((c.dtype, c.H_kv, K, c.Dv, c.page_size, c.num_pages, c.k_page, c.k_token, c.k_head,
+                               c.v_page, c.v_token, c.v_head), B, rows, H, width)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    rc = N.launch(N.lib().htree_draft_attention, dev, c, B, rows, H, width, block_table.stride(0),
+                  K ** -0.5 if scale is None else float(scale), q.data_ptr(), q_row, q_head, k_cache.data_ptr(),
+                  v_cache.data_ptr(), block_table.data_ptr(), lens.data_ptr(), starts.data_ptr(), N.address(parents),
+                  out.data_ptr(), H * c.Dv, c.Dv, N.address(ws), nbytes)
+    if rc:
+        N.check(rc, "htree_draft_attention")
     return out

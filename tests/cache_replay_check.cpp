@@ -52,21 +52,21 @@ int main() {
     CHECK(p.bytes == p.slots * p.R * (p.D + 2) * 4);
     const int KT = draft_tile(p.D, es, p.NW);
     CHECK(KT >= 16 && KT <= 64 && KT % 16 == 0);
-    int64_t tiles = 0;
+    float tiles = 0;
     std::vector<DraftReq> rq;
     for (int b = 0; b < B; ++b) {
       rq.push_back(draft_req(starts[b], starts[b + 1], lens[b], rows));
       const DraftReq& r = rq[b];
       CHECK(r.s0 >= 0 && r.n >= 0 && r.s0 + r.n <= rows && r.len >= 0);
-      tiles += draft_tiles(r, cap, KT) * draft_row_groups(r, G, p.R);
+      tiles += (float)draft_tiles(r, cap, KT) * draft_row_groups(r, G, p.R);
     }
     const int chunk = draft_chunk(tiles * Hkv, p.target);
-    int64_t units = 0, slots = 0, groups = 0;
+    int64_t units = 0, slots = 0;
     for (const DraftReq& r : rq) {
       const int nt = draft_tiles(r, cap, KT), nch = draft_chunks(nt, chunk);
       const int64_t rts = draft_row_groups(r, G, p.R);
-      units += nch * rts * Hkv;
-      if (nch > 1) slots += nch * rts * Hkv, groups += rts * Hkv;
+      units += draft_pieces(nch, (int)(rts * Hkv));
+      if (nch > 1) slots += draft_pieces(nch, (int)(rts * Hkv));
       for (int64_t rt = 0; rt < rts; rt += rts > 40 ? 1 + upto(9) : 1) {
         int next = 0;
         const DraftSpan whole = draft_span(r, rt * p.R, p.R, G, cap, KT, 0, 1 << 30);
@@ -104,10 +104,8 @@ int main() {
       }
     }
     CHECK(slots <= p.slots);
-    if (ascend) {
-      CHECK(units <= p.units);
-      CHECK(groups <= p.groups);
-    }
+    if (ascend) CHECK(units <= p.units);
+    CHECK((p.joins > 0) == (p.target > 0));
     // page tables: the new pages are those the launch has blocks for
     for (int b = 0; b < B; ++b) {
       const int64_t ctx = lens[b] < 0 ? 0 : lens[b], n = rq[b].n;
