@@ -432,6 +432,7 @@ extern "C" int htree_draft_attention(const htree_cache* c, int32_t B, int32_t ro
   a.B = B, a.rows = rows, a.H = H, a.Hkv = c->H_kv, a.G = H / c->H_kv, a.Dk = c->Dk, a.Dv = c->Dv;
   a.width = table_width, a.page_shift = log2i(c->page_size), a.num_pages = c->num_pages;
   a.target = p.target;
+  a.near = p.near;
   a.one_round = p.one_round;
   a.negate = scale < 0.f;
   a.c = fmaxf(fabsf(scale) * kLog2e, 1e-37f);  // a scale of 0 still multiplies -inf

@@ -31,11 +31,15 @@ __host__ __device__ constexpr int draft_tile(int D, int es, int NW = 1) {
                                                     : (NW > 1 ? 16384 : 8192) / (D * es);
 }
 
+// whether two blocks of the form with common rows fit a CU (256 registers a lane)
+__host__ __device__ constexpr bool draft_two(int D, int MT) { return D * MT <= 128; }
+
 // A call's split.  Units: blocks of the launch, R rows of a request and KV
 // head each.  Joins: blocks of the second launch, which joins the units of the
 // same rows and takes as many rounds as there are rows.
 struct DraftPlan {
   int D, MT, NW, R;
+  int near;    // groups of rows of a request, on average
   int target;  // units to split into (0: one unit per group of rows)
   bool one_round;  // every piece of the join has a block of its own
   int64_t units, joins, slots, bytes;  // at most
@@ -47,18 +51,20 @@ __host__ __device__ inline DraftPlan draft_plan(int Dk, int Dv, int es, int B, i
   p.D = m <= 32 ? 32 : m <= 64 ? 64 : m <= 128 ? 128 : 256;
   const int G = H / Hkv;
   const int64_t per = ((int64_t)rows * G + B - 1) / B;  // rows of a request, on average
-  p.MT = per <= 16 ? 1 : per <= 32 || p.D == 256 ? 2 : 4;
+  p.MT = per <= 16 ? 1 : per <= 32 || p.D == 256 ? 2 : es == 4 ? 3 : 4;
   p.NW = 1;
-  if (per > 64) {
+  if (per > 64 && es == 2) {
     const DraftForm f = draft_rows_form(p.D, es);
     p.MT = f.MT, p.NW = f.NW;
   }
   p.R = 16 * p.MT * p.NW;
   const int64_t rts = ((int64_t)rows * G / p.R + B) * Hkv;
   // blocks that fit the GPU at once
-  const int full = (p.NW > 1 || p.MT == 1) && p.D <= 128 ? 512 : 256;
+  const int full = (p.NW > 1 ? p.D <= 128 : draft_two(p.D, p.MT)) ? 512 : 256;
   p.target = (int64_t)width * page_size <= 1024 ? 0 : full;
-  p.units = rts + p.target;
+  p.near = (int)((per + p.R - 1) / p.R);
+  p.near = p.near > 64 ? 64 : p.near;
+  p.units = (rts + p.target + 8 * p.near - 1) / (8 * p.near) * (8 * p.near);
   // a group of rows makes R pieces of joining at most
   p.one_round = rts * p.R <= 1024;
   p.joins = p.target == 0 ? 0 : p.one_round ? rts * p.R : 1024;
@@ -66,6 +72,13 @@ __host__ __device__ inline DraftPlan draft_plan(int Dk, int Dv, int es, int B, i
   p.slots = 2 * (int64_t)p.target;
   p.bytes = p.slots * p.R * (p.D + 2) * 4;
   return p;
+}
+
+// The unit of block x: of 8 near blocks in a row, those 8 apart take `near`
+// units in a row.
+__host__ __device__ inline int64_t draft_near(int64_t x, int near) {
+  const int64_t all = 8 * (int64_t)near, y = x % all;
+  return x - y + y % 8 * near + y / 8;
 }
 
 // A request's lengths, held to what the buffers have
@@ -91,6 +104,12 @@ __host__ __device__ inline int draft_tiles(const DraftReq& r, int cap, int KT) {
 __host__ __device__ inline int draft_row_groups(const DraftReq& r, int G, int R) {
   return (int)((r.n * (int64_t)G + R - 1) / R);
 }
+// Rows of each of them: even parts of the request's, in whole 16 MT of a wave
+// (`step`), so that no group is left with a few rows and the time of a full one.
+__host__ __device__ inline int draft_even(const DraftReq& r, int G, int R, int step) {
+  const int n = r.n * G, groups = draft_row_groups(r, G, R);
+  return groups <= 1 ? R : ((n + groups - 1) / groups + step - 1) / step * step;
+}
 // Pieces of work of a request: groups of rows times pieces of each.  A call
 // has at most 2^24 (kDraftMaxUnits); damaged lengths that claim more are cut
 // there, so that a wave's sums stay in 32 bits.
@@ -106,10 +125,17 @@ __host__ __device__ inline int draft_pieces(int each, int groups) {
 __host__ __device__ inline int draft_chunk(float tiles, int target) {
   if (target <= 0) return 1 << 30;
   const float c = tiles * 1.0001f / target;
-  return c > (float)(1 << 29) ? 1 << 30 : c <= 8.f ? 8 : ((int)c + 4) / 4 * 4;
+  return c > (float)(1 << 29) ? 1 << 30 : ((int)c + 4) / 4 * 4;
 }
+__host__ __device__ inline int draft_wider(int chunk) { return chunk + chunk / 16 + 1; }
+// chunks of a request, and tiles of each: even parts
 __host__ __device__ inline int draft_chunks(int tiles, int chunk) {
   const int n = (int)(((int64_t)tiles + chunk - 1) / chunk);
+  return n < 1 ? 1 : n;
+}
+
+__host__ __device__ inline int draft_part(int tiles, int chunks) {
+  const int n = (tiles + chunks - 1) / chunks;
   return n < 1 ? 1 : n;
 }
 
@@ -117,6 +143,7 @@ __host__ __device__ inline int draft_chunks(int tiles, int chunk) {
 struct DraftSpan {
   int kend, t0, t1;
 };
+// (rows row0 .. row0 + R - 1 of it)
 __host__ __device__ inline DraftSpan draft_span(const DraftReq& r, int64_t row0, int R, int G, int cap,
                                                 int KT, int ch, int chunk) {
   const int64_t nrow = (int64_t)r.n * G, last = (row0 + R < nrow ? row0 + R : nrow) - 1;

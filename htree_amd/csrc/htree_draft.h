@@ -31,6 +31,7 @@ struct DraftArgs {
   int64_t q_row, q_head, o_row, o_head;                                // bytes
   int64_t k_page, k_token, k_head, v_page, v_token, v_head;            // bytes
   int32_t B, rows, H, Hkv, G, Dk, Dv, width, page_shift, num_pages;
+  int32_t near;    // units that share tokens, on average
   int32_t target;  // units to split into (0: one unit per group of rows)
   float c, inv_c;  // |scale| * log2(e), not 0
   int32_t one_round;  // the join's blocks take one piece of work each
@@ -88,17 +89,9 @@ __device__ __forceinline__ int draft_swz_v(int row, int chunk) {
   return CPR >= 16 ? chunk ^ ((row & 7) << 1) : CPR == 8 ? chunk ^ (((row >> 1) & 3) << 1) : chunk ^ (((row >> 2) & 1) << 1);
 }
 
-// LDS by its 32-bit address, for addresses made by exclusive or
-__device__ __forceinline__ uint32_t draft_lds(const char* p) {
-  return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)p;
-}
-template <typename V>
-__device__ __forceinline__ V draft_read(uint32_t at) {
-  return *(const __attribute__((address_space(3))) V*)(uintptr_t)at;
-}
-__device__ __forceinline__ uint2 draft_read_tr(uint32_t at) {
+__device__ __forceinline__ uint2 draft_read_tr(const char* p) {
   return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                       (__attribute__((address_space(3))) s16x4*)(uintptr_t)at));
+                                       (__attribute__((address_space(3))) s16x4*)(const __attribute__((address_space(3))) void*)p));
 }
 
 __device__ __forceinline__ DraftReq draft_request(const DraftArgs& a, int b) {
@@ -106,12 +99,12 @@ __device__ __forceinline__ DraftReq draft_request(const DraftArgs& a, int b) {
 }
 
 // Where a block's work is.  Every wave works it out from the lengths: with
-// `target` units wanted, a chunk is the same number of tiles everywhere, so a
-// long request gets more units than a short one.  The requests whose tokens
+// `target` units wanted, a chunk is about the same number of tiles everywhere,
+// so a long request gets more units than a short one.  The requests whose tokens
 // make more than one chunk get workspace slots, one per unit.
 struct DraftUnit {
   int b, nch;
-  int chunk;   // tiles of a chunk
+  int chunk;   // tiles of each chunk
   int slot;    // of the request's first unit
   int index;   // of the work within the request
   int groups;  // of rows, of one KV head
@@ -131,14 +124,32 @@ __device__ __forceinline__ bool draft_find(const DraftArgs& a, int64_t u, DraftU
     }
     w = add_xor32(add_xor16(row_sum16(w))) * a.Hkv;
   }
-  const int chunk = draft_chunk(w, a.target);
+  int chunk = draft_chunk(w, a.target);
+  if (a.target > 0 && a.B <= 64) {
+    // A chunk somewhat larger, where the units then all fit the GPU at once:
+    // else the last few of them start when the others are done.
+    int c = chunk;
+    for (int i = 0; i < 4; ++i) {
+      float units = 0.f;
+      if (lane < a.B) {
+        const DraftReq r = draft_request(a, lane);
+        units = (float)draft_chunks(draft_tiles(r, cap, KT), c) * draft_row_groups(r, a.G, R);
+      }
+      if (add_xor32(add_xor16(row_sum16(units))) * a.Hkv <= (float)a.target) {
+        chunk = c;
+        break;
+      }
+      c = draft_wider(c);
+    }
+  }
   int64_t first = 0, slot = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
     const int b = b0 + lane;
-    int nch = 0, rt = 0;
+    int nch = 0, rt = 0, tiles = 0;
     if (b < a.B) {
       const DraftReq r = draft_request(a, b);
-      nch = draft_chunks(draft_tiles(r, cap, KT), chunk);
+      tiles = draft_tiles(r, cap, KT);
+      nch = draft_chunks(tiles, chunk);
       rt = draft_row_groups(r, a.G, R) * a.Hkv;
     }
     const int mine = draft_pieces(per(nch), rt), sl = draft_pieces(nch > 1 ? nch : 0, rt);
@@ -153,7 +164,7 @@ __device__ __forceinline__ bool draft_find(const DraftArgs& a, int64_t u, DraftU
       const int l = __builtin_ctzll(hit);
       o->b = b0 + l;
       o->nch = __builtin_amdgcn_readlane(nch, l);
-      o->chunk = chunk;
+      o->chunk = draft_part(__builtin_amdgcn_readlane(tiles, l), o->nch);
       o->slot = (int)slot + __builtin_amdgcn_readlane(ps - sl, l);
       o->index = (int)(u - first) - __builtin_amdgcn_readlane(pu - mine, l);
       o->groups = __builtin_amdgcn_readlane(rt, l) / a.Hkv;
@@ -165,18 +176,21 @@ __device__ __forceinline__ bool draft_find(const DraftArgs& a, int64_t u, DraftU
   return false;
 }
 
-// A unit: KV head h (fastest), group of rows rt, chunk ch of a request
+// A unit: group of rows rt (fastest), KV head h, chunk ch of a request.  The
+// groups of rows of one head and chunk read the same tokens: `near` units in a
+// row go to blocks of one of the 8 dies (block x runs on die x % 8), whose L2
+// then serves all but the first.
 struct DraftPart {
   int h, rt, ch;
   int slot;  // -1: the request has one chunk
 };
 template <int KT, int R>
 __device__ __forceinline__ bool draft_unit(const DraftArgs& a, DraftUnit* u, DraftPart* p) {
-  if (!draft_find<KT, R>(a, blockIdx.x, u, [](int nch) { return nch; })) return false;
-  const uint32_t rest = (uint32_t)u->index / (uint32_t)a.Hkv;
-  p->h = uniform(u->index - rest * a.Hkv);
-  p->ch = uniform(rest / (uint32_t)u->groups);
-  p->rt = uniform(rest - p->ch * u->groups);
+  if (!draft_find<KT, R>(a, draft_near(blockIdx.x, a.near), u, [](int nch) { return nch; })) return false;
+  const uint32_t rest = (uint32_t)u->index / (uint32_t)u->groups;
+  p->rt = uniform(u->index - rest * u->groups);
+  p->ch = uniform(rest / (uint32_t)a.Hkv);
+  p->h = uniform(rest - p->ch * a.Hkv);
   p->slot = u->nch > 1 ? u->slot + u->index : -1;
   return true;
 }
@@ -229,12 +243,12 @@ __device__ __forceinline__ bool draft_odd(uint4 x) {
 struct DraftCtx {
   int s0, ctx, kend, t0, t1, used, shift;
   int full;  // tokens that every row sees, where their pages exist
-  int nrow;                // rows: new tokens x heads of the group
+  int row0, nrow;          // rows (new tokens x heads of the group) from .. to
   const char *kh, *vh;     // the KV head's keys and values
   const int32_t* tab;      // the request's table
   const int32_t* par;      // its new tokens' parents, or null
 };
-// The pages of a request's tokens, asked for in ascending order: 64 entries
+// The pages of a request's tokens, mostly asked for in ascending order: 64 entries
 // of the table in a register of the wave's lanes and the next 64 on their way.
 // (Read one by one through the scalar cache they held up the LDS reads, which
 // count on the same counter.)
@@ -254,23 +268,25 @@ struct DraftPages {
   __device__ __forceinline__ int page(int key) {
     const int pi = key >> shift;
     if (pi >> 6 != at) {
-      cur = nxt;
+      cur = pi >> 6 == at + 1 ? nxt : read(pi >> 6);
       nxt = read((at = pi >> 6) + 1);
     }
     return __builtin_amdgcn_readlane(cur, pi & 63);
   }
 };
-template <int KT, int R>
+template <int KT, int R, int STEP>
 __device__ __forceinline__ DraftCtx draft_ctx(const DraftArgs& a, const DraftUnit& u, const DraftPart& p, const DraftReq& rq) {
   DraftCtx c;
   c.s0 = uniform(rq.s0), c.ctx = uniform(rq.ctx);
   c.shift = a.page_shift;
-  c.nrow = uniform(rq.n * a.G);
-  const DraftSpan sp = draft_span(rq, p.rt * R, R, a.G, a.width << a.page_shift, KT, p.ch, u.chunk);
+  const int even = draft_even(rq, a.G, R, STEP);
+  c.row0 = uniform(p.rt * even);
+  c.nrow = uniform(min(rq.n * a.G, c.row0 + even));
+  const DraftSpan sp = draft_span(rq, c.row0, even, a.G, a.width << a.page_shift, KT, p.ch, u.chunk);
   c.kend = uniform(sp.kend), c.t0 = uniform(sp.t0), c.t1 = uniform(sp.t1);
   c.used = (c.kend + (1 << c.shift) - 1) >> c.shift;
   // rows behind the request's last see nothing, but are not stored either
-  c.full = min(a.parents ? c.ctx : c.ctx + p.rt * R / a.G + 1, c.kend);
+  c.full = min(a.parents ? c.ctx : c.ctx + c.row0 / a.G + 1, c.kend);
   c.kh = a.k + p.h * a.k_head;
   c.vh = a.v + p.h * a.v_head;
   c.tab = a.table + u.b * a.table_stride;
@@ -294,6 +310,7 @@ struct DraftWave {
   using S = DraftShape<T, D>;
   using Quad = DraftQuad<T, D>;
   static constexpr int NG = KT / 16, CPR = S::CPR, ROWB = S::ROWB, NQ = S::NQ;
+  static constexpr int GROUPS = MT, TILE = KT * ROWB;  // of rows; bytes of a tile's keys
   static constexpr bool F32 = S::F32;
   int n16, g, row0;
   f32x4 qf[MT][F32 ? D / 16 : 1];
@@ -355,33 +372,26 @@ struct DraftWave {
     return j >= 0 && c.ctx + j == key;
   }
 
-  // The weights of a tile's tokens, as the second operand of the product with
-  // their values: of the values' type, fp32 for fp32.
-  struct Weights {
-    typename std::conditional<F32, f32x4, uint2>::type p[MT][NG];
-  };
-
-  // One tile of KT tokens from key0, its keys staged at kb.  masked: not every
-  // row sees every token; there: the tokens (bits) that exist.
+  // Scores of one tile of KT tokens from key0, its keys staged at kb, and the
+  // rows' max moved where they call for it.  masked: not every row sees every
+  // token; there: the tokens (bits) that exist.
   __device__ __forceinline__ void scores(const DraftArgs& a, const DraftCtx& c, const char* kb, int key0,
-                                         bool masked, uint64_t there, Weights& wt) {
+                                         bool masked, uint64_t there, f32x4 (&sc)[MT][NG]) {
     const int lane = draft_lane_again(), n16 = lane & 15, g = lane >> 4;
     // ---- scores, token x row: a lane holds tokens 4 g .. 4 g + 3 of each
     // group of 16, of row n16.  The operands come from LDS four products
     // ahead (left to itself the compiler reads each where it is used, and the
     // wave waits for every one).
-    f32x4 sc[MT][NG];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
       for (int i = 0; i < NG; ++i) sc[mt][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     {
       constexpr int NS = NG * (F32 ? D / 16 : D / 32), AHEAD = NS < 4 ? NS : 4;
-      // (rows of 16 groups and buffers begin at multiples of 16 rows: the
-      // swizzle and the piece are bits of the address of their own)
-      const uint32_t k0 = draft_lds(kb) + n16 * ROWB + draft_swz<CPR>(n16, g) * 16;
+      // (a row's swizzle and the piece's number are bits of their own)
+      const uint32_t k0 = n16 * ROWB + draft_swz<CPR>(n16, g) * 16;
       auto key = [&](int x) {  // step x: 16-byte pieces of group x % NG
-        return draft_read<f32x4>((k0 ^ (x / NG * 64)) + x % NG * 16 * ROWB);
+        return *(const f32x4*)(kb + (k0 ^ (x / NG * 64)) + x % NG * 16 * ROWB);
       };
       f32x4 f[AHEAD];
 #pragma unroll
@@ -458,37 +468,27 @@ struct DraftWave {
           for (int q = 0; q < NQ; ++q) o[mt][q] *= al;
         }
       }
-#pragma unroll
-      for (int i = 0; i < NG; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          sc[mt][i][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[mt][i][e], a.c, nm[mt]));
-          if constexpr (F32) l[mt] += sc[mt][i][e];
-        }
     }
-
-    // P rounded to the values' type: a relative half step for each of many
-    // tokens, as large as the output's own rounding at most.  The sum is taken
-    // of the rounded P too, so that the weights still add up to one.
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int i = 0; i < NG; ++i) {
-        if constexpr (F32) {
-          wt.p[mt][i] = sc[mt][i];
-        } else {
-          typedef __attribute__((ext_vector_type(4))) T T4;
-          wt.p[mt][i] = __builtin_bit_cast(uint2, __builtin_convertvector(sc[mt][i], T4));
-        }
-      }
   }
 
-  // Adds the tile's values, staged at vb.  Output, dim x row: the tokens of a
-  // product's k index are those a lane holds, so the weights' registers are
-  // its second operand as they are.
-  __device__ __forceinline__ void values(const char* vb, const Weights& wt) {
+  // The weights of the tile's tokens and their values, staged at vb.  Output,
+  // dim x row: the tokens of a product's k index are those a lane holds, so the
+  // weights' registers are its second operand as they are.
+  __device__ __forceinline__ void values(const DraftArgs& a, const char* vb, f32x4 (&sc)[MT][NG]) {
     const int lane = draft_lane_again(), n16 = lane & 15, g = lane >> 4;
+    auto weigh = [&](int mt, int i, int e) {
+      sc[mt][i][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[mt][i][e], a.c, nm[mt]));
+    };
     if constexpr (F32) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int i = 0; i < NG; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            weigh(mt, i, e);
+            l[mt] += sc[mt][i][e];
+          }
 #pragma unroll
       for (int i = 0; i < NG; ++i)
 #pragma unroll
@@ -497,19 +497,19 @@ struct DraftWave {
 #pragma unroll
           for (int q = 0; q < NQ; q += S::VW) {
             if constexpr (S::VW == 4) {
-              const f32x4 x = draft_read<f32x4>(draft_lds(vb) + row * ROWB + draft_swz_v<CPR, F32>(row, 4 * q + n16) * 16);
+              const f32x4 x = *(const f32x4*)(vb + row * ROWB + draft_swz_v<CPR, F32>(row, 4 * q + n16) * 16);
 #pragma unroll
               for (int w = 0; w < 4; ++w)
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
-                  o[mt][q + w] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[w], wt.p[mt][i][e], o[mt][q + w], 0, 0, 0);
+                  o[mt][q + w] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[w], sc[mt][i][e], o[mt][q + w], 0, 0, 0);
             } else {
-              const f32x2 x = draft_read<f32x2>(draft_lds(vb) + row * ROWB + draft_swz_v<CPR, F32>(row, n16 >> 1) * 16 + (n16 & 1) * 8);
+              const f32x2 x = *(const f32x2*)(vb + row * ROWB + draft_swz_v<CPR, F32>(row, n16 >> 1) * 16 + (n16 & 1) * 8);
 #pragma unroll
               for (int w = 0; w < 2; ++w)
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
-                  o[mt][q + w] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[w], wt.p[mt][i][e], o[mt][q + w], 0, 0, 0);
+                  o[mt][q + w] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[w], sc[mt][i][e], o[mt][q + w], 0, 0, 0);
             }
           }
         }
@@ -517,27 +517,14 @@ struct DraftWave {
       // a transposing read gives lane n16 of group g four tokens of dim n16:
       // it addresses token 4 g + n16 / 4, dims 4 (n16 % 4) ..
       const int row = 4 * g + (n16 >> 2);
-      const uint32_t v0 = draft_lds(vb) + row * ROWB + draft_swz_v<CPR, F32>(row, (n16 & 3) >> 1) * 16 + (n16 & 1) * 8;
-      auto col = [&](int i, int q) { return draft_read_tr((v0 ^ (q * 32)) + i * 16 * ROWB); };
-      constexpr uint32_t one = std::is_same<T, __bf16>::value ? 0x3f803f80u : 0x3c003c00u;
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-        if constexpr (NG == 1) {
-          sum = DraftT<T>::mma_k16(__builtin_bit_cast(s16x4, make_uint2(one, one)),
-                                   __builtin_bit_cast(s16x4, wt.p[mt][0]), sum);
-        } else {
-          using V8 = typename DraftT<T>::V8;
-#pragma unroll
-          for (int i = 0; i < NG; i += 2)
-            sum = DraftT<T>::mma(
-                __builtin_bit_cast(V8, make_uint4(one, one, one, one)),
-                __builtin_bit_cast(V8, make_uint4(wt.p[mt][i].x, wt.p[mt][i].y, wt.p[mt][i + 1].x, wt.p[mt][i + 1].y)),
-                sum);
-        }
-        l[mt] += sum[0];
-      }
-      constexpr int PG = NG == 1 ? 1 : 2, NS = NG / PG * NQ, AHEAD = NS < 4 ? NS : 4;  // groups of a product
+      const uint32_t v0 = row * ROWB + draft_swz_v<CPR, F32>(row, (n16 & 3) >> 1) * 16 + (n16 & 1) * 8;
+      auto col = [&](int i, int q) { return draft_read_tr(vb + (v0 ^ (q * 32)) + i * 16 * ROWB); };
+      // Products of PG groups of 16 tokens at a time, the operands four products
+      // ahead.  The weights of the first tokens come before them, those of the
+      // next in their shadow: a product holds the matrix unit for four times as
+      // long as it holds the wave.
+      constexpr int PG = NG == 1 ? 1 : 2, NS = NG / PG * NQ, AHEAD = NS < 4 ? NS : 4;
+      constexpr int EL = PG * 4 * MT, EPS = (EL + NQ - 1) / NQ;  // weights of a product's tokens, of a step
       uint2 f[AHEAD][PG];
       auto value = [&](int x) {  // step x: dims x % NQ, groups from x / NQ
 #pragma unroll
@@ -545,26 +532,49 @@ struct DraftWave {
       };
 #pragma unroll
       for (int x = 0; x < AHEAD; ++x) value(x);
-#pragma unroll
-      for (int x = 0; x < NS; ++x) {
-        const int q = x % NQ, i = x / NQ * PG;
+      // P rounded to the values' type: a relative half step for each of many
+      // tokens, as large as the output's own rounding at most.  The sum is taken
+      // of the rounded P too, so that the weights still add up to one.
+      uint2 p[MT][PG];
+      auto round = [&](int i0) {
+        typedef __attribute__((ext_vector_type(4))) T T4;
+        constexpr uint32_t one = std::is_same<T, __bf16>::value ? 0x3f803f80u : 0x3c003c00u;
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
-          if constexpr (PG == 1) {
-            o[mt][q] = DraftT<T>::mma_k16(__builtin_bit_cast(s16x4, f[x % AHEAD][0]),
-                                          __builtin_bit_cast(s16x4, wt.p[mt][i]), o[mt][q]);
-          } else {
-            using V8 = typename DraftT<T>::V8;
-            const uint2 y0 = f[x % AHEAD][0], y1 = f[x % AHEAD][PG - 1];
-            o[mt][q] = DraftT<T>::mma(
-                __builtin_bit_cast(V8, make_uint4(y0.x, y0.y, y1.x, y1.y)),
-                __builtin_bit_cast(V8, make_uint4(wt.p[mt][i].x, wt.p[mt][i].y, wt.p[mt][i + PG - 1].x, wt.p[mt][i + PG - 1].y)),
-                o[mt][q]);
-          }
+#pragma unroll
+          for (int y = 0; y < PG; ++y) p[mt][y] = __builtin_bit_cast(uint2, __builtin_convertvector(sc[mt][i0 + y], T4));
+          f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+          l[mt] += product(make_uint2(one, one), make_uint2(one, one), p[mt][0], p[mt][PG - 1], sum)[0];
         }
+      };
+#pragma unroll
+      for (int x = 0; x < EL; ++x) weigh(x / (PG * 4), x / 4 % PG, x % 4);
+      round(0);
+#pragma unroll
+      for (int x = 0; x < NS; ++x) {
+        const int q = x % NQ, i0 = x / NQ * PG;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+          o[mt][q] = product(f[x % AHEAD][0], f[x % AHEAD][PG - 1], p[mt][0], p[mt][PG - 1], o[mt][q]);
         if (x + AHEAD < NS) value(x + AHEAD);
+        if (i0 + PG < NG) {
+#pragma unroll
+          for (int y = q * EPS; y < (q + 1) * EPS && y < EL; ++y) weigh(y / (PG * 4), i0 + PG + y / 4 % PG, y % 4);
+        }
         __builtin_amdgcn_sched_barrier(0);
+        if (q == NQ - 1 && i0 + PG < NG) round(i0 + PG);
       }
+    }
+  }
+
+  // a product over 32 tokens (two groups of 16), or 16 where a tile has no more
+  static __device__ __forceinline__ f32x4 product(uint2 a0, uint2 a1, uint2 b0, uint2 b1, f32x4 c) {
+    if constexpr (NG == 1) {
+      return DraftT<T>::mma_k16(__builtin_bit_cast(s16x4, a0), __builtin_bit_cast(s16x4, b0), c);
+    } else {
+      using V8 = typename DraftT<T>::V8;
+      return DraftT<T>::mma(__builtin_bit_cast(V8, make_uint4(a0.x, a0.y, a1.x, a1.y)),
+                            __builtin_bit_cast(V8, make_uint4(b0.x, b0.y, b1.x, b1.y)), c);
     }
   }
 
@@ -624,6 +634,14 @@ __device__ __forceinline__ f32x4 draft_got(const float* src, int row, int ch) {
   return *(const f32x4*)(src + row * D + ((ch ^ (row & DraftShape<T, D>::OS)) << 2));
 }
 
+// The kernel's arguments, read again: what is needed after the loop over the
+// tiles is not kept in scalar registers (spilled to vector lanes) across it.
+__device__ __forceinline__ const DraftArgs& draft_args_again() {
+  auto p = (const __attribute__((address_space(4))) DraftArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const DraftArgs*)p;
+}
+
 // Whether a token's values (row vp of Dv) hold an infinite or NaN one.
 template <typename T>
 __device__ __forceinline__ bool draft_odd_row(const DraftArgs& a, const char* vp) {
@@ -647,7 +665,7 @@ __device__ __forceinline__ void draft_store(const DraftArgs& a, int s0, int h, i
 // chunk's tiles in turn, each through LDS of its own, so that there is no
 // barrier before their states meet.
 template <typename T, int D, int MT>
-__global__ __launch_bounds__(256, (MT == 1 && D <= 128) ? 2 : 1) void draft_kernel(DraftArgs a) {
+__global__ __launch_bounds__(256, draft_two(D, MT) ? 2 : 1) void draft_kernel(DraftArgs a) {
   using S = DraftShape<T, D>;
   constexpr int KT = draft_tile(D, S::ES), NG = KT / 16, CPR = S::CPR, RPI = S::RPI, R = 16 * MT;
   constexpr int NI = KT / RPI, ROWB = S::ROWB, NW = kWavesPerBlock;
@@ -660,8 +678,8 @@ __global__ __launch_bounds__(256, (MT == 1 && D <= 128) ? 2 : 1) void draft_kern
   if (!draft_unit<KT, R>(a, &u, &part)) return;  // uniform over the block
   const int lane = threadIdx.x & 63, wv = uniform(threadIdx.x >> 6);
   const DraftReq rq = draft_request(a, u.b);
-  const DraftCtx c = draft_ctx<KT, R>(a, u, part, rq);
-  const int row0 = part.rt * R;
+  const DraftCtx c = draft_ctx<KT, R, 16 * MT>(a, u, part, rq);
+  const int row0 = c.row0;
   DraftWave<T, D, MT, KT> w;
   w.init(a, c, part.h, row0);
 
@@ -766,20 +784,21 @@ __global__ __launch_bounds__(256, (MT == 1 && D <= 128) ? 2 : 1) void draft_kern
       }
     }
     stage();
-    typename DraftWave<T, D, MT, KT>::Weights wt;
-    w.scores(a, c, kb, t * KT, some, there, wt);
-    w.values(vb, wt);
+    f32x4 sc[MT][NG];
+    w.scores(a, c, kb, t * KT, some, there, sc);
+    w.values(a, vb, sc);
     wave_sync();  // this tile's reads come before the next one's writes
   }
+  const DraftArgs& z = draft_args_again();
   if (odd) {
-    DraftPages again(a, c, (c.t0 + wv) * KT);
+    DraftPages again(z, c, (c.t0 + wv) * KT);
     for (t = c.t0 + wv; t < c.t1; t += NW) {
       pages_of(again, t, ent);
       if (!masked()) continue;
       for (uint64_t left = exist(); left; left &= left - 1) {
         const int key = t * KT + __builtin_ctzll(left), p = again.page(key);
-        if (draft_odd_row<T>(a, c.vh + p * a.v_page + (key & ((1 << c.shift) - 1)) * a.v_token))
-          w.odd_token(a, c, key, p);
+        if (draft_odd_row<T>(z, c.vh + p * z.v_page + (key & ((1 << c.shift) - 1)) * z.v_token))
+          w.odd_token(z, c, key, p);
       }
     }
   }
@@ -819,32 +838,54 @@ __global__ __launch_bounds__(256, (MT == 1 && D <= 128) ? 2 : 1) void draft_kern
         sum += mj == -INFINITY ? ml[j][rr][1] : ml[j][rr][1] * __builtin_amdgcn_exp2f(mj - big);
       }
       if (slot >= 0) {
-        *(f32x4*)(a.ws_o + (slot * R + rr) * D + ch * 4) = x;
+        *(f32x4*)(z.ws_o + (slot * R + rr) * D + ch * 4) = x;
         if (ch == 0) {
-          a.ws_ml[(slot * R + rr) * 2] = big;
-          a.ws_ml[(slot * R + rr) * 2 + 1] = sum;
+          z.ws_ml[(slot * R + rr) * 2] = big;
+          z.ws_ml[(slot * R + rr) * 2 + 1] = sum;
         }
       } else {
-        draft_store<T>(a, c.s0, part.h, row0 + rr, ch, x, sum);
+        draft_store<T>(z, c.s0, part.h, row0 + rr, ch, x, sum);
       }
     }
     __syncthreads();
   }
 }
 
+// 16 bytes of each lane into LDS, from `to` on in the order of the lanes
+__device__ __forceinline__ void draft_copy16(const char* from, char* to) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, (lds_void*)to, 16, 0, 0);
+}
+
+// A tile, while the next is copied (`copy`).  The buffers do not overlap and
+// are said not to: else the reads of one wait for the copies into the other.
+template <typename W, typename F>
+__device__ __forceinline__ void draft_step(const DraftArgs& a, const DraftCtx& c, W& w, int key0, bool masked,
+                                           uint64_t there, bool on, const char* __restrict__ now,
+                                           char* __restrict__ next, F copy) {
+  copy(next);
+  if (!on) return;
+  f32x4 sc[W::GROUPS][W::NG];
+  w.scores(a, c, now, key0, masked, there, sc);
+  w.values(a, now + W::TILE, sc);
+}
+
 // Many rows: each wave of a block has 16 MT rows of its own, and all of them
-// take the same tiles, which the block stages together in one of two LDS
-// buffers while it works on the other: one barrier a tile.
+// take the same tiles, which the block copies into one of two LDS buffers
+// (directly, without registers) while it works on the other: one barrier a
+// tile.
 template <typename T, int D, int MT, int NW, int KT>
 __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void draft_rows_kernel(DraftArgs a) {
   using S = DraftShape<T, D>;
+  using W = DraftWave<T, D, MT, KT>;
   constexpr int NG = KT / 16, CPR = S::CPR, RPI = S::RPI, R = 16 * MT * NW, ROWB = S::ROWB;
-  constexpr int WR = KT / NW;       // rows that a wave stages, in one page
+  constexpr int WR = KT / NW;       // rows that a wave copies, in one page
   constexpr int NI = WR / RPI;
-  static_assert(WR <= 16 && NI >= 1 && KT <= 64, "a wave stages rows of one page");
+  static_assert(WR <= 16 && NI >= 1 && KT <= 64, "a wave copies rows of one page");
   constexpr int STAGE = 2 * KT * ROWB;
   constexpr int PUT = NW * 16 * D * 4;  // the output passes through, 16 rows of each wave
-  __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE > PUT ? 2 * STAGE : PUT];
+  constexpr int BUF = 2 * STAGE > PUT ? STAGE : PUT / 2;
+  __shared__ __attribute__((aligned(1024))) char lds0[BUF];
+  __shared__ __attribute__((aligned(1024))) char lds1[BUF];
   __shared__ int odds[NW];
 
   DraftUnit u;
@@ -852,128 +893,122 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void draft_rows_kernel(D
   if (!draft_unit<KT, R>(a, &u, &part)) return;  // uniform over the block
   const int lane = threadIdx.x & 63, wv = uniform(threadIdx.x >> 6);
   const DraftReq rq = draft_request(a, u.b);
-  const DraftCtx c = draft_ctx<KT, R>(a, u, part, rq);
-  const int row0 = part.rt * R + wv * 16 * MT;
-  DraftWave<T, D, MT, KT> w;
+  const DraftCtx c = draft_ctx<KT, R, 16 * MT>(a, u, part, rq);
+  const int row0 = c.row0 + wv * 16 * MT;
+  const bool on = row0 < c.nrow;  // the wave has rows
+  W w;
   w.init(a, c, part.h, row0);
 
   const int lr = lane / CPR, lc = lane % CPR;
-  const bool kin = lc * 16 < a.Dk * S::ES, vin = lc * 16 < a.Dv * S::ES;
-  const bool whole = a.Dk == D && a.Dv == D;
-  const uint32_t koff = lr * (uint32_t)a.k_token + (kin ? lc * 16 : 0);
-  const uint32_t voff = lr * (uint32_t)a.v_token + (vin ? lc * 16 : 0);
-  const int r0 = wv * WR;  // first of the rows this wave stages
+  const int r0 = wv * WR;  // first of the rows this wave copies
+  const int kbytes = a.Dk * S::ES, vbytes = a.Dv * S::ES;
+  if (kbytes < ROWB || vbytes < ROWB) {
+    // the places past the head dims: no copy writes them
+    for (int i = threadIdx.x * 16; i < STAGE; i += 64 * NW * 16) {
+      *(uint4*)(lds0 + i) = make_uint4(0, 0, 0, 0);
+      *(uint4*)(lds1 + i) = make_uint4(0, 0, 0, 0);
+    }
+    __syncthreads();
+  }
 
-  uint4 kr[NI], vr[NI];
-  auto load_k = [&](int t, int e) {
-    const char* p = c.kh + (int64_t)max(e, 0) * a.k_page + ((t * KT + r0) & ((1 << c.shift) - 1)) * a.k_token;
+  // Lane x of a copy writes piece x of a KB of LDS: it reads the piece that
+  // belongs there.
+  const int row1 = r0 + lr, kc1 = draft_swz<CPR>(row1, lc), vc1 = draft_swz_v<CPR, S::F32>(row1, lc);
+  const uint32_t kl = lr * (uint32_t)a.k_token, vl = lr * (uint32_t)a.v_token;
+  auto copy = [&](char* buf, int t, int e) {
+    const int at = (t * KT + r0) & ((1 << c.shift) - 1);
+    const char* kp = c.kh + (int64_t)max(e, 0) * a.k_page + at * a.k_token;
+    const char* vp = c.vh + (int64_t)max(e, 0) * a.v_page + at * a.v_token;
 #pragma unroll
-    for (int x = 0; x < NI; ++x) kr[x] = *(const uint4*)(p + x * RPI * a.k_token + koff);
+    for (int x = 0; x < NI; ++x) {
+      // row row1 + x RPI: x's part of the swizzle has bits of its own
+      const int kc = (kc1 ^ draft_swz<CPR>(x * RPI, 0)) * 16, vc = (vc1 ^ draft_swz_v<CPR, S::F32>(x * RPI, 0)) * 16;
+      char* to = buf + (r0 + x * RPI) * ROWB;
+      if (kc < kbytes) draft_copy16(kp + x * RPI * a.k_token + (kl + kc), to);
+      if (vc < vbytes) draft_copy16(vp + x * RPI * a.v_token + (vl + vc), to + KT * ROWB);
+    }
   };
-  auto load_v = [&](int t, int e) {
-    const char* p = c.vh + (int64_t)max(e, 0) * a.v_page + ((t * KT + r0) & ((1 << c.shift) - 1)) * a.v_token;
-#pragma unroll
-    for (int x = 0; x < NI; ++x) vr[x] = *(const uint4*)(p + x * RPI * a.v_token + voff);
-  };
-  int ent[NG], nxt[NG], t = c.t0, own;
-  DraftPages pg(a, c, t * KT);
-  auto pages_of = [&](DraftPages& p, int t, int (&e)[NG]) {
-#pragma unroll
-    for (int i = 0; i < NG; ++i) e[i] = p.page(t * KT + 16 * i);
-  };
-  auto pages = [&](int t, int (&e)[NG]) { pages_of(pg, t, e); };
-  // the page of the rows that this wave stages (a tile's pages are in one
+  DraftPages pg(a, c, c.t0 * KT);
+  // the page of the rows that this wave copies (a tile's pages are in one
   // batch of entries)
   auto mine = [&](int t) { return pg.page(t * KT + r0 / 16 * 16); };
-  char *kb = lds, *vb = lds + KT * ROWB;
-  auto stage = [&]() {
-    kb = lds + ((t - c.t0) & 1) * STAGE;
-    vb = kb + KT * ROWB;
-    if (!whole) {
+  // groups of 16 tokens of a tile without a page
+  auto missing = [&](DraftPages& p, int t) {
+    uint32_t x = 0;
 #pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        if (!kin) kr[i] = make_uint4(0, 0, 0, 0);
-        if (!vin) vr[i] = make_uint4(0, 0, 0, 0);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      const int row = r0 + i * RPI + lr;
-      *(uint4*)(kb + row * ROWB + draft_swz<CPR>(row, lc) * 16) = kr[i];
-      *(uint4*)(vb + row * ROWB + draft_swz_v<CPR, S::F32>(row, lc) * 16) = vr[i];
-    }
-#pragma unroll
-    for (int i = 0; i < NG; ++i) ent[i] = nxt[i];
-    if (t + 1 < c.t1) load_k(t + 1, own);
-    pages(t + 2, nxt);
-    __syncthreads();
-  };
-  auto masked = [&]() {
-    bool x = (t + 1) * KT > c.full;
-#pragma unroll
-    for (int i = 0; i < NG; ++i) x |= ent[i] < 0;
+    for (int i = 0; i < NG; ++i) x |= p.page(t * KT + 16 * i) < 0 ? 1u << i : 0u;
     return x;
   };
-  auto exist = [&]() {
+  // tokens (bits) of tile t that exist
+  auto exist = [&](int t, uint32_t gone) {
     uint64_t x = 0;
 #pragma unroll
     for (int i = 0; i < NG; ++i) {
       const int left = min(max(c.kend - t * KT - 16 * i, 0), 16);
-      if (ent[i] >= 0) x |= (uint64_t)((1u << left) - 1u) << (16 * i);
+      if (!((gone >> i) & 1)) x |= (uint64_t)((1u << left) - 1u) << (16 * i);
     }
     return x;
   };
-  const bool on = row0 < c.nrow;  // the wave has rows
-  pages(t, ent);
-  if (t < c.t1) {
-    load_k(t, mine(t));
-    load_v(t, mine(t));
-  }
-  pages(t + 1, nxt);
-  own = mine(t + 1);
-  bool odd = false;  // this wave staged a token with infinite or NaN values
-  for (; t < c.t1; ++t) {
-    const bool some = masked();
+  // whether some row does not see all of tile t
+  auto masked = [&](int t, uint32_t gone) { return (t + 1) * KT > c.full || gone != 0; };
+
+  bool odd = false;  // this wave copied a token with infinite or NaN values
+  int t = c.t0;
+  if (t < c.t1) copy(lds0, t, mine(t));
+  auto step = [&](char* now, char* next) {
+    const uint32_t gone = missing(pg, t);
+    const bool some = masked(t, gone);
+    const int e = mine(t + 1);
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's copies have landed
+    __syncthreads();                     // all have, and the other buffer's readers are done
     uint64_t there = 0;
     if (some) {
-      there = exist();
+      // Values that a row does not see must not meet the product: 0 x NaN is
+      // NaN.  Each wave puts zeros in the place of those it copied that no row
+      // sees, and of infinite or NaN ones, which join at the end.
+      there = exist(t, gone);
+      const int lane2 = draft_lane_again();
 #pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        const int row = r0 + i * RPI + lr;
-        if (!((there >> row) & 1)) vr[i] = make_uint4(0, 0, 0, 0);
-        const uint64_t hit = __ballot(draft_odd<T>(vr[i]) && vin);
+      for (int x = 0; x < NI; ++x) {
+        const int row = r0 + x * RPI + lane2 / CPR;
+        uint4* p = (uint4*)(now + W::TILE + row * ROWB + lane2 % CPR * 16);
+        const bool in = (there >> row) & 1;
+        const uint64_t hit = __ballot(in && draft_odd<T>(*p));
         odd |= hit != 0;
-        if ((hit >> (lr * CPR)) & (CPR == 64 ? ~0ull : (1ull << (CPR & 63)) - 1)) vr[i] = make_uint4(0, 0, 0, 0);
+        if (!in || ((hit >> (lane2 / CPR * CPR)) & (CPR == 64 ? ~0ull : (1ull << (CPR & 63)) - 1)))
+          *p = make_uint4(0, 0, 0, 0);
       }
+      __syncthreads();
     }
-    stage();
-    typename DraftWave<T, D, MT, KT>::Weights wt;
-    if (on) w.scores(a, c, kb, t * KT, some, there, wt);
-    // only now, when the scores' registers are free
-    if (t + 1 < c.t1) load_v(t + 1, own);
-    own = mine(t + 2);
-    if (on) w.values(vb, wt);
-  }
+    draft_step(a, c, w, t * KT, some, there, on, now, next, [&](char* to) {
+      if (t + 1 < c.t1) copy(to, t + 1, e);
+    });
+    return ++t < c.t1;
+  };
+  if (t < c.t1)
+    while (step(lds0, lds1) && step(lds1, lds0)) {
+    }
+  const DraftArgs& z = draft_args_again();
   if (lane == 0) odds[wv] = odd;
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < NW; ++i) odd |= odds[i] != 0;
   if (odd && on) {
-    DraftPages again(a, c, c.t0 * KT);
+    DraftPages again(z, c, c.t0 * KT);
     for (t = c.t0; t < c.t1; ++t) {
-      pages_of(again, t, ent);
-      if (!masked()) continue;
-      for (uint64_t left = exist(); left; left &= left - 1) {
+      const uint32_t gone = missing(again, t);
+      if (!masked(t, gone)) continue;
+      for (uint64_t left = exist(t, gone); left; left &= left - 1) {
         const int key = t * KT + __builtin_ctzll(left), p = again.page(key);
-        if (draft_odd_row<T>(a, c.vh + p * a.v_page + (key & ((1 << c.shift) - 1)) * a.v_token))
-          w.odd_token(a, c, key, p);
+        if (draft_odd_row<T>(z, c.vh + p * z.v_page + (key & ((1 << c.shift) - 1)) * z.v_token))
+          w.odd_token(z, c, key, p);
       }
     }
   }
   __syncthreads();
 
   const int64_t slot = part.slot;
-  float* my = (float*)lds + wv * 16 * D;
+  float* my = (float*)(wv < NW / 2 ? lds0 : lds1) + wv % (NW / 2) * 16 * D;
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
     const float l = w.sum(mt), m = w.peak(mt);
@@ -988,13 +1023,13 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void draft_rows_kernel(D
       if (r >= c.nrow) continue;
       if (slot >= 0) {
         const int64_t at = slot * R + wv * 16 * MT + mt * 16 + row;
-        *(f32x4*)(a.ws_o + at * D + ch * 4) = x;
+        *(f32x4*)(z.ws_o + at * D + ch * 4) = x;
         if (ch == 0) {
-          a.ws_ml[at * 2] = big;
-          a.ws_ml[at * 2 + 1] = sum;
+          z.ws_ml[at * 2] = big;
+          z.ws_ml[at * 2 + 1] = sum;
         }
       } else {
-        draft_store<T>(a, c.s0, part.h, r, ch, x, sum);
+        draft_store<T>(z, c.s0, part.h, r, ch, x, sum);
       }
     }
     wave_sync();
@@ -1003,30 +1038,33 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void draft_rows_kernel(D
 
 // Joins the chunks of split requests.  The threads of a block are NP sets of
 // D / 4, a set holding a row.  Few chunks: each set takes a row and all its
-// chunks; many: the block takes a row and its sets share the chunks.
+// chunks; many chunks, or few rows in all: the block takes a row and its sets
+// share the chunks.
 constexpr int kJoinSerial = 16;
-template <typename T, int D, int KT, int R>
+template <typename T, int D, int KT, int R, int STEP>
 __global__ __launch_bounds__(256) void draft_join_kernel(DraftArgs a) {
-  constexpr int OC = D / 4, NP = 256 / OC, RB = R / NP > 1 ? R / NP : 1;
+  constexpr int OC = D / 4, NP = 256 / OC, RB = (R + NP - 1) / NP;
   __shared__ f32x4 acc[256];
   __shared__ float lsum[NP];
   const int tid = threadIdx.x, p = tid / OC, ch = tid % OC;
+  const int most = a.one_round ? 0 : kJoinSerial;
   for (int64_t at = blockIdx.x;; at += gridDim.x) {
     DraftUnit u;
-    if (!draft_find<KT, R>(a, at, &u, [](int nch) { return nch <= 1 ? 0 : nch <= kJoinSerial ? RB : R; }))
+    if (!draft_find<KT, R>(a, at, &u, [&](int nch) { return nch <= 1 ? 0 : nch <= most ? RB : R; }))
       return;  // uniform over the block
     const DraftReq rq = draft_request(a, u.b);
-    const bool serial = u.nch <= kJoinSerial;
+    const bool serial = u.nch <= most;
     const int per = serial ? RB : R, sub = u.index % per;
-    const int group = u.index / per, h = group % a.Hkv, rt = group / a.Hkv;
-    const int rr = serial ? sub * NP + p : sub, r = rt * R + rr, nrow = rq.n * a.G;
+    const int group = u.index / per, h = group / u.groups, rt = group % u.groups;
+    const int even = draft_even(rq, a.G, R, STEP), rr = serial ? sub * NP + p : sub, r0 = rt * even, r = r0 + rr;
+    const int nrow = min(rq.n * a.G, r0 + even);
     // (rows of a block ascend: the first one behind the last ends it)
-    if (rt * R + (serial ? sub * NP : sub) >= nrow) {
+    if (r0 + (serial ? sub * NP : sub) >= nrow) {
       if (a.one_round) return;
       continue;
     }
-    const bool on = rr < R && r < nrow;
-    const int64_t base = u.slot + (int64_t)rt * a.Hkv + h, step = (int64_t)u.groups * a.Hkv;
+    const bool on = r < nrow;
+    const int64_t base = u.slot + group, step = (int64_t)u.groups * a.Hkv;
     const int c0 = serial ? 0 : p, dc = serial ? 1 : NP;
     float big = -INFINITY;
     if (on) {
@@ -1079,7 +1117,7 @@ int draft_launch(const DraftArgs& a, int64_t units, int64_t joins, hipStream_t s
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return (int)e;
   if (joins > 0) {
-    hipLaunchKernelGGL((draft_join_kernel<T, D, KT, R>), dim3((unsigned)joins), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((draft_join_kernel<T, D, KT, R, 16 * MT>), dim3((unsigned)joins), dim3(256), 0, st, a);
     e = hipGetLastError();
   }
   return e == hipSuccess ? HTREE_OK : (int)e;
@@ -1090,11 +1128,14 @@ int draft_launch_type(const DraftArgs& a, const DraftPlan& p, hipStream_t st);
 
 template <typename T, int D>
 int draft_launch_dim(const DraftArgs& a, const DraftPlan& p, hipStream_t st) {
-  constexpr DraftForm f = draft_rows_form(D, (int)sizeof(T));
-  if (p.NW > 1) return draft_launch<T, D, f.MT, f.NW>(a, p.units, p.joins, st);
+  constexpr bool F32 = sizeof(T) == 4;
+  if constexpr (!F32) {
+    constexpr DraftForm f = draft_rows_form(D, (int)sizeof(T));
+    if (p.NW > 1) return draft_launch<T, D, f.MT, f.NW>(a, p.units, p.joins, st);
+  }
   if (p.MT == 1) return draft_launch<T, D, 1, 1>(a, p.units, p.joins, st);
   if constexpr (D <= 128) {
-    if (p.MT == 4) return draft_launch<T, D, 4, 1>(a, p.units, p.joins, st);
+    if (p.MT > 2) return draft_launch<T, D, F32 ? 3 : 4, 1>(a, p.units, p.joins, st);
   }
   return draft_launch<T, D, 2, 1>(a, p.units, p.joins, st);
 }

@@ -60,21 +60,25 @@ int main() {
       CHECK(r.s0 >= 0 && r.n >= 0 && r.s0 + r.n <= rows && r.len >= 0);
       tiles += (float)draft_tiles(r, cap, KT) * draft_row_groups(r, G, p.R);
     }
-    const int chunk = draft_chunk(tiles * Hkv, p.target);
+    int chunk = draft_chunk(tiles * Hkv, p.target);
+    for (int i = upto(3); i > 0 && p.target > 0; --i) chunk = draft_wider(chunk);
     int64_t units = 0, slots = 0;
     for (const DraftReq& r : rq) {
-      const int nt = draft_tiles(r, cap, KT), nch = draft_chunks(nt, chunk);
+      const int nt = draft_tiles(r, cap, KT), nch = draft_chunks(nt, chunk), part = draft_part(nt, nch);
+      CHECK((int64_t)part * nch >= nt && part <= (chunk > 1 ? chunk : 1));
       const int64_t rts = draft_row_groups(r, G, p.R);
       units += draft_pieces(nch, (int)(rts * Hkv));
       if (nch > 1) slots += draft_pieces(nch, (int)(rts * Hkv));
       for (int64_t rt = 0; rt < rts; rt += rts > 40 ? 1 + upto(9) : 1) {
         int next = 0;
-        const DraftSpan whole = draft_span(r, rt * p.R, p.R, G, cap, KT, 0, 1 << 30);
+        const int even = draft_even(r, G, p.R, 16 * p.MT), r0 = (int)rt * even;
+        CHECK(even <= p.R && even * rts >= (int64_t)r.n * G && r0 < r.n * G);
+        const DraftSpan whole = draft_span(r, r0, even, G, cap, KT, 0, 1 << 30);
         CHECK(whole.kend >= 0 && whole.kend <= cap && whole.kend <= r.len);
         const int used = (whole.kend + (1 << shift) - 1) >> shift;
         CHECK(used <= width);
         for (int ch = 0; ch < nch; ++ch) {
-          const DraftSpan s = draft_span(r, rt * p.R, p.R, G, cap, KT, ch, chunk);
+          const DraftSpan s = draft_span(r, r0, even, G, cap, KT, ch, part);
           ++units_seen;
           CHECK(s.kend == whole.kend && s.t0 <= s.t1);
           CHECK(s.t0 == next);
@@ -91,7 +95,7 @@ int main() {
         }
         CHECK(next == (whole.kend + KT - 1) / KT);
         // the rows' tokens and a walk to the root
-        for (int64_t x = rt * p.R; x < (rt + 1) * p.R && x < (int64_t)r.n * G; ++x) {
+        for (int64_t x = r0; x < r0 + even && x < (int64_t)r.n * G; ++x) {
           int j = (int)(x / G), steps = 0;
           CHECK(j < r.n && (int64_t)r.s0 + j < rows);
           while (j >= 0) {
@@ -106,6 +110,16 @@ int main() {
     CHECK(slots <= p.slots);
     if (ascend) CHECK(units <= p.units);
     CHECK((p.joins > 0) == (p.target > 0));
+    // every unit has one block
+    CHECK(p.units % (8 * p.near) == 0);
+    if (p.units < 100000) {
+      std::vector<char> had((size_t)p.units, 0);
+      for (int64_t x = 0; x < p.units; ++x) {
+        const int64_t u = draft_near(x, p.near);
+        CHECK(u >= 0 && u < p.units && !had[(size_t)u]);
+        if (u >= 0 && u < p.units) had[(size_t)u] = 1;
+      }
+    }
     // page tables: the new pages are those the launch has blocks for
     for (int b = 0; b < B; ++b) {
       const int64_t ctx = lens[b] < 0 ? 0 : lens[b], n = rq[b].n;
