@@ -150,6 +150,7 @@ struct AppendArgs {
   int64_t kc_page, kc_token, kc_head, vc_page, vc_token, vc_head;      // bytes
   int64_t num_slots;
   int32_t rows, H, Hkv, Dk, Dv, page_shift, rope_rows;
+  int32_t lanes;  // of a row: 2^n, at least the pieces of a half of a head (a head, of values)
 };
 
 template <int N>
@@ -174,15 +175,15 @@ __device__ __forceinline__ void rotate(const T* x1, const T* x2, const float* c,
   }
 }
 
-// heads of one row of q (or k): a lane takes one chunk of VB bytes of each
-// half of a head, 64 / (chunks of a half) heads at a time
+// heads of one row of q (or k): a lane of its `lanes` takes one chunk of VB
+// bytes of each half of a head, lanes / (chunks of a half) heads at a time
 template <typename T, int VB>
 __device__ __forceinline__ void append_rotate(const char* src, int64_t src_head, char* dst, int64_t dst_head,
                                               int heads, int half, const float* c, const float* s, int lane,
-                                              int part, int parts) {
+                                              int lanes, int part, int parts) {
   constexpr int NV = VB / (int)sizeof(T);
   typedef typename AppendVec<VB>::V V;
-  const int per = half / NV, hpi = 64 / per;
+  const int per = half / NV, hpi = lanes / per;
   const int h0 = lane / per, ch = lane - h0 * per;
   if (h0 >= hpi) return;
   float cc[NV], ss[NV];
@@ -217,21 +218,35 @@ __device__ __forceinline__ void append_rotate(const char* src, int64_t src_head,
 }
 
 __device__ __forceinline__ void append_copy(const char* src, int64_t src_head, char* dst, int64_t dst_head,
-                                            int heads, int bytes, int lane, int part, int parts) {
-  const int per = bytes / 16, hpi = 64 / per;
+                                            int heads, int bytes, int lane, int lanes, int part, int parts) {
+  const int per = bytes / 16, hpi = lanes / per;
   const int h0 = lane / per, ch = lane - h0 * per;
   if (h0 >= hpi) return;
-#pragma unroll 2
-  for (int h = part * hpi + h0; h < heads; h += parts * hpi)
-    *(uint4*)(dst + h * dst_head + ch * 16) = *(const uint4*)(src + h * src_head + ch * 16);
+  constexpr int U = 4;
+  for (int h = part * hpi + h0; h < heads; h += U * parts * hpi) {
+    f32x4 x[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int hh = h + i * parts * hpi;
+      if (hh < heads) x[i] = *(const f32x4*)(src + hh * src_head + ch * 16);
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int hh = h + i * parts * hpi;
+      if (hh < heads) *(f32x4*)(dst + hh * dst_head + ch * 16) = x[i];
+    }
+  }
 }
 
-// One wave per row (token); blockIdx.y splits its heads where there are few
-// rows.  Bound by memory: k, v and q once in, once out.
+// `lanes` lanes per row (token): a wave where the row has heads enough for
+// it, else as many as it has pieces of (keys and values of one head of dim 64,
+// 2M rows: 8 lanes a row; a wave each takes four times as long).  blockIdx.y
+// splits a row's heads where there are few rows.  Bound by memory: k, v and q
+// once in, once out.
 template <typename T, int VB>
 __global__ __launch_bounds__(256) void cache_append_kernel(AppendArgs a) {
-  const int lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * 4 + uniform(threadIdx.x >> 6);
+  const int lanes = a.lanes, lane = threadIdx.x & (lanes - 1);
+  const int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) / lanes;
   if (row >= a.rows) return;
   const int part = blockIdx.y, parts = gridDim.y;
   const int64_t slot = a.slots[row];
@@ -248,11 +263,11 @@ __global__ __launch_bounds__(256) void cache_append_kernel(AppendArgs a) {
   if (a.q) {
     char* qo = a.qo + row * a.o_row;
     if (at) {
-      append_rotate<T, VB>(a.q + row * a.q_row, a.q_head, qo, a.o_head, a.H, half, c, s, lane, part, parts);
+      append_rotate<T, VB>(a.q + row * a.q_row, a.q_head, qo, a.o_head, a.H, half, c, s, lane, lanes, part, parts);
     } else {
       // a row without a position has a query of zeros
       const int n = a.H * (a.Dk * (int)sizeof(T) / 16);
-      for (int i = part * 64 + lane; i < n; i += parts * 64) *(uint4*)(qo + (int64_t)i * 16) = make_uint4(0, 0, 0, 0);
+      for (int i = part * lanes + lane; i < n; i += parts * lanes) *(uint4*)(qo + (int64_t)i * 16) = make_uint4(0, 0, 0, 0);
     }
   }
   if (!at || slot < 0 || slot >= a.num_slots) return;
@@ -260,10 +275,10 @@ __global__ __launch_bounds__(256) void cache_append_kernel(AppendArgs a) {
   char* kd = a.kc + page * a.kc_page + off * a.kc_token;
   char* vd = a.vc + page * a.vc_page + off * a.vc_token;
   if (rope)
-    append_rotate<T, VB>(a.k + row * a.k_row, a.k_head, kd, a.kc_head, a.Hkv, half, c, s, lane, part, parts);
+    append_rotate<T, VB>(a.k + row * a.k_row, a.k_head, kd, a.kc_head, a.Hkv, half, c, s, lane, lanes, part, parts);
   else
-    append_copy(a.k + row * a.k_row, a.k_head, kd, a.kc_head, a.Hkv, a.Dk * (int)sizeof(T), lane, part, parts);
-  append_copy(a.v + row * a.v_row, a.v_head, vd, a.vc_head, a.Hkv, a.Dv * (int)sizeof(T), lane, part, parts);
+    append_copy(a.k + row * a.k_row, a.k_head, kd, a.kc_head, a.Hkv, a.Dk * (int)sizeof(T), lane, lanes, part, parts);
+  append_copy(a.v + row * a.v_row, a.v_head, vd, a.vc_head, a.Hkv, a.Dv * (int)sizeof(T), lane, lanes, part, parts);
 }
 
 // ------------------------------------------------------------------ host
@@ -371,12 +386,16 @@ extern "C" int htree_cache_append(const htree_cache* c, int32_t rows, int32_t H,
   a.num_slots = (int64_t)c->num_pages * c->page_size;
   a.rows = rows, a.H = q ? H : 0, a.Hkv = c->H_kv, a.Dk = c->Dk, a.Dv = c->Dv;
   a.page_shift = log2i(c->page_size), a.rope_rows = rope_rows;
-  const unsigned gx = (unsigned)((rows + 3ll) / 4);
+  // 16-byte chunks where a half of a head holds whole ones
+  const bool wide = c->Dk * es % 32 == 0;
+  const int per_k = rope ? c->Dk / 2 * es / (wide ? 16 : 8) : c->Dk * es / 16, per_v = c->Dv * es / 16;
+  const int heads = q ? H : c->H_kv, most = per_k > per_v ? per_k : per_v;
+  a.lanes = 1;
+  while (a.lanes < 64 && (a.lanes < most || a.lanes < heads * most)) a.lanes *= 2;
+  const unsigned gx = (unsigned)(((int64_t)rows * a.lanes + 255) / 256);
   const unsigned gy = gx >= 1024 ? 1 : gx >= 256 ? 2 : 4;
   const dim3 grid(gx, gy);
   hipStream_t s = (hipStream_t)stream;
-  // 16-byte chunks where a half of a head holds whole ones
-  const bool wide = c->Dk * es % 32 == 0;
 #define HTREE_APPEND(T)                                                                             \
   if (wide) hipLaunchKernelGGL((cache_append_kernel<T, 16>), grid, dim3(256), 0, s, a);             \
   else hipLaunchKernelGGL((cache_append_kernel<T, 8>), grid, dim3(256), 0, s, a)

@@ -32,7 +32,9 @@ __host__ __device__ constexpr int draft_tile(int D, int es, int NW = 1) {
 }
 
 // whether two blocks of the form with common rows fit a CU (256 registers a lane)
-__host__ __device__ constexpr bool draft_two(int D, int MT) { return D * MT <= 128; }
+__host__ __device__ constexpr bool draft_two(int D, int MT, int es) {
+  return es == 2 ? D * MT <= 128 : D * MT <= 64 || (MT == 1 && D <= 128);
+}
 
 // A call's split.  Units: blocks of the launch, R rows of a request and KV
 // head each.  Joins: blocks of the second launch, which joins the units of the
@@ -51,7 +53,7 @@ __host__ __device__ inline DraftPlan draft_plan(int Dk, int Dv, int es, int B, i
   p.D = m <= 32 ? 32 : m <= 64 ? 64 : m <= 128 ? 128 : 256;
   const int G = H / Hkv;
   const int64_t per = ((int64_t)rows * G + B - 1) / B;  // rows of a request, on average
-  p.MT = per <= 16 ? 1 : per <= 32 || p.D == 256 ? 2 : es == 4 ? 3 : 4;
+  p.MT = per <= 16 ? 1 : per <= 32 || p.D == 256 || es == 4 ? 2 : 4;
   p.NW = 1;
   if (per > 64 && es == 2) {
     const DraftForm f = draft_rows_form(p.D, es);
@@ -60,7 +62,7 @@ __host__ __device__ inline DraftPlan draft_plan(int Dk, int Dv, int es, int B, i
   p.R = 16 * p.MT * p.NW;
   const int64_t rts = ((int64_t)rows * G / p.R + B) * Hkv;
   // blocks that fit the GPU at once
-  const int full = (p.NW > 1 ? p.D <= 128 : draft_two(p.D, p.MT)) ? 512 : 256;
+  const int full = (p.NW > 1 ? p.D <= 128 : draft_two(p.D, p.MT, es)) ? 512 : 256;
   p.target = (int64_t)width * page_size <= 1024 ? 0 : full;
   p.near = (int)((per + p.R - 1) / p.R);
   p.near = p.near > 64 ? 64 : p.near;

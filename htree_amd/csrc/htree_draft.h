@@ -374,9 +374,11 @@ struct DraftWave {
 
   // Scores of one tile of KT tokens from key0, its keys staged at kb, and the
   // rows' max moved where they call for it.  masked: not every row sees every
-  // token; there: the tokens (bits) that exist.
+  // token; there: the tokens (bits) that exist; between(x, n): called after
+  // step x of n of the product.
+  template <typename F>
   __device__ __forceinline__ void scores(const DraftArgs& a, const DraftCtx& c, const char* kb, int key0,
-                                         bool masked, uint64_t there, f32x4 (&sc)[MT][NG]) {
+                                         bool masked, uint64_t there, f32x4 (&sc)[MT][NG], F between) {
     const int lane = draft_lane_again(), n16 = lane & 15, g = lane >> 4;
     // ---- scores, token x row: a lane holds tokens 4 g .. 4 g + 3 of each
     // group of 16, of row n16.  The operands come from LDS four products
@@ -386,6 +388,7 @@ struct DraftWave {
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
       for (int i = 0; i < NG; ++i) sc[mt][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    __builtin_amdgcn_s_setprio(1);
     {
       constexpr int NS = NG * (F32 ? D / 16 : D / 32), AHEAD = NS < 4 ? NS : 4;
       // (a row's swizzle and the piece's number are bits of their own)
@@ -413,10 +416,12 @@ struct DraftWave {
             sc[mt][i] = DraftT<T>::mma(__builtin_bit_cast(V8, f[x % AHEAD]), __builtin_bit_cast(V8, qh[mt][s]), sc[mt][i]);
         }
         if (x + AHEAD < NS) f[x % AHEAD] = key(x + AHEAD);
+        between(x, NS);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
 
+    __builtin_amdgcn_s_setprio(0);
     // ---- masks
     if (masked) {
 #pragma unroll
@@ -550,6 +555,7 @@ struct DraftWave {
 #pragma unroll
       for (int x = 0; x < EL; ++x) weigh(x / (PG * 4), x / 4 % PG, x % 4);
       round(0);
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int x = 0; x < NS; ++x) {
         const int q = x % NQ, i0 = x / NQ * PG;
@@ -564,6 +570,7 @@ struct DraftWave {
         __builtin_amdgcn_sched_barrier(0);
         if (q == NQ - 1 && i0 + PG < NG) round(i0 + PG);
       }
+      __builtin_amdgcn_s_setprio(0);
     }
   }
 
@@ -665,7 +672,7 @@ __device__ __forceinline__ void draft_store(const DraftArgs& a, int s0, int h, i
 // chunk's tiles in turn, each through LDS of its own, so that there is no
 // barrier before their states meet.
 template <typename T, int D, int MT>
-__global__ __launch_bounds__(256, draft_two(D, MT) ? 2 : 1) void draft_kernel(DraftArgs a) {
+__global__ __launch_bounds__(256, draft_two(D, MT, sizeof(T)) ? 2 : 1) void draft_kernel(DraftArgs a) {
   using S = DraftShape<T, D>;
   constexpr int KT = draft_tile(D, S::ES), NG = KT / 16, CPR = S::CPR, RPI = S::RPI, R = 16 * MT;
   constexpr int NI = KT / RPI, ROWB = S::ROWB, NW = kWavesPerBlock;
@@ -785,7 +792,7 @@ __global__ __launch_bounds__(256, draft_two(D, MT) ? 2 : 1) void draft_kernel(Dr
     }
     stage();
     f32x4 sc[MT][NG];
-    w.scores(a, c, kb, t * KT, some, there, sc);
+    w.scores(a, c, kb, t * KT, some, there, sc, [](int, int) {});
     w.values(a, vb, sc);
     wave_sync();  // this tile's reads come before the next one's writes
   }
@@ -856,16 +863,25 @@ __device__ __forceinline__ void draft_copy16(const char* from, char* to) {
   __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, (lds_void*)to, 16, 0, 0);
 }
 
-// A tile, while the next is copied (`copy`).  The buffers do not overlap and
-// are said not to: else the reads of one wait for the copies into the other.
-template <typename W, typename F>
+// A tile, while the next is copied: copy(next, i), i < COPIES, a piece at a
+// time between the products (all at once the copies held the wave for as long
+// as either product).  The buffers do not overlap and are said not to: else
+// the reads of one wait for the copies into the other.
+template <int COPIES, typename W, typename F>
 __device__ __forceinline__ void draft_step(const DraftArgs& a, const DraftCtx& c, W& w, int key0, bool masked,
                                            uint64_t there, bool on, const char* __restrict__ now,
                                            char* __restrict__ next, F copy) {
-  copy(next);
-  if (!on) return;
+  if (!on) {
+#pragma unroll
+    for (int i = 0; i < COPIES; ++i) copy(next, i);
+    return;
+  }
   f32x4 sc[W::GROUPS][W::NG];
-  w.scores(a, c, now, key0, masked, there, sc);
+  w.scores(a, c, now, key0, masked, there, sc, [&](int x, int n) {
+#pragma unroll
+    for (int i = 0; i < COPIES; ++i)
+      if (i * n / COPIES == x) copy(next, i);
+  });
   w.values(a, now + W::TILE, sc);
 }
 
@@ -873,7 +889,8 @@ __device__ __forceinline__ void draft_step(const DraftArgs& a, const DraftCtx& c
 // take the same tiles, which the block copies into one of two LDS buffers
 // (directly, without registers) while it works on the other: one barrier a
 // tile.
-template <typename T, int D, int MT, int NW, int KT>
+// WHOLE: the head dims are D.
+template <typename T, int D, int MT, int NW, int KT, bool WHOLE>
 __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void draft_rows_kernel(DraftArgs a) {
   using S = DraftShape<T, D>;
   using W = DraftWave<T, D, MT, KT>;
@@ -902,7 +919,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void draft_rows_kernel(D
   const int lr = lane / CPR, lc = lane % CPR;
   const int r0 = wv * WR;  // first of the rows this wave copies
   const int kbytes = a.Dk * S::ES, vbytes = a.Dv * S::ES;
-  if (kbytes < ROWB || vbytes < ROWB) {
+  if (!WHOLE) {
     // the places past the head dims: no copy writes them
     for (int i = threadIdx.x * 16; i < STAGE; i += 64 * NW * 16) {
       *(uint4*)(lds0 + i) = make_uint4(0, 0, 0, 0);
@@ -915,17 +932,21 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void draft_rows_kernel(D
   // belongs there.
   const int row1 = r0 + lr, kc1 = draft_swz<CPR>(row1, lc), vc1 = draft_swz_v<CPR, S::F32>(row1, lc);
   const uint32_t kl = lr * (uint32_t)a.k_token, vl = lr * (uint32_t)a.v_token;
-  auto copy = [&](char* buf, int t, int e) {
+  const char *kp, *vp;  // of the rows to copy
+  auto aim = [&](int t, int e) {
     const int at = (t * KT + r0) & ((1 << c.shift) - 1);
-    const char* kp = c.kh + (int64_t)max(e, 0) * a.k_page + at * a.k_token;
-    const char* vp = c.vh + (int64_t)max(e, 0) * a.v_page + at * a.v_token;
-#pragma unroll
-    for (int x = 0; x < NI; ++x) {
-      // row row1 + x RPI: x's part of the swizzle has bits of its own
-      const int kc = (kc1 ^ draft_swz<CPR>(x * RPI, 0)) * 16, vc = (vc1 ^ draft_swz_v<CPR, S::F32>(x * RPI, 0)) * 16;
-      char* to = buf + (r0 + x * RPI) * ROWB;
-      if (kc < kbytes) draft_copy16(kp + x * RPI * a.k_token + (kl + kc), to);
-      if (vc < vbytes) draft_copy16(vp + x * RPI * a.v_token + (vl + vc), to + KT * ROWB);
+    kp = c.kh + (int64_t)max(e, 0) * a.k_page + at * a.k_token;
+    vp = c.vh + (int64_t)max(e, 0) * a.v_page + at * a.v_token;
+  };
+  auto copy = [&](char* buf, int i) {
+    // row row1 + x RPI: x's part of the swizzle has bits of its own
+    const int x = i >> 1;
+    const int kc = (kc1 ^ draft_swz<CPR>(x * RPI, 0)) * 16, vc = (vc1 ^ draft_swz_v<CPR, S::F32>(x * RPI, 0)) * 16;
+    char* to = buf + (r0 + x * RPI) * ROWB;
+    if (i & 1) {
+      if (WHOLE || vc < vbytes) draft_copy16(vp + x * RPI * a.v_token + (vl + vc), to + KT * ROWB);
+    } else {
+      if (WHOLE || kc < kbytes) draft_copy16(kp + x * RPI * a.k_token + (kl + kc), to);
     }
   };
   DraftPages pg(a, c, c.t0 * KT);
@@ -954,11 +975,17 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void draft_rows_kernel(D
 
   bool odd = false;  // this wave copied a token with infinite or NaN values
   int t = c.t0;
-  if (t < c.t1) copy(lds0, t, mine(t));
+  if (t < c.t1) {
+    aim(t, mine(t));
+#pragma unroll
+    for (int i = 0; i < 2 * NI; ++i) copy(lds0, i);
+  }
   auto step = [&](char* now, char* next) {
     const uint32_t gone = missing(pg, t);
     const bool some = masked(t, gone);
-    const int e = mine(t + 1);
+    // (past the last tile: this one again, which no one reads)
+    const int t2 = min(t + 1, c.t1 - 1);
+    aim(t2, mine(t2));
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's copies have landed
     __syncthreads();                     // all have, and the other buffer's readers are done
     uint64_t there = 0;
@@ -980,14 +1007,13 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void draft_rows_kernel(D
       }
       __syncthreads();
     }
-    draft_step(a, c, w, t * KT, some, there, on, now, next, [&](char* to) {
-      if (t + 1 < c.t1) copy(to, t + 1, e);
-    });
+    draft_step<2 * NI>(a, c, w, t * KT, some, there, on, now, next, copy);
     return ++t < c.t1;
   };
   if (t < c.t1)
     while (step(lds0, lds1) && step(lds1, lds0)) {
     }
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the output passes through the buffers
   const DraftArgs& z = draft_args_again();
   if (lane == 0) odds[wv] = odd;
   __syncthreads();
@@ -1112,8 +1138,10 @@ int draft_launch(const DraftArgs& a, int64_t units, int64_t joins, hipStream_t s
   constexpr int KT = draft_tile(D, (int)sizeof(T), NW), R = 16 * MT * NW;
   if constexpr (NW == 1)
     hipLaunchKernelGGL((draft_kernel<T, D, MT>), dim3((unsigned)units), dim3(256), 0, st, a);
+  else if (a.Dk == D && a.Dv == D)
+    hipLaunchKernelGGL((draft_rows_kernel<T, D, MT, NW, KT, true>), dim3((unsigned)units), dim3(64 * NW), 0, st, a);
   else
-    hipLaunchKernelGGL((draft_rows_kernel<T, D, MT, NW, KT>), dim3((unsigned)units), dim3(64 * NW), 0, st, a);
+    hipLaunchKernelGGL((draft_rows_kernel<T, D, MT, NW, KT, false>), dim3((unsigned)units), dim3(64 * NW), 0, st, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return (int)e;
   if (joins > 0) {
