@@ -50,6 +50,13 @@ def _ints(t: torch.Tensor, name: str, n: int, device) -> None:
     assert t.device == device, f"{name} must be on {device}"
 
 
+def overlap(a: torch.Tensor, b: Optional[torch.Tensor]) -> bool:
+    """Whether two tensors' memory, gaps included, overlaps."""
+    def end(t):
+        return t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+    return b is not None and a.numel() > 0 and b.numel() > 0 and a.data_ptr() < end(b) and b.data_ptr() < end(a)
+
+
 def check_table(block_table: torch.Tensor, B: int, device) -> None:
     assert block_table.dtype is torch.int32 and block_table.dim() == 2, "block_table must be int32 [B, width]"
     assert block_table.shape[0] == B, f"block_table must have a row for each of the {B} requests"
@@ -113,7 +120,8 @@ def page_tables(ctx_lens: torch.Tensor, new_lens: torch.Tensor, block_table: tor
     index, within the request, of the token drafted before it, a smaller one
     (-1: none); positions are then those along each branch.
 
-    Returns PageTables (`out`: written there).  Rows behind the last request
+    Returns PageTables (`out`: written there; it does not overlap the
+    inputs).  Rows behind the last request
     have slot and position -1; so has the slot of a token past the table's
     width, or whose page free_pages was too short for (pages_used says how
     many are wanted).  page_size is a power of two."""
@@ -141,6 +149,10 @@ def page_tables(ctx_lens: torch.Tensor, new_lens: torch.Tensor, block_table: tor
         _ints(out.pages_used, "out.pages_used", 1, dev)
         assert out.slots.dtype is torch.int64 and out.slots.shape == (rows,) and out.slots.is_contiguous() \
             and out.slots.device == dev, f"out.slots must be a contiguous int64 tensor [{rows}] on {dev}"
+        # (the lengths of a step are a natural input of the next: the kernel
+        # would read some after writing them)
+        assert not any(overlap(x, y) for x in out for y in (ctx_lens, new_lens, free_pages, parents, block_table)), \
+            "out must not overlap the inputs"
     if B == 0:
         out.starts.zero_(), out.pages_used.zero_(), out.slots.fill_(-1), out.positions.fill_(-1)
         return out
@@ -167,7 +179,8 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     sums are fp32, rounded once.  Rows whose slot or position is out of range
     are not written, and a query without a position is zero.  The slots of a
     call are distinct; two rows with one slot leave either's values there,
-    or parts of both."""
+    or parts of both.  k, v and q are not parts of the cache that is written
+    (rows moved within it are copied out first: cache.view(...)[slots])."""
     c = native_cache(k_cache, v_cache)
     dtype, dev = k_cache.dtype, k_cache.device
     assert k.dim() == 3 and v.dim() == 3, "k / v must be [rows, H_kv, D]"

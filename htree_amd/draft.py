@@ -4,13 +4,14 @@ The cache, block tables and slots are cache.py's."""
 from __future__ import annotations
 
 import ctypes
+import math
 from functools import lru_cache
 from typing import Optional
 
 import torch
 
 from . import _native as N
-from .cache import MAX_REQUEST_TOKENS, _ints, aligned_rows, check_table, native_cache
+from .cache import MAX_REQUEST_TOKENS, _ints, aligned_rows, check_table, native_cache, overlap
 
 
 @lru_cache(maxsize=256)
@@ -72,6 +73,10 @@ def draft_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         assert out.shape == (rows, H, c.Dv) and out.dtype is dtype and out.is_contiguous() \
             and out.device == dev and out.data_ptr() % 16 == 0, \
             f"out must be a contiguous {dtype} tensor [{rows}, {H}, {c.Dv}] on {dev}"
+        assert not any(overlap(out, x) for x in (q, k_cache, v_cache, block_table, lens, starts, parents)), \
+            "out must not overlap the inputs"
+    scale = K ** -0.5 if scale is None else float(scale)
+    assert math.isfinite(scale), f"scale must be finite, got {scale}"
     if B == 0 or rows == 0:
         return out
     q = aligned_rows(q)
@@ -80,7 +85,7 @@ def draft_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                                c.v_page, c.v_token, c.v_head), B, rows, H, width)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     rc = N.launch(N.lib().htree_draft_attention, dev, c, B, rows, H, width, block_table.stride(0),
-                  K ** -0.5 if scale is None else float(scale), q.data_ptr(), q_row, q_head, k_cache.data_ptr(),
+                  scale, q.data_ptr(), q_row, q_head, k_cache.data_ptr(),
                   v_cache.data_ptr(), block_table.data_ptr(), lens.data_ptr(), starts.data_ptr(), N.address(parents),
                   out.data_ptr(), H * c.Dv, c.Dv, N.address(ws), nbytes)
     if rc:

@@ -237,6 +237,12 @@ def test_refusals():
         lambda: htree_amd.page_tables(i32([1]), i32([1]), i32(np.zeros((1, 2))), i32([1]), 16, 2, -1),
         lambda: htree_amd.page_tables(i32([1]), i32([1]), i32(np.zeros((1, 2))), i32([1]), 16, 2, 3, parents=i32([1])),
     ]
+    t = htree_amd.page_tables(i32([1]), i32([1]), i32(np.zeros((1, 2))), i32([1]), 16, 2, 3)
+    bad += [  # the last step's lengths as input of the next, written in place
+        lambda: htree_amd.page_tables(t.lens, i32([1]), i32(np.zeros((1, 2))), i32([1]), 16, 2, 3, out=t),
+        lambda: htree_amd.page_tables(i32([1]), i32([1]), i32(np.zeros((1, 2))), i32([1]), 16, 2, 3,
+                                      parents=t.positions, out=t),
+    ]
     for i, call in enumerate(bad):
         with pytest.raises(AssertionError):
             call()

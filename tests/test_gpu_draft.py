@@ -197,6 +197,70 @@ def test_pages_and_layouts(page, heads_first):
     c.check(c.run())
 
 
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("H,Hkv,K,V", HEADS + [(64, 1, 48, 128), (16, 1, 256, 200)])
+@pytest.mark.parametrize("kind", ["tree", None])
+def test_many_rows(dtype, H, Hkv, K, V, kind):
+    """Requests of many rows (new tokens x heads of a group), ragged, without
+    a cached token, split over their tokens; head dims that are not a
+    kernel's among them."""
+    c = Case([130, 300, 1400, 97], [130, 90, 200, 1], H, Hkv, K, V, dtype, kind=kind, seed=30)
+    c.check(c.run())
+
+
+def test_long_chunk_from_nothing():
+    """A whole prompt: every row sees another number of tokens."""
+    c = Case([1500], [1500], 4, 2, 32, 32, "bfloat16", seed=31)
+    c.check(c.run())
+
+
+def test_a_group_of_1024_heads():
+    c = Case([70, 3], [2, 1], 1024, 1, 32, 32, "float16", kind="tree", seed=32)
+    c.check(c.run())
+
+
+def test_requests_that_share_pages():
+    """A prefix in the same pages of two requests, and a table that names one
+    page twice."""
+    c = Case([96, 96, 40], [3, 5, 1], 8, 2, 64, 64, "bfloat16", kind="tree", seed=33)
+    c.table[1, :3] = c.table[0, :3]
+    c.table[2, 1] = c.table[2, 0]
+    for x in (c.k, c.v):
+        x[1][:48] = x[0][:48]
+        x[2][16:32] = x[2][:16]
+    c.check(c.run())
+
+
+def test_rows_that_begin_later():
+    """starts[0] > 0: the rows before it belong to no request."""
+    c = Case([40, 70], [3, 2], 8, 2, 64, 64, "bfloat16", seed=34, pad=4)
+    a, _ = c.args()
+    out = torch.full((9, 8, 64), 9.0, dtype=torch.bfloat16, device=DEV)
+    want = htree_amd.draft_attention(*a)
+    a[0] = torch.cat([torch.zeros_like(a[0][:4]), a[0][:5]])
+    a[5] = a[5] + 4
+    htree_amd.draft_attention(*a, out=out)
+    torch.cuda.synchronize()
+    assert bool((out[:4] == 9.0).all()) and torch.equal(out[4:], want[:5])
+
+
+@pytest.mark.parametrize("rows", [6, 400])
+def test_damaged_lengths_stay_in_bounds(rows):
+    """Starts and lengths that contradict each other (their indexes are
+    replayed on the host too): rows outside what any request claims are left."""
+    c = Case([200, 64, 90], [rows - 4, 2, 2], 8, 2, 64, 64, "bfloat16", seed=35, width=80)
+    a, _ = c.args()
+    for starts, lens in (([0, 3, 1, 5], [200, 64, 90]), ([2 ** 31 - 1, -2 ** 31, 3, 4], [200, 64, 90]),
+                         ([1, 2, 3, 2 ** 31 - 1], [2 ** 31 - 1, -1, -2 ** 31]), ([0, 0, 0, 0], [5, 5, 5])):
+        out = torch.full((rows, 8, 64), 9.0, dtype=torch.bfloat16, device=DEV)
+        htree_amd.draft_attention(a[0], a[1], a[2], a[3], i32(lens), i32(starts), out=out)
+        torch.cuda.synchronize()
+        claimed = torch.zeros(rows, dtype=torch.bool)
+        for s, e in zip(starts, starts[1:]):
+            claimed[min(max(s, 0), rows):min(max(e, 0), rows)] = True
+        assert bool((out[~claimed.to(DEV)] == 9.0).all())
+
+
 def test_many_requests():
     g = np.random.default_rng(0)
     lens = g.integers(1, 300, 333)
@@ -287,6 +351,37 @@ def test_branches_do_not_see_each_others_infinities(dtype, K, bad):
         else:
             assert torch.equal(x, y)
         assert torch.isfinite(x[:, ~hit]).all()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("K,V", [(64, 64), (128, 96), (256, 256)])
+def test_infinities_among_many_rows(dtype, K, V):
+    """The same with many rows, several such tokens (one of them cached, in a
+    tile with new ones) and pages missing."""
+    new, L = 40, 110
+    c = Case([L], [new], 16, 2, K, V, dtype, kind="tree", seed=36)
+    c.table[0, 2] = -1
+    a, p = c.args()
+    clean = htree_amd.draft_attention(*a, parents=p)
+    see = visible("tree", c.parents, new, L - new, L)
+    see[:, 32:48] = False
+    odd = [68, 75, 76, 90, 109]
+    for i, at in enumerate(odd):
+        c.vc[c.table[0, at // 16], at % 16, 1, i] = (float("inf"), float("nan"), -float("inf"))[i % 3]
+    out = htree_amd.draft_attention(*a, parents=p)
+    torch.cuda.synchronize()
+    _, bar = reference(c.q.double().numpy(), c.k[0], c.v[0], see, K ** -0.5, dtype)
+    bar = torch.as_tensor(bar, dtype=torch.float32, device=DEV)[:, 8:] * 1.0001
+    assert torch.equal(out[:, :8], clean[:, :8])
+    for j in range(new):
+        x, y = out[j, 8:].float(), clean[j, 8:].float()
+        hit = torch.zeros(V, dtype=torch.bool, device=DEV)
+        for i, at in enumerate(odd):
+            hit[i] = bool(see[j, at])
+        assert not torch.isfinite(x[:, hit]).any()
+        assert bool(((x - y).abs() <= 2 * bar[j])[:, ~hit].all())
+        if not hit.any():
+            assert torch.equal(x, y)
 
 
 def test_rows_behind_the_last_are_left():
@@ -408,7 +503,9 @@ def test_refusals():
         lambda: da(q, kc[:, :8], vc[:, :8], tab, lens, starts),
         lambda: da(q, kc, vc, tab, lens, starts, out=torch.empty(2, 8, 32, device=DEV)),
         lambda: da(q.clone().requires_grad_(), kc, vc, tab, lens, starts),
-        lambda: da(q[0], kc, vc, tab, lens, starts),
+        lambda: da(q[0], kc, vc, tab, lens, starts), lambda: da(q, kc, vc, tab, lens, starts, out=q),
+        lambda: da(q, kc, vc, tab, lens, starts, scale=float("nan")),
+        lambda: da(q, kc, vc, tab, lens, starts, scale=float("inf")),
     ]
     for i, call in enumerate(bad):
         with pytest.raises(AssertionError):
