@@ -444,6 +444,7 @@ extern "C" int htree_draft_attention(const htree_cache* c, int32_t B, int32_t ro
   a.table = block_table, a.lens = lens, a.starts = starts, a.parents = parents;
   a.ws_o = (float*)workspace;
   a.ws_ml = a.ws_o + p.slots * p.R * p.D;
+  a.ws_chunk = (int32_t*)(a.ws_ml + p.slots * p.R * 2);
   a.table_stride = table_stride;
   a.q_row = q_row * es, a.q_head = q_head * es, a.o_row = out_row * es, a.o_head = out_head * es;
   a.k_page = c->k_page * es, a.k_token = c->k_token * es, a.k_head = c->k_head * es;

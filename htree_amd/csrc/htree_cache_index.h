@@ -72,7 +72,7 @@ __host__ __device__ inline DraftPlan draft_plan(int Dk, int Dv, int es, int B, i
   p.joins = p.target == 0 ? 0 : p.one_round ? rts * p.R : 1024;
   // a split request has at most twice the chunks its tokens fill
   p.slots = 2 * (int64_t)p.target;
-  p.bytes = p.slots * p.R * (p.D + 2) * 4;
+  p.bytes = p.target == 0 ? 0 : p.slots * p.R * (p.D + 2) * 4 + 16;
   return p;
 }
 

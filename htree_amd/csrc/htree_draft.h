@@ -26,6 +26,7 @@ struct DraftArgs {
   char* out;
   const int32_t *table, *lens, *starts, *parents;
   float* ws_o;   // [slots][R][D] output of a unit, relative to its max
+  int32_t* ws_chunk;  // tiles of a chunk, for the join
   float* ws_ml;  // [slots][R][2] max (log2 units) and sum
   int64_t table_stride;
   int64_t q_row, q_head, o_row, o_head;                                // bytes
@@ -112,34 +113,42 @@ struct DraftUnit {
 
 // The u-th piece of work where each group of rows of a request of `nch`
 // chunks makes per(nch) pieces; false past the last.
-template <int KT, int R, typename F>
+template <int KT, int R, bool JOIN, typename F>
 __device__ __forceinline__ bool draft_find(const DraftArgs& a, int64_t u, DraftUnit* o, F per) {
   const int lane = threadIdx.x & 63;
   const int cap = a.width << a.page_shift;
-  float w = 0.f;
-  if (a.target > 0) {
-    for (int b = lane; b < a.B; b += 64) {
-      const DraftReq r = draft_request(a, b);
-      w += (float)draft_tiles(r, cap, KT) * draft_row_groups(r, a.G, R);
+  int chunk;
+  if constexpr (JOIN) {
+    chunk = max(*a.ws_chunk, 1);
+  } else {
+    float w = 0.f;
+    if (a.target > 0) {
+      for (int b = lane; b < a.B; b += 64) {
+        const DraftReq r = draft_request(a, b);
+        w += (float)draft_tiles(r, cap, KT) * draft_row_groups(r, a.G, R);
+      }
+      w = add_xor32(add_xor16(row_sum16(w))) * a.Hkv;
     }
-    w = add_xor32(add_xor16(row_sum16(w))) * a.Hkv;
-  }
-  int chunk = draft_chunk(w, a.target);
-  if (a.target > 0 && a.B <= 64) {
-    // A chunk somewhat larger, where the units then all fit the GPU at once:
-    // else the last few of them start when the others are done.
-    int c = chunk;
-    for (int i = 0; i < 4; ++i) {
-      float units = 0.f;
-      if (lane < a.B) {
-        const DraftReq r = draft_request(a, lane);
-        units = (float)draft_chunks(draft_tiles(r, cap, KT), c) * draft_row_groups(r, a.G, R);
+    chunk = draft_chunk(w, a.target);
+    if (a.target > 0) {
+      if (a.B <= 64) {
+        // A chunk somewhat larger, where the units then all fit the GPU at
+        // once: else the last few of them start when the others are done.
+        int c = chunk;
+        for (int i = 0; i < 4; ++i) {
+          float units = 0.f;
+          if (lane < a.B) {
+            const DraftReq r = draft_request(a, lane);
+            units = (float)draft_chunks(draft_tiles(r, cap, KT), c) * draft_row_groups(r, a.G, R);
+          }
+          if (add_xor32(add_xor16(row_sum16(units))) * a.Hkv <= (float)a.target) {
+            chunk = c;
+            break;
+          }
+          c = draft_wider(c);
+        }
       }
-      if (add_xor32(add_xor16(row_sum16(units))) * a.Hkv <= (float)a.target) {
-        chunk = c;
-        break;
-      }
-      c = draft_wider(c);
+      if (blockIdx.x == 0 && threadIdx.x == 0) *a.ws_chunk = chunk;
     }
   }
   int64_t first = 0, slot = 0;
@@ -186,7 +195,7 @@ struct DraftPart {
 };
 template <int KT, int R>
 __device__ __forceinline__ bool draft_unit(const DraftArgs& a, DraftUnit* u, DraftPart* p) {
-  if (!draft_find<KT, R>(a, draft_near(blockIdx.x, a.near), u, [](int nch) { return nch; })) return false;
+  if (!draft_find<KT, R, false>(a, draft_near(blockIdx.x, a.near), u, [](int nch) { return nch; })) return false;
   const uint32_t rest = (uint32_t)u->index / (uint32_t)u->groups;
   p->rt = uniform(u->index - rest * u->groups);
   p->ch = uniform(rest / (uint32_t)a.Hkv);
@@ -1066,17 +1075,17 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void draft_rows_kernel(D
 // D / 4, a set holding a row.  Few chunks: each set takes a row and all its
 // chunks; many chunks, or few rows in all: the block takes a row and its sets
 // share the chunks.
-constexpr int kJoinSerial = 16;
+constexpr int kJoinSerial = 16;  // or as many as a set has threads
 template <typename T, int D, int KT, int R, int STEP>
 __global__ __launch_bounds__(256) void draft_join_kernel(DraftArgs a) {
   constexpr int OC = D / 4, NP = 256 / OC, RB = (R + NP - 1) / NP;
   __shared__ f32x4 acc[256];
   __shared__ float lsum[NP];
   const int tid = threadIdx.x, p = tid / OC, ch = tid % OC;
-  const int most = a.one_round ? 0 : kJoinSerial;
+  const int most = a.one_round ? 0 : kJoinSerial < OC ? kJoinSerial : OC;
   for (int64_t at = blockIdx.x;; at += gridDim.x) {
     DraftUnit u;
-    if (!draft_find<KT, R>(a, at, &u, [&](int nch) { return nch <= 1 ? 0 : nch <= most ? RB : R; }))
+    if (!draft_find<KT, R, true>(a, at, &u, [&](int nch) { return nch <= 1 ? 0 : nch <= most ? RB : R; }))
       return;  // uniform over the block
     const DraftReq rq = draft_request(a, u.b);
     const bool serial = u.nch <= most;
@@ -1091,31 +1100,41 @@ __global__ __launch_bounds__(256) void draft_join_kernel(DraftArgs a) {
     }
     const bool on = r < nrow;
     const int64_t base = u.slot + group, step = (int64_t)u.groups * a.Hkv;
-    const int c0 = serial ? 0 : p, dc = serial ? 1 : NP;
-    float big = -INFINITY;
-    if (on) {
-      if (serial) {
-        for (int c = 0; c < u.nch; ++c) big = fmaxf(big, a.ws_ml[((base + c * step) * R + rr) * 2]);
-      } else {
-        for (int c = tid & 63; c < u.nch; c += 64) big = fmaxf(big, a.ws_ml[((base + c * step) * R + rr) * 2]);
-      }
-    }
-    if (!serial) big = wave_max(big);
     f32x4 x = {0.f, 0.f, 0.f, 0.f};
     float sum = 0.f;
-    if (on) {
+    // (a chunk whose tokens the row does not see has max -inf and zeros)
+    if (serial) {
+      // a lane of the set has a chunk's max and sum
+      float mc = -INFINITY, lc = 0.f;
+      if (on && ch < u.nch) {
+        const float* ml = a.ws_ml + ((base + ch * step) * R + rr) * 2;
+        mc = ml[0], lc = ml[1];
+      }
+      float big = mc;
+#pragma unroll
+      for (int m = 1; m < OC; m <<= 1) big = fmaxf(big, __shfl_xor(big, m));
+      const float f = mc == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mc - big);
+      sum = lc * f;
+#pragma unroll
+      for (int m = 1; m < OC; m <<= 1) sum += __shfl_xor(sum, m);
+#pragma unroll 8
+      for (int c = 0; c < u.nch; ++c) {
+        const float fc = __shfl(f, (tid & 63) / OC * OC + c);
+        if (on) x += *(const f32x4*)(a.ws_o + ((base + c * step) * R + rr) * D + ch * 4) * fc;
+      }
+    } else {
+      float big = -INFINITY;
+      for (int c = tid & 63; c < u.nch; c += 64) big = fmaxf(big, a.ws_ml[((base + c * step) * R + rr) * 2]);
+      big = wave_max(big);
 #pragma unroll 4
-      for (int c = c0; c < u.nch; c += dc) {
+      for (int c = p; c < u.nch; c += NP) {
         const int64_t i = (base + c * step) * R + rr;
         const float mc = a.ws_ml[i * 2], lc = a.ws_ml[i * 2 + 1];
         const f32x4 oc = *(const f32x4*)(a.ws_o + i * D + ch * 4);
-        // a chunk whose tokens the row does not see has max -inf and zeros
         const float f = mc == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mc - big);
         x += oc * f;
         sum += lc * f;
       }
-    }
-    if (!serial) {
       acc[tid] = x;
       if (ch == 0) lsum[p] = sum;
       __syncthreads();

@@ -49,7 +49,7 @@ int main() {
     if (rows == 0) continue;
     const DraftPlan p = draft_plan(Dk, Dv, es, B, rows, G * Hkv, Hkv, width, 1 << shift);
     CHECK(p.D >= Dk && p.D >= Dv && p.R == 16 * p.MT * p.NW);
-    CHECK(p.bytes == p.slots * p.R * (p.D + 2) * 4);
+    CHECK(p.bytes == (p.target ? p.slots * p.R * (p.D + 2) * 4 + 16 : 0));
     const int KT = draft_tile(p.D, es, p.NW);
     CHECK(KT >= 16 && KT <= 64 && KT % 16 == 0);
     float tiles = 0;
