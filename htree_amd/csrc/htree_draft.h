@@ -1175,15 +1175,10 @@ int draft_launch_type(const DraftArgs& a, const DraftPlan& p, hipStream_t st);
 
 template <typename T, int D>
 int draft_launch_dim(const DraftArgs& a, const DraftPlan& p, hipStream_t st) {
-  constexpr bool F32 = sizeof(T) == 4;
-  if constexpr (!F32) {
-    constexpr DraftForm f = draft_rows_form(D, (int)sizeof(T));
-    if (p.NW > 1) return draft_launch<T, D, f.MT, f.NW>(a, p.units, p.joins, st);
+  if constexpr (sizeof(T) == 2) {
+    if (p.NW > 1) return draft_launch<T, D, 2, 4>(a, p.units, p.joins, st);
   }
   if (p.MT == 1) return draft_launch<T, D, 1, 1>(a, p.units, p.joins, st);
-  if constexpr (D <= 128) {
-    if (p.MT > 2) return draft_launch<T, D, F32 ? 3 : 4, 1>(a, p.units, p.joins, st);
-  }
   return draft_launch<T, D, 2, 1>(a, p.units, p.joins, st);
 }
 
