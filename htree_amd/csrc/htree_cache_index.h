@@ -48,10 +48,11 @@ __host__ __device__ inline DraftPlan draft_plan(int Dk, int Dv, int es, int B, i
   const int G = H / Hkv;
   const int64_t per = ((int64_t)rows * G + B - 1) / B;  // rows of a request, on average
   // Blocks of 16 or 32 rows of the first form, or, above 32 rows a request and
-  // in 16 bits, of 128 rows of the second.  16 requests of 16384 tokens, 4 KV heads, bf16:
-  // at 64 rows 200 us in blocks of 64 rows of the first form and 157 us in the second
-  // (D 128), 51.8 and 42 us (D 64), 49.7 and 48.8 us (D 32); at 32 rows and
-  // D 128 173 and 148 us, but 16 requests of 1000 tokens 21.7 and 34.2 us.
+  // in 16 bits, of 128 rows of the second.  Requests of 16384 tokens, 4 KV
+  // heads, bf16, 64 rows a request: 32 of them at D 128 take 200 us in blocks
+  // of 64 rows of the first form and 157 us in the second, 16 at D 64 51.8 and
+  // 42 us, 16 at D 32 49.7 and 48.8 us.  At 32 rows and D 128 it is 173 and
+  // 148 us, but 16 requests of 1000 tokens take 21.7 and 34.2 us.
   p.MT = per <= 16 ? 1 : 2;
   p.NW = per > 32 && es == 2 ? 4 : 1;
   p.R = 16 * p.MT * p.NW;

@@ -494,39 +494,45 @@ struct DraftWave {
       sc[mt][i][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[mt][i][e], a.c, nm[mt]));
     };
     if constexpr (F32) {
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int i = 0; i < NG; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            weigh(mt, i, e);
-            l[mt] += sc[mt][i][e];
-          }
-#pragma unroll
-      for (int i = 0; i < NG; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int row = 16 * i + 4 * g + e;
-#pragma unroll
-          for (int q = 0; q < NQ; q += S::VW) {
-            if constexpr (S::VW == 4) {
-              const f32x4 x = *(const f32x4*)(vb + row * ROWB + draft_swz_v<CPR, F32>(row, 4 * q + n16) * 16);
-#pragma unroll
-              for (int w = 0; w < 4; ++w)
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
-                  o[mt][q + w] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[w], sc[mt][i][e], o[mt][q + w], 0, 0, 0);
-            } else {
-              const f32x2 x = *(const f32x2*)(vb + row * ROWB + draft_swz_v<CPR, F32>(row, n16 >> 1) * 16 + (n16 & 1) * 8);
-#pragma unroll
-              for (int w = 0; w < 2; ++w)
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
-                  o[mt][q + w] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[w], sc[mt][i][e], o[mt][q + w], 0, 0, 0);
-            }
-          }
+      // a step: the dims of one read (VW a lane) times the lane's token e of
+      // group i.  The weights of the next group go into the products' shadow.
+      constexpr int VW = S::VW, QS = NQ / VW, NS = NG * 4 * QS, AHEAD = 4;
+      f32x4 f[AHEAD];
+      auto value = [&](int x) {
+        const int row = 16 * (x / QS / 4) + 4 * g + x / QS % 4, q = x % QS * VW;
+        if constexpr (VW == 4) {
+          f[x % AHEAD] = *(const f32x4*)(vb + row * ROWB + draft_swz_v<CPR, F32>(row, 4 * q + n16) * 16);
+        } else {
+          const f32x2 y = *(const f32x2*)(vb + row * ROWB + draft_swz_v<CPR, F32>(row, n16 >> 1) * 16 + (n16 & 1) * 8);
+          f[x % AHEAD] = f32x4{y[0], y[1], 0.f, 0.f};
         }
+      };
+      auto weights = [&](int i, int e) {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          weigh(mt, i, e);
+          l[mt] += sc[mt][i][e];
+        }
+      };
+#pragma unroll
+      for (int x = 0; x < AHEAD; ++x) value(x);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) weights(0, e);
+      __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+      for (int x = 0; x < NS; ++x) {
+        const int i = x / QS / 4, e = x / QS % 4, q = x % QS * VW;
+        const f32x4 v = f[x % AHEAD];
+#pragma unroll
+        for (int w = 0; w < VW; ++w)
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+            o[mt][q + w] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[w], sc[mt][i][e], o[mt][q + w], 0, 0, 0);
+        if (x + AHEAD < NS) value(x + AHEAD);
+        if (x % QS == 0 && i + 1 < NG) weights(i + 1, e);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      __builtin_amdgcn_s_setprio(0);
     } else {
       // a transposing read gives lane n16 of group g four tokens of dim n16:
       // it addresses token 4 g + n16 / 4, dims 4 (n16 % 4) ..
