@@ -9,11 +9,31 @@
 // new tokens are the rows of one matrix product, so each cached row is read
 // once for all of them.
 //
-// One block of four waves takes a unit: 16 MT rows of one (request, KV head)
-// and a chunk of its tokens.  The waves take the chunk's tiles of KT tokens
-// in turn, each on its own: no barrier until the end, where the four running
-// (max, sum, output) states meet in LDS.  Units of one request meet in a
-// second launch (draft_join_kernel) through the workspace.
+// One pass: scores S^T = K Q^T, weights exp2 of the scores against a running
+// max, output O^T = V^T P^T, all in matrix products of 16 x 16.  With the
+// tokens as the scores' rows, a lane holds the weights of exactly the tokens
+// that the second product takes from it: P never leaves the registers.
+//
+// A block of four waves takes a unit: a group of rows of one (request, KV
+// head) and a chunk of its tokens.  Chunks are cut so that the units fill the
+// GPU once, whatever the lengths; each block finds its own from the lengths,
+// which never leave the device.  Units of one request meet in a second launch
+// (draft_join_kernel) through the workspace.
+//   draft_kernel: up to 32 rows.  The waves take the chunk's tiles of tokens
+//     in turn, each on its own: no barrier until the end, where the four
+//     running (max, sum, output) states meet in LDS.
+//   draft_rows_kernel: 128 rows.  Each wave has 32 rows of its own and all of
+//     them take the same tiles.
+//
+// What bounds them (bf16, D 128, 16-token pages, launch and join together):
+//   64 requests of up to 16384 tokens, one token each, 32/4 heads: the cache's
+//     bytes, 276 us (4.9 TB/s).
+//   One request of 131008 tokens, 64 drafted, 64/8 heads: 304 us, 903 TFLOP/s,
+//     where a library product of 8192 x 8192 reaches 1125: the matrix unit is
+//     busy 40% of the time; each tile's softmax, and the latency that two
+//     waves per SIMD do not cover, is the rest.
+//   One request of 2048 tokens, one token: 7.5 + 4 us, a chain of dependent
+//     reads (lengths, pages, keys, states) and two launches.
 #pragma once
 
 #include "htree_cache_index.h"
@@ -25,18 +45,18 @@ struct DraftArgs {
   const char *q, *k, *v;
   char* out;
   const int32_t *table, *lens, *starts, *parents;
-  float* ws_o;   // [slots][R][D] output of a unit, relative to its max
+  float* ws_o;        // [slots][R][D] output of a unit, relative to its max
+  float* ws_ml;       // [slots][R][2] max (log2 units) and sum
   int32_t* ws_chunk;  // tiles of a chunk, for the join
-  float* ws_ml;  // [slots][R][2] max (log2 units) and sum
   int64_t table_stride;
   int64_t q_row, q_head, o_row, o_head;                                // bytes
   int64_t k_page, k_token, k_head, v_page, v_token, v_head;            // bytes
   int32_t B, rows, H, Hkv, G, Dk, Dv, width, page_shift, num_pages;
-  int32_t near;    // units that share tokens, on average
-  int32_t target;  // units to split into (0: one unit per group of rows)
-  float c, inv_c;  // |scale| * log2(e), not 0
+  int32_t near;       // units that share tokens, on average
+  int32_t target;     // units to split into (0: one unit per group of rows)
   int32_t one_round;  // the join's blocks take one piece of work each
-  int32_t negate;  // the scale is negative: the queries change sign
+  int32_t negate;     // the scale is negative: the queries change sign
+  float c, inv_c;     // |scale| * log2(e), not 0
 };
 
 template <typename T>
@@ -685,7 +705,8 @@ __device__ __forceinline__ void draft_store(const DraftArgs& a, int s0, int h, i
 
 // Few rows: the four waves of a block have the same 16 MT rows and take the
 // chunk's tiles in turn, each through LDS of its own, so that there is no
-// barrier before their states meet.
+// barrier before their states meet.  While it works on a tile a wave has the
+// loads of its next one in flight: 16 KB a wave, 128 KB a CU.
 template <typename T, int D, int MT>
 __global__ __launch_bounds__(256, draft_two(D, MT, sizeof(T)) ? 2 : 1) void draft_kernel(DraftArgs a) {
   using S = DraftShape<T, D>;
@@ -903,7 +924,10 @@ __device__ __forceinline__ void draft_step(const DraftArgs& a, const DraftCtx& c
 // Many rows: each wave of a block has 16 MT rows of its own, and all of them
 // take the same tiles, which the block copies into one of two LDS buffers
 // (directly, without registers) while it works on the other: one barrier a
-// tile.
+// tile.  One request of 131008 tokens, 64 drafted, 64/8 heads of 128, bf16:
+// 718 us with 64 rows and tiles of a wave's own, 366 with common tiles, 322
+// with the copies straight into LDS, 304 with them spread between the products
+// and the waves' priority raised there.
 // WHOLE: the head dims are D.
 template <typename T, int D, int MT, int NW, int KT, bool WHOLE>
 __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void draft_rows_kernel(DraftArgs a) {
@@ -1080,7 +1104,8 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void draft_rows_kernel(D
 // Joins the chunks of split requests.  The threads of a block are NP sets of
 // D / 4, a set holding a row.  Few chunks: each set takes a row and all its
 // chunks; many chunks, or few rows in all: the block takes a row and its sets
-// share the chunks.
+// share the chunks.  Bound by the read of the states, and by the launch: 512
+// states of 128 rows of 128 (34 MB) 13 us, those of a single token 4 us.
 constexpr int kJoinSerial = 16;  // or as many as a set has threads
 template <typename T, int D, int KT, int R, int STEP>
 __global__ __launch_bounds__(256) void draft_join_kernel(DraftArgs a) {

@@ -340,7 +340,8 @@ int htree_page_tables(int32_t B, int32_t rows, int32_t page_size, int32_t num_pa
  * d + Dk/2), and so are the queries q [rows, H, Dk] (may be NULL) into q_out
  * [rows, H, Dk], contiguous.  Rows whose slot or position is out of range
  * are not written; without a position q_out is zero.  Two rows with one slot
- * leave either's values there, or parts of both. */
+ * leave either's values there, or parts of both.  k, v and q are not parts of
+ * the cache. */
 int htree_cache_append(const htree_cache* c, int32_t rows, int32_t H, const void* k,
                        int64_t k_row, int64_t k_head, const void* v, int64_t v_row,
                        int64_t v_head, const void* q, int64_t q_row, int64_t q_head,
@@ -358,7 +359,10 @@ int htree_draft_attention_workspace_bytes(const htree_cache* c, int32_t B, int32
  * the drafted tree (without parents: the new tokens before it) and itself.
  * Tokens in pages outside the cache (-1 entries) or past the table are not
  * there; a row that sees nothing gets zeros.  Rows of `out` [rows, H, Dv]
- * behind the last request are left as they were. */
+ * behind the last request are left as they were.
+ * HTREE_EUNSUPPORTED: a table of more than 2^30 tokens, tokens of a page more
+ * than 2^26 bytes apart, more than 2^24 blocks of work
+ * ((rows H / H_kv / 16 + B + 512) H_kv). */
 int htree_draft_attention(const htree_cache* c, int32_t B, int32_t rows, int32_t H,
                           int32_t table_width, int64_t table_stride, float scale,
                           const void* q, int64_t q_row, int64_t q_head, const void* k_cache,
