@@ -34,8 +34,10 @@ def draft_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     tokens (int32 [B]) of the request.  Row j of a request sees the tokens
     before the new ones, its ancestors by parents (int32 [rows]: the index
     within the request of the token drafted before it, a smaller one, -1:
-    none) and itself; without parents the new tokens up to itself.  scale
-    defaults to K^-0.5.  Queries and keys come rotated.
+    none) and itself; without parents the new tokens up to itself.  (Branches
+    are walked token by token: drafts of tens or hundreds of tokens.  A chunk
+    of thousands belongs in a call without parents.)  scale defaults to
+    K^-0.5.  Queries and keys come rotated.
 
     Returns [rows, H, V] in q's dtype (`out`: written there, contiguous, no
     overlap with the inputs).  Rows that see nothing are zero; rows behind
