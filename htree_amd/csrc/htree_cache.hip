@@ -455,7 +455,7 @@ extern "C" int htree_draft_attention(const htree_cache* c, int32_t B, int32_t ro
   a.q_row = q_row * es, a.q_head = q_head * es, a.o_row = out_row * es, a.o_head = out_head * es;
   a.k_page = c->k_page * es, a.k_token = c->k_token * es, a.k_head = c->k_head * es;
   a.v_page = c->v_page * es, a.v_token = c->v_token * es, a.v_head = c->v_head * es;
-  a.B = B, a.rows = rows, a.H = H, a.Hkv = c->H_kv, a.G = H / c->H_kv, a.Dk = c->Dk, a.Dv = c->Dv;
+  a.B = B, a.rows = rows, a.Hkv = c->H_kv, a.G = H / c->H_kv, a.Dk = c->Dk, a.Dv = c->Dv;
   a.width = table_width, a.page_shift = log2i(c->page_size), a.num_pages = c->num_pages;
   a.target = p.target;
   a.near = p.near;

@@ -51,7 +51,7 @@ struct DraftArgs {
   int64_t table_stride;
   int64_t q_row, q_head, o_row, o_head;                                // bytes
   int64_t k_page, k_token, k_head, v_page, v_token, v_head;            // bytes
-  int32_t B, rows, H, Hkv, G, Dk, Dv, width, page_shift, num_pages;
+  int32_t B, rows, Hkv, G, Dk, Dv, width, page_shift, num_pages;
   int32_t near;       // units that share tokens, on average
   int32_t target;     // units to split into (0: one unit per group of rows)
   int32_t one_round;  // the join's blocks take one piece of work each
