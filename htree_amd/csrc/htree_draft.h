@@ -358,6 +358,12 @@ struct DraftWave {
   static constexpr bool F16 = std::is_same<T, _Float16>::value;
   static constexpr float kUp = F16 ? 11.f : 0.f, kLag = F16 ? 4.f : 8.f;
   float nm[MT], top[MT];
+  // Where the max is past kFar log2 units, the product's rounding to fp32 no
+  // longer leaves a weight where it belongs (half a unit at 2^24, and past 2^31
+  // the max's own weight overflows or is zero).  There the max itself, `top`, is
+  // subtracted from the scores before the product, and nm is kUp.
+  static constexpr float kFar = 4194304.f;  // 2^22
+  int was_far;  // some row of the wave has been there (the same in all lanes)
   // the weights' sum: whole for 16-bit types, which have it from a product
   // with ones, a quarter of it in each lane for fp32
   float l[MT];
@@ -400,6 +406,7 @@ struct DraftWave {
 #pragma unroll
       for (int q = 0; q < NQ; ++q) o[mt][q] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
+    was_far = 0;
   }
 
   // whether row mt's token sees the request's token `key` < kend
@@ -502,15 +509,37 @@ struct DraftWave {
         for (int e = 0; e < 4; ++e) mx = fmaxf(mx, sc[mt][i][e]);
       if (__any(mx > top[mt])) {
         mx = max_xor32(max_xor16(mx));
+        float t = mx + kLag * a.inv_c;
+        if (__any(mx > top[mt] && fabsf(t) * a.c >= kFar)) was_far = 1;
         if (mx > top[mt]) {
-          const float mn = kUp - mx * a.c, al = top[mt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mn - nm[mt]);
+          float mn = kUp - mx * a.c, al = mn - nm[mt];
+          if (was_far) {
+            const bool was = far(a, mt);
+            if (was) al = top[mt] * a.c - mx * a.c;
+            if (fabsf(t) * a.c >= kFar) {
+              t = mx;
+              if (was) al = (top[mt] - mx) * a.c;
+              if (fabsf(mx) * a.c >= kFar) mn = kUp;
+            }
+          }
           // (before the first score there is nothing to rescale, but NaN stays)
+          al = top[mt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(al);
           nm[mt] = mn;
-          top[mt] = mx + kLag * a.inv_c;
+          top[mt] = t;
           l[mt] *= al;
 #pragma unroll
           for (int q = 0; q < NQ; ++q) o[mt][q] *= al;
         }
+      }
+    }
+    if (was_far) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        const float m = far(a, mt) ? top[mt] : 0.f;
+#pragma unroll
+        for (int i = 0; i < NG; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[mt][i][e] -= m;
       }
     }
   }
@@ -650,9 +679,11 @@ struct DraftWave {
           const int d = F32 ? 16 * s + 4 * g + e : 32 * s + 8 * g + e;
           if (d < a.Dk) x += q_at(mt, s, e) * Io<T>::ld(kp + d);
         }
-      x = add_xor32(add_xor16(x)) * a.c;
+      x = add_xor32(add_xor16(x));
       const bool see = sees(a, c, mt, key);
-      const float p = __builtin_amdgcn_exp2f(x + nm[mt]);
+      // (the sum's order is another than the product's: past kFar a score could
+      // pass the max by more than a weight can hold)
+      const float p = __builtin_amdgcn_exp2f((far(a, mt) ? fminf(x - top[mt], 0.f) * a.c : x * a.c) + nm[mt]);
 #pragma unroll
       for (int q = 0; q < NQ; ++q)
 #pragma unroll
@@ -671,7 +702,13 @@ struct DraftWave {
   __device__ __forceinline__ float sum(int mt) const {
     return F32 ? add_xor32(add_xor16(l[mt])) : l[mt];
   }
-  __device__ __forceinline__ float peak(int mt) const { return top[mt] == -INFINITY ? -INFINITY : -nm[mt]; }
+  __device__ __forceinline__ float peak(const DraftArgs& a, int mt) const {
+    return top[mt] == -INFINITY ? -INFINITY : far(a, mt) ? top[mt] * a.c - kUp : -nm[mt];
+  }
+  // whether the max is past kFar (`top` is then the max itself)
+  __device__ __forceinline__ bool far(const DraftArgs& a, int mt) const {
+    return fabsf(top[mt]) * a.c >= kFar && top[mt] != -INFINITY;
+  }
 
   // the lane's part of row n16 of group mt, times f, into 16 fp32 rows at dst
   __device__ __forceinline__ void put(float* dst, int mt, float f) const {
@@ -864,7 +901,7 @@ __global__ __launch_bounds__(256, draft_two(D, MT, sizeof(T)) ? 2 : 1) void draf
   for (int mt = 0; mt < MT; ++mt) {
     const float sum = w.sum(mt);
     if (w.g == 0) {
-      ml[wv][mt * 16 + w.n16][0] = w.peak(mt);
+      ml[wv][mt * 16 + w.n16][0] = w.peak(z, mt);
       ml[wv][mt * 16 + w.n16][1] = sum;
     }
   }
@@ -877,7 +914,7 @@ __global__ __launch_bounds__(256, draft_two(D, MT, sizeof(T)) ? 2 : 1) void draf
     for (int i = 0; i < NW; ++i) mm = fmaxf(mm, ml[i][mt * 16 + w.n16][0]);
     // a wave that saw no token of the row adds nothing (NaN scores leave the
     // max alone and make sums NaN, which stay)
-    const float pk = w.peak(mt);
+    const float pk = w.peak(z, mt);
     w.put((float*)(lds + wv * WAVE_LDS), mt, pk == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(pk - mm));
     __syncthreads();
     for (int i = threadIdx.x; i < 16 * S::OC; i += 256) {
@@ -1089,7 +1126,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void draft_rows_kernel(D
   float* my = (float*)(wv < NW / 2 ? lds0 : lds1) + wv % (NW / 2) * 16 * D;
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
-    const float l = w.sum(mt), m = w.peak(mt);
+    const float l = w.sum(mt), m = w.peak(z, mt);
     w.put(my, mt, 1.f);
     wave_sync();
 #pragma unroll
