@@ -4,6 +4,8 @@
 // (htree_draft.h).
 #include "htree_draft.h"
 
+#include <cmath>
+
 namespace htree {
 
 // ---------------------------------------------------------------- tables
@@ -434,6 +436,7 @@ extern "C" int htree_draft_attention(const htree_cache* c, int32_t B, int32_t ro
                                      void* workspace, int64_t workspace_bytes, void* stream) {
   const int rc = draft_check(c, B, rows, H, table_width);
   if (rc) return rc;
+  if (!std::isfinite(scale * kLog2e)) return HTREE_ESHAPE;
   if (B == 0 || rows == 0) return HTREE_OK;
   if (!q || !k_cache || !v_cache || !lens || !starts || !out || (table_width && !block_table)) return HTREE_ENULL;
   if (B > 1 && table_stride < table_width) return HTREE_ESHAPE;

@@ -4,7 +4,6 @@ The cache, block tables and slots are cache.py's."""
 from __future__ import annotations
 
 import ctypes
-import math
 from functools import lru_cache
 from typing import Optional
 
@@ -12,6 +11,8 @@ import torch
 
 from . import _native as N
 from .cache import MAX_REQUEST_TOKENS, _ints, aligned_rows, check_table, native_cache, overlap
+
+MAX_SCALE = 2.35e38  # scale * log2(e) is an fp32 number
 
 
 @lru_cache(maxsize=256)
@@ -37,7 +38,7 @@ def draft_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     none) and itself; without parents the new tokens up to itself.  (Branches
     are walked token by token: drafts of tens or hundreds of tokens.  A chunk
     of thousands belongs in a call without parents.)  scale defaults to
-    K^-0.5.  Queries and keys come rotated.
+    K^-0.5, and is at most MAX_SCALE in size.  Queries and keys come rotated.
 
     Returns [rows, H, V] in q's dtype (`out`: written there, contiguous, no
     overlap with the inputs).  Rows that see nothing are zero; rows behind
@@ -78,7 +79,7 @@ def draft_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         assert not any(overlap(out, x) for x in (q, k_cache, v_cache, block_table, lens, starts, parents)), \
             "out must not overlap the inputs"
     scale = K ** -0.5 if scale is None else float(scale)
-    assert math.isfinite(scale), f"scale must be finite, got {scale}"
+    assert abs(scale) <= MAX_SCALE, f"scale must be a number of at most {MAX_SCALE} in size, got {scale}"
     if B == 0 or rows == 0:
         return out
     q = aligned_rows(q)

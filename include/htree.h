@@ -362,6 +362,7 @@ int htree_draft_attention_workspace_bytes(const htree_cache* c, int32_t B, int32
  * behind the last request are left as they were.
  * Branches of the tree are walked token by token, for tens or hundreds of
  * drafts; a chunk of thousands of tokens belongs in a call without parents.
+ * HTREE_ESHAPE: scale * log2(e) is not a finite fp32 number (among others).
  * HTREE_EUNSUPPORTED: a table of more than 2^30 tokens, tokens of a page more
  * than 2^26 bytes apart, more than 2^24 blocks of work
  * ((rows H / H_kv / 16 + B + 512) H_kv). */
