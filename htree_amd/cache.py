@@ -25,6 +25,7 @@ from functools import lru_cache
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as N
 
@@ -55,6 +56,16 @@ def overlap(a: torch.Tensor, b: Optional[torch.Tensor]) -> bool:
     def end(t):
         return t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
     return b is not None and a.numel() > 0 and b.numel() > 0 and a.data_ptr() < end(b) and b.data_ptr() < end(a)
+
+
+def no_derivatives(name: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Refuses tensors whose gradient or forward-mode tangent a call would lose."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            assert t is None or not t.requires_grad, f"{name} has no backward"
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            assert t is None or forward_ad.unpack_dual(t).tangent is None, f"{name} has no forward-mode derivative"
 
 
 def check_table(block_table: torch.Tensor, B: int, device) -> None:
@@ -199,9 +210,7 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
         assert n == 1 or (x > 0 and y > 0), "k_cache and v_cache must not be expanded"
     assert slots.dtype is torch.int64 and slots.shape == (rows,) and slots.is_contiguous() \
         and slots.device == dev, f"slots must be a contiguous int64 tensor [{rows}] on {dev}"
-    if torch.is_grad_enabled():
-        assert not (k.requires_grad or v.requires_grad or (q is not None and q.requires_grad)), \
-            "cache_append has no backward"
+    no_derivatives("cache_append", k, v, q, cos, sin, k_cache, v_cache)
     assert (cos is None) == (sin is None) == (positions is None), "positions, cos and sin go together"
     H, rope_rows, q_out, q_row, q_head = 0, 0, None, 0, 0
     if cos is not None:

@@ -10,7 +10,7 @@ from typing import Optional
 import torch
 
 from . import _native as N
-from .cache import MAX_REQUEST_TOKENS, _ints, aligned_rows, check_table, native_cache, overlap
+from .cache import MAX_REQUEST_TOKENS, _ints, aligned_rows, check_table, native_cache, no_derivatives, overlap
 
 MAX_SCALE = 2.35e38  # scale * log2(e) is an fp32 number
 
@@ -67,9 +67,7 @@ def draft_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         f"a request's table holds at most {MAX_REQUEST_TOKENS} tokens, got {width * c.page_size}"
     if parents is not None:
         _ints(parents, "parents", rows, dev)
-    if torch.is_grad_enabled():
-        assert not (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad), \
-            "draft_attention has no backward"
+    no_derivatives("draft_attention", q, k_cache, v_cache, out)
     if out is None:
         out = torch.empty((rows, H, c.Dv), dtype=dtype, device=dev)
     else:
