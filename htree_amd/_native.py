@@ -23,6 +23,7 @@ HTREE_ECONFIG = -3
 HTREE_EUNSUPPORTED = -4
 HTREE_EWORKSPACE = -5
 HTREE_ESCRATCH = -6
+HTREE_EOVERLAP = -7
 
 DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 

@@ -196,8 +196,8 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     sums are fp32, rounded once.  Rows whose slot or position is out of range
     are not written, and a query without a position is zero.  The slots of a
     call are distinct; two rows with one slot leave either's values there,
-    or parts of both.  k, v and q are not parts of the cache that is written
-    (rows moved within it are copied out first: cache.view(...)[slots])."""
+    or parts of both.  k, v and q may be parts of the cache: where their
+    memory's range overlaps its, they are copied before anything is written."""
     c = native_cache(k_cache, v_cache)
     dtype, dev = k_cache.dtype, k_cache.device
     assert k.dim() == 3 and v.dim() == 3, "k / v must be [rows, H_kv, D]"
@@ -228,14 +228,20 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
         assert q.dtype is dtype and q.device == dev, "q must have k's dtype and device"
         H = q.shape[1]
         q = aligned_rows(q)
-        q_row, q_head, _ = q.stride()
         q_out = torch.empty((rows, H, c.Dk), dtype=dtype, device=dev)
     k, v = aligned_rows(k), aligned_rows(v)
-    k_row, k_head, _ = k.stride()
-    v_row, v_head, _ = v.stride()
-    rc = N.launch(N.lib().htree_cache_append, dev, c, rows, H, k.data_ptr(), k_row, k_head, v.data_ptr(), v_row, v_head,
-                  N.address(q), q_row, q_head, slots.data_ptr(), N.address(positions), N.address(cos), N.address(sin),
-                  rope_rows, N.address(q_out), k_cache.data_ptr(), v_cache.data_ptr())
+    for copied in (False, True):
+        if copied:
+            k, v, q = (None if x is None else x.clone(memory_format=torch.contiguous_format) for x in (k, v, q))
+        k_row, k_head, _ = k.stride()
+        v_row, v_head, _ = v.stride()
+        if q is not None:
+            q_row, q_head, _ = q.stride()
+        rc = N.launch(N.lib().htree_cache_append, dev, c, rows, H, k.data_ptr(), k_row, k_head, v.data_ptr(), v_row,
+                      v_head, N.address(q), q_row, q_head, slots.data_ptr(), N.address(positions), N.address(cos),
+                      N.address(sin), rope_rows, N.address(q_out), k_cache.data_ptr(), v_cache.data_ptr())
+        if rc != N.HTREE_EOVERLAP:
+            break
     if rc:
         N.check(rc, "htree_cache_append")
     return q_out

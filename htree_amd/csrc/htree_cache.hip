@@ -307,6 +307,14 @@ static int cache_check(const htree_cache* c) {
   if (c->k_token * es > (1 << 26) || c->v_token * es > (1 << 26)) return HTREE_EUNSUPPORTED;
   return HTREE_OK;
 }
+struct Range {
+  const void* at;
+  int64_t bytes;
+};
+static bool overlap(const Range& a, const Range& b) {
+  const char *x = (const char*)a.at, *y = (const char*)b.at;
+  return a.bytes > 0 && b.bytes > 0 && x < y + b.bytes && y < x + a.bytes;
+}
 static bool off16(const void* p) { return ((uintptr_t)p & 15) != 0; }
 static int log2i(int x) { return __builtin_ctz((unsigned)x); }
 
@@ -382,6 +390,21 @@ extern "C" int htree_cache_append(const htree_cache* c, int32_t rows, int32_t H,
   for (int64_t s : st)
     if (s < 0 || s * es % 16) return HTREE_EUNSUPPORTED;
   if (off16(k) || off16(v) || off16(q) || off16(q_out) || off16(k_cache) || off16(v_cache)) return HTREE_EUNSUPPORTED;
+  // A source in the cache's range: a row could be read after another one's
+  // write.  (The two caches' ranges may overlap: keys beside values in a page.)
+  const auto rows_end = [&](int64_t row, int64_t head, int heads, int D) {
+    return ((rows - 1) * row + (heads - 1) * head + D) * es;
+  };
+  const auto cache_end = [&](int64_t page, int64_t token, int64_t head, int D) {
+    return ((c->num_pages - 1) * page + (c->page_size - 1) * token + (c->H_kv - 1) * head + D) * es;
+  };
+  const Range from[3] = {{k, rows_end(k_row, k_head, c->H_kv, c->Dk)}, {v, rows_end(v_row, v_head, c->H_kv, c->Dv)},
+                         {q, q ? rows_end(q_row, q_head, H, c->Dk) : 0}};
+  const Range to[2] = {{k_cache, cache_end(c->k_page, c->k_token, c->k_head, c->Dk)},
+                       {v_cache, cache_end(c->v_page, c->v_token, c->v_head, c->Dv)}};
+  for (const Range& x : from)
+    for (const Range& y : to)
+      if (overlap(x, y)) return HTREE_EOVERLAP;
   AppendArgs a;
   a.k = (const char*)k, a.v = (const char*)v, a.q = (const char*)q;
   a.kc = (char*)k_cache, a.vc = (char*)v_cache, a.qo = (char*)q_out;

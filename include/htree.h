@@ -54,8 +54,10 @@ enum htree_status {
                               backward level of 2^31 or more entries
                               (B * T * H_kv * min(top_k, parents)) */
   HTREE_EWORKSPACE = -5,   /* workspace too small */
-  HTREE_ESCRATCH = -6      /* htree_backward_noalloc: the problem's backward
+  HTREE_ESCRATCH = -6,     /* htree_backward_noalloc: the problem's backward
                               needs more than HTREE_NOALLOC_SCRATCH_BYTES */
+  HTREE_EOVERLAP = -7      /* htree_cache_append: k, v or q lies in the range
+                              of the cache that is written */
 };
 
 /* Size of the device array htree_backward_noalloc works in (one per GPU). */
@@ -341,7 +343,9 @@ int htree_page_tables(int32_t B, int32_t rows, int32_t page_size, int32_t num_pa
  * [rows, H, Dk], contiguous.  Rows whose slot or position is out of range
  * are not written; without a position q_out is zero.  Two rows with one slot
  * leave either's values there, or parts of both.  k, v and q are not parts of
- * the cache. */
+ * the cache: rows that another one's write could change first.
+ * HTREE_EOVERLAP: one of them shares its range of memory, gaps included, with
+ * k_cache's or v_cache's; copy it out first. */
 int htree_cache_append(const htree_cache* c, int32_t rows, int32_t H, const void* k,
                        int64_t k_row, int64_t k_head, const void* v, int64_t v_row,
                        int64_t v_head, const void* q, int64_t q_row, int64_t q_head,
