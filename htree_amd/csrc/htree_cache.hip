@@ -52,17 +52,6 @@ __device__ __forceinline__ int64_t tab_scan(int B, int32_t most, int32_t* dst, i
   return all;
 }
 
-// last b with s[b] <= x (s ascending, s[0] = 0, x >= 0); B >= 1
-__device__ __forceinline__ int tab_find(const int32_t* s, int B, int x) {
-  int lo = 0, hi = B;  // s[lo] <= x, and s[hi] > x or hi == B
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (s[mid] <= x) lo = mid;
-    else hi = mid;
-  }
-  return lo;
-}
-
 // Blocks 0 .. page_blocks - 1 write the new pages' table entries, the others
 // the rows' slots and positions, `tiles` times 256 each.  Each block sums the
 // lengths again (two loads and two scans), which is less than a second launch;
@@ -102,7 +91,7 @@ __global__ __launch_bounds__(256) void page_tables_kernel(TabArgs a) {
     for (int x = 0; x < a.tiles; ++x) {
       const int64_t i = ((int64_t)blockIdx.x * a.tiles + x) * kTabTile + tid;
       if (i >= total) return;
-      const int b = tab_find(first, a.B, (int)i);
+      const int b = table_find(first, a.B, (int)i);
       const int64_t j = had(b) + i - first[b];
       if (j < a.width) a.table[b * a.table_stride + j] = fresh(i);
     }
@@ -121,7 +110,7 @@ __global__ __launch_bounds__(256) void page_tables_kernel(TabArgs a) {
     int64_t slot = -1;
     int pos = -1;
     if (row < starts[a.B]) {
-      const int b = tab_find(starts, a.B, (int)row);
+      const int b = table_find(starts, a.B, (int)row);
       const int ctx = max(a.ctx[b], 0), s0 = starts[b], j = (int)row - s0;
       const int64_t at = (int64_t)ctx + j;
       const int64_t pi = at >> a.page_shift, h = had(b);

@@ -1,9 +1,11 @@
 // Index arithmetic of the paged cache's kernels (htree_cache.hip,
 // htree_draft.h): how an attention call is split into units, which rows,
-// tokens and pages a unit touches, and which pages and slots a request's new
-// tokens get.  Lengths, tables and lists are device data that no host checks,
-// so everything read from them goes through these functions, and the host
-// replay over damaged inputs (tests/cache_replay_check.cpp) runs the same ones.
+// tokens and pages a unit touches, which states a piece of the join reads, and
+// which pages a request's new tokens get.  Lengths, tables and lists are device
+// data that no host checks: the host replays over ordinary and damaged ones
+// (tests/cache_replay_check.cpp, tests/cache_units_check.cpp) run these same
+// functions.  The kernels alone have the sums over lanes, and the rows' slots
+// and positions.
 #ifndef HTREE_CACHE_INDEX_H_
 #define HTREE_CACHE_INDEX_H_
 
@@ -128,6 +130,17 @@ __host__ __device__ inline int draft_chunk(float tiles, int target) {
   return c > (float)(1 << 29) ? 1 << 30 : ((int)c + 4) / 4 * 4;
 }
 __host__ __device__ inline int draft_wider(int chunk) { return chunk + chunk / 16 + 1; }
+// A chunk somewhat larger, where the units(chunk) of the call then all fit the
+// GPU at once: else the last few of them start when the others are done.
+template <typename F>
+__host__ __device__ inline int draft_widen(int chunk, int target, F units) {
+  int c = chunk;
+  for (int i = 0; i < 4; ++i) {
+    if (units(c) <= (float)target) return c;
+    c = draft_wider(c);
+  }
+  return chunk;
+}
 // chunks of a request, and tiles of each: even parts
 __host__ __device__ inline int draft_chunks(int tiles, int chunk) {
   const int n = (int)(((int64_t)tiles + chunk - 1) / chunk);
@@ -137,6 +150,85 @@ __host__ __device__ inline int draft_chunks(int tiles, int chunk) {
 __host__ __device__ inline int draft_part(int tiles, int chunks) {
   const int n = (tiles + chunks - 1) / chunks;
   return n < 1 ? 1 : n;
+}
+
+// Where a block's work is.  The requests whose tokens make more than one chunk
+// get workspace slots, one per unit.
+struct DraftUnit {
+  int b, nch;
+  int chunk;   // tiles of each chunk
+  int slot;    // of the request's first unit
+  int index;   // of the work within the request
+  int groups;  // of rows, of one KV head
+};
+// What a request has of a call's work, where each group of rows of a request
+// of `nch` chunks makes per(nch) pieces.
+struct DraftShare {
+  int nch, tiles;
+  int groups;  // of rows, of all KV heads
+  int pieces, slots;
+};
+template <typename F>
+__host__ __device__ inline DraftShare draft_share(const DraftReq& r, int cap, int KT, int G, int R, int Hkv,
+                                                  int chunk, F per) {
+  DraftShare s;
+  s.tiles = draft_tiles(r, cap, KT);
+  s.nch = draft_chunks(s.tiles, chunk);
+  s.groups = draft_row_groups(r, G, R) * Hkv;
+  s.pieces = draft_pieces(per(s.nch), s.groups);
+  s.slots = draft_pieces(s.nch > 1 ? s.nch : 0, s.groups);
+  return s;
+}
+// the work of request b's share that is `index` pieces into it, `slot` the
+// first of the request's slots
+__host__ __device__ inline DraftUnit draft_pick(int b, int nch, int tiles, int groups, int64_t slot,
+                                                int64_t index, int Hkv) {
+  return DraftUnit{b, nch, draft_part(tiles, nch), (int)slot, (int)index, groups / Hkv};
+}
+
+// A unit: group of rows rt (fastest), KV head h, chunk ch of a request.  The
+// groups of rows of one head and chunk read the same tokens: `near` units in a
+// row go to blocks of one of the 8 dies (block x runs on die x % 8), whose L2
+// then serves all but the first.
+struct DraftPart {
+  int h, rt, ch;
+  int slot;  // -1: the request has one chunk
+};
+__host__ __device__ inline DraftPart draft_unit_part(const DraftUnit& u, int Hkv) {
+  const uint32_t rest = (uint32_t)u.index / (uint32_t)u.groups;
+  DraftPart p;
+  p.rt = (int)(u.index - rest * u.groups);
+  p.ch = (int)(rest / (uint32_t)Hkv);
+  p.h = (int)(rest - p.ch * Hkv);
+  p.slot = u.nch > 1 ? u.slot + u.index : -1;
+  return p;
+}
+
+// A piece of the join: a row of a group of rows, its chunks shared by a
+// block's sets, or, of requests of up to `most` chunks, a row for each of the
+// `sets`.
+__host__ __device__ inline int draft_join_pieces(int nch, int most, int R, int sets) {
+  return nch <= 1 ? 0 : nch <= most ? (R + sets - 1) / sets : R;
+}
+struct DraftJoin {
+  int h, rt;
+  int r0, nrow;        // rows of the group, from .. to
+  int row;             // the first row's place in the group
+  bool serial;         // a row for each set
+  int64_t base, step;  // slot of chunk c: base + c step
+};
+__host__ __device__ inline DraftJoin draft_join(const DraftUnit& u, const DraftReq& r, int G, int Hkv, int R,
+                                                int step, int sets, int most) {
+  DraftJoin j;
+  j.serial = u.nch <= most;
+  const int per = draft_join_pieces(u.nch, most, R, sets), sub = u.index % per, group = u.index / per;
+  j.h = group / u.groups, j.rt = group % u.groups;
+  const int even = draft_even(r, G, R, step), end = r.n * G;
+  j.r0 = j.rt * even;
+  j.nrow = end < j.r0 + even ? end : j.r0 + even;
+  j.row = j.serial ? sub * sets : sub;
+  j.base = u.slot + group, j.step = (int64_t)u.groups * Hkv;
+  return j;
 }
 
 // What a unit's rows see: tokens [0, kend), tiles [t0, t1) in its chunk
@@ -168,6 +260,17 @@ __host__ __device__ inline int draft_parent(int p, int j) { return p >= 0 && p <
 // pages of n tokens
 __host__ __device__ inline int64_t table_pages(int64_t tokens, int shift) {
   return (tokens + (((int64_t)1 << shift) - 1)) >> shift;
+}
+
+// last b with s[b] <= x (s ascending, s[0] = 0, x >= 0); B >= 1
+__host__ __device__ inline int table_find(const int32_t* s, int B, int x) {
+  int lo = 0, hi = B;  // s[lo] <= x, and s[hi] > x or hi == B
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (s[mid] <= x) lo = mid;
+    else hi = mid;
+  }
+  return lo;
 }
 
 }  // namespace htree

@@ -121,15 +121,7 @@ __device__ __forceinline__ DraftReq draft_request(const DraftArgs& a, int b) {
 
 // Where a block's work is.  Every wave works it out from the lengths: with
 // `target` units wanted, a chunk is about the same number of tiles everywhere,
-// so a long request gets more units than a short one.  The requests whose tokens
-// make more than one chunk get workspace slots, one per unit.
-struct DraftUnit {
-  int b, nch;
-  int chunk;   // tiles of each chunk
-  int slot;    // of the request's first unit
-  int index;   // of the work within the request
-  int groups;  // of rows, of one KV head
-};
+// so a long request gets more units than a short one.
 
 // The u-th piece of work where each group of rows of a request of `nch`
 // chunks makes per(nch) pieces; false past the last.
@@ -151,38 +143,24 @@ __device__ __forceinline__ bool draft_find(const DraftArgs& a, int64_t u, DraftU
     }
     chunk = draft_chunk(w, a.target);
     if (a.target > 0) {
-      if (a.B <= 64) {
-        // A chunk somewhat larger, where the units then all fit the GPU at
-        // once: else the last few of them start when the others are done.
-        int c = chunk;
-        for (int i = 0; i < 4; ++i) {
+      if (a.B <= 64)
+        chunk = draft_widen(chunk, a.target, [&](int c) {
           float units = 0.f;
           if (lane < a.B) {
             const DraftReq r = draft_request(a, lane);
             units = (float)draft_chunks(draft_tiles(r, cap, KT), c) * draft_row_groups(r, a.G, R);
           }
-          if (add_xor32(add_xor16(row_sum16(units))) * a.Hkv <= (float)a.target) {
-            chunk = c;
-            break;
-          }
-          c = draft_wider(c);
-        }
-      }
+          return add_xor32(add_xor16(row_sum16(units))) * a.Hkv;
+        });
       if (blockIdx.x == 0 && threadIdx.x == 0) *a.ws_chunk = chunk;
     }
   }
   int64_t first = 0, slot = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
     const int b = b0 + lane;
-    int nch = 0, rt = 0, tiles = 0;
-    if (b < a.B) {
-      const DraftReq r = draft_request(a, b);
-      tiles = draft_tiles(r, cap, KT);
-      nch = draft_chunks(tiles, chunk);
-      rt = draft_row_groups(r, a.G, R) * a.Hkv;
-    }
-    const int mine = draft_pieces(per(nch), rt), sl = draft_pieces(nch > 1 ? nch : 0, rt);
-    int pu = mine, ps = sl;
+    DraftShare mine = {};
+    if (b < a.B) mine = draft_share(draft_request(a, b), cap, KT, a.G, R, a.Hkv, chunk, per);
+    int pu = mine.pieces, ps = mine.slots;
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) {
       const int x = __shfl_up(pu, m), y = __shfl_up(ps, m);
@@ -191,12 +169,9 @@ __device__ __forceinline__ bool draft_find(const DraftArgs& a, int64_t u, DraftU
     const uint64_t hit = __ballot(first + pu > u);
     if (hit) {
       const int l = __builtin_ctzll(hit);
-      o->b = b0 + l;
-      o->nch = __builtin_amdgcn_readlane(nch, l);
-      o->chunk = draft_part(__builtin_amdgcn_readlane(tiles, l), o->nch);
-      o->slot = (int)slot + __builtin_amdgcn_readlane(ps - sl, l);
-      o->index = (int)(u - first) - __builtin_amdgcn_readlane(pu - mine, l);
-      o->groups = __builtin_amdgcn_readlane(rt, l) / a.Hkv;
+      *o = draft_pick(b0 + l, __builtin_amdgcn_readlane(mine.nch, l), __builtin_amdgcn_readlane(mine.tiles, l),
+                      __builtin_amdgcn_readlane(mine.groups, l), slot + __builtin_amdgcn_readlane(ps - mine.slots, l),
+                      u - first - __builtin_amdgcn_readlane(pu - mine.pieces, l), a.Hkv);
       return true;
     }
     first += __builtin_amdgcn_readlane(pu, 63);
@@ -205,22 +180,12 @@ __device__ __forceinline__ bool draft_find(const DraftArgs& a, int64_t u, DraftU
   return false;
 }
 
-// A unit: group of rows rt (fastest), KV head h, chunk ch of a request.  The
-// groups of rows of one head and chunk read the same tokens: `near` units in a
-// row go to blocks of one of the 8 dies (block x runs on die x % 8), whose L2
-// then serves all but the first.
-struct DraftPart {
-  int h, rt, ch;
-  int slot;  // -1: the request has one chunk
-};
+// the unit of this block
 template <int KT, int R>
 __device__ __forceinline__ bool draft_unit(const DraftArgs& a, DraftUnit* u, DraftPart* p) {
   if (!draft_find<KT, R, false>(a, draft_near(blockIdx.x, a.near), u, [](int nch) { return nch; })) return false;
-  const uint32_t rest = (uint32_t)u->index / (uint32_t)u->groups;
-  p->rt = uniform(u->index - rest * u->groups);
-  p->ch = uniform(rest / (uint32_t)a.Hkv);
-  p->h = uniform(rest - p->ch * a.Hkv);
-  p->slot = u->nch > 1 ? u->slot + u->index : -1;
+  *p = draft_unit_part(*u, a.Hkv);
+  p->rt = uniform(p->rt), p->ch = uniform(p->ch), p->h = uniform(p->h);
   return true;
 }
 
@@ -1159,28 +1124,26 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void draft_rows_kernel(D
 constexpr int kJoinSerial = 16;  // or as many as a set has threads
 template <typename T, int D, int KT, int R, int STEP>
 __global__ __launch_bounds__(256) void draft_join_kernel(DraftArgs a) {
-  constexpr int OC = D / 4, NP = 256 / OC, RB = (R + NP - 1) / NP;
+  constexpr int OC = D / 4, NP = 256 / OC;
   __shared__ f32x4 acc[256];
   __shared__ float lsum[NP];
   const int tid = threadIdx.x, p = tid / OC, ch = tid % OC;
   const int most = a.one_round ? 0 : kJoinSerial < OC ? kJoinSerial : OC;
   for (int64_t at = blockIdx.x;; at += gridDim.x) {
     DraftUnit u;
-    if (!draft_find<KT, R, true>(a, at, &u, [&](int nch) { return nch <= 1 ? 0 : nch <= most ? RB : R; }))
+    if (!draft_find<KT, R, true>(a, at, &u, [&](int nch) { return draft_join_pieces(nch, most, R, NP); }))
       return;  // uniform over the block
     const DraftReq rq = draft_request(a, u.b);
-    const bool serial = u.nch <= most;
-    const int per = serial ? RB : R, sub = u.index % per;
-    const int group = u.index / per, h = group / u.groups, rt = group % u.groups;
-    const int even = draft_even(rq, a.G, R, STEP), rr = serial ? sub * NP + p : sub, r0 = rt * even, r = r0 + rr;
-    const int nrow = min(rq.n * a.G, r0 + even);
+    const DraftJoin j = draft_join(u, rq, a.G, a.Hkv, R, STEP, NP, most);
     // (rows of a block ascend: the first one behind the last ends it)
-    if (r0 + (serial ? sub * NP : sub) >= nrow) {
+    if (j.r0 + j.row >= j.nrow) {
       if (a.one_round) return;
       continue;
     }
-    const bool on = r < nrow;
-    const int64_t base = u.slot + group, step = (int64_t)u.groups * a.Hkv;
+    const bool serial = j.serial;
+    const int rr = serial ? j.row + p : j.row, r = j.r0 + rr, h = j.h;
+    const bool on = r < j.nrow;
+    const int64_t base = j.base, step = j.step;
     f32x4 x = {0.f, 0.f, 0.f, 0.f};
     float sum = 0.f;
     // (a chunk whose tokens the row does not see has max -inf and zeros)
