@@ -9,7 +9,7 @@
 namespace htree {
 
 // ---------------------------------------------------------------- tables
-constexpr int kMaxRequests = 4096;  // the lengths' sums sit in one block's LDS
+// (the lengths' sums of all requests sit in a block's LDS)
 constexpr int kTabTile = 256;       // rows, or new pages, that a block takes at a time
 
 struct TabArgs {
@@ -315,7 +315,7 @@ static int draft_check(const htree_cache* c, int32_t B, int32_t rows, int32_t H,
   const int rc = cache_check(c);
   if (rc) return rc;
   if (B < 0 || rows < 0 || H <= 0 || H % c->H_kv || width < 0) return HTREE_ESHAPE;
-  if ((int64_t)width * c->page_size > (1 << 30)) return HTREE_EUNSUPPORTED;
+  if ((int64_t)width * c->page_size > (1 << 30) || B > kCacheMaxRequests) return HTREE_EUNSUPPORTED;
   // 32-bit rows (new tokens x heads of a group), and the units of 16 rows at least
   if ((int64_t)rows * (H / c->H_kv) >= 0x7fffff00ll ||
       ((int64_t)rows * (H / c->H_kv) / 16 + B + 512) * c->H_kv > kDraftMaxUnits)
@@ -335,7 +335,7 @@ extern "C" int htree_page_tables(int32_t B, int32_t rows, int32_t page_size, int
                                  void* stream) {
   if (B < 0 || rows < 0 || num_pages < 0 || table_width < 0 || n_free < 0) return HTREE_ESHAPE;
   if (B > 1 && table_stride < table_width) return HTREE_ESHAPE;
-  if (page_size < 1 || (page_size & (page_size - 1)) || B > kMaxRequests) return HTREE_EUNSUPPORTED;
+  if (page_size < 1 || (page_size & (page_size - 1)) || B > kCacheMaxRequests) return HTREE_EUNSUPPORTED;
   if (B == 0 && rows == 0) return HTREE_OK;
   if (B == 0) return HTREE_ESHAPE;
   if (!ctx_lens || !new_lens || !starts || !lens || !pages_used) return HTREE_ENULL;

@@ -14,6 +14,12 @@
 
 namespace htree {
 
+// Requests of a call, of the page tables and of the attention.  Every block
+// sums the lengths of all of them, 64 at a time, so a call's time grows with
+// the square: 4096 single tokens over 64 tokens each take 360 us, where their
+// bytes take 28; 65536 took 77 ms.
+constexpr int kCacheMaxRequests = 4096;
+
 // ------------------------------------------------------- attention's split
 // A block's form.  NW = 1: four waves with the same 16 MT rows and tiles of
 // their own (few rows); NW = 4: four waves with 16 MT rows each and common
@@ -120,10 +126,23 @@ __host__ __device__ inline int draft_pieces(int each, int groups) {
   const int64_t n = (int64_t)each * groups;
   return n < kDraftMaxUnits ? (int)n : kDraftMaxUnits;
 }
-// Tiles of a chunk, from the tiles of all groups of rows (an fp32 sum, raised
-// by more than its rounding: the workspace is sized for the exact one): the
-// same for every request, a multiple of the block's 4 waves, two tiles a wave
-// at least.
+// Tiles of all groups of rows of the requests that a lane sums: lane, lane +
+// 64, ...
+template <typename F>
+__host__ __device__ inline float draft_lane_tiles(int lane, int B, int cap, int KT, int G, int R, F req) {
+  float w = 0.f;
+  for (int b = lane; b < B; b += 64) {
+    const DraftReq r = req(b);
+    w += (float)draft_tiles(r, cap, KT) * draft_row_groups(r, G, R);
+  }
+  return w;
+}
+// Tiles of a chunk, from the tiles of all groups of rows: an fp32 sum of 64
+// terms a lane at most and of 64 lanes, rounded fewer than 100 times on the way
+// of any term (100 x 2^-24 is 6e-6), and raised by more than that: the workspace
+// is sized for the exact one.  The same for every request, a multiple of the
+// block's 4 waves, and so one tile a wave at least.  (A wider chunk and a
+// request's even parts are no such multiples.)
 __host__ __device__ inline int draft_chunk(float tiles, int target) {
   if (target <= 0) return 1 << 30;
   const float c = tiles * 1.0001f / target;

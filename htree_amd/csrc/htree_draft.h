@@ -135,10 +135,7 @@ __device__ __forceinline__ bool draft_find(const DraftArgs& a, int64_t u, DraftU
   } else {
     float w = 0.f;
     if (a.target > 0) {
-      for (int b = lane; b < a.B; b += 64) {
-        const DraftReq r = draft_request(a, b);
-        w += (float)draft_tiles(r, cap, KT) * draft_row_groups(r, a.G, R);
-      }
+      w = draft_lane_tiles(lane, a.B, cap, KT, a.G, R, [&](int b) { return draft_request(a, b); });
       w = add_xor32(add_xor16(row_sum16(w))) * a.Hkv;
     }
     chunk = draft_chunk(w, a.target);

@@ -10,7 +10,7 @@ from typing import Optional
 import torch
 
 from . import _native as N
-from .cache import MAX_REQUEST_TOKENS, _ints, aligned_rows, check_table, native_cache, no_derivatives, overlap
+from .cache import MAX_REQUEST_TOKENS, MAX_REQUESTS, _ints, aligned_rows, check_table, native_cache, no_derivatives, overlap
 
 MAX_SCALE = 2.35e38  # scale * log2(e) is an fp32 number
 
@@ -59,6 +59,7 @@ def draft_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     assert q.device == dev, "q and the cache must be on one device"
     assert lens.dim() == 1, "lens must be int32 [B]"
     B = lens.shape[0]
+    assert B <= MAX_REQUESTS, f"at most {MAX_REQUESTS} requests, got {B}"
     _ints(lens, "lens", B, dev)
     _ints(starts, "starts", B + 1, dev)
     check_table(block_table, B, dev)

@@ -303,8 +303,8 @@ int htree_topk_rows(const float* values, int64_t rows, int32_t n, int32_t k,
  * on the host: whatever they hold, nothing outside the buffers is touched.
  * The limits of a call are: page_size a power of two (16 .. 4096 for the
  * cache itself), Dk and Dv up to 256 in rows of whole 16-byte pieces, every
- * stride and base 16-byte aligned, at most 4096 requests in
- * htree_page_tables, table_width * page_size <= 2^30 tokens a request. */
+ * stride and base 16-byte aligned, at most 4096 requests,
+ * table_width * page_size <= 2^30 tokens a request. */
 
 typedef struct htree_cache {
   int32_t dtype;      /* enum htree_dtype of keys, values, queries, output   */
@@ -367,6 +367,8 @@ int htree_draft_attention_workspace_bytes(const htree_cache* c, int32_t B, int32
  * Branches of the tree are walked token by token, for tens or hundreds of
  * drafts; a chunk of thousands of tokens belongs in a call without parents.
  * HTREE_ESHAPE: scale * log2(e) is not a finite fp32 number (among others).
+ * Each block sums the lengths of all requests: 4096 of them over 64 tokens each
+ * take 13 times as long as their bytes.
  * HTREE_EUNSUPPORTED: a table of more than 2^30 tokens, tokens of a page more
  * than 2^26 bytes apart, more than 2^24 blocks of work
  * ((rows H / H_kv / 16 + B + 512) H_kv). */
