@@ -34,6 +34,7 @@ MAX_HEAD_DIM = 256
 PAGE_SIZES = (16, 4096)       # of the cache: powers of two in this range
 MAX_REQUEST_TOKENS = 1 << 30  # block table width * page_size
 MAX_TOKEN_BYTES = 1 << 26     # between a page's tokens
+INT32 = 1 << 31               # sizes below: the C ABI's are int32
 
 
 class PageTables(NamedTuple):
@@ -92,7 +93,7 @@ def _describe(kshape, kstride, vshape, vstride, dtype) -> "N.HtreeCache":
     V = vshape[3]
     assert vshape[:3] == kshape[:3], "k_cache and v_cache must have the same pages and heads"
     assert dtype in N.DTYPE_CODE, "the cache's dtype must be float32, bfloat16 or float16"
-    assert pages > 0 and heads > 0, "the cache needs a page and a head"
+    assert 0 < pages < INT32 and 0 < heads < INT32, "the cache needs a page and a head, and less than 2^31 of either"
     assert PAGE_SIZES[0] <= page <= PAGE_SIZES[1] and page & (page - 1) == 0, \
         f"page_size must be a power of two from {PAGE_SIZES[0]} to {PAGE_SIZES[1]}, got {page}"
     es = dtype.itemsize
@@ -146,7 +147,9 @@ def page_tables(ctx_lens: torch.Tensor, new_lens: torch.Tensor, block_table: tor
     _ints(free_pages, "free_pages", F, dev)
     check_table(block_table, B, dev)
     assert page_size > 0 and page_size & (page_size - 1) == 0, f"page_size must be a power of two, got {page_size}"
-    assert 0 <= rows < 2 ** 31 and num_pages >= 0, "rows and num_pages must not be negative"
+    assert 0 <= rows < INT32 and 0 <= num_pages < INT32, "rows and num_pages must not be negative, nor pass 31 bits"
+    assert page_size < INT32 and F < INT32 and block_table.shape[1] < INT32, \
+        "page_size, free_pages and block_table's width must not pass 31 bits"
     if parents is not None:
         _ints(parents, "parents", rows, dev)
     if out is None:
@@ -202,6 +205,7 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     dtype, dev = k_cache.dtype, k_cache.device
     assert k.dim() == 3 and v.dim() == 3, "k / v must be [rows, H_kv, D]"
     rows = k.shape[0]
+    assert rows < INT32, f"rows must be below 2^31, got {rows}"
     assert k.shape == (rows, c.H_kv, c.Dk) and v.shape == (rows, c.H_kv, c.Dv), \
         f"k / v must be [rows, {c.H_kv}, {c.Dk} / {c.Dv}], got {list(k.shape)} / {list(v.shape)}"
     assert k.dtype is dtype and v.dtype is dtype, "k, v and the cache must share one dtype"
@@ -216,14 +220,14 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     if cos is not None:
         assert c.Dk % 2 == 0, "rotating needs an even head dim K"
         rope_rows, half = cos.shape[0], c.Dk // 2
-        assert rope_rows > 0 and cos.shape == (rope_rows, half) and sin.shape == (rope_rows, half) \
+        assert 0 < rope_rows < INT32 and cos.shape == (rope_rows, half) and sin.shape == (rope_rows, half) \
             and cos.dtype is torch.float32 and sin.dtype is torch.float32 \
             and cos.is_contiguous() and sin.is_contiguous() and cos.device == dev and sin.device == dev, \
             f"cos and sin must be contiguous fp32 tensors [n, {half}] on {dev}"
         _ints(positions, "positions", rows, dev)
     if q is not None:
         assert cos is not None, "q is taken to be rotated: it needs positions, cos and sin"
-        assert q.dim() == 3 and q.shape[0] == rows and q.shape[2] == c.Dk and q.shape[1] > 0, \
+        assert q.dim() == 3 and q.shape[0] == rows and q.shape[2] == c.Dk and 0 < q.shape[1] < INT32, \
             f"q must be [{rows}, H, {c.Dk}], got {list(q.shape)}"
         assert q.dtype is dtype and q.device == dev, "q must have k's dtype and device"
         H = q.shape[1]

@@ -10,7 +10,8 @@ from typing import Optional
 import torch
 
 from . import _native as N
-from .cache import MAX_REQUEST_TOKENS, MAX_REQUESTS, _ints, aligned_rows, check_table, native_cache, no_derivatives, overlap
+from .cache import (INT32, MAX_REQUEST_TOKENS, MAX_REQUESTS, _ints, aligned_rows, check_table, native_cache,
+                    no_derivatives, overlap)
 
 MAX_SCALE = 2.35e38  # scale * log2(e) is an fp32 number
 
@@ -54,6 +55,7 @@ def draft_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     assert q.dim() == 3, "q must be [rows, H, K]"
     rows, H, K = q.shape
     assert K == c.Dk, f"q and the cache must share the head dim K ({K} vs {c.Dk})"
+    assert rows < INT32 and H < INT32, f"rows and heads must be below 2^31, got {rows} and {H}"
     assert H > 0 and H % c.H_kv == 0, f"H ({H}) must be divisible by H_kv ({c.H_kv})"
     assert q.dtype is dtype, "q and the cache must share one dtype"
     assert q.device == dev, "q and the cache must be on one device"
