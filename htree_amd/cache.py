@@ -73,6 +73,7 @@ def check_table(block_table: torch.Tensor, B: int, device) -> None:
     assert block_table.dtype is torch.int32 and block_table.dim() == 2, "block_table must be int32 [B, width]"
     assert block_table.shape[0] == B, f"block_table must have a row for each of the {B} requests"
     assert block_table.stride(1) == 1 or block_table.shape[1] <= 1 or B == 0, "block_table rows must be contiguous"
+    assert B <= 1 or block_table.stride(0) >= block_table.shape[1], "block_table must not be expanded"
     assert block_table.device == device, f"block_table must be on {device}"
 
 

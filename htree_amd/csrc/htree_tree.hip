@@ -465,7 +465,8 @@ const char* htree_strerror(int status) {
     case HTREE_ESHAPE:
       return "invalid shape: need B,T,H,H_kv,D > 0, even D, H % H_kv == 0, dtype and grad_dtype "
              "in {f32,bf16,f16}, kv_share in {0,1,2,4} (H_kv a multiple of kv_share), "
-             "0 <= group_pad < H/H_kv";
+             "0 <= group_pad < H/H_kv; serving: no negative sizes, H % H_kv == 0, block table rows "
+             "at least their width apart, a finite scale";
     case HTREE_ECONFIG:
       return "invalid tree configuration: compression_rate, top_k_per_layer and max_top_nodes "
              "must be powers of two with max_top_nodes <= top_k_per_layer * compression_rate "
@@ -477,8 +478,10 @@ const char* htree_strerror(int status) {
              "top_k_per_layer * compression_rate <= 65536, with D <= 128 where "
              "top_k_per_layer > 1024 or top_k_per_layer * compression_rate > 16384; the "
              "backward also needs B * T * H_kv * min(top_k_per_layer, parents of a level) < 2^31 "
-             "per level";
-    case HTREE_EWORKSPACE: return "workspace smaller than htree_tree_workspace_bytes()";
+             "per level; serving: pages of 16 to 4096 tokens (a power of two), head dims of whole "
+             "16-byte pieces up to 256, strides and bases at 16-byte steps, at most 4096 requests, "
+             "2^30 tokens of a table, 2^26 bytes between tokens and 2^24 blocks of work";
+    case HTREE_EWORKSPACE: return "workspace smaller than the call's ..._workspace_bytes()";
     case HTREE_ESCRATCH:
       return "backward needs more scratch than htree_backward_noalloc's device array "
              "(HTREE_NOALLOC_SCRATCH_BYTES) holds: use htree_backward with a workspace";
