@@ -153,6 +153,12 @@ def page_tables(ctx_lens: torch.Tensor, new_lens: torch.Tensor, block_table: tor
         "page_size, free_pages and block_table's width must not pass 31 bits"
     if parents is not None:
         _ints(parents, "parents", rows, dev)
+    ins = [(ctx_lens.data_ptr(), B), (new_lens.data_ptr(), B), (free_pages.data_ptr(), F)]
+    if parents is not None:
+        ins.append((parents.data_ptr(), rows))
+    table = (block_table.data_ptr(), (B - 1) * block_table.stride(0) + block_table.shape[1] if block_table.numel() else 0)
+    for p, n in ins:
+        assert p >= table[0] + 4 * table[1] or table[0] >= p + 4 * n, "block_table, which is written, overlaps an input"
     if out is None:
         starts, positions, lens, used = torch.empty(2 * B + 2 + rows, dtype=torch.int32, device=dev).split_with_sizes(
             (B + 1, rows, B, 1))
@@ -166,13 +172,9 @@ def page_tables(ctx_lens: torch.Tensor, new_lens: torch.Tensor, block_table: tor
             and out.slots.device == dev, f"out.slots must be a contiguous int64 tensor [{rows}] on {dev}"
         # (the lengths of a step are a natural input of the next: the kernel
         # would read some after writing them)
-        ins = [(ctx_lens.data_ptr(), B), (new_lens.data_ptr(), B), (free_pages.data_ptr(), F),
-               (block_table.data_ptr(), max(B - 1, 0) * block_table.stride(0) + block_table.shape[1])]
-        if parents is not None:
-            ins.append((parents.data_ptr(), rows))
         outs = ((out.starts.data_ptr(), B + 1), (out.slots.data_ptr(), 2 * rows), (out.positions.data_ptr(), rows),
                 (out.lens.data_ptr(), B), (out.pages_used.data_ptr(), 1))
-        assert not any(p < q + 4 * m and q < p + 4 * n for p, n in ins for q, m in outs), \
+        assert not any(p < q + 4 * m and q < p + 4 * n for p, n in (*ins, table) for q, m in outs), \
             "out must not overlap the inputs"
     if B == 0:
         out.starts.zero_(), out.pages_used.zero_(), out.slots.fill_(-1), out.positions.fill_(-1)

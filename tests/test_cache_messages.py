@@ -2,7 +2,6 @@
 import pytest
 import torch
 
-import htree_amd
 from htree_amd import _native as N
 from htree_amd.cache import check_table
 
@@ -20,4 +19,3 @@ def test_expanded_tables_are_refused_as_such():
     with pytest.raises(AssertionError, match="expanded"):
         check_table(t.expand(3, 4), 3, t.device)
     check_table(t[:, :0].expand(3, 0), 3, t.device)  # no entries
-    assert htree_amd.draft_attention
