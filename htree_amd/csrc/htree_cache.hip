@@ -279,6 +279,14 @@ __global__ __launch_bounds__(256) void cache_append_kernel(AppendArgs a) {
 }
 
 // ------------------------------------------------------------------ host
+struct Range {
+  const void* at;
+  int64_t bytes;
+};
+static bool overlap(const Range& a, const Range& b) {
+  const char *x = (const char*)a.at, *y = (const char*)b.at;
+  return a.bytes > 0 && b.bytes > 0 && x < y + b.bytes && y < x + a.bytes;
+}
 static int cache_es(const htree_cache* c) { return c->dtype == HTREE_F32 ? 4 : 2; }
 
 // sizes, types and alignment of the cache
@@ -295,14 +303,6 @@ static int cache_check(const htree_cache* c) {
   // lanes hold 32-bit offsets into 16 tokens
   if (c->k_token * es > (1 << 26) || c->v_token * es > (1 << 26)) return HTREE_EUNSUPPORTED;
   return HTREE_OK;
-}
-struct Range {
-  const void* at;
-  int64_t bytes;
-};
-static bool overlap(const Range& a, const Range& b) {
-  const char *x = (const char*)a.at, *y = (const char*)b.at;
-  return a.bytes > 0 && b.bytes > 0 && x < y + b.bytes && y < x + a.bytes;
 }
 static bool off16(const void* p) { return ((uintptr_t)p & 15) != 0; }
 static int log2i(int x) { return __builtin_ctz((unsigned)x); }
@@ -340,6 +340,18 @@ extern "C" int htree_page_tables(int32_t B, int32_t rows, int32_t page_size, int
   if (B == 0) return HTREE_ESHAPE;
   if (!ctx_lens || !new_lens || !starts || !lens || !pages_used) return HTREE_ENULL;
   if ((table_width && !block_table) || (n_free && !free_pages) || (rows && (!slots || !positions))) return HTREE_ENULL;
+  // (the lengths of a step are a natural input of the next: a block would read
+  // some after another has written them)
+  const Range in[4] = {{ctx_lens, B * 4ll}, {new_lens, B * 4ll}, {parents, parents ? rows * 4ll : 0},
+                       {free_pages, n_free * 4ll}};
+  const Range table = {block_table, table_width ? ((B - 1) * table_stride + table_width) * 4 : 0};
+  const Range written[6] = {table, {starts, (B + 1) * 4ll}, {slots, rows * 8ll}, {positions, rows * 4ll},
+                            {lens, B * 4ll}, {pages_used, 4}};
+  for (const Range& x : written)
+    for (const Range& y : in)
+      if (overlap(x, y)) return HTREE_EOVERLAP;
+  for (const Range& x : written)
+    if (&x != written && overlap(x, table)) return HTREE_EOVERLAP;
   TabArgs a;
   a.ctx = ctx_lens, a.add = new_lens, a.parents = parents, a.free_pages = free_pages;
   a.table = block_table, a.starts = starts, a.positions = positions, a.lens = lens, a.used = pages_used;

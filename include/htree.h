@@ -56,8 +56,8 @@ enum htree_status {
   HTREE_EWORKSPACE = -5,   /* workspace too small */
   HTREE_ESCRATCH = -6,     /* htree_backward_noalloc: the problem's backward
                               needs more than HTREE_NOALLOC_SCRATCH_BYTES */
-  HTREE_EOVERLAP = -7      /* htree_cache_append: k, v or q lies in the range
-                              of the cache that is written */
+  HTREE_EOVERLAP = -7      /* serving: an input shares memory with what the
+                              call writes */
 };
 
 /* Size of the device array htree_backward_noalloc works in (one per GPU). */
@@ -328,7 +328,9 @@ typedef struct htree_cache {
  *              ctx + index); -1 behind the last request
  *   lens       [B] ctx + new (these and positions end at 2^31 - 1)
  *   pages_used [1] pages wanted; more than n_free: the last ones are missing
- *              (their entries are -1) */
+ *              (their entries are -1)
+ * HTREE_EOVERLAP: one of them or the block table, which is written, shares
+ * its range of memory with an input, or an output with the table. */
 int htree_page_tables(int32_t B, int32_t rows, int32_t page_size, int32_t num_pages,
                       int32_t table_width, int64_t table_stride, int32_t n_free,
                       const int32_t* ctx_lens, const int32_t* new_lens,

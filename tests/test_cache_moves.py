@@ -90,3 +90,29 @@ def test_neighbours_are_no_overlap():
     both = torch.zeros(4, 2, 16, 1, D, device=dev)
     htree_amd.cache_append(k, v, both[:, 0], both[:, 1], slots)
     assert torch.equal(both[:, 0].reshape(-1, 1, D)[slots], k0) and torch.equal(both[:, 1].reshape(-1, 1, D)[slots], v0)
+
+
+@pytest.mark.parametrize("name", ["ctx", "new", "parents", "free"])
+@pytest.mark.parametrize("over", ["table", "starts", "slots", "positions", "lens", "used"])
+def test_page_tables_refuses_inputs_that_it_writes(name, over):
+    """4 requests, 6 rows, 3 pages, a table of 4 x 10."""
+    at = {n: (i + 1) * FAR for i, n in enumerate(("ctx", "new", "parents", "free", "table", "starts", "slots",
+                                                 "positions", "lens", "used"))}
+    size = dict(table=160, starts=20, slots=48, positions=24, lens=16, used=4)[over]
+    for shift in (0, size - 4):
+        at[name] = at[over] + shift
+        p = lambda n: ctypes.c_void_p(at[n])
+        assert N.lib().htree_page_tables(4, 6, 16, 9, 10, 10, 3, p("ctx"), p("new"), p("parents"), p("table"),
+                                         p("free"), p("starts"), p("slots"), p("positions"), p("lens"), p("used"),
+                                         None) == N.HTREE_EOVERLAP
+
+
+@pytest.mark.parametrize("over", ["starts", "slots", "positions", "lens", "used"])
+def test_page_tables_refuses_outputs_in_the_table(over):
+    at = {n: (i + 1) * FAR for i, n in enumerate(("ctx", "new", "parents", "free", "table", "starts", "slots",
+                                                 "positions", "lens", "used"))}
+    at[over] = at["table"] + 156
+    p = lambda n: ctypes.c_void_p(at[n])
+    assert N.lib().htree_page_tables(4, 6, 16, 9, 10, 10, 3, p("ctx"), p("new"), p("parents"), p("table"), p("free"),
+                                     p("starts"), p("slots"), p("positions"), p("lens"), p("used"),
+                                     None) == N.HTREE_EOVERLAP
