@@ -771,10 +771,16 @@ __global__ __launch_bounds__(256, draft_two(D, MT, sizeof(T)) ? 2 : 1) void draf
     }
   };
 
+  // The lane again, for places in LDS: at D 32, 32 rows, a third block fits a CU
+  // then (168 registers; 2000 requests of up to 900 tokens, 64/4 heads, fp16:
+  // 414 us, with two blocks 557).  fp32 has the registers, and kept places are
+  // 2% faster there.
+  auto place = [&]() { return S::F32 ? lane : draft_lane_again(); };
   // the staged tile into LDS; the loads of the wave's next one go out
   int ent[NG], nxt[NG];
   int t = c.t0 + wv;
   auto stage = [&]() {
+    const int lane2 = place(), lr = lane2 / CPR, lc = lane2 % CPR;
     if (!whole) {
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
@@ -829,6 +835,7 @@ __global__ __launch_bounds__(256, draft_two(D, MT, sizeof(T)) ? 2 : 1) void draf
       // Values that a row does not see must not meet the product: 0 x NaN is
       // NaN.  Zeros take the place of those that no row sees, and of
       // infinite or NaN ones, which join at the end.
+      const int lr = place() / CPR;
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
         const int row = i * RPI + lr;
