@@ -28,11 +28,11 @@
 // What bounds them (bf16, D 128, 16-token pages, launch and join together):
 //   64 requests of up to 16384 tokens, one token each, 32/4 heads: the cache's
 //     bytes, 276 us (4.9 TB/s).
-//   One request of 131008 tokens, 64 drafted, 64/8 heads: 304 us, 903 TFLOP/s,
+//   One request of 131008 tokens, 64 drafted, 64/8 heads: 303 us, 906 TFLOP/s,
 //     where a library product of 8192 x 8192 reaches 1125: the matrix unit is
 //     busy 40% of the time; each tile's softmax, and the latency that two
 //     waves per SIMD do not cover, is the rest.
-//   One request of 2048 tokens, one token: 7.5 + 4 us, a chain of dependent
+//   One request of 2048 tokens, one token: 7.8 + 4.7 us, a chain of dependent
 //     reads (lengths, pages, keys, states) and two launches.
 #pragma once
 
@@ -315,7 +315,7 @@ struct DraftWave {
   // and each is off by half a step, or 2^-36 of the max.  Against a max of 1,
   // 4096 tokens 20 log2 units below one whose values are zero were 1e-2 off.
   // Moving after 4 and not 8 costs a rescale here and there: two chunks of up
-  // to 777 tokens over 1500, 8/2 heads of 64, take 27.8 us for 27.4, a prompt of
+  // to 777 tokens over 1500, 8/2 heads of 64, took 27.8 us for 27.4, a prompt of
   // 2048, 32/4 heads of 128, 78.6 for 76.8.
   static constexpr bool F16 = std::is_same<T, _Float16>::value;
   static constexpr float kUp = F16 ? 11.f : 0.f, kLag = F16 ? 4.f : 8.f;
@@ -771,11 +771,11 @@ __global__ __launch_bounds__(256, draft_two(D, MT, sizeof(T)) ? 2 : 1) void draf
     }
   };
 
-  // The lane again, for places in LDS: at D 32, 32 rows, a third block fits a CU
-  // then (168 registers; 2000 requests of up to 900 tokens, 64/4 heads, fp16:
-  // 414 us, with two blocks 557).  fp32 has the registers, and kept places are
-  // 2% faster there.
-  auto place = [&]() { return S::F32 ? lane : draft_lane_again(); };
+  // The lane again, for places in LDS: at D 32 in 16 bits a third block of 32
+  // rows fits a CU then (168 registers; 2000 requests of up to 900 tokens, 64/4
+  // heads, fp16: 414 us, with two blocks 557).  Elsewhere LDS allows no more
+  // blocks, and kept places are up to 2% faster (fp32 at D 32).
+  auto place = [&]() { return D == 32 && !S::F32 ? draft_lane_again() : lane; };
   // the staged tile into LDS; the loads of the wave's next one go out
   int ent[NG], nxt[NG];
   int t = c.t0 + wv;
@@ -945,7 +945,7 @@ __device__ __forceinline__ void draft_step(const DraftArgs& a, const DraftCtx& c
 // (directly, without registers) while it works on the other: one barrier a
 // tile.  One request of 131008 tokens, 64 drafted, 64/8 heads of 128, bf16:
 // 718 us with 64 rows and tiles of a wave's own, 366 with common tiles, 322
-// with the copies straight into LDS, 304 with them spread between the products
+// with the copies straight into LDS, 303 with them spread between the products
 // and the waves' priority raised there.
 // WHOLE: the head dims are D.
 template <typename T, int D, int MT, int NW, int KT, bool WHOLE>
@@ -1124,7 +1124,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void draft_rows_kernel(D
 // D / 4, a set holding a row.  Few chunks: each set takes a row and all its
 // chunks; many chunks, or few rows in all: the block takes a row and its sets
 // share the chunks.  Bound by the read of the states, and by the launch: 512
-// states of 128 rows of 128 (34 MB) 13 us, those of a single token 4 us.
+// states of 128 rows of 128 (34 MB) 11 us, those of a single token 4.7 us.
 constexpr int kJoinSerial = 16;  // or as many as a set has threads
 template <typename T, int D, int KT, int R, int STEP>
 __global__ __launch_bounds__(256) void draft_join_kernel(DraftArgs a) {
