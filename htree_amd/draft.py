@@ -38,16 +38,21 @@ def draft_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     within the request of the token drafted before it, a smaller one, -1:
     none) and itself; without parents the new tokens up to itself.  (Branches
     are walked token by token: drafts of tens or hundreds of tokens.  A chunk
-    of thousands belongs in a call without parents.)  scale defaults to
-    K^-0.5, and is at most MAX_SCALE in size.  Queries and keys come rotated.
+    of thousands belongs in a call without parents: a chain of 2048 takes
+    9 ms instead of 0.3, and at least four times that for twice the tokens.)
+    scale defaults to K^-0.5, and is at most MAX_SCALE in size.  Queries and
+    keys come rotated.
 
     Returns [rows, H, V] in q's dtype (`out`: written there, contiguous, no
-    overlap with the inputs).  Rows that see nothing are zero; rows behind
-    the last request are not written.  Pages outside the cache hold no
-    tokens, neither does the request past its table.
+    overlap with the inputs).  Rows that see nothing are zero, and so are
+    those all of whose scores are -inf; rows behind the last request are not
+    written.  Pages outside the cache hold no tokens, neither does the request
+    past its table.
 
     Scores and the softmax are fp32 (fp32 products for fp32 inputs); for
-    16-bit types P is rounded to the type for the product with the values.
+    16-bit types P is rounded to the type for the product with the values
+    (fp16: each weight to half a step, or 2^-36 of the row's largest).
+    At most MAX_REQUESTS requests: each block sums all of their lengths.
     Results do not depend on the other requests' values, but a request's
     split, and so the last bits, depends on all lengths."""
     c = native_cache(k_cache, v_cache)

@@ -347,7 +347,8 @@ int htree_page_tables(int32_t B, int32_t rows, int32_t page_size, int32_t num_pa
  * leave either's values there, or parts of both.  k, v and q are not parts of
  * the cache: rows that another one's write could change first.
  * HTREE_EOVERLAP: one of them shares its range of memory, gaps included, with
- * k_cache's or v_cache's; copy it out first. */
+ * k_cache's or v_cache's; copy it out first.  q_out shares none with any of
+ * them. */
 int htree_cache_append(const htree_cache* c, int32_t rows, int32_t H, const void* k,
                        int64_t k_row, int64_t k_head, const void* v, int64_t v_row,
                        int64_t v_head, const void* q, int64_t q_row, int64_t q_head,
@@ -367,7 +368,9 @@ int htree_draft_attention_workspace_bytes(const htree_cache* c, int32_t B, int32
  * there; a row that sees nothing gets zeros.  Rows of `out` [rows, H, Dv]
  * behind the last request are left as they were.
  * Branches of the tree are walked token by token, for tens or hundreds of
- * drafts; a chunk of thousands of tokens belongs in a call without parents.
+ * drafts; a chunk of thousands of tokens belongs in a call without parents
+ * (a chain of 2048: 9 ms instead of 0.3, and at least four times that for
+ * twice the tokens).  `out` and the workspace share no memory with the inputs.
  * HTREE_ESHAPE: scale * log2(e) is not a finite fp32 number (among others).
  * Each block sums the lengths of all requests: 4096 of them over 64 tokens each
  * take 13 times as long as their bytes.
