@@ -116,3 +116,31 @@ def test_page_tables_refuses_outputs_in_the_table(over):
     assert N.lib().htree_page_tables(4, 6, 16, 9, 10, 10, 3, p("ctx"), p("new"), p("parents"), p("table"), p("free"),
                                      p("starts"), p("slots"), p("positions"), p("lens"), p("used"),
                                      None) == N.HTREE_EOVERLAP
+
+
+@pytest.mark.gpu
+def test_a_captured_move():
+    """The copies are part of the capture: every replay moves the rows as they
+    are then."""
+    dev, n, D = "cuda:0", 100, 64
+    g = torch.Generator().manual_seed(5)
+    kc, vc = torch.zeros(12, 16, 2, D, device=dev), torch.zeros(12, 16, 2, D, device=dev)
+    kf, vf = kc.view(-1, 2, D), vc.view(-1, 2, D)
+    slots = torch.arange(3, 3 + n, device=dev)
+    call = lambda k, v: htree_amd.cache_append(kf[:n], vf[:n], k, v, slots)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call(kc, vc)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(kc, vc)
+    for _ in range(4):
+        kc.copy_(torch.randn(kc.shape, generator=g))
+        vc.copy_(torch.randn(vc.shape, generator=g))
+        wk, wv = kf.clone(), vf.clone()
+        wk[slots], wv[slots] = kf[:n].clone(), vf[:n].clone()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(kf, wk) and torch.equal(vf, wv)
