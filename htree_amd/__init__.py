@@ -12,6 +12,13 @@ and, for serving, attention of new tokens over a paged key/value cache:
     page_tables(ctx_lens, new_lens, block_table, free_pages, ...) -> PageTables
     cache_append(k, v, k_cache, v_cache, slots, q, positions, cos, sin) -> rotated q
     draft_attention(q, k_cache, v_cache, block_table, lens, starts, parents)
+with what surrounds it in a step:
+    head_norm(q, k, q_weight, k_weight, ...) -> (q, k)   (for training too)
+    verify_drafts(target_probs, tokens, starts, uniforms, draws, ...) -> Verified
+    keep_drafts(k_caches, v_caches, slots, starts, path, kept)
+    fork_requests(block_table, lens, source, free_pages, ...) -> Forked
+    copy_pages(k_caches, v_caches, copy_from, copy_to, copy_tokens)
+    unused_pages(block_table, lens, page_size, num_pages, held) -> UnusedPages
 """
 from .parallel import (HTREE_SCORE_NEG_INF, HTREE_SCORE_VALID_THRESHOLD, htree_forward,
                        htree_forward_parents, rope_cache)
@@ -21,6 +28,9 @@ from .trace import LayerTrace, compare_traces, run_parallel_with_trace
 from .topk import topk_rows
 from .cache import PageTables, cache_append, page_tables
 from .draft import draft_attention
+from .norm import head_norm
+from .pages import Forked, UnusedPages, copy_pages, fork_requests, keep_drafts, unused_pages
+from .verify import Verified, verify_drafts
 
 
 __all__ = [
@@ -29,4 +39,6 @@ __all__ = [
     "HTreeFunction", "rope_cache",
     "HTREE_SCORE_NEG_INF", "HTREE_SCORE_VALID_THRESHOLD", "LayerTrace", "run_parallel_with_trace",
     "compare_traces", "topk_rows", "PageTables", "page_tables", "cache_append", "draft_attention",
+    "head_norm", "Verified", "verify_drafts", "keep_drafts", "Forked", "fork_requests", "copy_pages",
+    "UnusedPages", "unused_pages",
 ]

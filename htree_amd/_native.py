@@ -36,6 +36,10 @@ EXPORTS = (
     "htree_forward_trace", "htree_topk_rows", "htree_backward_noalloc_bytes",
     "htree_backward_noalloc", "htree_select", "htree_page_tables", "htree_cache_append",
     "htree_draft_attention_workspace_bytes", "htree_draft_attention",
+    "htree_verify_drafts_workspace_bytes", "htree_verify_drafts", "htree_keep_drafts",
+    "htree_fork_requests", "htree_copy_pages", "htree_unused_pages_workspace_bytes",
+    "htree_unused_pages", "htree_head_norm", "htree_head_norm_backward_workspace_bytes",
+    "htree_head_norm_backward",
 )
 
 
@@ -121,6 +125,27 @@ def lib() -> ctypes.CDLL:
     L.htree_draft_attention.restype = ctypes.c_int
     L.htree_draft_attention.argtypes = [CP, I32, I32, I32, I32, I64, F, P, I64, I64, P, P, P, P, P, P,
                                         P, I64, I64, P, I64, P]
+    L.htree_verify_drafts_workspace_bytes.restype = ctypes.c_int
+    L.htree_verify_drafts_workspace_bytes.argtypes = [I32, I32, ctypes.POINTER(I64)]
+    L.htree_verify_drafts.restype = ctypes.c_int
+    L.htree_verify_drafts.argtypes = [I32] * 4 + [P, I64, P, I64] + [P] * 9 + [I64, P]
+    L.htree_keep_drafts.restype = ctypes.c_int
+    L.htree_keep_drafts.argtypes = [CP, I32, P, P, I32, I32] + [P] * 5
+    L.htree_fork_requests.restype = ctypes.c_int
+    L.htree_fork_requests.argtypes = [I32] * 5 + [I64, I64, I32] + [P] * 11
+    L.htree_copy_pages.restype = ctypes.c_int
+    L.htree_copy_pages.argtypes = [CP, I32, P, P, I32] + [P] * 4
+    L.htree_unused_pages_workspace_bytes.restype = ctypes.c_int
+    L.htree_unused_pages_workspace_bytes.argtypes = [I32, ctypes.POINTER(I64)]
+    L.htree_unused_pages.restype = ctypes.c_int
+    L.htree_unused_pages.argtypes = [I32] * 4 + [I64, P, P, I32, P, P, P, P, I64, P]
+    L.htree_head_norm.restype = ctypes.c_int
+    L.htree_head_norm.argtypes = [I32] * 6 + [F] + [P, I64, I64] * 2 + [P] * 5 + [I32, P, P, P]
+    L.htree_head_norm_backward_workspace_bytes.restype = ctypes.c_int
+    L.htree_head_norm_backward_workspace_bytes.argtypes = [I32, ctypes.POINTER(I64)]
+    L.htree_head_norm_backward.restype = ctypes.c_int
+    L.htree_head_norm_backward.argtypes = ([I32] * 6 + [F] + [P, I64, I64] * 4 + [P] * 5 + [I32]
+                                           + [P] * 5 + [I64, P])
     _lib = L
     return L
 

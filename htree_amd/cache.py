@@ -64,6 +64,11 @@ def no_derivatives(name: str, *tensors: Optional[torch.Tensor]) -> None:
     if torch.is_grad_enabled():
         for t in tensors:
             assert t is None or not t.requires_grad, f"{name} has no backward"
+    no_tangents(name, *tensors)
+
+
+def no_tangents(name: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Refuses tensors whose forward-mode tangent a call would lose."""
     if forward_ad._current_level >= 0:
         for t in tensors:
             assert t is None or forward_ad.unpack_dual(t).tangent is None, f"{name} has no forward-mode derivative"

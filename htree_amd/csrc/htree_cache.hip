@@ -2,6 +2,8 @@
 // request lengths, new keys and values written to their slots (rotated by
 // their positions), and the entry point of the attention over the cache
 // (htree_draft.h).
+#include "htree_cache_host.h"
+#include "htree_cache_scan.h"
 #include "htree_draft.h"
 
 #include <cmath>
@@ -19,38 +21,6 @@ struct TabArgs {
   int64_t table_stride;
   int32_t B, rows, page_shift, num_pages, width, n_free, page_blocks, tiles;
 };
-
-// Exclusive sums over the requests in `dst[0 .. B]`, of f(b), saturated at
-// `most`.  All 256 threads; `red` holds the waves' sums.
-template <typename F>
-__device__ __forceinline__ int64_t tab_scan(int B, int32_t most, int32_t* dst, int64_t* red, F f) {
-  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-  const int per = (B + 255) / 256, b0 = tid * per, b1 = min(b0 + per, B);
-  int64_t mine = 0;
-  for (int b = b0; b < b1; ++b) mine += f(b);
-  int64_t inc = mine;
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
-    const int64_t x = __shfl_up((long long)inc, m);
-    if (lane >= m) inc += x;
-  }
-  __syncthreads();  // `red` of an earlier scan has been read
-  if (lane == 63) red[wv] = inc;
-  __syncthreads();
-  int64_t at = inc - mine, all = 0;
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    if (w < wv) at += red[w];
-    all += red[w];
-  }
-  for (int b = b0; b < b1; ++b) {
-    dst[b] = (int32_t)min(at, (int64_t)most);
-    at += f(b);
-  }
-  if (tid == 0) dst[B] = (int32_t)min(all, (int64_t)most);
-  __syncthreads();
-  return all;
-}
 
 // Blocks 0 .. page_blocks - 1 write the new pages' table entries, the others
 // the rows' slots and positions, `tiles` times 256 each.  Each block sums the
@@ -279,34 +249,6 @@ __global__ __launch_bounds__(256) void cache_append_kernel(AppendArgs a) {
 }
 
 // ------------------------------------------------------------------ host
-struct Range {
-  const void* at;
-  int64_t bytes;
-};
-static bool overlap(const Range& a, const Range& b) {
-  const char *x = (const char*)a.at, *y = (const char*)b.at;
-  return a.bytes > 0 && b.bytes > 0 && x < y + b.bytes && y < x + a.bytes;
-}
-static int cache_es(const htree_cache* c) { return c->dtype == HTREE_F32 ? 4 : 2; }
-
-// sizes, types and alignment of the cache
-static int cache_check(const htree_cache* c) {
-  if (!c) return HTREE_ENULL;
-  if (c->dtype != HTREE_F32 && c->dtype != HTREE_BF16 && c->dtype != HTREE_F16) return HTREE_ESHAPE;
-  if (c->H_kv <= 0 || c->Dk <= 0 || c->Dv <= 0 || c->num_pages <= 0) return HTREE_ESHAPE;
-  if (c->page_size < 16 || c->page_size > 4096 || (c->page_size & (c->page_size - 1))) return HTREE_EUNSUPPORTED;
-  const int es = cache_es(c);
-  if (c->Dk > 256 || c->Dv > 256 || c->Dk * es % 16 || c->Dv * es % 16) return HTREE_EUNSUPPORTED;
-  const int64_t st[6] = {c->k_page, c->k_token, c->k_head, c->v_page, c->v_token, c->v_head};
-  for (int64_t s : st)
-    if (s < 0 || s * es % 16) return HTREE_EUNSUPPORTED;
-  // lanes hold 32-bit offsets into 16 tokens
-  if (c->k_token * es > (1 << 26) || c->v_token * es > (1 << 26)) return HTREE_EUNSUPPORTED;
-  return HTREE_OK;
-}
-static bool off16(const void* p) { return ((uintptr_t)p & 15) != 0; }
-static int log2i(int x) { return __builtin_ctz((unsigned)x); }
-
 static DraftPlan draft_plan(const htree_cache* c, int B, int rows, int H, int width) {
   return draft_plan(c->Dk, c->Dv, cache_es(c), B, rows, H, c->H_kv, width, c->page_size);
 }

@@ -1,0 +1,151 @@
+"""Norms of queries and keys by head, rotated by their positions in the same
+pass: before htree_forward in training (which rotates by itself), before
+cache_append in serving."""
+from __future__ import annotations
+
+import ctypes
+from functools import lru_cache
+from typing import Optional, Tuple
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _native as N
+from .cache import INT32, MAX_HEAD_DIM, aligned_rows, no_tangents
+
+
+@lru_cache(maxsize=16)
+def _workspace_bytes(D: int) -> int:
+    n = ctypes.c_int64()
+    N.check(N.lib().htree_head_norm_backward_workspace_bytes(D, n), "htree_head_norm_backward_workspace_bytes")
+    return n.value
+
+
+def _rows(x: torch.Tensor) -> torch.Tensor:
+    """x as the kernels read it: [rows, heads, D], rows and heads at 16-byte steps."""
+    return aligned_rows(x if x.dim() == 3 else x.reshape(-1, *x.shape[-2:]))
+
+
+def _sizes(q: torch.Tensor, weight: Optional[torch.Tensor]):
+    code = N.DTYPE_CODE[q.dtype]
+    return code, code if weight is None else N.DTYPE_CODE[weight.dtype]
+
+
+def _forward(q, k, q_weight, k_weight, eps, positions, cos, sin):
+    dev, dtype, D = q.device, q.dtype, q.shape[-1]
+    q_out, k_out = (torch.empty(x.shape, dtype=dtype, device=dev) for x in (q, k))
+    q3, k3 = _rows(q), _rows(k)
+    rows = q3.shape[0]
+    if rows:
+        rc = N.launch(N.lib().htree_head_norm, dev, *_sizes(q, k_weight if q_weight is None else q_weight), rows,
+                      q3.shape[1], k3.shape[1], D, eps, q3.data_ptr(), q3.stride(0), q3.stride(1), k3.data_ptr(),
+                      k3.stride(0), k3.stride(1), N.address(q_weight), N.address(k_weight), N.address(positions),
+                      N.address(cos), N.address(sin), 0 if cos is None else cos.shape[0], q_out.data_ptr(),
+                      k_out.data_ptr())
+        if rc:
+            N.check(rc, "htree_head_norm")
+    return q_out, k_out
+
+
+class _HeadNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, eps, positions, cos, sin):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(q, k, q_weight, k_weight, positions, cos, sin)
+        ctx.eps = eps
+        return _forward(q, k, q_weight, k_weight, eps, positions, cos, sin)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dq_out, dk_out):
+        q, k, q_weight, k_weight, positions, cos, sin = ctx.saved_tensors
+        dev, D = q.device, q.shape[-1]
+        grads, args, strides, H, ws = [None, None, None, None], [], [], [0, 0], None
+        for i, (x, dy, w) in enumerate(((q, dq_out, q_weight), (k, dk_out, k_weight))):
+            wanted = dy is not None and (ctx.needs_input_grad[i] or ctx.needs_input_grad[2 + i])
+            if not wanted:
+                args.append((None, None, None, None))
+                strides += [(0, 0), (0, 0)]
+                continue
+            dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
+            dw = torch.zeros_like(w) if ctx.needs_input_grad[2 + i] else None
+            x3, dy3 = _rows(x), _rows(dy)
+            H[i] = x.shape[-2]
+            args.append((x3, dy3, dx, dw))
+            strides += [x3.stride(), dy3.stride()]
+            grads[i] = dx if ctx.needs_input_grad[i] else None
+            grads[2 + i] = dw
+        (q3, dq3, dq, dqw), (k3, dk3, dk, dkw) = args
+        rows = q.shape[:-2].numel()
+        if rows and any(H):
+            nbytes = _workspace_bytes(D) if dqw is not None or dkw is not None else 0
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+            (qr, qh, *_), (yr, yh, *_), (kr, kh, *_), (zr, zh, *_) = strides
+            rc = N.launch(N.lib().htree_head_norm_backward, dev, *_sizes(q, k_weight if q_weight is None else q_weight),
+                          rows, H[0], H[1], D, ctx.eps, N.address(q3), qr, qh, N.address(k3), kr, kh, N.address(dq3),
+                          yr, yh, N.address(dk3), zr, zh, N.address(q_weight), N.address(k_weight),
+                          N.address(positions), N.address(cos), N.address(sin), 0 if cos is None else cos.shape[0],
+                          N.address(dq), N.address(dk), N.address(dqw), N.address(dkw), N.address(ws), nbytes)
+            if rc:
+                N.check(rc, "htree_head_norm_backward")
+        return (*grads, None, None, None, None)
+
+
+def head_norm(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tensor] = None,
+              k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+              positions: Optional[torch.Tensor] = None, cos: Optional[torch.Tensor] = None,
+              sin: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Each head's x (mean x^2 + eps)^-1/2 weight, of queries q [..., H, D] and
+    keys k [..., H_kv, D] ([rows, H, D] in serving, [B, T, H, D] in training).
+
+    q_weight and k_weight ([D], both float32 or both of q's dtype; None: ones)
+    are shared by the heads.  With positions (int32 [...], one a row) and the
+    tables cos / sin (fp32 [n, D/2], htree_amd.rope_cache) heads are rotated
+    as cache_append rotates them, pairs (d, d + D/2); cache_append and
+    draft_attention then take the results as they are.  htree_forward rotates
+    by itself: there positions stay out.  Rows whose position is outside the
+    tables are zero.
+
+    Products and sums are fp32, rounded once at the end; sizes of up to 1e18
+    (their squares are summed).  D is at most 256, in whole 16-byte pieces;
+    inputs at other steps than 16 bytes are copied first, and so are those
+    whose leading dims are no one step apart.  Returns contiguous tensors.
+
+    Gradients of q, k and the weights: dx = r (g - x r^2 mean(g x)) with g the
+    output's gradient rotated back, times the weight; the weights' are summed
+    over rows and heads in fp32, in a fixed order.  There is no second
+    derivative and no forward mode; cos and sin have no gradient."""
+    dev, dtype = q.device, q.dtype
+    assert dev.type == "cuda", "htree_amd runs on the GPU (no CPU fallback)"
+    assert dtype in N.DTYPE_CODE, "q must be float32, bfloat16 or float16"
+    assert k.dtype is dtype and k.device == dev, "q and k must share one dtype and device"
+    assert q.dim() >= 3 and q.dim() == k.dim() and q.shape[:-2] == k.shape[:-2] and q.shape[-1] == k.shape[-1], \
+        f"q and k must be [..., H, D] and [..., H_kv, D], got {list(q.shape)} and {list(k.shape)}"
+    D, lead = q.shape[-1], q.shape[:-2]
+    assert 0 < D <= MAX_HEAD_DIM and D * dtype.itemsize % 16 == 0, \
+        f"the head dim must be whole 16-byte pieces and at most {MAX_HEAD_DIM}, got {D}"
+    assert q.shape[-2] > 0 and k.shape[-2] > 0, "q and k need a head each"
+    rows = lead.numel()
+    assert rows * (q.shape[-2] + k.shape[-2]) < INT32, "rows times heads must be below 2^31"
+    eps = float(eps)
+    assert 0.0 <= eps < 3.4e38, f"eps must not be negative, nor infinite, got {eps}"
+    for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+        assert w is None or (w.shape == (D,) and w.dtype in (torch.float32, dtype) and w.is_contiguous()
+                             and w.device == dev), f"{name} must be a contiguous [{D}] tensor, float32 or {dtype}, on {dev}"
+    assert q_weight is None or k_weight is None or q_weight.dtype is k_weight.dtype, \
+        "q_weight and k_weight must share one dtype"
+    assert (cos is None) == (sin is None) == (positions is None), "positions, cos and sin go together"
+    if cos is not None:
+        n = cos.shape[0]
+        assert 0 < n < INT32 and cos.shape == (n, D // 2) and sin.shape == (n, D // 2) \
+            and cos.dtype is torch.float32 and sin.dtype is torch.float32 and cos.is_contiguous() \
+            and sin.is_contiguous() and cos.device == dev and sin.device == dev, \
+            f"cos and sin must be contiguous fp32 tensors [n, {D // 2}] on {dev}"
+        assert positions.dtype is torch.int32 and positions.shape == lead and positions.is_contiguous() \
+            and positions.device == dev, f"positions must be a contiguous int32 tensor {list(lead)} on {dev}"
+        if torch.is_grad_enabled():
+            assert not cos.requires_grad and not sin.requires_grad, "cos and sin have no gradient"
+    no_tangents("head_norm", q, k, q_weight, k_weight, cos, sin)
+    if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, q_weight, k_weight)):
+        return _HeadNorm.apply(q, k, q_weight, k_weight, eps, positions, cos, sin)
+    return _forward(q, k, q_weight, k_weight, eps, positions, cos, sin)

@@ -385,6 +385,112 @@ int htree_draft_attention(const htree_cache* c, int32_t B, int32_t rows, int32_t
                           void* out, int64_t out_row, int64_t out_head, void* workspace,
                           int64_t workspace_bytes, void* stream);
 
+/* Verification of drafted tokens.  target_probs / draft_probs [rows, V]
+ * (dtype, rows target_row / draft_row elements apart): the target's and the
+ * drafter's probabilities after each row.  The first row of a request is the
+ * token its last step decided on and is kept; a row c behind it is a draft of
+ * tokens[c] after row parents[c] (without parents: the row before), which is a
+ * smaller one of the request; other rows are never kept, nor is anything
+ * drafted after them.  At a kept row its drafts are tried in order, T being
+ * the target's probabilities there, S = 1:
+ *   with draft_probs (each drawn from draft_probs' row on its own): accepted
+ *     if uniforms[c] S q(token) < T(token), else T = max(T - S q, 0), S = sum T
+ *   without: accepted if uniforms[c] S < T(token), else T(token) = 0 and
+ *     S -= T(token)
+ * An accepted one is kept and the walk goes on there.  Where none is, the next
+ * token is the first whose cumulative T passes draws[b] sum T (T: the target's
+ * probabilities if nothing is left of them).  Sums are fp64.  Entries that are
+ * no positive finite numbers count as 0, and so do uniforms and draws that
+ * are not positive.
+ *   kept        [B] rows kept; 0 for a request without rows
+ *   path        [rows] from starts[b] on the kept rows' indices within their
+ *               request, ascending; -1 elsewhere
+ *   next_tokens [B]; -1 without rows or without any mass
+ * The first 1024 rows of a request are looked at. */
+int htree_verify_drafts_workspace_bytes(int32_t B, int32_t V, int64_t* bytes);
+int htree_verify_drafts(int32_t dtype, int32_t B, int32_t rows, int32_t V, const void* target_probs,
+                        int64_t target_row, const void* draft_probs, int64_t draft_row,
+                        const int64_t* tokens, const int32_t* starts, const int32_t* parents,
+                        const float* uniforms, const float* draws, int32_t* kept, int32_t* path,
+                        int64_t* next_tokens, void* workspace, int64_t workspace_bytes,
+                        void* stream);
+
+/* The accepted drafts of a step to the front of their request's new tokens, in
+ * the caches of `layers` layers (host arrays of device pointers; c describes
+ * each): what is in slot slots[starts[b] + path[starts[b] + j]] goes to slot
+ * slots[starts[b] + j], for j < kept[b].  path ascends (path[j] >= j); entries
+ * that do not are left out, and so are slots outside the cache. */
+int htree_keep_drafts(const htree_cache* c, int32_t layers, void* const* k_layers,
+                      void* const* v_layers, int32_t B, int32_t rows, const int64_t* slots,
+                      const int32_t* starts, const int32_t* path, const int32_t* kept,
+                      void* stream);
+
+/* N new requests out of B: new request i carries on from request source[i]
+ * (outside 0 .. B - 1: an empty one).  Full pages are shared.  A partly filled
+ * last page stays with the first new request of its source; each further one
+ * gets a fresh page, from free_pages [n_free] from the front, and the page's
+ * tokens have to be copied.
+ *   out_table   [N][out_stride] entries; -1 behind the last page
+ *   out_lens    [N]
+ *   copy_from, copy_to, copy_tokens [N] pages and tokens to copy
+ *               (htree_copy_pages), -1, -1 and 0 where there are none
+ *   pages_used  [1] pages wanted; more than n_free: the last ones are missing
+ *               (their entries are -1)
+ * HTREE_EOVERLAP: an output shares memory with an input or another output. */
+int htree_fork_requests(int32_t B, int32_t N, int32_t page_size, int32_t num_pages,
+                        int32_t table_width, int64_t table_stride, int64_t out_stride,
+                        int32_t n_free, const int32_t* block_table, const int32_t* lens,
+                        const int32_t* source, const int32_t* free_pages, int32_t* out_table,
+                        int32_t* out_lens, int32_t* copy_from, int32_t* copy_to,
+                        int32_t* copy_tokens, int32_t* pages_used, void* stream);
+
+/* The first tokens[i] tokens (NULL: all) of page from[i] to page to[i], in the
+ * caches of `layers` layers.  Pages outside the cache: nothing.  No page of
+ * `to` is in `from` too, nor twice in `to`. */
+int htree_copy_pages(const htree_cache* c, int32_t layers, void* const* k_layers,
+                     void* const* v_layers, int32_t n, const int32_t* from, const int32_t* to,
+                     const int32_t* tokens, void* stream);
+
+/* The pages of 0 .. num_pages - 1 that are in no live entry of the table
+ * (entries 0 .. ceil(lens[b] / page_size) - 1) and not among held [n_held]:
+ * pages [num_pages], ascending, -1 behind them, and count [1]. */
+int htree_unused_pages_workspace_bytes(int32_t num_pages, int64_t* bytes);
+int htree_unused_pages(int32_t B, int32_t page_size, int32_t num_pages, int32_t table_width,
+                       int64_t table_stride, const int32_t* block_table, const int32_t* lens,
+                       int32_t n_held, const int32_t* held, int32_t* pages, int32_t* count,
+                       void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Norms of queries [rows, H, D] and keys [rows, H_kv, D] by head, rotated in
+ * the same pass (strides in elements; outputs contiguous):
+ *   n = x (mean x^2 + eps)^-1/2 weight,  out = n rotated by the row's position
+ * with pairs (d, d + D/2) as htree_forward rotates them.  Weights [D] are fp32
+ * or of the inputs' type (w_dtype), NULL: ones; without positions and tables
+ * (all NULL) nothing is rotated.  Rows whose position is outside the tables
+ * are zero.  Everything is fp32, rounded once.  H or H_kv may be 0.
+ * HTREE_EUNSUPPORTED: D above 256 or not in whole 16-byte pieces, strides or
+ * bases off 16 bytes, rows (H + H_kv) past 31 bits. */
+int htree_head_norm(int32_t dtype, int32_t w_dtype, int32_t rows, int32_t H, int32_t H_kv,
+                    int32_t D, float eps, const void* q, int64_t q_row, int64_t q_head,
+                    const void* k, int64_t k_row, int64_t k_head, const void* q_weight,
+                    const void* k_weight, const int32_t* positions, const float* cos_table,
+                    const float* sin_table, int32_t rope_rows, void* q_out, void* k_out,
+                    void* stream);
+
+/* Its gradients: dq, dk (contiguous) from those of the outputs, dq_out and
+ * dk_out, and the weights' (w_dtype; NULL: not wanted; without both no
+ * workspace is needed).  Sums are fp32, in a fixed order. */
+int htree_head_norm_backward_workspace_bytes(int32_t D, int64_t* bytes);
+int htree_head_norm_backward(int32_t dtype, int32_t w_dtype, int32_t rows, int32_t H,
+                             int32_t H_kv, int32_t D, float eps, const void* q, int64_t q_row,
+                             int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
+                             const void* dq_out, int64_t dq_row, int64_t dq_head,
+                             const void* dk_out, int64_t dk_row, int64_t dk_head,
+                             const void* q_weight, const void* k_weight,
+                             const int32_t* positions, const float* cos_table,
+                             const float* sin_table, int32_t rope_rows, void* dq, void* dk,
+                             void* dq_weight, void* dk_weight, void* workspace,
+                             int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
