@@ -10,7 +10,8 @@ namespace htree {
 
 // ----------------------------------------------------------- moving tokens
 constexpr int kMoveLayers = 64;  // layers of a launch: their pointers are its arguments
-constexpr int kMoveUnroll = 8;   // tokens that a thread reads before it writes the first
+constexpr int kMoveTokens = 4;   // tokens and layers that a thread reads before it writes the first
+constexpr int kMoveAtOnce = 4;
 
 struct MoveArgs {
   char *k[kMoveLayers], *v[kMoveLayers];
@@ -18,6 +19,7 @@ struct MoveArgs {
   int32_t k_pieces, v_pieces;    // 16-byte pieces of a head
   int32_t pieces, k_all;         // of a token, and those of its keys
   int32_t page_shift, num_pages;
+  int32_t layers, by;            // of the launch, of a block (blockIdx.y)
 };
 
 struct KeepArgs {
@@ -34,29 +36,60 @@ struct CopyArgs {
 };
 
 // The column of a token's bytes that a thread owns: one 16-byte piece of a
-// head, in the keys' cache or the values'.
+// head, in the keys' caches or the values'.
 struct MoveColumn {
-  char* base;
-  int64_t page, token;
+  bool keys;
+  int64_t at, page, token;
 };
-__device__ __forceinline__ MoveColumn move_column(const MoveArgs& m, int layer, int piece) {
+__device__ __forceinline__ MoveColumn move_column(const MoveArgs& m, int piece) {
   MoveColumn c;
-  if (piece < m.k_all) {
-    const int h = piece / m.k_pieces;
-    c.base = m.k[layer] + h * m.k_head + (int64_t)(piece - h * m.k_pieces) * 16;
-    c.page = m.k_page, c.token = m.k_token;
-  } else {
-    piece -= m.k_all;
-    const int h = piece / m.v_pieces;
-    c.base = m.v[layer] + h * m.v_head + (int64_t)(piece - h * m.v_pieces) * 16;
-    c.page = m.v_page, c.token = m.v_token;
-  }
+  c.keys = piece < m.k_all;
+  if (!c.keys) piece -= m.k_all;
+  const int per = c.keys ? m.k_pieces : m.v_pieces, h = piece / per;
+  c.at = h * (c.keys ? m.k_head : m.v_head) + (int64_t)(piece - h * per) * 16;
+  c.page = c.keys ? m.k_page : m.v_page, c.token = c.keys ? m.k_token : m.v_token;
   return c;
+}
+
+// The column's pieces of kMoveTokens tokens (from / to: bytes from a layer's
+// base, to < 0: read, not written) in the block's layers: all tokens of four
+// layers are read before the first of them is written.
+__device__ __forceinline__ void move_tokens(const MoveArgs& m, const MoveColumn& c, const int64_t* from,
+                                            const int64_t* to) {
+  const int l1 = min((int)(blockIdx.y + 1) * m.by, m.layers);
+  for (int l0 = blockIdx.y * m.by; l0 < l1; l0 += kMoveAtOnce) {
+    char* base[kMoveAtOnce];
+    f32x4 x[kMoveAtOnce][kMoveTokens] = {};
+#pragma unroll
+    for (int l = 0; l < kMoveAtOnce; ++l) {
+      const int at = min(l0 + l, l1 - 1);
+      base[l] = c.keys ? m.k[at] : m.v[at];
+    }
+#pragma unroll
+    for (int l = 0; l < kMoveAtOnce; ++l) {
+      if (l0 + l >= l1) break;
+#pragma unroll
+      for (int i = 0; i < kMoveTokens; ++i) x[l][i] = *(const f32x4*)(base[l] + from[i]);
+    }
+    // one wait for all that was read: where the stores are conditional the
+    // compiler would wait at each, for the stores before it too
+#pragma unroll
+    for (int l = 0; l < kMoveAtOnce; ++l)
+#pragma unroll
+      for (int i = 0; i < kMoveTokens; ++i) asm volatile("" : "+v"(x[l][i]));
+#pragma unroll
+    for (int l = 0; l < kMoveAtOnce; ++l) {
+      if (l0 + l >= l1) break;
+#pragma unroll
+      for (int i = 0; i < kMoveTokens; ++i)
+        if (to[i] >= 0) *(f32x4*)(base[l] + to[i]) = x[l][i];
+    }
+  }
 }
 
 // Accepted drafts to the front of their request's new tokens: token j comes
 // from path[j] >= j.  A thread owns a piece of every token of its request, so
-// that the order in which tokens are read and written is its own: eight are
+// that the order in which tokens are read and written is its own: four are
 // read before the first of them is written, later ones come from places behind
 // all that were written.
 __global__ __launch_bounds__(256) void keep_drafts_kernel(KeepArgs a) {
@@ -64,27 +97,26 @@ __global__ __launch_bounds__(256) void keep_drafts_kernel(KeepArgs a) {
   if (piece >= a.m.pieces) return;
   const int s0 = min(max(a.starts[b], 0), a.rows), s1 = min(max(a.starts[b + 1], s0), a.rows);
   const int n = s1 - s0, kept = min(a.kept[b], n);
-  const MoveColumn c = move_column(a.m, blockIdx.y, piece);
+  const MoveColumn c = move_column(a.m, piece);
   const int64_t slots = (int64_t)a.m.num_pages << a.m.page_shift;
   const int64_t mask = ((int64_t)1 << a.m.page_shift) - 1;
-  for (int j0 = 0; j0 < kept; j0 += kMoveUnroll) {
-    uint4 x[kMoveUnroll];
-    int64_t to[kMoveUnroll];
+  for (int j0 = 0; j0 < kept; j0 += kMoveTokens) {
+    int64_t from[kMoveTokens], to[kMoveTokens];
+    bool any = false;
 #pragma unroll
-    for (int i = 0; i < kMoveUnroll; ++i) {
+    for (int i = 0; i < kMoveTokens; ++i) {
       const int j = j0 + i;
-      to[i] = -1;
+      from[i] = c.at, to[i] = -1;
       if (j >= kept) continue;
       const int p = a.path[s0 + j];
       if (p <= j || p >= n) continue;  // in its place already, or damaged
       const int64_t s = a.slots[s0 + p], d = a.slots[s0 + j];
       if (s < 0 || s >= slots || d < 0 || d >= slots) continue;
-      to[i] = d;
-      x[i] = *(const uint4*)(c.base + (s >> a.m.page_shift) * c.page + (s & mask) * c.token);
+      from[i] = c.at + (s >> a.m.page_shift) * c.page + (s & mask) * c.token;
+      to[i] = c.at + (d >> a.m.page_shift) * c.page + (d & mask) * c.token;
+      any = true;
     }
-#pragma unroll
-    for (int i = 0; i < kMoveUnroll; ++i)
-      if (to[i] >= 0) *(uint4*)(c.base + (to[i] >> a.m.page_shift) * c.page + (to[i] & mask) * c.token) = x[i];
+    if (any) move_tokens(a.m, c, from, to);
   }
 }
 
@@ -98,17 +130,16 @@ __global__ __launch_bounds__(256) void copy_pages_kernel(CopyArgs a) {
   const int col = threadIdx.x % a.columns, step = 256 / a.columns;
   const int piece = blockIdx.z * a.columns + col;
   if (piece >= a.m.pieces || (int)threadIdx.x >= step * a.columns) return;
-  const MoveColumn c = move_column(a.m, blockIdx.y, piece);
-  const char* src = c.base + from * c.page;
-  char* dst = c.base + to * c.page;
-  for (int t0 = threadIdx.x / a.columns; t0 < n; t0 += kMoveUnroll * step) {
-    uint4 x[kMoveUnroll];
+  const MoveColumn c = move_column(a.m, piece);
+  for (int t0 = threadIdx.x / a.columns; t0 < n; t0 += kMoveTokens * step) {
+    int64_t src[kMoveTokens], dst[kMoveTokens];
 #pragma unroll
-    for (int u = 0; u < kMoveUnroll; ++u)
-      if (t0 + u * step < n) x[u] = *(const uint4*)(src + (t0 + u * step) * c.token);
-#pragma unroll
-    for (int u = 0; u < kMoveUnroll; ++u)
-      if (t0 + u * step < n) *(uint4*)(dst + (t0 + u * step) * c.token) = x[u];
+    for (int u = 0; u < kMoveTokens; ++u) {
+      const int t = t0 + u * step;
+      src[u] = c.at + from * c.page + min(t, n - 1) * c.token;
+      dst[u] = t < n ? c.at + to * c.page + t * c.token : -1;
+    }
+    move_tokens(a.m, c, src, dst);
   }
 }
 
@@ -176,39 +207,181 @@ struct UnusedArgs {
   int64_t table_stride;
   int32_t B, width, page_shift, num_pages, n_held, tiles;
 };
-constexpr int kUnusedTile = 4096;  // pages a block counts or lists: 16 a thread
+constexpr int kUnusedTile = 4096;        // pages a block counts or lists: 16 a thread
+constexpr int kUnusedChunk = 1024;       // entries of a row that a wave reads at once: four times 4 a lane
+constexpr int kUnusedSmall = 1 << 16;    // entries, and held pages, of a call in one launch,
+constexpr int kUnusedSmallRows = 256;    // its requests
+constexpr int kUnusedSmallPages = 1 << 18;  // and pages, whose bits fill 32 KB of LDS
+constexpr int kUnusedSmallTile = 8192;   // pages a block lists: 8 a thread
 
-__global__ __launch_bounds__(256) void unused_clear_kernel(uint8_t* flags, int64_t n) {
-  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 16;
-  if (i < n) *(uint4*)(flags + i) = make_uint4(0, 0, 0, 0);
-}
+struct __attribute__((packed, aligned(4))) Entries {
+  int32_t v[4];
+};
 
-// Whoever holds a page writes the same 1: no atomics.
-__global__ __launch_bounds__(256) void unused_mark_kernel(UnusedArgs a) {
-  const int b = blockIdx.y;
-  if (b == a.B) {
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.n_held; i += (int64_t)gridDim.x * 256) {
-      const int pg = cache_page(a.held[i], a.num_pages);
-      if (pg >= 0) a.flags[pg] = 1;
-    }
+// Entries j0 .. j0 + kUnusedChunk - 1 of a request, by a wave.  A row's last
+// reads start earlier, not past its end: the entries that they see twice are
+// marked twice.  (Rows of less than four entries: one each.)
+struct Chunk {
+  Entries x[4];
+  int64_t at[4];
+};
+__device__ __forceinline__ void load_chunk(const UnusedArgs& a, int b, int64_t j0, Chunk* c) {
+  const int lane = threadIdx.x & 63;
+  const int32_t* row = a.table + b * a.table_stride;
+  if (a.width < 4) {
+    c->at[0] = lane;
+    c->x[0].v[0] = lane < a.width ? row[lane] : -1;
     return;
   }
-  const int64_t live = min(table_pages(max(a.lens[b], 0), a.page_shift), (int64_t)a.width);
-  const int32_t* row = a.table + b * a.table_stride;
-  for (int64_t j = (int64_t)blockIdx.x * 256 + threadIdx.x; j < live; j += (int64_t)gridDim.x * 256) {
-    const int pg = cache_page(row[j], a.num_pages);
-    if (pg >= 0) a.flags[pg] = 1;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    c->at[u] = min(j0 + u * 256 + lane * 4, (int64_t)a.width - 4);
+    c->x[u] = *(const Entries*)(row + c->at[u]);
   }
 }
+// f(page) for those before entry `live`
+template <typename F>
+__device__ __forceinline__ void mark_chunk(const UnusedArgs& a, const Chunk& c, int64_t live, F f) {
+  if (a.width < 4) {
+    if (c.at[0] < live) f(cache_page(c.x[0].v[0], a.num_pages));
+    return;
+  }
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (c.at[u] + e < live) f(cache_page(c.x[u].v[e], a.num_pages));
+}
+__device__ __forceinline__ int64_t live_pages(const UnusedArgs& a, int len) {
+  return min(table_pages(max(len, 0), a.page_shift), (int64_t)a.width);
+}
 
-// sum over the block's 256 threads, to all; `red` 4 ints
+// sum over the block's threads, to all; `red` an int for each wave
+template <int WAVES>
 __device__ __forceinline__ int block_sum(int x, int* red) {
 #pragma unroll
   for (int m = 32; m; m >>= 1) x += __shfl_xor(x, m);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
   __syncthreads();
-  return red[0] + red[1] + red[2] + red[3];
+  int all = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) all += red[w];
+  return all;
+}
+
+// Lists a block's unused pages, bit i of `bits`: page p0 + i of the thread's N,
+// from place `before` of the list on, and -1 in the block's places behind the
+// last of `all`.  They go through LDS, so that places are written in order.
+template <int WAVES, int N>
+__device__ __forceinline__ void list_pages(const UnusedArgs& a, uint32_t bits, int before, int all, int32_t* buf,
+                                           int* red) {
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+  const int64_t p0 = (int64_t)blockIdx.x * (WAVES * 64 * N);
+  int inc = __popc(bits);
+  const int mine = inc;
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) {
+    const int x = __shfl_up(inc, m);
+    if (lane >= m) inc += x;
+  }
+  __syncthreads();
+  if (lane == 63) red[wv] = inc;
+  __syncthreads();
+  int at = inc - mine, here = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) {
+    if (w < wv) at += red[w];
+    here += red[w];
+  }
+  for (; bits; bits &= bits - 1) buf[at++] = (int)(p0 + tid * N + __builtin_ctz(bits));
+  __syncthreads();
+  for (int i = tid; i < here; i += WAVES * 64) a.pages[(int64_t)before + i] = buf[i];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int64_t p = p0 + i * (WAVES * 64) + tid;
+    if (p >= all && p < a.num_pages) a.pages[p] = -1;
+  }
+  if (blockIdx.x == 0 && tid == 0) a.count[0] = all;
+}
+
+// A call in one launch: every block marks all pages that are held, in the bits
+// of its LDS, and lists its own part of the others.
+__global__ __launch_bounds__(1024) void unused_small_kernel(UnusedArgs a) {
+  extern __shared__ uint32_t small_bits[];  // 1: held; pages past the last one too
+  __shared__ int32_t buf[kUnusedSmallTile];
+  __shared__ int red[16];
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+  const int words = a.tiles * (kUnusedSmallTile / 32);
+  for (int i = tid; i < words; i += 1024) {
+    const int left = a.num_pages - i * 32;
+    small_bits[i] = left >= 32 ? 0u : left <= 0 ? ~0u : ~0u << left;
+  }
+  // lane r: the length of the wave's r-th request
+  const int mine = lane * 16 + wv, len = mine < a.B && lane < kUnusedSmallRows / 16 ? a.lens[mine] : 0;
+  __syncthreads();
+  auto mark = [&](int page) {
+    if (page >= 0) atomicOr(&small_bits[page >> 5], 1u << (page & 31));
+  };
+  // two requests' first chunks in flight
+  for (int r = 0, b = wv; b < a.B; r += 2, b += 32) {
+    const bool two = b + 16 < a.B;
+    const int64_t live[2] = {live_pages(a, __shfl(len, r)), two ? live_pages(a, __shfl(len, r + 1)) : 0};
+    Chunk c[2];
+    load_chunk(a, b, 0, &c[0]);
+    if (two) load_chunk(a, b + 16, 0, &c[1]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (live[i]) mark_chunk(a, c[i], live[i], mark);
+      for (int64_t j = kUnusedChunk; j < live[i]; j += kUnusedChunk) {
+        load_chunk(a, b + i * 16, j, &c[i]);
+        mark_chunk(a, c[i], live[i], mark);
+      }
+    }
+  }
+  for (int i = tid; i < a.n_held; i += 1024) mark(cache_page(a.held[i], a.num_pages));
+  __syncthreads();
+  const int first = blockIdx.x * (kUnusedSmallTile / 32);
+  int before = 0, all = 0;
+  for (int i = tid; i < words; i += 1024) {
+    const int n = 32 - __popc(small_bits[i]);
+    all += n;
+    if (i < first) before += n;
+  }
+  before = block_sum<16>(before, red);
+  all = block_sum<16>(all, red);
+  const uint32_t bits = ~(small_bits[first + tid / 4] >> (tid % 4 * 8)) & 255u;
+  list_pages<16, 8>(a, bits, before, all, buf, red);
+}
+
+__global__ __launch_bounds__(256) void unused_clear_kernel(uint8_t* flags, int64_t n) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 16;
+  if (i < n) *(uint4*)(flags + i) = make_uint4(0, 0, 0, 0);
+}
+
+// A wave a chunk of a request's entries (wave b + c B: chunk c of request b, so
+// that the first chunks, which have most of the live entries, are spread over
+// the dies); the last blocks mark the held pages.  Whoever holds a page writes
+// the same 1: no atomics.
+__global__ __launch_bounds__(256) void unused_mark_kernel(UnusedArgs a) {
+  const int64_t chunks = ((int64_t)a.width + kUnusedChunk - 1) / kUnusedChunk;
+  const int64_t blocks = (a.B * chunks + 3) / 4;
+  if (blockIdx.x >= blocks) {
+    const int64_t i = (blockIdx.x - blocks) * 256 + threadIdx.x;
+    const int page = i < a.n_held ? cache_page(a.held[i], a.num_pages) : -1;
+    if (page >= 0) a.flags[page] = 1;
+    return;
+  }
+  const int64_t wave = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t c = wave / a.B, b = wave - c * a.B;
+  if (c >= chunks) return;
+  const int64_t live = live_pages(a, a.lens[b]);
+  if (c * kUnusedChunk >= live) return;
+  Chunk x;
+  load_chunk(a, (int)b, c * kUnusedChunk, &x);
+  mark_chunk(a, x, live, [&](int page) {
+    if (page >= 0) a.flags[page] = 1;
+  });
 }
 
 // bit i: page p0 + i is unused
@@ -225,41 +398,23 @@ __device__ __forceinline__ uint32_t unused_bits(const UnusedArgs& a, int64_t p0)
 __global__ __launch_bounds__(256) void unused_count_kernel(UnusedArgs a) {
   __shared__ int red[4];
   const int64_t p0 = (int64_t)blockIdx.x * kUnusedTile + threadIdx.x * 16;
-  const int n = block_sum(__popc(unused_bits(a, p0)), red);
+  const int n = block_sum<4>(__popc(unused_bits(a, p0)), red);
   if (threadIdx.x == 0) a.counts[blockIdx.x] = n;
 }
 
 __global__ __launch_bounds__(256) void unused_list_kernel(UnusedArgs a) {
+  __shared__ int32_t buf[kUnusedTile];
   __shared__ int red[4];
-  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+  const uint32_t bits = unused_bits(a, (int64_t)blockIdx.x * kUnusedTile + threadIdx.x * 16);
   int before = 0, all = 0;
-  for (int t = tid; t < a.tiles; t += 256) {
+  for (int t = threadIdx.x; t < a.tiles; t += 256) {
     const int n = a.counts[t];
     all += n;
     if (t < (int)blockIdx.x) before += n;
   }
-  before = block_sum(before, red);
-  all = block_sum(all, red);
-  const int64_t p0 = (int64_t)blockIdx.x * kUnusedTile + tid * 16;
-  uint32_t bits = unused_bits(a, p0);
-  int inc = __popc(bits);
-  const int mine = inc;
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
-    const int x = __shfl_up(inc, m);
-    if (lane >= m) inc += x;
-  }
-  __syncthreads();
-  if (lane == 63) red[wv] = inc;
-  __syncthreads();
-  int at = before + inc - mine;
-  for (int w = 0; w < wv; ++w) at += red[w];
-  for (; bits; bits &= bits - 1) a.pages[at++] = (int)(p0 + __builtin_ctz(bits));
-  // the list's places behind the last unused page
-#pragma unroll
-  for (int i = 0; i < 16; ++i)
-    if (p0 + i >= all && p0 + i < a.num_pages) a.pages[p0 + i] = -1;
-  if (blockIdx.x == 0 && tid == 0) a.count[0] = all;
+  before = block_sum<4>(before, red);
+  all = block_sum<4>(all, red);
+  list_pages<4, 16>(a, bits, before, all, buf, red);
 }
 
 // ------------------------------------------------------------------ host
@@ -285,13 +440,16 @@ static int move_args(const htree_cache* c, int32_t layers, void* const* k, void*
   return HTREE_OK;
 }
 
-// runs f(layers of this launch) for 64 layers at a time
+// runs f(blocks in y) for 64 layers at a time; `blocks` in x and z
 template <typename F>
-static int by_layers(int32_t layers, void* const* k, void* const* v, MoveArgs* m, F f) {
+static int by_layers(int32_t layers, void* const* k, void* const* v, int64_t blocks, MoveArgs* m, F f) {
   for (int l = 0; l < layers; l += kMoveLayers) {
     const int n = layers - l < kMoveLayers ? layers - l : kMoveLayers;
     for (int i = 0; i < n; ++i) m->k[i] = (char*)k[l + i], m->v[i] = (char*)v[l + i];
-    f(n);
+    // a block for each layer until the GPU is full, then as many layers each
+    m->layers = n;
+    m->by = blocks * n <= 1024 ? 1 : 4;
+    f((n + m->by - 1) / m->by);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return (int)e;
   }
@@ -315,8 +473,8 @@ extern "C" int htree_keep_drafts(const htree_cache* c, int32_t layers, void* con
   a.slots = slots, a.starts = starts, a.path = path, a.kept = kept, a.rows = rows;
   const unsigned threads = a.m.pieces >= 256 ? 256 : (a.m.pieces + 63) / 64 * 64;
   const unsigned z = (a.m.pieces + threads - 1) / threads;
-  return by_layers(layers, k_layers, v_layers, &a.m, [&](int n) {
-    hipLaunchKernelGGL(keep_drafts_kernel, dim3(B, n, z), dim3(threads), 0, (hipStream_t)stream, a);
+  return by_layers(layers, k_layers, v_layers, (int64_t)B * z, &a.m, [&](int y) {
+    hipLaunchKernelGGL(keep_drafts_kernel, dim3(B, y, z), dim3(threads), 0, (hipStream_t)stream, a);
   });
 }
 
@@ -332,8 +490,8 @@ extern "C" int htree_copy_pages(const htree_cache* c, int32_t layers, void* cons
   a.from = from, a.to = to, a.tokens = tokens, a.n = n;
   a.columns = a.m.pieces < 256 ? a.m.pieces : 256;
   const unsigned z = (a.m.pieces + a.columns - 1) / a.columns;
-  return by_layers(layers, k_layers, v_layers, &a.m, [&](int l) {
-    hipLaunchKernelGGL(copy_pages_kernel, dim3(n, l, z), dim3(256), 0, (hipStream_t)stream, a);
+  return by_layers(layers, k_layers, v_layers, (int64_t)n * z, &a.m, [&](int y) {
+    hipLaunchKernelGGL(copy_pages_kernel, dim3(n, y, z), dim3(256), 0, (hipStream_t)stream, a);
   });
 }
 
@@ -373,11 +531,18 @@ extern "C" int htree_fork_requests(int32_t B, int32_t N, int32_t page_size, int3
   return e == hipSuccess ? HTREE_OK : (int)e;
 }
 
-extern "C" int htree_unused_pages_workspace_bytes(int32_t num_pages, int64_t* bytes) {
+// whether a call runs in one launch
+static bool unused_small(int32_t B, int32_t num_pages, int32_t table_width, int32_t n_held) {
+  return num_pages <= kUnusedSmallPages && B <= kUnusedSmallRows && n_held <= kUnusedSmall &&
+         (int64_t)B * table_width <= kUnusedSmall;
+}
+
+extern "C" int htree_unused_pages_workspace_bytes(int32_t B, int32_t num_pages, int32_t table_width, int32_t n_held,
+                                                  int64_t* bytes) {
   if (!bytes) return HTREE_ENULL;
-  if (num_pages < 0) return HTREE_ESHAPE;
+  if (B < 0 || num_pages < 0 || table_width < 0 || n_held < 0) return HTREE_ESHAPE;
   const int64_t tiles = ((int64_t)num_pages + kUnusedTile - 1) / kUnusedTile;
-  *bytes = tiles * (kUnusedTile + 4);
+  *bytes = unused_small(B, num_pages, table_width, n_held) ? 0 : tiles * (kUnusedTile + 4);
   return HTREE_OK;
 }
 
@@ -385,15 +550,16 @@ extern "C" int htree_unused_pages(int32_t B, int32_t page_size, int32_t num_page
                                   int64_t table_stride, const int32_t* block_table, const int32_t* lens,
                                   int32_t n_held, const int32_t* held, int32_t* pages, int32_t* count,
                                   void* workspace, int64_t workspace_bytes, void* stream) {
-  if (B < 0 || num_pages < 0 || table_width < 0 || n_held < 0) return HTREE_ESHAPE;
+  int64_t need = 0;
+  const int rc = htree_unused_pages_workspace_bytes(B, num_pages, table_width, n_held, &need);
+  if (rc) return rc;
   if (B > 1 && table_stride < table_width) return HTREE_ESHAPE;
   if (page_size < 1 || (page_size & (page_size - 1)) || B > kCacheMaxRequests) return HTREE_EUNSUPPORTED;
   if (num_pages == 0) return HTREE_OK;
-  if (!pages || !count || !workspace || (n_held && !held) || (B && !lens) || (B && table_width && !block_table))
+  if (!pages || !count || (need && !workspace) || (n_held && !held) || (B && !lens) ||
+      (B && table_width && !block_table))
     return HTREE_ENULL;
   if (off16(workspace)) return HTREE_EUNSUPPORTED;
-  int64_t need = 0;
-  htree_unused_pages_workspace_bytes(num_pages, &need);
   if (workspace_bytes < need) return HTREE_EWORKSPACE;
   const Range in[3] = {{block_table, B && table_width ? ((B - 1) * table_stride + table_width) * 4 : 0},
                        {lens, B * 4ll}, {held, n_held * 4ll}};
@@ -406,20 +572,26 @@ extern "C" int htree_unused_pages(int32_t B, int32_t page_size, int32_t num_page
   }
   UnusedArgs a;
   a.table = block_table, a.lens = lens, a.held = held;
-  a.tiles = (int)(((int64_t)num_pages + kUnusedTile - 1) / kUnusedTile);
-  a.flags = (uint8_t*)workspace;
-  a.counts = (int32_t*)(a.flags + (int64_t)a.tiles * kUnusedTile);
   a.pages = pages, a.count = count;
   a.table_stride = table_stride;
   a.B = B, a.width = table_width, a.page_shift = log2i(page_size), a.num_pages = num_pages, a.n_held = n_held;
   hipStream_t s = (hipStream_t)stream;
-  hipLaunchKernelGGL(unused_clear_kernel, dim3(a.tiles), dim3(256), 0, s, a.flags, (int64_t)a.tiles * kUnusedTile);
-  const int64_t most = table_width > n_held ? table_width : n_held;
-  const unsigned gx = (unsigned)(most <= 1024 ? 1 : most >= 16384 ? 16 : (most + 1023) / 1024);
-  if (B + (n_held > 0) > 0)
-    hipLaunchKernelGGL(unused_mark_kernel, dim3(gx, B + (n_held > 0)), dim3(256), 0, s, a);
-  hipLaunchKernelGGL(unused_count_kernel, dim3(a.tiles), dim3(256), 0, s, a);
-  hipLaunchKernelGGL(unused_list_kernel, dim3(a.tiles), dim3(256), 0, s, a);
+  if (unused_small(B, num_pages, table_width, n_held)) {
+    a.tiles = (num_pages + kUnusedSmallTile - 1) / kUnusedSmallTile;
+    a.flags = nullptr, a.counts = nullptr;
+    hipLaunchKernelGGL(unused_small_kernel, dim3(a.tiles), dim3(1024), a.tiles * (kUnusedSmallTile / 8), s, a);
+  } else {
+    a.tiles = (int)(((int64_t)num_pages + kUnusedTile - 1) / kUnusedTile);
+    a.flags = (uint8_t*)workspace;
+    a.counts = (int32_t*)(a.flags + (int64_t)a.tiles * kUnusedTile);
+    const int64_t chunks = ((int64_t)table_width + kUnusedChunk - 1) / kUnusedChunk;
+    const int64_t blocks = (B * chunks + 3) / 4 + ((int64_t)n_held + 255) / 256;
+    if (blocks > 0x7fffffff) return HTREE_EUNSUPPORTED;
+    hipLaunchKernelGGL(unused_clear_kernel, dim3(a.tiles), dim3(256), 0, s, a.flags, (int64_t)a.tiles * kUnusedTile);
+    if (blocks) hipLaunchKernelGGL(unused_mark_kernel, dim3((unsigned)blocks), dim3(256), 0, s, a);
+    hipLaunchKernelGGL(unused_count_kernel, dim3(a.tiles), dim3(256), 0, s, a);
+    hipLaunchKernelGGL(unused_list_kernel, dim3(a.tiles), dim3(256), 0, s, a);
+  }
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? HTREE_OK : (int)e;
 }

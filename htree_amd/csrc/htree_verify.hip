@@ -21,27 +21,36 @@
 namespace htree {
 
 constexpr int kVerifyRows = 1024;    // of a request that are looked at
-constexpr int kVerifySegment = 8192; // elements of a row that a block sums: 8 a thread, 4 times (pick: once)
-constexpr int kVerifySum = 256, kVerifyPick = 1024;  // threads
+constexpr int kVerifyThreads = 1024;
+constexpr int kVerifyWaves = kVerifyThreads / 64;
+constexpr int kVerifyStep = 64 * 8;  // elements that a wave takes at once: 8 a lane
+constexpr int kVerifySteps = 4;      // steps in a range, at least; of 16-bit types as many are in flight
 
-// where a request's walk ended
+// Few requests over a large vocabulary: `parts` blocks share a request's sums.
+constexpr int kVerifyParts = 4;        // at most: their waves' sums fill a wave
+constexpr int kVerifySplit = 1 << 17;  // elements of a row of p (and q) from which on they do,
+constexpr int kVerifyPart = 1 << 14;   // and that a part has at least
+constexpr int kVerifyFull = 256;       // blocks that fill the GPU
+
+// where a request's walk ended, for verify_draw_kernel
 struct VerifyEnd {
-  double off;      // a: T = max(p - a q, 0)
-  int32_t row;     // of p and q, -1: the request has no rows
-  int32_t node;    // the same within the request; its children are all rejected
+  double off;
+  int32_t row, node, n;  // row -1: the request has none
+  int32_t unused;
 };
 
 struct VerifyArgs {
+  VerifyEnd* ends;  // [B]
+  double* sums;     // [B][parts][waves]
+  int32_t parts;
   const char *p, *q;
   const int64_t* tokens;
   const int32_t *starts, *parents;
   const float *uniforms, *draws;
   int32_t *kept, *path;
   int64_t* next;
-  VerifyEnd* ends;  // [B]
-  double* sums;     // [B][segments][2] of T and of p
   int64_t p_row, q_row;  // elements
-  int32_t B, rows, V, segments;
+  int32_t B, rows, V;
 };
 
 // NV elements from anywhere: rows of an odd vocabulary begin at any element
@@ -53,27 +62,41 @@ struct __attribute__((packed, aligned(sizeof(T)))) Elements {
 // what an entry counts for: nothing if it is no positive number
 template <typename T>
 __device__ __forceinline__ float mass(T x) {
-  const float f = (float)x;
-  return f > 0.f && f < INFINITY ? f : 0.f;
+  const float f = fmaxf((float)x, 0.f);  // (of a NaN: 0)
+  return f < INFINITY ? f : 0.f;
 }
 __device__ __forceinline__ double left_of(float p, float q, double a) { return fmax((double)p - a * (double)q, 0.0); }
 
-__device__ __forceinline__ double wave_sum(double x) {
-#pragma unroll
-  for (int m = 32; m; m >>= 1) x += __shfl_xor(x, m);
+// the value that DPP pattern CTRL brings to a lane, 0 where it brings none
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double from_lane(double x) {
+  const int lo = __builtin_amdgcn_update_dpp(0, __double2loint(x), CTRL, ROWS, 0xf, true);
+  const int hi = __builtin_amdgcn_update_dpp(0, __double2hiint(x), CTRL, ROWS, 0xf, true);
+  return __hiloint2double(hi, lo);
+}
+// Sums up to a lane, in the same order whoever asks: within rows of 16 lanes,
+// then the rows in front.  A quarter of the time of shuffles through LDS.
+__device__ __forceinline__ double wave_scan(double x) {
+  x += from_lane<0x111, 0xf>(x);  // from the lane in front,
+  x += from_lane<0x112, 0xf>(x);  // two,
+  x += from_lane<0x114, 0xf>(x);  // four
+  x += from_lane<0x118, 0xf>(x);  // and eight in front
+  x += from_lane<0x142, 0xa>(x);  // rows 1, 3: the last lane of the row in front
+  x += from_lane<0x143, 0xc>(x);  // rows 2, 3: lane 31
   return x;
 }
-
-// rows s0 .. s0 + n - 1 are request b's
-__device__ __forceinline__ int verify_rows(const VerifyArgs& a, int b, int* s0) {
-  *s0 = min(max(a.starts[b], 0), a.rows);
-  return min(max(a.starts[b + 1], *s0), a.rows) - *s0;
+__device__ __forceinline__ double lane_value(double x, int lane) {
+  return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(x), lane),
+                          __builtin_amdgcn_readlane(__double2loint(x), lane));
 }
+__device__ __forceinline__ double wave_sum(double x) { return lane_value(wave_scan(x), 63); }
 
 struct VerifyLds {
   int32_t parent[kVerifyRows], token[kVerifyRows];
   float p[kVerifyRows], q[kVerifyRows], u[kVerifyRows];
-  double red[kVerifyPick / 64];
+  double red[kVerifyWaves];
+  double sums[kVerifyParts * kVerifyWaves];  // of the ranges
+  int32_t found;
 };
 
 // The first child of `node` behind row c, -1: none.  The same in every wave.
@@ -96,323 +119,400 @@ __device__ __forceinline__ bool had_token(const VerifyLds& l, int node, int c) {
   return false;
 }
 
-// A block a request: its drafts' tests, one after another, and the path.
+// What is left of the target's probabilities at a row: max(p - a q, 0), p
+// itself (a = 0), or p without the tokens of the row's children.
 template <typename T>
-__global__ __launch_bounds__(kVerifyPick) void verify_walk_kernel(VerifyArgs a) {
+struct Left {
+  const T *p, *q;  // q: nullptr, nothing of it is taken off
+  double off;
+  int node, n;     // children that take their tokens away are rows of this parent; n = 0: none do
+};
+
+template <typename T>
+struct Eight {
+  Elements<T, 8> p, q;
+};
+// The eight elements from e on; where the row ends before, its last eight.
+// (V >= 8.)
+template <typename T>
+__device__ __forceinline__ void load_p(const Left<T>& l, int64_t e, int V, Eight<T>* x) {
+  x->p = *(const Elements<T, 8>*)(l.p + min(e, (int64_t)V - 8));
+}
+template <typename T>
+__device__ __forceinline__ void load_q(const Left<T>& l, int64_t e, int V, Eight<T>* x) {
+  x->q = *(const Elements<T, 8>*)(l.q + min(e, (int64_t)V - 8));
+}
+
+// The largest of eight bit patterns, as unsigned numbers: below infinity's
+// all of them are numbers that are not negative.
+__device__ __forceinline__ uint32_t most_bits(const Elements<float, 8>& x) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, __builtin_bit_cast(uint32_t, x.v[i]));
+  return m;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t most_bits(const Elements<T, 8>& x) {
+  typedef __attribute__((ext_vector_type(8))) unsigned short u16x8;
+  typedef __attribute__((ext_vector_type(2))) unsigned short u16x2;
+  const u16x8 v = __builtin_bit_cast(u16x8, x);
+  const u16x2 m = __builtin_elementwise_max(__builtin_elementwise_max(v.s01, v.s23),
+                                            __builtin_elementwise_max(v.s45, v.s67));
+  return max((uint32_t)m.x, (uint32_t)m.y);
+}
+__device__ __forceinline__ uint32_t infinity_bits(float) { return 0x7f800000u; }
+__device__ __forceinline__ uint32_t infinity_bits(__bf16) { return 0x7f80u; }
+__device__ __forceinline__ uint32_t infinity_bits(_Float16) { return 0x7c00u; }
+
+// t of those eight elements.  mass() of each would be a third of the instructions:
+// only eights that hold something else than finite numbers >= 0 go through it.
+template <typename T>
+__device__ __forceinline__ void left_eight(const Left<T>& l, Eight<T>& x, double* t) {
+  if (most_bits(x.p) >= infinity_bits(T())) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x.p.v[i] = (T)mass(x.p.v[i]);
+  }
+  if (l.q) {
+    if (most_bits(x.q) >= infinity_bits(T())) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x.q.v[i] = (T)mass(x.q.v[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = left_of((float)x.p.v[i], (float)x.q.v[i], l.off);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = (double)(float)x.p.v[i];
+  }
+}
+
+// What a lane's eight elements from e on count for: those that are there, and
+// whose tokens the row's children do not take away (`some`: there may be such).
+// The wave's elements are e0 .. e0 + 511.
+template <typename T>
+__device__ __forceinline__ void count_eight(const Left<T>& l, const VerifyLds& s, Eight<T>& x, int64_t e0, int V,
+                                            bool some, double* t) {
+  const int lane = threadIdx.x & 63;
+  const int64_t e = e0 + lane * 8;
+  left_eight(l, x, t);
+  int at = lane * 8;  // of the first element, from e0
+  if (e0 + kVerifyStep > V) {
+    const int64_t over = e - min(e, (int64_t)V - 8);  // elements that the lanes in front have
+    at -= (int)over;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = i < over ? 0.0 : t[i];
+  }
+  if (!some) return;
+  for (int c0 = l.node + 1; c0 < l.n; c0 += 64) {
+    const int c = min(c0 + lane, kVerifyRows - 1);
+    const int64_t token = s.token[c] - e0;
+    uint64_t hit = __ballot(c0 + lane < l.n && s.parent[c] == l.node && token >= 0 && token < kVerifyStep);
+    for (; hit; hit &= hit - 1) {
+      const int gone = __shfl((int)token, __builtin_ctzll(hit));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) t[i] = at + i == gone ? 0.0 : t[i];
+    }
+  }
+}
+
+// Element e alone, for vocabularies of less than eight.
+template <typename T>
+__device__ __forceinline__ double count_one(const Left<T>& l, const VerifyLds& s, int e) {
+  for (int c = l.node + 1; c < l.n; ++c)
+    if (s.parent[c] == l.node && s.token[c] == e) return 0.0;
+  return l.q ? left_of(mass(l.p[e]), mass(l.q[e]), l.off) : (double)mass(l.p[e]);
+}
+
+// Range w is the elements w size .. (w + 1) size - 1.
+__device__ __forceinline__ int64_t range_size(int V, int ranges) {
+  constexpr int once = kVerifySteps * kVerifyStep;
+  return (((int64_t)V + once - 1) / once + ranges - 1) / ranges * once;
+}
+
+// A wave's sum of range w.  (Taking the children's tokens off the sum
+// afterwards would round away what is left beside them.)
+template <typename T>
+__device__ __forceinline__ double range_sum(const Left<T>& l, const VerifyLds& s, int V, int w, int ranges) {
+  constexpr int U = sizeof(T) == 4 ? kVerifySteps / 2 : kVerifySteps;  // steps in flight
+  const int lane = threadIdx.x & 63;
+  const int64_t size = range_size(V, ranges), e0 = w * size, e1 = min(e0 + size, (int64_t)V);
+  bool some = false;  // a child's token in this range
+  for (int i = l.node + 1 + lane; i < l.n; i += 64)
+    some |= s.parent[i] == l.node && s.token[i] >= e0 && s.token[i] < e1;
+  some = __any(some);
+  double sum = 0.0;
+  for (int64_t e = e0; e < e1; e += U * kVerifyStep) {
+    Eight<T> x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) load_p(l, e + u * kVerifyStep + lane * 8, V, &x[u]);
+    if (l.q) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) load_q(l, e + u * kVerifyStep + lane * 8, V, &x[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      double t[8];
+      count_eight(l, s, x[u], e + u * kVerifyStep, V, some, t);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum += t[i];
+    }
+  }
+  return wave_sum(sum);
+}
+
+// The thread whose share of a cumulative sum first passes t: every thread
+// comes with its share `mine` and gets the sum before it, from `base` on.
+// Returns that thread, -1 where rounding or the range leaves none; `all` is the
+// sum behind the last thread.
+__device__ __forceinline__ int find_share(double mine, double base, double t, VerifyLds& s, double* before,
+                                          double* all) {
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const double inc = wave_scan(mine);
+  __syncthreads();  // what an earlier call left has been read
+  if (tid == 0) s.found = 0x7fffffff;
+  if (lane == 63) s.red[wv] = inc;
+  __syncthreads();
+  const double waves = wave_scan(lane < kVerifyWaves ? s.red[lane] : 0.0);
+  const double front = base + (wv ? lane_value(waves, wv - 1) : 0.0);
+  *all = base + lane_value(waves, 63);
+  // the sum before a thread is the one up to its neighbour, to the bit
+  const double up = __shfl_up(inc, 1);
+  *before = lane ? front + up : front;
+  const uint64_t hit = __ballot(mine > 0.0 && front + inc > t);
+  if (hit && lane == 0) atomicMin(&s.found, wv * 64 + __builtin_ctzll(hit));
+  __syncthreads();
+  return s.found == 0x7fffffff ? -1 : s.found;
+}
+
+// The first element whose cumulative sum passes `draw` of the total, or where
+// rounding leaves none the last with any mass; -1: there is no mass.  The
+// ranges' sums (64 at most) are in s.sums.
+template <typename T>
+__device__ __forceinline__ int64_t find_element(const Left<T>& l, VerifyLds& s, int V, int ranges, float draw) {
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const double part = draw > 0.f ? (double)draw : 0.0;
+  if (V < 8) {
+    double total = 0.0, sum = 0.0;
+    for (int e = 0; e < V; ++e) total += count_one(l, s, e);
+    int at = -1;
+    for (int e = 0; e < V && !(sum > part * total); ++e) {
+      const double x = count_one(l, s, e);
+      if (x > 0.0) at = e;
+      sum += x;
+    }
+    return at;
+  }
+  // its range: the same choice in every wave
+  const double mine = lane < ranges ? s.sums[lane] : 0.0, up_to = wave_scan(mine);
+  const double t = part * lane_value(up_to, 63);
+  const uint64_t any = __ballot(mine > 0.0), pass = __ballot(mine > 0.0 && up_to > t);
+  if (!any) return -1;
+  const int w = pass ? __builtin_ctzll(pass) : 63 - __builtin_clzll(any);
+  double base = w ? lane_value(up_to, w - 1) : 0.0;
+  const int64_t size = range_size(V, ranges), e0 = w * size, e1 = min(e0 + size, (int64_t)V);
+  __shared__ int64_t token;
+  __syncthreads();
+  if (tid == 0) token = -1;
+  for (int64_t e = e0; e < e1; e += kVerifyThreads * 8) {
+    // ranges are whole steps: a wave's elements are in this one or behind it
+    const int64_t first = e + wv * kVerifyStep, at = min(first + lane * 8, (int64_t)V - 8);
+    double x[8], share = 0.0, before, all;
+    if (first < e1) {
+      Eight<T> v;
+      load_p(l, at, V, &v);
+      if (l.q) load_q(l, at, V, &v);
+      count_eight(l, s, v, first, V, l.n > 0, x);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) share += x[i];
+    }
+    int who = find_share(share, base, t, s, &before, &all);
+    const bool passed = who >= 0;
+    if (!passed) {
+      // the last thread with a share, for when none passes
+      __syncthreads();
+      if (tid == 0) s.found = -1;
+      __syncthreads();
+      const uint64_t hit = __ballot(share > 0.0);
+      if (hit && (tid & 63) == 0) atomicMax(&s.found, (tid | 63) - __builtin_clzll(hit));
+      __syncthreads();
+      who = s.found;
+    }
+    if (tid == who) {
+      int last = 0;
+      double run = before;
+      bool done = false;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (!done && x[i] > 0.0) {
+          last = i;
+          run += x[i];
+          done = passed && run > t;
+        }
+      token = at + last;
+    }
+    if (passed) break;
+    base = all;
+  }
+  __syncthreads();
+  return token;
+}
+
+// The sum over a row, or over part `part` of `parts` of it, by the whole block:
+// its waves' shares in s.sums.
+template <typename T>
+__device__ __forceinline__ double row_sum(const Left<T>& l, VerifyLds& s, int V, int part, int parts) {
+  if (V < 8) {
+    double all = 0.0;
+    for (int e = 0; e < V; ++e) all += count_one(l, s, e);
+    return all;
+  }
+  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const double x = range_sum(l, s, V, part * kVerifyWaves + wv, parts * kVerifyWaves);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) s.sums[wv] = x;
+  __syncthreads();
+  const int lane = threadIdx.x & 63;
+  return wave_sum(lane < kVerifyWaves ? s.sums[lane] : 0.0);
+}
+
+__device__ __forceinline__ int load_row(const VerifyArgs& a, VerifyLds& l, int s0, int i) {
+  const int64_t x = a.tokens[s0 + i];
+  int up = a.parents ? draft_parent(a.parents[s0 + i], i) : i - 1;
+  if (x < 0 || x >= a.V) up = -1;  // no token: no draft
+  l.parent[i] = up;
+  l.token[i] = (int)x;
+  return up;
+}
+
+// A block a request: its drafts' tests one after another, the path, then the
+// next token from what is left at the last kept row.  With `parts` blocks a
+// request each makes the same tests, and a part of the last sums.
+template <typename T>
+__global__ __launch_bounds__(kVerifyThreads) void verify_drafts_kernel(VerifyArgs a) {
   __shared__ VerifyLds l;
-  const int b = blockIdx.x, tid = threadIdx.x, wv = tid >> 6;
+  const int b = blockIdx.x, part = blockIdx.y, tid = threadIdx.x;
   const T *P = (const T*)a.p, *Q = (const T*)a.q;
-  int s0;
-  const int rows = verify_rows(a, b, &s0), n = min(rows, kVerifyRows);
-  for (int i = tid; i < rows; i += kVerifyPick) a.path[s0 + i] = i ? -1 : 0;
-  // rows of no request
-  if (b == 0)
-    for (int i = tid; i < s0; i += kVerifyPick) a.path[i] = -1;
-  if (b == a.B - 1)
-    for (int i = s0 + rows + tid; i < a.rows; i += kVerifyPick) a.path[i] = -1;
+  const int s0 = min(max(a.starts[b], 0), a.rows), s1 = min(max(a.starts[b + 1], s0), a.rows);
+  const int rows = s1 - s0, n = min(rows, kVerifyRows);
+  if (part == 0) {
+    for (int i = tid; i < rows; i += kVerifyThreads) a.path[s0 + i] = i ? -1 : 0;
+    // rows of no request
+    if (b == 0)
+      for (int i = tid; i < s0; i += kVerifyThreads) a.path[i] = -1;
+    if (b == a.B - 1)
+      for (int i = s1 + tid; i < a.rows; i += kVerifyThreads) a.path[i] = -1;
+  }
+  const bool writes = part == 0 && tid == 0;
   if (n == 0) {
-    if (tid == 0) {
-      a.kept[b] = 0;
-      a.ends[b] = {0.0, -1, -1};
+    if (writes) {
+      a.kept[b] = 0, a.next[b] = -1;
+      if (a.parts > 1) a.ends[b].row = -1;
     }
     return;
   }
-  for (int i = tid; i < n; i += kVerifyPick) {
-    const int64_t x = a.tokens[s0 + i];
-    int up = a.parents ? draft_parent(a.parents[s0 + i], i) : i - 1;
-    if (x < 0 || x >= a.V) up = -1;  // no token: no draft
-    l.parent[i] = up;
-    l.token[i] = (int)x;
+  for (int i = tid; i < n; i += kVerifyThreads) {
+    const int up = load_row(a, l, s0, i);
     if (up >= 0) {
-      l.p[i] = mass(P[(s0 + up) * a.p_row + x]);
-      l.q[i] = Q ? mass(Q[(s0 + up) * a.q_row + x]) : 1.f;
+      l.p[i] = mass(P[(s0 + up) * a.p_row + l.token[i]]);
+      l.q[i] = Q ? mass(Q[(s0 + up) * a.q_row + l.token[i]]) : 1.f;
       const float u = a.uniforms[s0 + i];
       l.u[i] = u > 0.f ? u : 0.f;
     }
   }
+  const float draw = a.draws[b];
   __syncthreads();  // also: the path's -1s are written before its places
-  int node = 0, kept = 1;
-  double off = 0.0, S = 1.0;
-  for (int c = next_child(l, n, 0, 0); c >= 0;) {
-    const double px = l.p[c], qx = l.q[c], u = l.u[c];
-    bool ok, gone = false;
-    if (Q) {
-      ok = u * S * qx < px - off * qx;
-    } else {
-      gone = had_token(l, node, c);
-      ok = !gone && u * S < px;
-    }
-    if (ok) {
-      node = c, off = 0.0, S = 1.0;
-      if (tid == 0) a.path[s0 + kept] = c;
-      ++kept;
-      c = next_child(l, n, node, c);
-      continue;
-    }
-    c = next_child(l, n, node, c);
-    if (!Q) {
-      if (!gone) S -= px;
-      continue;
-    }
-    off += S;
-    if (c < 0) break;
-    // the mass that is left for the next sibling
-    constexpr int NV = 16 / (int)sizeof(T);
-    const T *pr = P + (s0 + node) * a.p_row, *qr = Q + (s0 + node) * a.q_row;
-    double sum = 0.0;
-    for (int e = tid * NV; e < a.V; e += kVerifyPick * NV) {
-      if (e + NV <= a.V) {
-        const Elements<T, NV> x = *(const Elements<T, NV>*)(pr + e), y = *(const Elements<T, NV>*)(qr + e);
-#pragma unroll
-        for (int i = 0; i < NV; ++i) sum += left_of(mass(x.v[i]), mass(y.v[i]), off);
+  Left<T> left = {P + s0 * a.p_row, nullptr, 0.0, 0, 0};
+  int node = 0, kept = 1, c = next_child(l, n, 0, 0);
+  double S = 1.0, total;
+  // one place for the sums over a row, whichever they are for: the code of three
+  // would be read from memory by every block
+  for (;;) {
+    while (c >= 0) {
+      const double px = l.p[c], qx = l.q[c], u = l.u[c];
+      bool ok, gone = false;
+      if (Q) {
+        ok = u * S * qx < px - left.off * qx;
       } else {
-        for (int i = e; i < a.V; ++i) sum += left_of(mass(pr[i]), mass(qr[i]), off);
+        gone = had_token(l, node, c);
+        ok = !gone && u * S < px;
       }
+      if (ok) {
+        node = c, S = 1.0;
+        left = {P + (s0 + node) * a.p_row, nullptr, 0.0, node, 0};
+        if (writes) a.path[s0 + kept] = c;
+        ++kept;
+      }
+      c = next_child(l, n, node, c);
+      if (ok) continue;
+      if (Q) {
+        left.q = Q + (s0 + node) * a.q_row;
+        left.off += S;
+        break;  // for S, what is left of the mass
+      }
+      left.node = node, left.n = n;
+      if (!gone) S -= px;
     }
-    sum = wave_sum(sum);
-    __syncthreads();
-    if ((tid & 63) == 0) l.red[wv] = sum;
-    __syncthreads();
-    S = 0.0;
-    for (int w = 0; w < kVerifyPick / 64; ++w) S += l.red[w];
-  }
-  if (tid == 0) {
-    a.kept[b] = kept;
-    a.ends[b] = {off, s0 + node, node};
-  }
-}
-
-// Bits of the tokens of a segment that the walk's rejected children took away.
-__device__ __forceinline__ void taken_bits(const VerifyArgs& a, int b, int node, int64_t e0, uint32_t* bits,
-                                           int threads) {
-  for (int i = threadIdx.x; i < kVerifySegment / 32; i += threads) bits[i] = 0;
-  __syncthreads();
-  int s0;
-  const int n = min(verify_rows(a, b, &s0), kVerifyRows);
-  for (int i = node + 1 + threadIdx.x; i < n; i += threads) {
-    const int up = a.parents ? draft_parent(a.parents[s0 + i], i) : i - 1;
-    const int64_t x = a.tokens[s0 + i] - e0;
-    if (up == node && x >= 0 && x < kVerifySegment && x + e0 < a.V) atomicOr(&bits[x >> 5], 1u << (x & 31));
-  }
-  __syncthreads();
-}
-
-// T and p of the 8 elements from e on; `at` the first one's place in the segment
-template <typename T>
-__device__ __forceinline__ void load_left(const T* pr, const T* qr, int64_t e, int64_t V, double off,
-                                          const uint32_t* bits, int at, double* t, float* p) {
-  float q[8];
-  if (e + 8 <= V) {
-    const Elements<T, 8> x = *(const Elements<T, 8>*)(pr + e);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) p[i] = mass(x.v[i]);
-    if (qr) {
-      const Elements<T, 8> y = *(const Elements<T, 8>*)(qr + e);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) q[i] = mass(y.v[i]);
+    const bool ended = c < 0;
+    total = row_sum(left, l, a.V, ended ? part : 0, ended ? a.parts : 1);
+    if (!ended) {
+      S = total;
+      continue;
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      p[i] = e + i < V ? mass(pr[e + i]) : 0.f;
-      if (qr) q[i] = e + i < V ? mass(qr[e + i]) : 0.f;
-    }
+    if (a.parts > 1 || total > 0.0 || !(left.q || left.n)) break;
+    left.q = nullptr, left.n = 0;  // nothing left: from p itself
   }
-  if (qr) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) t[i] = left_of(p[i], q[i], off);
-  } else {
-    const uint32_t gone = bits[at >> 5] >> (at & 31);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) t[i] = (gone >> i) & 1 ? 0.0 : (double)p[i];
+  if (writes) a.kept[b] = kept;
+  if (a.parts > 1) {
+    if (tid < kVerifyWaves) a.sums[((int64_t)b * a.parts + part) * kVerifyWaves + tid] = l.sums[tid];
+    if (writes) a.ends[b] = {left.off, s0 + node, node, left.n, 0};
+    return;
   }
+  const int64_t token = find_element(left, l, a.V, kVerifyWaves, draw);
+  if (writes) a.next[b] = token;
 }
 
-// Sums of T and p over a segment (blockIdx.x) of a request's last row.
+// The next token of a request whose parts' sums are there.
 template <typename T>
-__global__ __launch_bounds__(kVerifySum) void verify_sum_kernel(VerifyArgs a) {
-  __shared__ uint32_t bits[kVerifySegment / 32];
-  __shared__ double red[2][kVerifySum / 64];
-  const int b = blockIdx.y, tid = threadIdx.x;
-  const VerifyEnd end = a.ends[b];
-  if (end.row < 0) return;
-  const int64_t e0 = (int64_t)blockIdx.x * kVerifySegment;
-  const T* pr = (const T*)a.p + end.row * a.p_row;
-  const T* qr = a.q ? (const T*)a.q + end.row * a.q_row : nullptr;
-  if (!qr) taken_bits(a, b, end.node, e0, bits, kVerifySum);
-  double st = 0.0, sp = 0.0;
-#pragma unroll
-  for (int r = 0; r < kVerifySegment / (kVerifySum * 8); ++r) {
-    const int at = (r * kVerifySum + tid) * 8;
-    if (e0 + at >= a.V) break;
-    double t[8];
-    float p[8];
-    load_left(pr, qr, e0 + at, (int64_t)a.V, end.off, bits, at, t, p);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) st += t[i], sp += (double)p[i];
-  }
-  st = wave_sum(st), sp = wave_sum(sp);
-  if ((tid & 63) == 0) red[0][tid >> 6] = st, red[1][tid >> 6] = sp;
-  __syncthreads();
-  if (tid < 2) {
-    double s = 0.0;
-    for (int w = 0; w < kVerifySum / 64; ++w) s += red[tid][w];
-    a.sums[((int64_t)b * a.segments + blockIdx.x) * 2 + tid] = s;
-  }
-}
-
-// The thread whose share of a cumulative sum first passes t: every thread
-// comes with its share `mine` and gets the sum before it.  Returns that thread,
-// or where rounding leaves none the last one with a share, -1 without any.
-// red: kVerifyPick / 64 doubles, found: an int
-__device__ __forceinline__ int find_share(double mine, double t, double* red, int* found, double* before) {
-  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-  double inc = mine;
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
-    const double x = __shfl_up(inc, m);
-    if (lane >= m) inc += x;
-  }
-  __syncthreads();
-  if (tid == 0) *found = 0x7fffffff;
-  if (lane == 63) red[wv] = inc;
-  __syncthreads();
-  double base = 0.0;
-  for (int w = 0; w < wv; ++w) base += red[w];
-  // the sum before a thread is the sum up to the one in front of it, to the bit
-  const double up = __shfl_up(inc, 1);
-  *before = lane ? base + up : base;
-  const bool pass = mine > 0.0 && base + inc > t;
-  uint64_t hit = __ballot(pass);
-  if (hit && lane == 0) atomicMin(found, wv * 64 + __builtin_ctzll(hit));
-  __syncthreads();
-  int at = *found;
-  if (at == 0x7fffffff) {
-    __syncthreads();
-    if (tid == 0) *found = -1;
-    __syncthreads();
-    hit = __ballot(mine > 0.0);
-    if (hit && lane == 0) atomicMax(found, wv * 64 + 63 - __builtin_clzll(hit));
-    __syncthreads();
-    at = *found;
-  }
-  return at;
-}
-
-// A block a request: the segment whose sum passes the draw, then the token.
-template <typename T>
-__global__ __launch_bounds__(kVerifyPick) void verify_pick_kernel(VerifyArgs a) {
-  __shared__ uint32_t bits[kVerifySegment / 32];
-  __shared__ double red[kVerifyPick / 64], pass_s;
-  __shared__ int found, seg_s;
-  __shared__ double total_s[2];
+__global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(VerifyArgs a) {
+  __shared__ VerifyLds l;
   const int b = blockIdx.x, tid = threadIdx.x;
   const VerifyEnd end = a.ends[b];
-  if (end.row < 0) {
-    if (tid == 0) a.next[b] = -1;
-    return;
-  }
-  const double* sums = a.sums + (int64_t)b * a.segments * 2;
-  const int per = (a.segments + kVerifyPick - 1) / kVerifyPick;
-  const int g0 = min(tid * per, a.segments), g1 = min(g0 + per, a.segments);
-  double mine[2] = {0.0, 0.0};
-  for (int g = g0; g < g1; ++g) mine[0] += sums[2 * g], mine[1] += sums[2 * g + 1];
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const double s = wave_sum(mine[k]);
-    __syncthreads();
-    if ((tid & 63) == 0) red[tid >> 6] = s;
-    __syncthreads();
-    if (tid == 0) {
-      double all = 0.0;
-      for (int w = 0; w < kVerifyPick / 64; ++w) all += red[w];
-      total_s[k] = all;
-    }
-  }
+  if (end.row < 0) return;
+  const float draw = a.draws[b];
+  const T *P = (const T*)a.p, *Q = (const T*)a.q;
+  Left<T> left = {P + end.row * a.p_row, Q && end.off > 0.0 ? Q + end.row * a.q_row : nullptr, end.off, end.node,
+                  end.n};
+  int ranges = a.parts * kVerifyWaves;
+  if (tid < ranges) l.sums[tid] = a.sums[(int64_t)b * ranges + tid];
+  for (int i = tid; i < left.n; i += kVerifyThreads) load_row(a, l, end.row - end.node, i);
   __syncthreads();
-  // no mass left: from p itself, and without any of that no token
-  const int k = total_s[0] > 0.0 ? 0 : 1;
-  const double total = total_s[k];
-  const float d = a.draws[b];
-  const double t = (d > 0.f ? (double)d : 0.0) * total;
-  double before;
-  int at = find_share(mine[k], t, red, &found, &before);
-  if (at < 0) {
-    if (tid == 0) a.next[b] = -1;
-    return;
+  const int lane = tid & 63;
+  if (!(wave_sum(lane < ranges ? l.sums[lane] : 0.0) > 0.0)) {  // nothing left: from p itself
+    left.q = nullptr, left.n = 0, ranges = kVerifyWaves;
+    row_sum(left, l, a.V, 0, 1);
   }
-  if (tid == at) {
-    int last = -1, g = g0;
-    double sum = before, had = before;
-    for (; g < g1; ++g) {
-      const double s = sums[2 * g + k];
-      if (s > 0.0) {
-        last = g, had = sum;
-        sum += s;
-        if (sum > t) break;
-      }
-    }
-    seg_s = last, pass_s = had;
-  }
-  __syncthreads();
-  const int64_t e0 = (int64_t)seg_s * kVerifySegment;
-  const double rest = t - pass_s;
-  const bool plain = k == 1;
-  const T* pr = (const T*)a.p + end.row * a.p_row;
-  const T* qr = a.q ? (const T*)a.q + end.row * a.q_row : nullptr;
-  if (!qr) taken_bits(a, b, end.node, e0, bits, kVerifyPick);
-  double tt[8];
-  float p[8];
-  const int first = tid * 8;
-  if (e0 + first < a.V) {
-    load_left(pr, qr, e0 + first, (int64_t)a.V, end.off, bits, first, tt, p);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) tt[i] = 0.0, p[i] = 0.f;
-  }
-  double share = 0.0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    if (plain) tt[i] = (double)p[i];
-    share += tt[i];
-  }
-  at = find_share(share, rest, red, &found, &before);
-  if (tid == at) {
-    double sum = before;
-    int last = 0;
-    bool done = false;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (!done && tt[i] > 0.0) {
-        last = i;
-        sum += tt[i];
-        done = sum > rest;
-      }
-    }
-    a.next[b] = e0 + first + last;
-  }
+  const int64_t token = find_element(left, l, a.V, ranges, draw);
+  if (tid == 0) a.next[b] = token;
 }
 
-template <typename T>
-static int verify_launch(const VerifyArgs& a, hipStream_t s) {
-  hipLaunchKernelGGL((verify_walk_kernel<T>), dim3(a.B), dim3(kVerifyPick), 0, s, a);
-  hipLaunchKernelGGL((verify_sum_kernel<T>), dim3(a.segments, a.B), dim3(kVerifySum), 0, s, a);
-  hipLaunchKernelGGL((verify_pick_kernel<T>), dim3(a.B), dim3(kVerifyPick), 0, s, a);
-  const hipError_t e = hipGetLastError();
-  return e == hipSuccess ? HTREE_OK : (int)e;
+// Blocks that share a request's sums: as many as have a CU to themselves.
+static int verify_parts(int32_t B, int32_t V, bool drawn) {
+  const int64_t all = (int64_t)V * (drawn ? 2 : 1);
+  if (all < kVerifySplit || 2 * B > kVerifyFull) return 1;
+  int64_t parts = kVerifyFull / B;
+  if (parts > kVerifyParts) parts = kVerifyParts;
+  return (int)(all / kVerifyPart < parts ? all / kVerifyPart : parts);
 }
-
-static int verify_segments(int32_t V) { return (int)(((int64_t)V + kVerifySegment - 1) / kVerifySegment); }
 
 }  // namespace htree
 
 using namespace htree;
 
-extern "C" int htree_verify_drafts_workspace_bytes(int32_t B, int32_t V, int64_t* bytes) {
+extern "C" int htree_verify_drafts_workspace_bytes(int32_t B, int32_t V, int32_t drawn, int64_t* bytes) {
   if (!bytes) return HTREE_ENULL;
   if (B < 0 || V < 1) return HTREE_ESHAPE;
   if (B > kCacheMaxRequests) return HTREE_EUNSUPPORTED;
-  *bytes = (int64_t)B * ((int64_t)sizeof(VerifyEnd) + verify_segments(V) * 16ll);
+  const int parts = B ? verify_parts(B, V, drawn) : 1;
+  *bytes = parts > 1 ? B * ((int64_t)sizeof(VerifyEnd) + parts * kVerifyWaves * 8) : 0;
   return HTREE_OK;
 }
 
@@ -421,14 +521,15 @@ extern "C" int htree_verify_drafts(int32_t dtype, int32_t B, int32_t rows, int32
                                    const int64_t* tokens, const int32_t* starts, const int32_t* parents,
                                    const float* uniforms, const float* draws, int32_t* kept, int32_t* path,
                                    int64_t* next_tokens, void* workspace, int64_t workspace_bytes, void* stream) {
-  int64_t need = 0;
-  const int rc = htree_verify_drafts_workspace_bytes(B, V, &need);
-  if (rc) return rc;
   if (dtype != HTREE_F32 && dtype != HTREE_BF16 && dtype != HTREE_F16) return HTREE_ESHAPE;
   if (rows < 0 || target_row < 0 || draft_row < 0) return HTREE_ESHAPE;
+  int64_t need = 0;
+  const int rc = htree_verify_drafts_workspace_bytes(B, V, draft_probs != nullptr, &need);
+  if (rc) return rc;
   if (B == 0) return HTREE_OK;
-  if (!starts || !draws || !kept || !next_tokens || !workspace) return HTREE_ENULL;
+  if (!starts || !draws || !kept || !next_tokens) return HTREE_ENULL;
   if (rows && (!target_probs || !tokens || !uniforms || !path)) return HTREE_ENULL;
+  if (need && !workspace) return HTREE_ENULL;
   if (off16(workspace)) return HTREE_EUNSUPPORTED;
   if (workspace_bytes < need) return HTREE_EWORKSPACE;
   const int es = dtype == HTREE_F32 ? 4 : 2;
@@ -447,12 +548,21 @@ extern "C" int htree_verify_drafts(int32_t dtype, int32_t B, int32_t rows, int32
   a.p = (const char*)target_probs, a.q = (const char*)draft_probs;
   a.tokens = tokens, a.starts = starts, a.parents = parents, a.uniforms = uniforms, a.draws = draws;
   a.kept = kept, a.path = path, a.next = next_tokens;
+  a.p_row = target_row, a.q_row = draft_row;
+  a.B = B, a.rows = rows, a.V = V;
+  a.parts = verify_parts(B, V, draft_probs != nullptr);
   a.ends = (VerifyEnd*)workspace;
   a.sums = (double*)(a.ends + B);
-  a.p_row = target_row, a.q_row = draft_row;
-  a.B = B, a.rows = rows, a.V = V, a.segments = verify_segments(V);
   hipStream_t s = (hipStream_t)stream;
-  if (dtype == HTREE_F32) return verify_launch<float>(a, s);
-  if (dtype == HTREE_BF16) return verify_launch<__bf16>(a, s);
-  return verify_launch<_Float16>(a, s);
+#define HTREE_VERIFY(T)                                                                                     \
+  do {                                                                                                      \
+    hipLaunchKernelGGL((verify_drafts_kernel<T>), dim3(B, a.parts), dim3(kVerifyThreads), 0, s, a);         \
+    if (a.parts > 1) hipLaunchKernelGGL((verify_draw_kernel<T>), dim3(B), dim3(kVerifyThreads), 0, s, a);   \
+  } while (0)
+  if (dtype == HTREE_F32) HTREE_VERIFY(float);
+  else if (dtype == HTREE_BF16) HTREE_VERIFY(__bf16);
+  else HTREE_VERIFY(_Float16);
+#undef HTREE_VERIFY
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? HTREE_OK : (int)e;
 }

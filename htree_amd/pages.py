@@ -191,9 +191,9 @@ def fork_requests(block_table: torch.Tensor, lens: torch.Tensor, source: torch.T
 
 
 @lru_cache(maxsize=64)
-def _unused_workspace_bytes(num_pages: int) -> int:
+def _unused_workspace_bytes(B: int, num_pages: int, width: int, held: int) -> int:
     n = ctypes.c_int64()
-    N.check(N.lib().htree_unused_pages_workspace_bytes(num_pages, n), "htree_unused_pages_workspace_bytes")
+    N.check(N.lib().htree_unused_pages_workspace_bytes(B, num_pages, width, held, n), "htree_unused_pages_workspace_bytes")
     return n.value
 
 
@@ -230,11 +230,11 @@ def unused_pages(block_table: torch.Tensor, lens: torch.Tensor, page_size: int, 
     if num_pages == 0:
         out.count.zero_()
         return out
-    nbytes = _unused_workspace_bytes(num_pages)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    rc = N.launch(N.lib().htree_unused_pages, dev, B, page_size, num_pages, block_table.shape[1],
-                  block_table.stride(0), block_table.data_ptr(), lens.data_ptr(), M, N.address(held),
-                  out.pages.data_ptr(), out.count.data_ptr(), ws.data_ptr(), nbytes)
+    width = block_table.shape[1]
+    nbytes = _unused_workspace_bytes(B, num_pages, width, M)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    rc = N.launch(N.lib().htree_unused_pages, dev, B, page_size, num_pages, width, block_table.stride(0), block_table.data_ptr(), lens.data_ptr(), M, N.address(held),
+                  out.pages.data_ptr(), out.count.data_ptr(), N.address(ws), nbytes)
     if rc:
         assert rc != N.HTREE_EOVERLAP, "out must not overlap the inputs, nor its parts each other"
         N.check(rc, "htree_unused_pages")

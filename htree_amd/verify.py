@@ -24,9 +24,9 @@ class Verified(NamedTuple):
 
 
 @lru_cache(maxsize=256)
-def _workspace_bytes(B: int, V: int) -> int:
+def _workspace_bytes(B: int, V: int, drawn: bool) -> int:
     n = ctypes.c_int64()
-    N.check(N.lib().htree_verify_drafts_workspace_bytes(B, V, n), "htree_verify_drafts_workspace_bytes")
+    N.check(N.lib().htree_verify_drafts_workspace_bytes(B, V, drawn, n), "htree_verify_drafts_workspace_bytes")
     return n.value
 
 
@@ -108,12 +108,12 @@ def verify_drafts(target_probs: torch.Tensor, tokens: torch.Tensor, starts: torc
     if B == 0:
         out.path.fill_(-1)
         return out
-    nbytes = _workspace_bytes(B, V)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    nbytes = _workspace_bytes(B, V, draft_probs is not None)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     rc = N.launch(N.lib().htree_verify_drafts, dev, N.DTYPE_CODE[dtype], B, rows, V, target_probs.data_ptr(),
                   target_probs.stride(0), N.address(draft_probs), 0 if draft_probs is None else draft_probs.stride(0),
                   tokens.data_ptr(), starts.data_ptr(), N.address(parents), uniforms.data_ptr(), draws.data_ptr(),
-                  out.kept.data_ptr(), out.path.data_ptr(), out.next_tokens.data_ptr(), ws.data_ptr(), nbytes)
+                  out.kept.data_ptr(), out.path.data_ptr(), out.next_tokens.data_ptr(), N.address(ws), nbytes)
     if rc:
         assert rc != N.HTREE_EOVERLAP, "out must not overlap the inputs, nor its parts each other"
         N.check(rc, "htree_verify_drafts")

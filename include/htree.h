@@ -406,8 +406,9 @@ int htree_draft_attention(const htree_cache* c, int32_t B, int32_t rows, int32_t
  *   path        [rows] from starts[b] on the kept rows' indices within their
  *               request, ascending; -1 elsewhere
  *   next_tokens [B]; -1 without rows or without any mass
- * The first 1024 rows of a request are looked at. */
-int htree_verify_drafts_workspace_bytes(int32_t B, int32_t V, int64_t* bytes);
+ * The first 1024 rows of a request are looked at.  Few requests over a large
+ * vocabulary need a workspace (drawn: with draft_probs). */
+int htree_verify_drafts_workspace_bytes(int32_t B, int32_t V, int32_t drawn, int64_t* bytes);
 int htree_verify_drafts(int32_t dtype, int32_t B, int32_t rows, int32_t V, const void* target_probs,
                         int64_t target_row, const void* draft_probs, int64_t draft_row,
                         const int64_t* tokens, const int32_t* starts, const int32_t* parents,
@@ -454,7 +455,8 @@ int htree_copy_pages(const htree_cache* c, int32_t layers, void* const* k_layers
 /* The pages of 0 .. num_pages - 1 that are in no live entry of the table
  * (entries 0 .. ceil(lens[b] / page_size) - 1) and not among held [n_held]:
  * pages [num_pages], ascending, -1 behind them, and count [1]. */
-int htree_unused_pages_workspace_bytes(int32_t num_pages, int64_t* bytes);
+int htree_unused_pages_workspace_bytes(int32_t B, int32_t num_pages, int32_t table_width,
+                                       int32_t n_held, int64_t* bytes);
 int htree_unused_pages(int32_t B, int32_t page_size, int32_t num_pages, int32_t table_width,
                        int64_t table_stride, const int32_t* block_table, const int32_t* lens,
                        int32_t n_held, const int32_t* held, int32_t* pages, int32_t* count,

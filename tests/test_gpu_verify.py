@@ -115,7 +115,8 @@ def case(new, V, dtype, tree, drawn, seed, sharp=4.0, grid=None):
 @pytest.mark.parametrize("new,V,dtype", [
     ([6], 32000, "float32"), ([1, 2, 3], 1, "float32"), ([24] * 5, 7, "bfloat16"), ([2, 9, 1, 30], 8192, "float16"),
     ([5, 5], 8193, "float32"), ([64], 16385, "bfloat16"), ([65, 3], 777, "float32"), ([3] * 70, 301, "bfloat16"),
-    ([0, 4, 0, 5, 0], 1001, "float32"), ([200, 1], 50, "float16"), ([7, 8], 150001, "bfloat16")])
+    ([0, 4, 0, 5, 0], 1001, "float32"), ([200, 1], 50, "float16"), ([7, 8], 150001, "bfloat16"),
+    ([6], 300007, "float32"), ([5, 0, 12, 1], 131072, "float16")])
 def test_matches_the_walk(new, V, dtype, tree, drawn):
     kept = [check(*case(new, V, dtype, tree, drawn, seed))[0].sum() for seed in range(3)]
     assert max(kept) > 0

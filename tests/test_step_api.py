@@ -19,7 +19,7 @@ def size(f, *args):
 
 
 def verify(dtype=0, B=2, rows=6, V=100, p=at(1), p_row=100, q=None, q_row=0, tokens=at(2), starts=at(3), parents=None,
-           u=at(4), d=at(5), kept=at(6), path=at(7), nxt=at(8), ws=at(9), n=1 << 19):
+           u=at(4), d=at(5), kept=at(6), path=at(7), nxt=at(8), ws=None, n=0):
     return N.lib().htree_verify_drafts(dtype, B, rows, V, p, p_row, q, q_row, tokens, starts, parents, u, d, kept, path,
                                        nxt, ws, n, None)
 
@@ -31,22 +31,29 @@ def test_verify_refusals():
     assert verify(V=0) == N.HTREE_ESHAPE
     assert verify(p_row=-1) == N.HTREE_ESHAPE
     assert verify(B=4097) == N.HTREE_EUNSUPPORTED
-    for name in ("p", "tokens", "starts", "u", "d", "kept", "path", "nxt", "ws"):
+    for name in ("p", "tokens", "starts", "u", "d", "kept", "path", "nxt"):
         assert verify(**{name: None}) == N.HTREE_ENULL, name
-    assert verify(ws=ctypes.c_void_p((9 << 20) + 8)) == N.HTREE_EUNSUPPORTED
-    need = size("htree_verify_drafts_workspace_bytes", 2, 100)[1]
-    assert need > 0 and verify(n=need - 1) == N.HTREE_EWORKSPACE
-    for name in ("kept", "path", "nxt", "ws"):
+    for name in ("kept", "path", "nxt"):
         for x in range(1, 6):
             assert verify(**{name: at(x)}) == N.HTREE_EOVERLAP, (name, x)
         assert verify(q=at(20), q_row=100, **{name: at(20)}) == N.HTREE_EOVERLAP
         assert verify(parents=at(20), **{name: at(20)}) == N.HTREE_EOVERLAP
     assert verify(kept=at(7)) == N.HTREE_EOVERLAP and verify(path=at(8)) == N.HTREE_EOVERLAP
-    assert verify(ws=at(8)) == N.HTREE_EOVERLAP
     assert verify(B=0, p=None) == N.HTREE_OK
-    assert size("htree_verify_drafts_workspace_bytes", 4, 0)[0] == N.HTREE_ESHAPE
-    assert N.lib().htree_verify_drafts_workspace_bytes(1, 1, None) == N.HTREE_ENULL
-    assert size("htree_verify_drafts_workspace_bytes", 4096, 2 ** 31 - 1)[1] > 2 ** 33
+    # few requests over a large vocabulary need a workspace
+    need = lambda *a: size("htree_verify_drafts_workspace_bytes", *a)
+    assert need(2, 100, 1) == (N.HTREE_OK, 0) and need(129, 1 << 20, 1) == (N.HTREE_OK, 0)
+    rc, n = need(2, 1 << 17, 0)
+    assert rc == N.HTREE_OK and 0 < n < 4096 and need(2, 1 << 16, 1) == (N.HTREE_OK, n)
+    big = dict(V=1 << 17, p=at(4000), p_row=1 << 17, n=n)
+    assert verify(**big) == N.HTREE_ENULL
+    assert verify(**dict(big, n=n - 1), ws=at(9)) == N.HTREE_EWORKSPACE
+    assert verify(**big, ws=ctypes.c_void_p((9 << 20) + 8)) == N.HTREE_EUNSUPPORTED
+    for x in (2, 3, 4, 5, 6, 7, 8, 4000):
+        assert verify(**big, ws=at(x)) == N.HTREE_EOVERLAP
+    assert need(4, 0, 0)[0] == N.HTREE_ESHAPE and need(-1, 5, 0)[0] == N.HTREE_ESHAPE
+    assert need(4097, 5, 0)[0] == N.HTREE_EUNSUPPORTED
+    assert N.lib().htree_verify_drafts_workspace_bytes(1, 1, 0, None) == N.HTREE_ENULL
 
 
 def pointers(n, first=4096):
@@ -117,16 +124,26 @@ def test_unused_refusals():
         assert unused(**kw) == N.HTREE_ESHAPE, kw
     for kw in (dict(page=0), dict(page=24), dict(B=4097), dict(ws=ctypes.c_void_p((6 << 20) + 4))):
         assert unused(**kw) == N.HTREE_EUNSUPPORTED, kw
-    for name in ("table", "lens", "held", "out", "count", "ws"):
+    for name in ("table", "lens", "held", "out", "count"):
         assert unused(**{name: None}) == N.HTREE_ENULL, name
-    assert unused(n=size("htree_unused_pages_workspace_bytes", 9)[1] - 1) == N.HTREE_EWORKSPACE
-    for name in ("out", "count", "ws"):
+    # small calls need no workspace
+    need = lambda *a: size("htree_unused_pages_workspace_bytes", *a)
+    assert need(64, 1 << 18, 1024, 1 << 16) == (N.HTREE_OK, 0)
+    for many in ((64, (1 << 18) + 1, 1024, 0), (65, 100, 1024, 0), (257, 100, 1, 0), (1, 100, 1, (1 << 16) + 1)):
+        rc, n = need(*many)
+        assert rc == N.HTREE_OK and n > 0
+        big = dict(B=many[0], pages=many[1], width=many[2], stride=many[2], n_held=many[3], out=at(400), count=at(500))
+        assert unused(ws=at(600), n=n - 1, **big) == N.HTREE_EWORKSPACE
+        assert unused(ws=None, n=n, **big) == N.HTREE_ENULL
+        assert unused(ws=at(1), n=n, **big) == N.HTREE_EOVERLAP and unused(ws=at(500), n=n, **big) == N.HTREE_EOVERLAP
+    for name in ("out", "count"):
         for x in (1, 2, 3):
             assert unused(**{name: at(x)}) == N.HTREE_EOVERLAP
-    assert unused(out=at(5)) == N.HTREE_EOVERLAP and unused(ws=at(4)) == N.HTREE_EOVERLAP
+    assert unused(out=at(5)) == N.HTREE_EOVERLAP
     assert unused(pages=0, table=None) == N.HTREE_OK
-    assert size("htree_unused_pages_workspace_bytes", -1)[0] == N.HTREE_ESHAPE
-    assert size("htree_unused_pages_workspace_bytes", 2 ** 31 - 1)[1] > 2 ** 31
+    assert need(1, -1, 1, 1)[0] == N.HTREE_ESHAPE
+    assert need(1, 2 ** 31 - 1, 1, 1)[1] > 2 ** 31
+    assert N.lib().htree_unused_pages_workspace_bytes(1, 1, 1, 1, None) == N.HTREE_ENULL
 
 
 def norm(dtype=1, w=0, rows=4, H=8, Hkv=2, D=64, eps=1e-6, q=FAKE, qr=512, k=FAKE, pos=None, cos=None, sin=None, rope=0,
