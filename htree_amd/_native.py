@@ -227,7 +227,7 @@ def address(t):
 def launch(fn, dev, *args) -> int:
     """fn(*args, stream) on dev's current stream, with dev the current device."""
     index = dev.index
-    if torch.cuda.current_device() == index:  # the context manager costs as much as a call
+    if torch._C._cuda_getDevice() == index:  # the context manager costs as much as a call
         return fn(*args, torch._C._cuda_getCurrentRawStream(index))
     with torch.cuda.device(index):
         return fn(*args, torch._C._cuda_getCurrentRawStream(index))

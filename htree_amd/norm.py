@@ -26,22 +26,25 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
     return aligned_rows(x if x.dim() == 3 else x.reshape(-1, *x.shape[-2:]))
 
 
-def _sizes(q: torch.Tensor, weight: Optional[torch.Tensor]):
+def _codes(q: torch.Tensor, q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor]):
+    """The inputs' type and the weights'."""
+    w = k_weight if q_weight is None else q_weight
     code = N.DTYPE_CODE[q.dtype]
-    return code, code if weight is None else N.DTYPE_CODE[weight.dtype]
+    return code, code if w is None else N.DTYPE_CODE[w.dtype]
 
 
 def _forward(q, k, q_weight, k_weight, eps, positions, cos, sin):
-    dev, dtype, D = q.device, q.dtype, q.shape[-1]
-    q_out, k_out = (torch.empty(x.shape, dtype=dtype, device=dev) for x in (q, k))
+    dev, dtype, shape = q.device, q.dtype, q.shape
+    q_out = torch.empty(shape, dtype=dtype, device=dev)
+    k_out = torch.empty(k.shape, dtype=dtype, device=dev)
     q3, k3 = _rows(q), _rows(k)
-    rows = q3.shape[0]
+    rows, H, D = q3.shape
     if rows:
-        rc = N.launch(N.lib().htree_head_norm, dev, *_sizes(q, k_weight if q_weight is None else q_weight), rows,
-                      q3.shape[1], k3.shape[1], D, eps, q3.data_ptr(), q3.stride(0), q3.stride(1), k3.data_ptr(),
-                      k3.stride(0), k3.stride(1), N.address(q_weight), N.address(k_weight), N.address(positions),
-                      N.address(cos), N.address(sin), 0 if cos is None else cos.shape[0], q_out.data_ptr(),
-                      k_out.data_ptr())
+        (qr, qh, _), (kr, kh, _) = q3.stride(), k3.stride()
+        rc = N.launch(N.lib().htree_head_norm, dev, *_codes(q, q_weight, k_weight), rows, H, k3.shape[1], D, eps,
+                      q3.data_ptr(), qr, qh, k3.data_ptr(), kr, kh, N.address(q_weight), N.address(k_weight),
+                      N.address(positions), N.address(cos), N.address(sin), 0 if cos is None else cos.shape[0],
+                      q_out.data_ptr(), k_out.data_ptr())
         if rc:
             N.check(rc, "htree_head_norm")
     return q_out, k_out
@@ -81,7 +84,7 @@ class _HeadNorm(torch.autograd.Function):
             nbytes = _workspace_bytes(D) if dqw is not None or dkw is not None else 0
             ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
             (qr, qh, *_), (yr, yh, *_), (kr, kh, *_), (zr, zh, *_) = strides
-            rc = N.launch(N.lib().htree_head_norm_backward, dev, *_sizes(q, k_weight if q_weight is None else q_weight),
+            rc = N.launch(N.lib().htree_head_norm_backward, dev, *_codes(q, q_weight, k_weight),
                           rows, H[0], H[1], D, ctx.eps, N.address(q3), qr, qh, N.address(k3), kr, kh, N.address(dq3),
                           yr, yh, N.address(dk3), zr, zh, N.address(q_weight), N.address(k_weight),
                           N.address(positions), N.address(cos), N.address(sin), 0 if cos is None else cos.shape[0],
@@ -89,6 +92,11 @@ class _HeadNorm(torch.autograd.Function):
             if rc:
                 N.check(rc, "htree_head_norm_backward")
         return (*grads, None, None, None, None)
+
+
+def _check_weight(name: str, w: torch.Tensor, D: int, dtype, dev) -> None:
+    assert w.shape == (D,) and (w.dtype is torch.float32 or w.dtype is dtype) and w.is_contiguous() \
+        and w.device == dev, f"{name} must be a contiguous [{D}] tensor, float32 or {dtype}, on {dev}"
 
 
 def head_norm(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tensor] = None,
@@ -115,37 +123,37 @@ def head_norm(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tensor]
     output's gradient rotated back, times the weight; the weights' are summed
     over rows and heads in fp32, in a fixed order.  There is no second
     derivative and no forward mode; cos and sin have no gradient."""
-    dev, dtype = q.device, q.dtype
+    dev, dtype, shape, kshape = q.device, q.dtype, q.shape, k.shape
     assert dev.type == "cuda", "htree_amd runs on the GPU (no CPU fallback)"
     assert dtype in N.DTYPE_CODE, "q must be float32, bfloat16 or float16"
     assert k.dtype is dtype and k.device == dev, "q and k must share one dtype and device"
-    assert q.dim() >= 3 and q.dim() == k.dim() and q.shape[:-2] == k.shape[:-2] and q.shape[-1] == k.shape[-1], \
-        f"q and k must be [..., H, D] and [..., H_kv, D], got {list(q.shape)} and {list(k.shape)}"
-    D, lead = q.shape[-1], q.shape[:-2]
+    lead = shape[:-2]
+    assert len(shape) >= 3 and len(shape) == len(kshape) and lead == kshape[:-2] and shape[-1] == kshape[-1], \
+        f"q and k must be [..., H, D] and [..., H_kv, D], got {list(shape)} and {list(kshape)}"
+    H, D, H_kv = shape[-2], shape[-1], kshape[-2]
     assert 0 < D <= MAX_HEAD_DIM and D * dtype.itemsize % 16 == 0, \
         f"the head dim must be whole 16-byte pieces and at most {MAX_HEAD_DIM}, got {D}"
-    assert q.shape[-2] > 0 and k.shape[-2] > 0, "q and k need a head each"
-    rows = lead.numel()
-    assert rows * (q.shape[-2] + k.shape[-2]) < INT32, "rows times heads must be below 2^31"
-    eps = float(eps)
+    assert H > 0 and H_kv > 0, "q and k need a head each"
+    assert lead.numel() * (H + H_kv) < INT32, "rows times heads must be below 2^31"
     assert 0.0 <= eps < 3.4e38, f"eps must not be negative, nor infinite, got {eps}"
-    for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
-        assert w is None or (w.shape == (D,) and w.dtype in (torch.float32, dtype) and w.is_contiguous()
-                             and w.device == dev), f"{name} must be a contiguous [{D}] tensor, float32 or {dtype}, on {dev}"
-    assert q_weight is None or k_weight is None or q_weight.dtype is k_weight.dtype, \
-        "q_weight and k_weight must share one dtype"
+    if q_weight is not None:
+        _check_weight("q_weight", q_weight, D, dtype, dev)
+    if k_weight is not None:
+        _check_weight("k_weight", k_weight, D, dtype, dev)
+        assert q_weight is None or q_weight.dtype is k_weight.dtype, "q_weight and k_weight must share one dtype"
     assert (cos is None) == (sin is None) == (positions is None), "positions, cos and sin go together"
     if cos is not None:
-        n = cos.shape[0]
-        assert 0 < n < INT32 and cos.shape == (n, D // 2) and sin.shape == (n, D // 2) \
+        n, half = cos.shape[0], D // 2
+        assert 0 < n < INT32 and cos.shape == (n, half) and sin.shape == (n, half) \
             and cos.dtype is torch.float32 and sin.dtype is torch.float32 and cos.is_contiguous() \
             and sin.is_contiguous() and cos.device == dev and sin.device == dev, \
-            f"cos and sin must be contiguous fp32 tensors [n, {D // 2}] on {dev}"
+            f"cos and sin must be contiguous fp32 tensors [n, {half}] on {dev}"
         assert positions.dtype is torch.int32 and positions.shape == lead and positions.is_contiguous() \
             and positions.device == dev, f"positions must be a contiguous int32 tensor {list(lead)} on {dev}"
-        if torch.is_grad_enabled():
-            assert not cos.requires_grad and not sin.requires_grad, "cos and sin have no gradient"
     no_tangents("head_norm", q, k, q_weight, k_weight, cos, sin)
-    if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, q_weight, k_weight)):
-        return _HeadNorm.apply(q, k, q_weight, k_weight, eps, positions, cos, sin)
-    return _forward(q, k, q_weight, k_weight, eps, positions, cos, sin)
+    if torch.is_grad_enabled():
+        assert cos is None or not (cos.requires_grad or sin.requires_grad), "cos and sin have no gradient"
+        if q.requires_grad or k.requires_grad or (q_weight is not None and q_weight.requires_grad) \
+                or (k_weight is not None and k_weight.requires_grad):
+            return _HeadNorm.apply(q, k, q_weight, k_weight, float(eps), positions, cos, sin)
+    return _forward(q, k, q_weight, k_weight, float(eps), positions, cos, sin)

@@ -9,6 +9,7 @@ in one launch.  Nothing here synchronises."""
 from __future__ import annotations
 
 import ctypes
+from array import array
 from functools import lru_cache
 from typing import NamedTuple, Optional, Sequence, Union
 
@@ -38,16 +39,17 @@ class UnusedPages(NamedTuple):
 
 
 def _bases(caches: Caches, name: str):
-    """A layer's shape and stride, its tensor's type and device, and the
+    """A layer's shape and stride, a tensor of its type and device, and the
     address of each layer."""
     if isinstance(caches, torch.Tensor):
-        if caches.dim() == 4:
-            return caches.shape, caches.stride(), caches, (caches.data_ptr(),)
-        assert caches.dim() == 5, f"{name} must be [pages, page_size, H_kv, D] or [layers, pages, page_size, H_kv, D]"
-        layers, base, step = caches.shape[0], caches.data_ptr(), caches.stride(0) * caches.element_size()
+        shape, stride, at = caches.shape, caches.stride(), caches.data_ptr()
+        if len(shape) == 4:
+            return shape, stride, caches, (at,)
+        assert len(shape) == 5, f"{name} must be [pages, page_size, H_kv, D] or [layers, pages, page_size, H_kv, D]"
+        layers, step = shape[0], stride[0] * caches.element_size()
         assert 0 < layers <= MAX_LAYERS, f"{name} must have 1 to {MAX_LAYERS} layers"
         assert layers == 1 or step > 0, f"{name} must not be expanded"
-        return caches.shape[1:], caches.stride()[1:], caches, [base + i * step for i in range(layers)]
+        return shape[1:], stride[1:], caches, range(at, at + layers * step, step) if step else (at,)
     caches = list(caches)
     assert 0 < len(caches) <= MAX_LAYERS, f"{name} must have 1 to {MAX_LAYERS} layers"
     first = caches[0]
@@ -58,25 +60,31 @@ def _bases(caches: Caches, name: str):
     return shape, stride, first, [c.data_ptr() for c in caches]
 
 
+@lru_cache(maxsize=256)
+def _layout(kshape, kstride, vshape, vstride, dtype) -> "N.HtreeCache":
+    """The description of layers that are written to."""
+    c = _describe(kshape, kstride, vshape, vstride, dtype)
+    for size, a, b in zip(kshape, kstride, vstride):
+        assert size == 1 or (a > 0 and b > 0), "k_caches and v_caches must not be expanded"
+    return c
+
+
 def _layers(name: str, k_caches: Caches, v_caches: Caches):
     """Checks the layers; their description and addresses for the C ABI."""
     ks, kt, k, k_at = _bases(k_caches, "k_caches")
     vs, vt, v, v_at = _bases(v_caches, "v_caches")
-    dev = k.device
+    dev, n = k.device, len(k_at)
     assert dev.type == "cuda", "htree_amd runs on the GPU (no CPU fallback)"
     assert v.dtype is k.dtype and v.device == dev, "k_caches and v_caches must share one dtype and device"
-    n = len(k_at)
     assert len(v_at) == n, f"k_caches and v_caches must have as many layers, got {n} and {len(v_at)}"
-    c = _describe(ks, kt, vs, vt, k.dtype)
-    for size, a, b in zip(ks, kt, vt):
-        assert size == 1 or (a > 0 and b > 0), "k_caches and v_caches must not be expanded"
+    c = _layout(ks, kt, vs, vt, k.dtype)
     assert len({*k_at, *v_at}) == 2 * n, "each layer's keys and values must be tensors of their own"
-    for x in (k_caches, v_caches):
-        no_derivatives(name, *((x,) if isinstance(x, torch.Tensor) else x))
-    kind = ctypes.c_void_p * n
-    k_ptr, v_ptr = kind(*k_at), kind(*v_at)
-    for a in (k_at, v_at):
-        assert not any(p & 15 for p in a), "the cache must begin at a 16-byte step"
+    if k is k_caches and v is v_caches:
+        no_derivatives(name, k, v)
+    else:
+        for x in (k_caches, v_caches):
+            no_derivatives(name, *((x,) if isinstance(x, torch.Tensor) else x))
+    k_ptr, v_ptr = array("Q", k_at), array("Q", v_at)
     return c, n, k_ptr, v_ptr, dev
 
 
@@ -103,7 +111,7 @@ def keep_drafts(k_caches: Caches, v_caches: Caches, slots: torch.Tensor, starts:
     _ints(starts, "starts", B + 1, dev)
     _ints(path, "path", rows, dev)
     _ints(kept, "kept", B, dev)
-    rc = N.launch(N.lib().htree_keep_drafts, dev, c, layers, k_ptr, v_ptr, B, rows, slots.data_ptr(),
+    rc = N.launch(N.lib().htree_keep_drafts, dev, c, layers, k_ptr.buffer_info()[0], v_ptr.buffer_info()[0], B, rows, slots.data_ptr(),
                   starts.data_ptr(), path.data_ptr(), kept.data_ptr())
     if rc:
         N.check(rc, "htree_keep_drafts")
@@ -124,8 +132,8 @@ def copy_pages(k_caches: Caches, v_caches: Caches, copy_from: torch.Tensor, copy
     _ints(copy_to, "copy_to", n, dev)
     if copy_tokens is not None:
         _ints(copy_tokens, "copy_tokens", n, dev)
-    rc = N.launch(N.lib().htree_copy_pages, dev, c, layers, k_ptr, v_ptr, n, copy_from.data_ptr(),
-                  copy_to.data_ptr(), N.address(copy_tokens))
+    rc = N.launch(N.lib().htree_copy_pages, dev, c, layers, k_ptr.buffer_info()[0], v_ptr.buffer_info()[0], n,
+                  copy_from.data_ptr(), copy_to.data_ptr(), N.address(copy_tokens))
     if rc:
         N.check(rc, "htree_copy_pages")
 
