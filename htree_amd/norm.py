@@ -34,8 +34,9 @@ def _codes(q: torch.Tensor, q_weight: Optional[torch.Tensor], k_weight: Optional
 
 
 def _forward(q, k, q_weight, k_weight, eps, positions, cos, sin):
-    dev, dtype, shape = q.device, q.dtype, q.shape
-    q_out = torch.empty(shape, dtype=dtype, device=dev)
+    """The outputs, and q and k as the kernels read them."""
+    dev, dtype = q.device, q.dtype
+    q_out = torch.empty(q.shape, dtype=dtype, device=dev)
     k_out = torch.empty(k.shape, dtype=dtype, device=dev)
     q3, k3 = _rows(q), _rows(k)
     rows, H, D = q3.shape
@@ -47,51 +48,52 @@ def _forward(q, k, q_weight, k_weight, eps, positions, cos, sin):
                       q_out.data_ptr(), k_out.data_ptr())
         if rc:
             N.check(rc, "htree_head_norm")
-    return q_out, k_out
+    return q_out, k_out, q3, k3
 
 
 class _HeadNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, q_weight, k_weight, eps, positions, cos, sin):
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(q, k, q_weight, k_weight, positions, cos, sin)
-        ctx.eps = eps
-        return _forward(q, k, q_weight, k_weight, eps, positions, cos, sin)
+        q_out, k_out, q3, k3 = _forward(q, k, q_weight, k_weight, eps, positions, cos, sin)
+        ctx.save_for_backward(q3, k3, q_weight, k_weight, positions, cos, sin)
+        ctx.eps, ctx.shapes, ctx.codes = eps, (q.shape, k.shape), _codes(q, q_weight, k_weight)
+        return q_out, k_out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dq_out, dk_out):
         q, k, q_weight, k_weight, positions, cos, sin = ctx.saved_tensors
-        dev, D = q.device, q.shape[-1]
-        grads, args, strides, H, ws = [None, None, None, None], [], [], [0, 0], None
-        for i, (x, dy, w) in enumerate(((q, dq_out, q_weight), (k, dk_out, k_weight))):
-            wanted = dy is not None and (ctx.needs_input_grad[i] or ctx.needs_input_grad[2 + i])
-            if not wanted:
-                args.append((None, None, None, None))
-                strides += [(0, 0), (0, 0)]
-                continue
-            dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
-            dw = torch.zeros_like(w) if ctx.needs_input_grad[2 + i] else None
-            x3, dy3 = _rows(x), _rows(dy)
-            H[i] = x.shape[-2]
-            args.append((x3, dy3, dx, dw))
-            strides += [x3.stride(), dy3.stride()]
-            grads[i] = dx if ctx.needs_input_grad[i] else None
-            grads[2 + i] = dw
-        (q3, dq3, dq, dqw), (k3, dk3, dk, dkw) = args
-        rows = q.shape[:-2].numel()
-        if rows and any(H):
-            nbytes = _workspace_bytes(D) if dqw is not None or dkw is not None else 0
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-            (qr, qh, *_), (yr, yh, *_), (kr, kh, *_), (zr, zh, *_) = strides
-            rc = N.launch(N.lib().htree_head_norm_backward, dev, *_codes(q, q_weight, k_weight),
-                          rows, H[0], H[1], D, ctx.eps, N.address(q3), qr, qh, N.address(k3), kr, kh, N.address(dq3),
-                          yr, yh, N.address(dk3), zr, zh, N.address(q_weight), N.address(k_weight),
-                          N.address(positions), N.address(cos), N.address(sin), 0 if cos is None else cos.shape[0],
-                          N.address(dq), N.address(dk), N.address(dqw), N.address(dkw), N.address(ws), nbytes)
+        needs, dev, dtype, (rows, H, D), H_kv = ctx.needs_input_grad, q.device, q.dtype, q.shape, k.shape[1]
+        dq = dk = dq_weight = dk_weight = ws = None
+        new = torch.empty if rows else torch.zeros
+        qr = qh = kr = kh = yr = yh = zr = zh = nbytes = 0
+        if dq_out is None or not (needs[0] or needs[2]):
+            q, dq_out, H = None, None, 0
+        else:
+            dq_out = _rows(dq_out)
+            dq = torch.empty(ctx.shapes[0], dtype=dtype, device=dev)
+            dq_weight = new(D, dtype=q_weight.dtype, device=dev) if needs[2] else None
+            (qr, qh, _), (yr, yh, _) = q.stride(), dq_out.stride()
+        if dk_out is None or not (needs[1] or needs[3]):
+            k, dk_out, H_kv = None, None, 0
+        else:
+            dk_out = _rows(dk_out)
+            dk = torch.empty(ctx.shapes[1], dtype=dtype, device=dev)
+            dk_weight = new(D, dtype=k_weight.dtype, device=dev) if needs[3] else None
+            (kr, kh, _), (zr, zh, _) = k.stride(), dk_out.stride()
+        if rows and (H or H_kv):
+            if dq_weight is not None or dk_weight is not None:
+                nbytes = _workspace_bytes(D)
+                ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            ptr = N.address
+            rc = N.launch(N.lib().htree_head_norm_backward, dev, *ctx.codes, rows, H, H_kv, D, ctx.eps, ptr(q), qr, qh,
+                          ptr(k), kr, kh, ptr(dq_out), yr, yh, ptr(dk_out), zr, zh, ptr(q_weight), ptr(k_weight),
+                          ptr(positions), ptr(cos), ptr(sin), 0 if cos is None else cos.shape[0], ptr(dq), ptr(dk),
+                          ptr(dq_weight), ptr(dk_weight), ptr(ws), nbytes)
             if rc:
                 N.check(rc, "htree_head_norm_backward")
-        return (*grads, None, None, None, None)
+        return (dq if needs[0] else None, dk if needs[1] else None, dq_weight, dk_weight, None, None, None, None)
 
 
 def _check_weight(name: str, w: torch.Tensor, D: int, dtype, dev) -> None:
@@ -156,4 +158,4 @@ def head_norm(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tensor]
         if q.requires_grad or k.requires_grad or (q_weight is not None and q_weight.requires_grad) \
                 or (k_weight is not None and k_weight.requires_grad):
             return _HeadNorm.apply(q, k, q_weight, k_weight, float(eps), positions, cos, sin)
-    return _forward(q, k, q_weight, k_weight, float(eps), positions, cos, sin)
+    return _forward(q, k, q_weight, k_weight, float(eps), positions, cos, sin)[:2]
