@@ -35,9 +35,9 @@ def _codes(q: torch.Tensor, q_weight: Optional[torch.Tensor], k_weight: Optional
 
 def _forward(q, k, q_weight, k_weight, eps, positions, cos, sin):
     """The outputs, and q and k as the kernels read them."""
-    dev, dtype = q.device, q.dtype
-    q_out = torch.empty(q.shape, dtype=dtype, device=dev)
-    k_out = torch.empty(k.shape, dtype=dtype, device=dev)
+    dev = q.device
+    q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
     q3, k3 = _rows(q), _rows(k)
     rows, H, D = q3.shape
     if rows:
@@ -64,23 +64,23 @@ class _HeadNorm(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dq_out, dk_out):
         q, k, q_weight, k_weight, positions, cos, sin = ctx.saved_tensors
-        needs, dev, dtype, (rows, H, D), H_kv = ctx.needs_input_grad, q.device, q.dtype, q.shape, k.shape[1]
+        needs, dev, (rows, H, D), H_kv = ctx.needs_input_grad, q.device, q.shape, k.shape[1]
         dq = dk = dq_weight = dk_weight = ws = None
-        new = torch.empty if rows else torch.zeros
+        new = torch.empty_like if rows else torch.zeros_like
         qr = qh = kr = kh = yr = yh = zr = zh = nbytes = 0
         if dq_out is None or not (needs[0] or needs[2]):
             q, dq_out, H = None, None, 0
         else:
             dq_out = _rows(dq_out)
-            dq = torch.empty(ctx.shapes[0], dtype=dtype, device=dev)
-            dq_weight = new(D, dtype=q_weight.dtype, device=dev) if needs[2] else None
+            dq = q.new_empty(ctx.shapes[0])
+            dq_weight = new(q_weight) if needs[2] else None
             (qr, qh, _), (yr, yh, _) = q.stride(), dq_out.stride()
         if dk_out is None or not (needs[1] or needs[3]):
             k, dk_out, H_kv = None, None, 0
         else:
             dk_out = _rows(dk_out)
-            dk = torch.empty(ctx.shapes[1], dtype=dtype, device=dev)
-            dk_weight = new(D, dtype=k_weight.dtype, device=dev) if needs[3] else None
+            dk = k.new_empty(ctx.shapes[1])
+            dk_weight = new(k_weight) if needs[3] else None
             (kr, kh, _), (zr, zh, _) = k.stride(), dk_out.stride()
         if rows and (H or H_kv):
             if dq_weight is not None or dk_weight is not None:

@@ -178,8 +178,8 @@ def fork_requests(block_table: torch.Tensor, lens: torch.Tensor, source: torch.T
     _sizes(page_size, num_pages, block_table)
     width = block_table.shape[1]
     if out is None:
-        ints = torch.empty(4 * n + 1, dtype=torch.int32, device=dev).split_with_sizes((n, n, n, n, 1))
-        out = Forked(torch.empty((n, width), dtype=torch.int32, device=dev), *ints)
+        out = Forked(block_table.new_empty((n, width)),
+                     *source.new_empty(4 * n + 1).split_with_sizes((n, n, n, n, 1)))
     else:
         check_table(out.block_table, n, dev)
         assert out.block_table.shape[1] == width, f"out.block_table must be [{n}, {width}]"
@@ -231,7 +231,7 @@ def unused_pages(block_table: torch.Tensor, lens: torch.Tensor, page_size: int, 
         M = held.shape[0]
         _ints(held, "held", M, dev)
     if out is None:
-        out = UnusedPages(*torch.empty(num_pages + 1, dtype=torch.int32, device=dev).split_with_sizes((num_pages, 1)))
+        out = UnusedPages(*lens.new_empty(num_pages + 1).split_with_sizes((num_pages, 1)))
     else:
         _ints(out.pages, "out.pages", num_pages, dev)
         _ints(out.count, "out.count", 1, dev)
@@ -240,7 +240,7 @@ def unused_pages(block_table: torch.Tensor, lens: torch.Tensor, page_size: int, 
         return out
     width = block_table.shape[1]
     nbytes = _unused_workspace_bytes(B, num_pages, width, M)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    ws = lens.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     rc = N.launch(N.lib().htree_unused_pages, dev, B, page_size, num_pages, width, block_table.stride(0), block_table.data_ptr(), lens.data_ptr(), M, N.address(held),
                   out.pages.data_ptr(), out.count.data_ptr(), N.address(ws), nbytes)
     if rc:

@@ -97,8 +97,8 @@ def verify_drafts(target_probs: torch.Tensor, tokens: torch.Tensor, starts: torc
     if parents is not None:
         _ints(parents, "parents", rows, dev)
     if out is None:
-        kept, path = torch.empty(B + rows, dtype=torch.int32, device=dev).split_with_sizes((B, rows))
-        out = Verified(kept, path, torch.empty(B, dtype=torch.int64, device=dev))
+        out = Verified(torch.empty_like(draws, dtype=torch.int32), torch.empty_like(uniforms, dtype=torch.int32),
+                       torch.empty_like(draws, dtype=torch.int64))
     else:
         _ints(out.kept, "out.kept", B, dev)
         _ints(out.path, "out.path", rows, dev)
@@ -109,7 +109,7 @@ def verify_drafts(target_probs: torch.Tensor, tokens: torch.Tensor, starts: torc
         out.path.fill_(-1)
         return out
     nbytes = _workspace_bytes(B, V, draft_probs is not None)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    ws = draws.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     rc = N.launch(N.lib().htree_verify_drafts, dev, N.DTYPE_CODE[dtype], B, rows, V, target_probs.data_ptr(),
                   target_probs.stride(0), N.address(draft_probs), 0 if draft_probs is None else draft_probs.stride(0),
                   tokens.data_ptr(), starts.data_ptr(), N.address(parents), uniforms.data_ptr(), draws.data_ptr(),
