@@ -126,7 +126,7 @@ def lib() -> ctypes.CDLL:
     L.htree_draft_attention.argtypes = [CP, I32, I32, I32, I32, I64, F, P, I64, I64, P, P, P, P, P, P,
                                         P, I64, I64, P, I64, P]
     L.htree_verify_drafts_workspace_bytes.restype = ctypes.c_int
-    L.htree_verify_drafts_workspace_bytes.argtypes = [I32, I32, I32, ctypes.POINTER(I64)]
+    L.htree_verify_drafts_workspace_bytes.argtypes = [I32] * 6 + [ctypes.POINTER(I64)]
     L.htree_verify_drafts.restype = ctypes.c_int
     L.htree_verify_drafts.argtypes = [I32] * 4 + [P, I64, P, I64] + [P] * 9 + [I64, P]
     L.htree_keep_drafts.restype = ctypes.c_int

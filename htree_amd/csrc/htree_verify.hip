@@ -31,6 +31,7 @@ constexpr int kVerifyParts = 4;        // at most: their waves' sums fill a wave
 constexpr int kVerifySplit = 1 << 17;  // elements of a row of p (and q) from which on they do,
 constexpr int kVerifyPart = 1 << 14;   // and that a part has at least
 constexpr int kVerifyFull = 256;       // blocks that fill the GPU
+constexpr int64_t kVerifyAll = 1 << 28;  // bytes of a call whose rows are all searched, greedily
 
 // where a request's walk ended, for verify_draw_kernel
 struct VerifyEnd {
@@ -42,6 +43,7 @@ struct VerifyEnd {
 struct VerifyArgs {
   VerifyEnd* ends;  // [B]
   double* sums;     // [B][parts][waves]
+  int32_t* largest; // [rows], greedily
   int32_t parts;
   const char *p, *q;
   const int64_t* tokens;
@@ -93,6 +95,7 @@ __device__ __forceinline__ double wave_sum(double x) { return lane_value(wave_sc
 
 struct VerifyLds {
   int32_t parent[kVerifyRows], token[kVerifyRows];
+  int32_t largest[kVerifyWaves], best[kVerifyRows];
   float p[kVerifyRows], q[kVerifyRows], u[kVerifyRows];
   double red[kVerifyWaves];
   double sums[kVerifyParts * kVerifyWaves];  // of the ranges
@@ -383,6 +386,30 @@ __device__ __forceinline__ int load_row(const VerifyArgs& a, VerifyLds& l, int s
   return up;
 }
 
+// A request's first row and how many of its rows are looked at.  Its path, but
+// for the kept rows behind the first, is written by part 0; a request without
+// rows is done with this.
+struct Request {
+  int s0, n;
+};
+__device__ __forceinline__ Request open_request(const VerifyArgs& a, int b, int part) {
+  const int tid = threadIdx.x;
+  const int s0 = min(max(a.starts[b], 0), a.rows), s1 = min(max(a.starts[b + 1], s0), a.rows);
+  if (part == 0) {
+    for (int i = s0 + tid; i < s1; i += kVerifyThreads) a.path[i] = i == s0 ? 0 : -1;
+    // rows of no request
+    if (b == 0)
+      for (int i = tid; i < s0; i += kVerifyThreads) a.path[i] = -1;
+    if (b == a.B - 1)
+      for (int i = s1 + tid; i < a.rows; i += kVerifyThreads) a.path[i] = -1;
+    if (s0 == s1 && tid == 0) {
+      a.kept[b] = 0, a.next[b] = -1;
+      if (a.parts > 1) a.ends[b].row = -1;
+    }
+  }
+  return {s0, min(s1 - s0, kVerifyRows)};
+}
+
 // A block a request: its drafts' tests one after another, the path, then the
 // next token from what is left at the last kept row.  With `parts` blocks a
 // request each makes the same tests, and a part of the last sums.
@@ -391,24 +418,9 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_drafts_kernel(VerifyArg
   __shared__ VerifyLds l;
   const int b = blockIdx.x, part = blockIdx.y, tid = threadIdx.x;
   const T *P = (const T*)a.p, *Q = (const T*)a.q;
-  const int s0 = min(max(a.starts[b], 0), a.rows), s1 = min(max(a.starts[b + 1], s0), a.rows);
-  const int rows = s1 - s0, n = min(rows, kVerifyRows);
-  if (part == 0) {
-    for (int i = tid; i < rows; i += kVerifyThreads) a.path[s0 + i] = i ? -1 : 0;
-    // rows of no request
-    if (b == 0)
-      for (int i = tid; i < s0; i += kVerifyThreads) a.path[i] = -1;
-    if (b == a.B - 1)
-      for (int i = s1 + tid; i < a.rows; i += kVerifyThreads) a.path[i] = -1;
-  }
+  const auto [s0, n] = open_request(a, b, part);
+  if (n == 0) return;
   const bool writes = part == 0 && tid == 0;
-  if (n == 0) {
-    if (writes) {
-      a.kept[b] = 0, a.next[b] = -1;
-      if (a.parts > 1) a.ends[b].row = -1;
-    }
-    return;
-  }
   for (int i = tid; i < n; i += kVerifyThreads) {
     const int up = load_row(a, l, s0, i);
     if (up >= 0) {
@@ -494,6 +506,92 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(VerifyArgs 
   if (tid == 0) a.next[b] = token;
 }
 
+// The index of a row's largest entry, of several the first; -1 where none is
+// above -infinity (a NaN is not).  By the whole block.
+template <typename T>
+__device__ __forceinline__ int row_largest(const T* row, VerifyLds& s, int V) {
+  constexpr int U = sizeof(T) == 4 ? kVerifySteps / 2 : kVerifySteps;
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  float most = -INFINITY;
+  int at = -1;
+  if (V < 8) {
+    for (int e = 0; e < V; ++e) {
+      const float x = (float)row[e];
+      if (x > most) most = x, at = e;
+    }
+    return at;
+  }
+  const int64_t size = range_size(V, kVerifyWaves), e0 = wv * size, e1 = min(e0 + size, (int64_t)V);
+  for (int64_t e = e0; e < e1; e += U * kVerifyStep) {
+    Elements<T, 8> x[U];
+    int64_t from[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {  // past the end: the last eight again
+      from[u] = min(e + u * kVerifyStep + lane * 8, (int64_t)V - 8);
+      x[u] = *(const Elements<T, 8>*)(row + from[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float v = (float)x[u].v[i];
+        if (v > most) most = v, at = (int)from[u] + i;
+      }
+  }
+  // (an index of -1 is the largest unsigned one)
+  auto better = [&](float v, int i) {
+    if (v > most || (v == most && (uint32_t)i < (uint32_t)at)) most = v, at = i;
+  };
+#pragma unroll
+  for (int m = 32; m; m >>= 1) better(__shfl_xor(most, m), __shfl_xor(at, m));
+  __syncthreads();
+  if (lane == 0) s.p[wv] = most, s.largest[wv] = at;
+  __syncthreads();
+  most = -INFINITY, at = -1;
+  for (int w = 0; w < kVerifyWaves; ++w) better(s.p[w], s.largest[w]);
+  return at;
+}
+
+// A block a row: its largest entry.
+template <typename T>
+__global__ __launch_bounds__(kVerifyThreads) void verify_largest_kernel(VerifyArgs a) {
+  __shared__ VerifyLds l;
+  const int at = row_largest((const T*)a.p + blockIdx.x * a.p_row, l, a.V);
+  if (threadIdx.x == 0) a.largest[blockIdx.x] = at;
+}
+
+// A block a request, greedily: a draft is kept if its token is the largest
+// entry's after the row it was drafted after.  Those of all rows are there
+// already, or are found row by row as the walk comes to them.
+template <typename T>
+__global__ __launch_bounds__(kVerifyThreads) void verify_greedy_kernel(VerifyArgs a) {
+  __shared__ VerifyLds l;
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+  const T* P = (const T*)a.p;
+  const auto [s0, n] = open_request(a, b, 0);
+  if (n == 0) return;
+  for (int i = tid; i < n; i += kVerifyThreads) {
+    load_row(a, l, s0, i);
+    if (a.largest) l.best[i] = a.largest[s0 + i];
+  }
+  __syncthreads();
+  int node = 0, kept = 1, token;
+  for (;;) {
+    token = a.largest ? l.best[node] : row_largest(P + (s0 + node) * a.p_row, l, a.V);
+    int next = -1;
+    for (int g = node + 1; g < n && next < 0; g += 64) {
+      const int i = min(g + lane, kVerifyRows - 1);
+      const uint64_t hit = __ballot(g + lane < n && l.parent[i] == node && l.token[i] == token);
+      if (hit) next = g + __builtin_ctzll(hit);
+    }
+    if (next < 0) break;
+    node = next;
+    if (tid == 0) a.path[s0 + kept] = node;
+    ++kept;
+  }
+  if (tid == 0) a.kept[b] = kept, a.next[b] = token;
+}
+
 // Blocks that share a request's sums: as many as have a CU to themselves.
 static int verify_parts(int32_t B, int32_t V, bool drawn) {
   const int64_t all = (int64_t)V * (drawn ? 2 : 1);
@@ -503,16 +601,29 @@ static int verify_parts(int32_t B, int32_t V, bool drawn) {
   return (int)(all / kVerifyPart < parts ? all / kVerifyPart : parts);
 }
 
+// Whether all rows are searched for their largest entry at once, or only those
+// that the walk comes to: one after another, so that the longest path counts.
+// 64 requests of 9 rows, 128000 16-bit entries (147 MB): 38 us at once, 67 one
+// after another; 256 of 13 rows, 32768 fp32 (436 MB): 80 and 67.
+static bool verify_all(int32_t dtype, int32_t rows, int32_t V) {
+  return (int64_t)rows * V * (dtype == HTREE_F32 ? 4 : 2) <= kVerifyAll;
+}
+
 }  // namespace htree
 
 using namespace htree;
 
-extern "C" int htree_verify_drafts_workspace_bytes(int32_t B, int32_t V, int32_t drawn, int64_t* bytes) {
+extern "C" int htree_verify_drafts_workspace_bytes(int32_t dtype, int32_t B, int32_t rows, int32_t V, int32_t drawn,
+                                                   int32_t greedy, int64_t* bytes) {
   if (!bytes) return HTREE_ENULL;
-  if (B < 0 || V < 1) return HTREE_ESHAPE;
+  if (dtype != HTREE_F32 && dtype != HTREE_BF16 && dtype != HTREE_F16) return HTREE_ESHAPE;
+  if (B < 0 || rows < 0 || V < 1 || (greedy && drawn)) return HTREE_ESHAPE;
   if (B > kCacheMaxRequests) return HTREE_EUNSUPPORTED;
-  const int parts = B ? verify_parts(B, V, drawn) : 1;
-  *bytes = parts > 1 ? B * ((int64_t)sizeof(VerifyEnd) + parts * kVerifyWaves * 8) : 0;
+  *bytes = 0;
+  if (B == 0) return HTREE_OK;
+  const int parts = verify_parts(B, V, drawn);
+  if (greedy) *bytes = verify_all(dtype, rows, V) ? rows * 4ll : 0;
+  else if (parts > 1) *bytes = B * ((int64_t)sizeof(VerifyEnd) + parts * kVerifyWaves * 8);
   return HTREE_OK;
 }
 
@@ -521,14 +632,14 @@ extern "C" int htree_verify_drafts(int32_t dtype, int32_t B, int32_t rows, int32
                                    const int64_t* tokens, const int32_t* starts, const int32_t* parents,
                                    const float* uniforms, const float* draws, int32_t* kept, int32_t* path,
                                    int64_t* next_tokens, void* workspace, int64_t workspace_bytes, void* stream) {
-  if (dtype != HTREE_F32 && dtype != HTREE_BF16 && dtype != HTREE_F16) return HTREE_ESHAPE;
-  if (rows < 0 || target_row < 0 || draft_row < 0) return HTREE_ESHAPE;
+  const bool greedy = !uniforms && !draws;
   int64_t need = 0;
-  const int rc = htree_verify_drafts_workspace_bytes(B, V, draft_probs != nullptr, &need);
+  const int rc = htree_verify_drafts_workspace_bytes(dtype, B, rows, V, draft_probs != nullptr, greedy, &need);
   if (rc) return rc;
+  if (target_row < 0 || draft_row < 0) return HTREE_ESHAPE;
   if (B == 0) return HTREE_OK;
-  if (!starts || !draws || !kept || !next_tokens) return HTREE_ENULL;
-  if (rows && (!target_probs || !tokens || !uniforms || !path)) return HTREE_ENULL;
+  if (!starts || (!greedy && !draws) || !kept || !next_tokens) return HTREE_ENULL;
+  if (rows && (!target_probs || !tokens || (!greedy && !uniforms) || !path)) return HTREE_ENULL;
   if (need && !workspace) return HTREE_ENULL;
   if (off16(workspace)) return HTREE_EUNSUPPORTED;
   if (workspace_bytes < need) return HTREE_EWORKSPACE;
@@ -536,7 +647,7 @@ extern "C" int htree_verify_drafts(int32_t dtype, int32_t B, int32_t rows, int32
   const Range in[7] = {{target_probs, rows ? ((rows - 1) * target_row + V) * es : 0},
                        {draft_probs, rows && draft_probs ? ((rows - 1) * draft_row + V) * es : 0},
                        {tokens, rows * 8ll}, {starts, (B + 1) * 4ll}, {parents, parents ? rows * 4ll : 0},
-                       {uniforms, rows * 4ll}, {draws, B * 4ll}};
+                       {uniforms, uniforms ? rows * 4ll : 0}, {draws, draws ? B * 4ll : 0}};
   const Range out[4] = {{kept, B * 4ll}, {path, rows * 4ll}, {next_tokens, B * 8ll}, {workspace, need}};
   for (int i = 0; i < 4; ++i) {
     for (const Range& y : in)
@@ -550,12 +661,19 @@ extern "C" int htree_verify_drafts(int32_t dtype, int32_t B, int32_t rows, int32
   a.kept = kept, a.path = path, a.next = next_tokens;
   a.p_row = target_row, a.q_row = draft_row;
   a.B = B, a.rows = rows, a.V = V;
-  a.parts = verify_parts(B, V, draft_probs != nullptr);
+  a.parts = greedy ? 1 : verify_parts(B, V, draft_probs != nullptr);
   a.ends = (VerifyEnd*)workspace;
   a.sums = (double*)(a.ends + B);
+  a.largest = greedy && need ? (int32_t*)workspace : nullptr;
   hipStream_t s = (hipStream_t)stream;
 #define HTREE_VERIFY(T)                                                                                     \
   do {                                                                                                      \
+    if (greedy) {                                                                                           \
+      if (a.largest)                                                                                        \
+        hipLaunchKernelGGL((verify_largest_kernel<T>), dim3(rows), dim3(kVerifyThreads), 0, s, a);          \
+      hipLaunchKernelGGL((verify_greedy_kernel<T>), dim3(B), dim3(kVerifyThreads), 0, s, a);                \
+      break;                                                                                                \
+    }                                                                                                       \
     hipLaunchKernelGGL((verify_drafts_kernel<T>), dim3(B, a.parts), dim3(kVerifyThreads), 0, s, a);         \
     if (a.parts > 1) hipLaunchKernelGGL((verify_draw_kernel<T>), dim3(B), dim3(kVerifyThreads), 0, s, a);   \
   } while (0)

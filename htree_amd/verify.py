@@ -24,9 +24,10 @@ class Verified(NamedTuple):
 
 
 @lru_cache(maxsize=256)
-def _workspace_bytes(B: int, V: int, drawn: bool) -> int:
+def _workspace_bytes(dtype, B: int, rows: int, V: int, drawn: bool, greedy: bool) -> int:
     n = ctypes.c_int64()
-    N.check(N.lib().htree_verify_drafts_workspace_bytes(B, V, drawn, n), "htree_verify_drafts_workspace_bytes")
+    N.check(N.lib().htree_verify_drafts_workspace_bytes(N.DTYPE_CODE[dtype], B, rows, V, drawn, greedy, n),
+            "htree_verify_drafts_workspace_bytes")
     return n.value
 
 
@@ -37,7 +38,7 @@ def _probs(p: torch.Tensor, name: str, rows: int, V: int, dtype, device) -> None
 
 
 def verify_drafts(target_probs: torch.Tensor, tokens: torch.Tensor, starts: torch.Tensor,
-                  uniforms: torch.Tensor, draws: torch.Tensor,
+                  uniforms: Optional[torch.Tensor] = None, draws: Optional[torch.Tensor] = None,
                   draft_probs: Optional[torch.Tensor] = None, parents: Optional[torch.Tensor] = None,
                   out: Optional[Verified] = None) -> Verified:
     """Accepts or rejects drafted tokens so that what is kept is distributed
@@ -65,13 +66,18 @@ def verify_drafts(target_probs: torch.Tensor, tokens: torch.Tensor, starts: torc
     accepted, or there are none, the next token is drawn from T: the first
     whose cumulative T passes draws[b] sum T (if nothing is left of T, from
     the target's probabilities).  uniforms (float32 [rows]; those of first
-    rows are not used) and draws (float32 [B]) are from [0, 1).  For greedy
-    decoding the target's probabilities are ones and zeros.
+    rows are not used) and draws (float32 [B]) are from [0, 1).
+
+    Without uniforms, draws and draft_probs the drafts are verified greedily:
+    one is accepted if its token is that of the largest entry after the row
+    it was drafted after, and that token is the next one where none is.
+    target_probs may be any scores then; of equal entries the first counts, a
+    NaN does not.
 
     Sums are 64-bit.  Entries that are no positive finite numbers count as
     zero, and so do uniforms and draws that are not positive.  A request
-    without rows keeps 0 and has next token -1, and so has one without any
-    mass.  Of a request the first 1024 rows are looked at.
+    without rows keeps 0 and has next token -1; without any mass (greedily: any
+    entry above -infinity) the next token is -1 too.  Of a request the first 1024 rows are looked at.
 
     Returns Verified (`out`: written there; no overlap with the inputs).
     Nothing synchronises; the numbers are the same every run."""
@@ -85,20 +91,24 @@ def verify_drafts(target_probs: torch.Tensor, tokens: torch.Tensor, starts: torc
     _probs(target_probs, "target_probs", rows, V, dtype, dev)
     if draft_probs is not None:
         _probs(draft_probs, "draft_probs", rows, V, dtype, dev)
-    assert draws.dim() == 1, "draws must be float32 [B]"
-    B = draws.shape[0]
+    assert starts.dim() == 1 and starts.shape[0] > 0, "starts must be int32 [B + 1]"
+    B = starts.shape[0] - 1
     assert B <= MAX_REQUESTS, f"at most {MAX_REQUESTS} requests, got {B}"
     _ints(starts, "starts", B + 1, dev)
-    for t, name, n in ((uniforms, "uniforms", rows), (draws, "draws", B)):
-        assert t.dtype is torch.float32 and t.shape == (n,) and t.is_contiguous() and t.device == dev, \
-            f"{name} must be a contiguous float32 tensor [{n}] on {dev}"
+    greedy = uniforms is None
+    assert greedy == (draws is None), "uniforms and draws go together"
+    if greedy:
+        assert draft_probs is None, "draft_probs need uniforms and draws"
+    else:
+        for t, name, n in ((uniforms, "uniforms", rows), (draws, "draws", B)):
+            assert t.dtype is torch.float32 and t.shape == (n,) and t.is_contiguous() and t.device == dev, \
+                f"{name} must be a contiguous float32 tensor [{n}] on {dev}"
     assert tokens.dtype is torch.int64 and tokens.shape == (rows,) and tokens.is_contiguous() and tokens.device == dev, \
         f"tokens must be a contiguous int64 tensor [{rows}] on {dev}"
     if parents is not None:
         _ints(parents, "parents", rows, dev)
     if out is None:
-        out = Verified(torch.empty_like(draws, dtype=torch.int32), torch.empty_like(uniforms, dtype=torch.int32),
-                       torch.empty_like(draws, dtype=torch.int64))
+        out = Verified(starts.new_empty(B), torch.empty_like(tokens, dtype=torch.int32), tokens.new_empty(B))
     else:
         _ints(out.kept, "out.kept", B, dev)
         _ints(out.path, "out.path", rows, dev)
@@ -108,11 +118,11 @@ def verify_drafts(target_probs: torch.Tensor, tokens: torch.Tensor, starts: torc
     if B == 0:
         out.path.fill_(-1)
         return out
-    nbytes = _workspace_bytes(B, V, draft_probs is not None)
-    ws = draws.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    nbytes = _workspace_bytes(dtype, B, rows, V, draft_probs is not None, greedy)
+    ws = starts.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     rc = N.launch(N.lib().htree_verify_drafts, dev, N.DTYPE_CODE[dtype], B, rows, V, target_probs.data_ptr(),
                   target_probs.stride(0), N.address(draft_probs), 0 if draft_probs is None else draft_probs.stride(0),
-                  tokens.data_ptr(), starts.data_ptr(), N.address(parents), uniforms.data_ptr(), draws.data_ptr(),
+                  tokens.data_ptr(), starts.data_ptr(), N.address(parents), N.address(uniforms), N.address(draws),
                   out.kept.data_ptr(), out.path.data_ptr(), out.next_tokens.data_ptr(), N.address(ws), nbytes)
     if rc:
         assert rc != N.HTREE_EOVERLAP, "out must not overlap the inputs, nor its parts each other"

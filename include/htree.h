@@ -402,13 +402,18 @@ int htree_draft_attention(const htree_cache* c, int32_t B, int32_t rows, int32_t
  * probabilities if nothing is left of them).  Sums are fp64.  Entries that are
  * no positive finite numbers count as 0, and so do uniforms and draws that
  * are not positive.
+ * Without uniforms and draws (both NULL, nor draft_probs) greedily: a draft is
+ * accepted if its token is that of the largest entry of target_probs, which
+ * may be any scores then (the first of equal ones, NaN is none), and that is
+ * the next token where none is.
  *   kept        [B] rows kept; 0 for a request without rows
  *   path        [rows] from starts[b] on the kept rows' indices within their
  *               request, ascending; -1 elsewhere
  *   next_tokens [B]; -1 without rows or without any mass
- * The first 1024 rows of a request are looked at.  Few requests over a large
- * vocabulary need a workspace (drawn: with draft_probs). */
-int htree_verify_drafts_workspace_bytes(int32_t B, int32_t V, int32_t drawn, int64_t* bytes);
+ * The first 1024 rows of a request are looked at.  Some sizes need a workspace
+ * (drawn: with draft_probs, greedy: without the numbers). */
+int htree_verify_drafts_workspace_bytes(int32_t dtype, int32_t B, int32_t rows, int32_t V,
+                                        int32_t drawn, int32_t greedy, int64_t* bytes);
 int htree_verify_drafts(int32_t dtype, int32_t B, int32_t rows, int32_t V, const void* target_probs,
                         int64_t target_row, const void* draft_probs, int64_t draft_row,
                         const int64_t* tokens, const int32_t* starts, const int32_t* parents,

@@ -131,6 +131,8 @@ def test_decoding_with_drafts(layout):
         probs = torch.nn.functional.one_hot(scores.argmax(-1), VOCAB).float()
         v = htree_amd.verify_drafts(probs, tokens, t.starts, torch.rand(sum(n), device=DEV), torch.rand(B, device=DEV),
                                     parents=parents)
+        greedy = htree_amd.verify_drafts(scores, tokens, t.starts, parents=parents)
+        assert all(torch.equal(x, y) for x, y in zip(v, greedy))
         htree_amd.keep_drafts(kc, vc, t.slots, t.starts, v.path, v.kept)
         held = sum(-(-int(x) // PAGE) for x in lens + v.kept)
         lens = lens + v.kept

@@ -131,6 +131,76 @@ def test_ties_and_borders(tree, drawn):
         check(*case([9, 5, 17], 40, "float32", tree, drawn, seed, sharp=2.0, grid=16))
 
 
+def greedy_walk(p, tokens, starts, parents):
+    p = np.asarray(p, np.float64)
+    p = np.where(np.isnan(p), -np.inf, p)
+    B, V = len(starts) - 1, p.shape[1]
+    kept, path, nxt = np.zeros(B, int), np.full(p.shape[0], -1), np.full(B, -1)
+    for b in range(B):
+        s0, n = starts[b], min(starts[b + 1] - starts[b], 1024)
+        if n <= 0:
+            continue
+        keep = [0]
+        while True:
+            best = int(p[s0 + keep[-1]].argmax())
+            best = best if p[s0 + keep[-1]][best] > -np.inf else -1
+            hit = [j for j in range(keep[-1] + 1, n) if (j - 1 if parents is None else parents[s0 + j]) == keep[-1]
+                   and 0 <= tokens[s0 + j] < V and tokens[s0 + j] == best]
+            if not hit:
+                break
+            keep.append(hit[0])
+        kept[b], path[s0:s0 + len(keep)], nxt[b] = len(keep), keep, best
+    return kept, path, nxt
+
+
+def check_greedy(p, tokens, starts, parents):
+    i32 = lambda x: None if x is None else torch.as_tensor(np.asarray(x, np.int32)).to(DEV)
+    want = greedy_walk(p.double().cpu().numpy(), tokens, starts, parents)
+    got = htree_amd.verify_drafts(p.to(DEV), torch.as_tensor(np.asarray(tokens, np.int64)).to(DEV), i32(starts),
+                                  parents=i32(parents))
+    for name, a, b in zip(got._fields, got, want):
+        assert np.array_equal(a.cpu().numpy(), b), (name, a.cpu().numpy()[:20], b[:20])
+    return want
+
+
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize("new,V,dtype", [([6], 32000, "float32"), ([1, 0, 3], 1, "float32"), ([24] * 5, 7, "bfloat16"),
+                                         ([9, 5], 8, "float16"), ([2, 9, 1, 30], 8192, "float16"), ([5, 5], 8193, "float32"),
+                                         ([64, 65], 2047, "bfloat16"), ([3] * 300, 301, "bfloat16"), ([7, 8], 150001, "bfloat16"),
+                                         ([1200], 40, "float32"),
+                                         ([40, 1, 30], 1000003, "float32")])
+def test_greedily(new, V, dtype, tree):
+    """Scores of any size, equal ones among them, drafts half of which are what
+    the target says."""
+    kept = 0
+    for seed in range(3):
+        p, _, tokens, starts, parents, _, _ = case(new, V, dtype, tree, False, seed)
+        g = np.random.default_rng(seed)
+        scores = (torch.randn(p.shape, generator=torch.Generator().manual_seed(seed)) * 8).round() / 4
+        scores = (scores * (10.0 ** 3 if seed else 1.0)).to(DT[dtype])
+        best = scores.float().numpy().argmax(1)
+        for b in range(len(new)):
+            for j in range(1, new[b]):
+                if g.random() < 0.5:
+                    tokens[starts[b] + j] = best[starts[b] + (j - 1 if parents is None else parents[starts[b] + j])]
+        if seed == 2:
+            scores[g.random(p.shape) < 0.3] = float("nan")
+            scores[::3] = scores[::3].clamp(max=0) - float("inf")
+            scores[1::5, V // 2] = float("inf")
+            if len(scores) > 1:
+                scores[-1] = float("nan")
+        kept = max(kept, check_greedy(scores, tokens, starts, parents)[0].max())
+    assert kept > 1 or sum(new) < 20  # the larger cases accept something
+
+
+def test_greedily_is_what_ones_and_zeros_give():
+    p, _, tokens, starts, parents, u, d = case([20, 20, 20], 300, "float32", True, False, 3)
+    one = torch.nn.functional.one_hot(p.argmax(1), 300).float()
+    a = check_greedy(p, tokens, starts, parents)
+    b = check(one, None, tokens, starts, parents, u, d)
+    assert all(np.array_equal(x, y) for x, y in zip(a, b))
+
+
 @pytest.mark.parametrize("drawn", [False, True])
 def test_more_rows_than_are_looked_at(drawn):
     new, V = [1500, 3], 20
@@ -267,7 +337,8 @@ def test_refusals():
     bad = [dict(target_probs=f(3, 9, t=torch.float64)), dict(target_probs=f(3, 9, 1)), dict(target_probs=f(3, 0)),
            dict(target_probs=f(9, 3).t()), dict(target_probs=f(4, 9)), dict(tokens=f(3, t=i32)), dict(tokens=f(2, t=i64)),
            dict(tokens=f(6, t=i64)[::2]), dict(starts=f(3, t=i32)), dict(starts=f(2, t=i64)),
-           dict(uniforms=f(3, t=torch.float64)), dict(uniforms=f(4)), dict(draws=f(1, 1)), dict(draws=f(4097)),
+           dict(uniforms=f(3, t=torch.float64)), dict(uniforms=f(4)), dict(draws=f(1, 1)), dict(draws=f(2)), dict(starts=f(4098, t=i32), draws=f(4097)), dict(uniforms=None), dict(draws=None),
+           dict(uniforms=None, draws=None, draft_probs=f(3, 9)), dict(starts=f(0, t=i32)),
            dict(draft_probs=f(3, 8)), dict(draft_probs=f(3, 9, t=torch.bfloat16)), dict(parents=f(3, t=i64)),
            dict(parents=f(4, t=i32)), dict(tokens=torch.zeros(3, dtype=i64)), dict(draft_probs=torch.zeros(3, 9)),
            dict(out=htree_amd.Verified(f(2, t=i32), f(3, t=i32), f(1, t=i64))),

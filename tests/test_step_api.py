@@ -41,7 +41,8 @@ def test_verify_refusals():
     assert verify(kept=at(7)) == N.HTREE_EOVERLAP and verify(path=at(8)) == N.HTREE_EOVERLAP
     assert verify(B=0, p=None) == N.HTREE_OK
     # few requests over a large vocabulary need a workspace
-    need = lambda *a: size("htree_verify_drafts_workspace_bytes", *a)
+    need = lambda B, V, drawn, greedy=0, rows=6, dtype=0: \
+        size("htree_verify_drafts_workspace_bytes", dtype, B, rows, V, drawn, greedy)
     assert need(2, 100, 1) == (N.HTREE_OK, 0) and need(129, 1 << 20, 1) == (N.HTREE_OK, 0)
     rc, n = need(2, 1 << 17, 0)
     assert rc == N.HTREE_OK and 0 < n < 4096 and need(2, 1 << 16, 1) == (N.HTREE_OK, n)
@@ -52,8 +53,18 @@ def test_verify_refusals():
     for x in (2, 3, 4, 5, 6, 7, 8, 4000):
         assert verify(**big, ws=at(x)) == N.HTREE_EOVERLAP
     assert need(4, 0, 0)[0] == N.HTREE_ESHAPE and need(-1, 5, 0)[0] == N.HTREE_ESHAPE
+    assert need(4, 5, 0, rows=-1)[0] == N.HTREE_ESHAPE and need(4, 5, 0, dtype=3)[0] == N.HTREE_ESHAPE
     assert need(4097, 5, 0)[0] == N.HTREE_EUNSUPPORTED
-    assert N.lib().htree_verify_drafts_workspace_bytes(1, 1, 0, None) == N.HTREE_ENULL
+    assert N.lib().htree_verify_drafts_workspace_bytes(0, 1, 1, 1, 0, 0, None) == N.HTREE_ENULL
+    # greedily: no numbers at all, nor a drafter's probabilities
+    greedy = dict(u=None, d=None)
+    assert need(2, 100, 0, 1) == (N.HTREE_OK, 24) and need(2, 1 << 20, 0, 1, rows=65) == (N.HTREE_OK, 0)
+    assert need(2, 1 << 20, 0, 1, rows=128, dtype=1) == (N.HTREE_OK, 512)
+    assert verify(**greedy, q=at(20), q_row=100) == N.HTREE_ESHAPE and need(2, 100, 1, 1)[0] == N.HTREE_ESHAPE
+    assert verify(**greedy, p=None, ws=at(9), n=24) == N.HTREE_ENULL
+    assert verify(**greedy) == N.HTREE_ENULL and verify(**greedy, ws=at(9), n=23) == N.HTREE_EWORKSPACE
+    assert verify(**greedy, ws=at(9), n=24, kept=at(2)) == N.HTREE_EOVERLAP
+    assert verify(**greedy, ws=at(1), n=24) == N.HTREE_EOVERLAP
 
 
 def pointers(n, first=4096):
