@@ -20,7 +20,7 @@ struct NormSide {  // queries, or keys
   char* y;                              // the backward's dx
   const void* w;
   int64_t x_row, x_head, dy_row, dy_head;  // bytes; y is contiguous
-  int32_t heads, groups;                // of U heads
+  int32_t heads;
 };
 
 struct NormArgs {
@@ -28,7 +28,7 @@ struct NormArgs {
   const int32_t* positions;
   const float *cs, *sn;
   float* partial;   // backward: [2][blocks][D]
-  int64_t items;    // rows x (groups of heads of both)
+  int64_t items;    // rows x heads of both sides
   int32_t rows, D, per, lanes, rope_rows, w_f32;
   float eps, inv_d;
 };
@@ -79,66 +79,60 @@ __device__ __forceinline__ bool load_turn(const NormArgs& a, int row, int at, fl
 }
 
 // A head has `lanes` lanes (2^n: LANES, or 0: as the arguments say), the first
-// `per` of them with VB bytes of each half.  U heads of a row at a time.
-template <typename T, int VB, int LANES, int U>
+// `per` of them with VB bytes of each half, so that a lane has both elements of
+// its pairs.  (Four heads of a row a lane, which reads the rotation and the
+// weights once for them, took 1 to 2 us longer up to 1000 rows and 234 us instead
+// of 227 for 65536.)  Bound by memory, in and out once: 65536 rows of 32/2 heads
+// of 128, rotated, bf16, 227 us (5.2 TB/s); 64 such rows 3.5 us, most of it the
+// launch.
+template <typename T, int VB, int LANES>
 __global__ __launch_bounds__(kNormThreads) void head_norm_kernel(NormArgs a) {
   constexpr int NV = VB / (int)sizeof(T);
   typedef typename NormVec<VB>::V V;
   const int L = LANES ? LANES : a.lanes, lane = threadIdx.x & (L - 1);
   const int64_t item = ((int64_t)blockIdx.x * kNormThreads + threadIdx.x) / L;
   if (item >= a.items) return;
-  const int all = a.side[0].groups + a.side[1].groups;
+  const int all = a.side[0].heads + a.side[1].heads;
   const int row = (int)((uint32_t)item / (uint32_t)all);
-  int g = (int)((uint32_t)item - (uint32_t)row * all);
-  const int which = g >= a.side[0].groups;
-  if (which) g -= a.side[0].groups;
+  int h = (int)((uint32_t)item - (uint32_t)row * all);
+  const int which = h >= a.side[0].heads;
+  if (which) h -= a.side[0].heads;
   const NormSide& sd = a.side[which];
-  const int half = a.D / 2, at = lane * NV, heads = sd.heads;
+  const int half = a.D / 2, at = lane * NV;
   const bool on = lane < a.per;
-  const int64_t hb = (int64_t)half * sizeof(T), h0 = (int64_t)g * U;
-  const char* x = sd.x + row * sd.x_row + h0 * sd.x_head + lane * VB;
-  V v1[U], v2[U];
-#pragma unroll
-  for (int u = 0; u < U; ++u)
-    if (on && h0 + u < heads) {
-      v1[u] = *(const V*)(x + u * sd.x_head);
-      v2[u] = *(const V*)(x + u * sd.x_head + hb);
-    }
-  float w1[NV], w2[NV], c[NV], s[NV];
+  const int64_t hb = (int64_t)half * sizeof(T);
+  V v1, v2;
+  float w1[NV], w2[NV], c[NV], s[NV], ss = 0.f;
   bool there = true;
+  const T *p1 = (const T*)&v1, *p2 = (const T*)&v2;
   if (on) {
+    const char* x = sd.x + row * sd.x_row + h * sd.x_head + lane * VB;
+    v1 = *(const V*)x, v2 = *(const V*)(x + hb);
     load_weight<T, NV>(a, sd.w, at, w1);
     load_weight<T, NV>(a, sd.w, half + at, w2);
     there = load_turn<NV>(a, row, at, c, s);
+#pragma unroll
+    for (int e = 0; e < NV; ++e) ss += (float)p1[e] * (float)p1[e] + (float)p2[e] * (float)p2[e];
   }
-  char* y = sd.y + (((int64_t)row * heads + h0) * a.D) * sizeof(T) + lane * VB;
+  const float r = rsqrtf(lanes_sum(ss, L) * a.inv_d + a.eps);
+  if (!on) return;
+  V o1, o2;
+  T *q1 = (T*)&o1, *q2 = (T*)&o2;
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const bool mine = on && h0 + u < heads;
-    const T *p1 = (const T*)&v1[u], *p2 = (const T*)&v2[u];
-    float ss = 0.f;
-    if (mine) {
-#pragma unroll
-      for (int e = 0; e < NV; ++e) ss += (float)p1[e] * (float)p1[e] + (float)p2[e] * (float)p2[e];
-    }
-    const float r = rsqrtf(lanes_sum(ss, L) * a.inv_d + a.eps);
-    if (!mine) continue;
-    V o1, o2;
-    T *q1 = (T*)&o1, *q2 = (T*)&o2;
-#pragma unroll
-    for (int e = 0; e < NV; ++e) {
-      const float n1 = (float)p1[e] * r * w1[e], n2 = (float)p2[e] * r * w2[e];
-      q1[e] = (T)(there ? n1 * c[e] - n2 * s[e] : 0.f);
-      q2[e] = (T)(there ? n2 * c[e] + n1 * s[e] : 0.f);
-    }
-    *(V*)(y + (int64_t)u * a.D * sizeof(T)) = o1;
-    *(V*)(y + (int64_t)u * a.D * sizeof(T) + hb) = o2;
+  for (int e = 0; e < NV; ++e) {
+    const float n1 = (float)p1[e] * r * w1[e], n2 = (float)p2[e] * r * w2[e];
+    q1[e] = (T)(there ? n1 * c[e] - n2 * s[e] : 0.f);
+    q2[e] = (T)(there ? n2 * c[e] + n1 * s[e] : 0.f);
   }
+  char* y = sd.y + ((int64_t)row * sd.heads + h) * a.D * (int64_t)sizeof(T) + lane * VB;
+  *(V*)y = o1;
+  *(V*)(y + hb) = o2;
 }
 
 // The gradients of x, and each block's share of the weights'.  Blocks walk over
 // a side's items in steps of the grid, queries first, so that a lane's sums of
-// dw stay in registers.
+// dw stay in registers.  Bound by memory, x and dy in, dx out once: 65536 rows
+// of 32/4 heads of 128, bf16, 380 us (4.8 TB/s).
 template <typename T, int VB, int LANES>
 __global__ __launch_bounds__(kNormThreads, 4) void head_norm_bwd_kernel(NormArgs a) {
   constexpr int NV = VB / (int)sizeof(T);
@@ -241,7 +235,8 @@ struct NormSumArgs {
 };
 
 // The weights' gradients from the blocks' shares: block x, y sums 16 of the D
-// columns of side y, 64 threads a column, in a fixed order.
+// columns of side y, 64 threads a column, in a fixed order.  5.4 us of 1024
+// shares, eight loads of a thread in flight (9.4 one after another).
 template <typename T>
 __global__ __launch_bounds__(1024) void head_norm_sum_kernel(NormSumArgs a) {
   __shared__ float red[64][17];
@@ -268,13 +263,6 @@ static int norm_lanes(int per) {
   int L = 1;
   while (L < per) L *= 2;
   return L;
-}
-
-template <typename T, int VB, int LANES>
-static void norm_forward(const NormArgs& a, int u, hipStream_t s) {
-  const unsigned blocks = (unsigned)((a.items * a.lanes + kNormThreads - 1) / kNormThreads);
-  if (u == 1) hipLaunchKernelGGL((head_norm_kernel<T, VB, LANES, 1>), dim3(blocks), dim3(kNormThreads), 0, s, a);
-  else hipLaunchKernelGGL((head_norm_kernel<T, VB, LANES, 4>), dim3(blocks), dim3(kNormThreads), 0, s, a);
 }
 
 static int norm_blocks(int64_t items, int L) {
@@ -338,18 +326,16 @@ extern "C" int htree_head_norm(int32_t dtype, int32_t w_dtype, int32_t rows, int
   const bool wide = D * es % 32 == 0;
   a.per = D / 2 * es / (wide ? 16 : 8);
   const int L = a.lanes = norm_lanes(a.per);
-  // few rows: a head at a time, for the latency; many: four, and the row's
-  // rotation and weights read once for them
-  const int u = (int64_t)rows * (H + H_kv) * L <= 256 * 1024 ? 1 : 4;
-  a.side[0] = {(const char*)q, nullptr, (char*)q_out, q_weight, q_row * es, q_head * es, 0, 0, H, (H + u - 1) / u};
-  a.side[1] = {(const char*)k, nullptr, (char*)k_out, k_weight, k_row * es, k_head * es, 0, 0, H_kv,
-               (H_kv + u - 1) / u};
+  a.side[0] = {(const char*)q, nullptr, (char*)q_out, q_weight, q_row * es, q_head * es, 0, 0, H};
+  a.side[1] = {(const char*)k, nullptr, (char*)k_out, k_weight, k_row * es, k_head * es, 0, 0, H_kv};
   a.positions = positions, a.cs = cos_table, a.sn = sin_table;
-  a.items = (int64_t)rows * (a.side[0].groups + a.side[1].groups);
+  a.items = (int64_t)rows * (H + H_kv);
   a.rows = rows, a.D = D, a.rope_rows = rope_rows, a.w_f32 = w_dtype == HTREE_F32;
   a.eps = eps, a.inv_d = 1.f / D;
   hipStream_t s = (hipStream_t)stream;
-#define HTREE_NORM_FWD(T, VB, LANES) norm_forward<T, VB, LANES>(a, u, s)
+  const unsigned blocks = (unsigned)((a.items * L + kNormThreads - 1) / kNormThreads);
+#define HTREE_NORM_FWD(T, VB, LANES) \
+  hipLaunchKernelGGL((head_norm_kernel<T, VB, LANES>), dim3(blocks), dim3(kNormThreads), 0, s, a)
   HTREE_NORM_TYPES(HTREE_NORM_FWD)
 #undef HTREE_NORM_FWD
   const hipError_t e = hipGetLastError();
@@ -392,9 +378,9 @@ extern "C" int htree_head_norm_backward(int32_t dtype, int32_t w_dtype, int32_t 
   a.per = D / 2 * es / (wide ? 16 : 8);
   const int L = a.lanes = norm_lanes(a.per);
   a.side[0] = {(const char*)q, (const char*)dq_out, (char*)dq, q_weight, q_row * es, q_head * es, dq_row * es,
-               dq_head * es, H, H};
+               dq_head * es, H};
   a.side[1] = {(const char*)k, (const char*)dk_out, (char*)dk, k_weight, k_row * es, k_head * es, dk_row * es,
-               dk_head * es, H_kv, H_kv};
+               dk_head * es, H_kv};
   a.positions = positions, a.cs = cos_table, a.sn = sin_table;
   a.partial = weights ? (float*)workspace : nullptr;
   a.rows = rows, a.D = D, a.rope_rows = rope_rows, a.w_f32 = w_dtype == HTREE_F32;

@@ -97,7 +97,9 @@ __device__ __forceinline__ void move_tokens(const MoveArgs& m, const MoveColumn&
 // from path[j] >= j.  A thread owns a piece of every token of its request, so
 // that the order in which tokens are read and written is its own: four are
 // read before the first of them is written, later ones come from places behind
-// all that were written.
+// all that were written.  Bound by the chain start -> path -> slot -> token and
+// by memory: 16 requests, one layer 3.9 us; 256 requests, 32 layers of 8 x 128
+// bf16 39 us (162 MB, 4.1 TB/s).
 __global__ __launch_bounds__(256) void keep_drafts_kernel(KeepArgs a) {
   const int piece = blockIdx.z * blockDim.x + threadIdx.x, b = blockIdx.x;
   if (piece >= a.m.pieces) return;
@@ -126,7 +128,9 @@ __global__ __launch_bounds__(256) void keep_drafts_kernel(KeepArgs a) {
   }
 }
 
-// The first tokens[i] tokens of page from[i] to page to[i].
+// The first tokens[i] tokens of page from[i] to page to[i]: 192 pages of 8
+// tokens on average, 16 layers of 4 x 128 bf16, 13.7 us (33 MB); a page to seven
+// others, 16 layers 4.8 us, a launch and two loads one after the other.
 __global__ __launch_bounds__(256) void copy_pages_kernel(CopyArgs a) {
   const int i = blockIdx.x;
   const int from = cache_page(a.from[i], a.m.num_pages), to = cache_page(a.to[i], a.m.num_pages);
@@ -159,7 +163,8 @@ struct ForkArgs {
 
 // New requests blockIdx.x, + gridDim.x ..: their rows of the table.  Each block
 // finds the first child of every request and sums the fresh pages over all new
-// ones itself, which is less than a second launch.
+// ones itself, which is less than a second launch: 4.2 us for 8 new requests,
+// 5.3 for 256 out of 256.
 __global__ __launch_bounds__(256) void fork_requests_kernel(ForkArgs a) {
   extern __shared__ int32_t fork_lds[];
   __shared__ int64_t red[4];
@@ -214,52 +219,73 @@ struct UnusedArgs {
   int32_t B, width, page_shift, num_pages, n_held, tiles;
 };
 constexpr int kUnusedTile = 4096;        // pages a block counts or lists: 16 a thread
-constexpr int kUnusedChunk = 1024;       // entries of a row that a wave reads at once: four times 4 a lane
-constexpr int kUnusedSmall = 1 << 16;    // entries, and held pages, of a call in one launch,
-constexpr int kUnusedSmallRows = 256;    // its requests
-constexpr int kUnusedSmallPages = 1 << 18;  // and pages, whose bits fill 32 KB of LDS
+constexpr int kUnusedPiece = 256;        // entries of a row that a wave reads at once, 4 a lane,
+constexpr int kUnusedPieces = 4;         // of so many rows
+// Calls in one launch: pieces, requests and held pages at most, and pages, whose
+// bits fill 32 KB of LDS.  Against the other form's four launches: 64 pieces 6.9
+// us (11.7), 128 9.2 (11.4), 256 12.4 to 14 (10 to 12.5, and 7 us more of the
+// host's time); 1024 38 (12.7).
+constexpr int kUnusedSmall = 256, kUnusedSmallRows = 256, kUnusedSmallHeld = 4096;
+constexpr int kUnusedSmallPages = 1 << 18;
 constexpr int kUnusedSmallTile = 8192;   // pages a block lists: 8 a thread
 
 struct __attribute__((packed, aligned(4))) Entries {
   int32_t v[4];
 };
 
-// Entries j0 .. j0 + kUnusedChunk - 1 of a request, by a wave.  A row's last
-// reads start earlier, not past its end: the entries that they see twice are
-// marked twice.  (Rows of less than four entries: one each.)
-struct Chunk {
-  Entries x[4];
-  int64_t at[4];
+__device__ __forceinline__ int live_pages(const UnusedArgs& a, int len) {
+  return (int)min(table_pages(max(len, 0), a.page_shift), (int64_t)a.width);
+}
+
+// Four pieces of the table, from piece p0 on: piece p is the (p / B)-th 256
+// entries of request p % B, so that first pieces, which have most of the live
+// entries, come first.  Reads that would pass a row's end start earlier; what the
+// lanes in front have is not marked again, 64 lanes would wait for one word: of a
+// lane's four entries those from `lo` to before `hi` count.  (Rows of less than
+// four entries: one a lane.)
+struct Pieces {
+  Entries x[kUnusedPieces];
+  int lo[kUnusedPieces], hi[kUnusedPieces];
+  bool live[kUnusedPieces];  // any of the piece
 };
-__device__ __forceinline__ void load_chunk(const UnusedArgs& a, int b, int64_t j0, Chunk* c) {
+// (less than 2^31 of them)
+__device__ __forceinline__ uint32_t piece_count(const UnusedArgs& a) {
+  return ((uint32_t)a.width + kUnusedPiece - 1) / kUnusedPiece * a.B;
+}
+// length(b): of request b
+template <typename L>
+__device__ __forceinline__ void load_pieces(const UnusedArgs& a, uint32_t p0, L length, Pieces* c) {
   const int lane = threadIdx.x & 63;
-  const int32_t* row = a.table + b * a.table_stride;
-  if (a.width < 4) {
-    c->at[0] = lane;
-    c->x[0].v[0] = lane < a.width ? row[lane] : -1;
-    return;
-  }
+  const uint32_t all = piece_count(a);
+  uint32_t q = p0 / (uint32_t)a.B, b = p0 - q * a.B;
 #pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    c->at[u] = min(j0 + u * 256 + lane * 4, (int64_t)a.width - 4);
-    c->x[u] = *(const Entries*)(row + c->at[u]);
+  for (int u = 0; u < kUnusedPieces; ++u) {
+    const int32_t* row = a.table + (int64_t)b * a.table_stride;
+    const int live = p0 + u < all ? live_pages(a, length((int)b)) : 0;
+    if (a.width < 4) {
+      c->x[u].v[0] = row[min(lane, a.width - 1)];
+      c->live[u] = live > 0;
+      c->lo[u] = 0, c->hi[u] = lane < live ? 1 : 0;
+    } else {
+      const int mine = (int)q * kUnusedPiece + lane * 4, at = min(mine, a.width - 4);
+      c->x[u] = *(const Entries*)(row + at);
+      c->live[u] = live > (int)q * kUnusedPiece;
+      c->lo[u] = mine - at, c->hi[u] = live - at;
+    }
+    // (past the last piece: that one again)
+    if (p0 + u + 1 < all && ++b == (uint32_t)a.B) b = 0, ++q;
   }
 }
-// f(page) for those before entry `live`
+// f(page) for the pages that count
 template <typename F>
-__device__ __forceinline__ void mark_chunk(const UnusedArgs& a, const Chunk& c, int64_t live, F f) {
-  if (a.width < 4) {
-    if (c.at[0] < live) f(cache_page(c.x[0].v[0], a.num_pages));
-    return;
-  }
+__device__ __forceinline__ void mark_pieces(const UnusedArgs& a, const Pieces& c, F f) {
 #pragma unroll
-  for (int u = 0; u < 4; ++u)
+  for (int u = 0; u < kUnusedPieces; ++u)
+    if (c.live[u])
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (c.at[u] + e < live) f(cache_page(c.x[u].v[e], a.num_pages));
-}
-__device__ __forceinline__ int64_t live_pages(const UnusedArgs& a, int len) {
-  return min(table_pages(max(len, 0), a.page_shift), (int64_t)a.width);
+      for (int e = 0; e < 4; ++e)
+        if (e >= c.lo[u] && e < c.hi[u] && (uint32_t)c.x[u].v[e] < (uint32_t)a.num_pages)
+          f(c.x[u].v[e]);
 }
 
 // sum over the block's threads, to all; `red` an int for each wave
@@ -312,40 +338,30 @@ __device__ __forceinline__ void list_pages(const UnusedArgs& a, uint32_t bits, i
 }
 
 // A call in one launch: every block marks all pages that are held, in the bits
-// of its LDS, and lists its own part of the others.
+// of its LDS, and lists its own part of the others.  Bound by the marks, atomics
+// on random words: 41600 live entries of 64 requests, 46620 pages 12.8 us.
 __global__ __launch_bounds__(1024) void unused_small_kernel(UnusedArgs a) {
   extern __shared__ uint32_t small_bits[];  // 1: held; pages past the last one too
-  __shared__ int32_t buf[kUnusedSmallTile];
+  __shared__ int32_t buf[kUnusedSmallTile], lens[kUnusedSmallRows];
   __shared__ int red[16];
-  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+  const int tid = threadIdx.x, wv = tid >> 6;
   const int words = a.tiles * (kUnusedSmallTile / 32);
   for (int i = tid; i < words; i += 1024) {
     const int left = a.num_pages - i * 32;
     small_bits[i] = left >= 32 ? 0u : left <= 0 ? ~0u : ~0u << left;
   }
-  // lane r: the length of the wave's r-th request
-  const int mine = lane * 16 + wv, len = mine < a.B && lane < kUnusedSmallRows / 16 ? a.lens[mine] : 0;
+  for (int i = tid; i < a.B; i += 1024) lens[i] = a.lens[i];
   __syncthreads();
-  auto mark = [&](int page) {
-    if (page >= 0) atomicOr(&small_bits[page >> 5], 1u << (page & 31));
-  };
-  // two requests' first chunks in flight
-  for (int r = 0, b = wv; b < a.B; r += 2, b += 32) {
-    const bool two = b + 16 < a.B;
-    const int64_t live[2] = {live_pages(a, __shfl(len, r)), two ? live_pages(a, __shfl(len, r + 1)) : 0};
-    Chunk c[2];
-    load_chunk(a, b, 0, &c[0]);
-    if (two) load_chunk(a, b + 16, 0, &c[1]);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      if (live[i]) mark_chunk(a, c[i], live[i], mark);
-      for (int64_t j = kUnusedChunk; j < live[i]; j += kUnusedChunk) {
-        load_chunk(a, b + i * 16, j, &c[i]);
-        mark_chunk(a, c[i], live[i], mark);
-      }
-    }
+  auto mark = [&](int page) { atomicOr(&small_bits[page >> 5], 1u << (page & 31)); };
+  auto length = [&](int b) { return __builtin_amdgcn_readfirstlane(lens[b]); };
+  const uint32_t pieces = piece_count(a);
+  for (uint32_t p = __builtin_amdgcn_readfirstlane(wv) * kUnusedPieces; p < pieces; p += 16 * kUnusedPieces) {
+    Pieces c;
+    load_pieces(a, p, length, &c);
+    mark_pieces(a, c, mark);
   }
-  for (int i = tid; i < a.n_held; i += 1024) mark(cache_page(a.held[i], a.num_pages));
+  for (int i = tid; i < a.n_held; i += 1024)
+    if ((uint32_t)a.held[i] < (uint32_t)a.num_pages) mark(a.held[i]);
   __syncthreads();
   const int first = blockIdx.x * (kUnusedSmallTile / 32);
   int before = 0, all = 0;
@@ -365,29 +381,23 @@ __global__ __launch_bounds__(256) void unused_clear_kernel(uint8_t* flags, int64
   if (i < n) *(uint4*)(flags + i) = make_uint4(0, 0, 0, 0);
 }
 
-// A wave a chunk of a request's entries (wave b + c B: chunk c of request b, so
-// that the first chunks, which have most of the live entries, are spread over
-// the dies); the last blocks mark the held pages.  Whoever holds a page writes
-// the same 1: no atomics.
+// A wave four pieces of the table (spread over the dies as pieces are numbered: a
+// die that had all the first ones took six times as long); the last blocks mark
+// the held pages.  Whoever holds a page writes the same 1: no atomics.
+// 1.3M entries, each a store to a line of its own, 12 us; all four launches 24.
 __global__ __launch_bounds__(256) void unused_mark_kernel(UnusedArgs a) {
-  const int64_t chunks = ((int64_t)a.width + kUnusedChunk - 1) / kUnusedChunk;
-  const int64_t blocks = (a.B * chunks + 3) / 4;
+  const uint32_t pieces = piece_count(a), blocks = (pieces + 4 * kUnusedPieces - 1) / (4 * kUnusedPieces);
   if (blockIdx.x >= blocks) {
-    const int64_t i = (blockIdx.x - blocks) * 256 + threadIdx.x;
+    const int64_t i = (int64_t)(blockIdx.x - blocks) * 256 + threadIdx.x;
     const int page = i < a.n_held ? cache_page(a.held[i], a.num_pages) : -1;
     if (page >= 0) a.flags[page] = 1;
     return;
   }
-  const int64_t wave = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int64_t c = wave / a.B, b = wave - c * a.B;
-  if (c >= chunks) return;
-  const int64_t live = live_pages(a, a.lens[b]);
-  if (c * kUnusedChunk >= live) return;
-  Chunk x;
-  load_chunk(a, (int)b, c * kUnusedChunk, &x);
-  mark_chunk(a, x, live, [&](int page) {
-    if (page >= 0) a.flags[page] = 1;
-  });
+  const uint32_t p = (blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * kUnusedPieces;
+  if (p >= pieces) return;
+  Pieces c;
+  load_pieces(a, p, [&](int b) { return a.lens[b]; }, &c);
+  mark_pieces(a, c, [&](int page) { a.flags[page] = 1; });
 }
 
 // bit i: page p0 + i is unused
@@ -540,10 +550,13 @@ extern "C" int htree_fork_requests(int32_t B, int32_t N, int32_t page_size, int3
   return e == hipSuccess ? HTREE_OK : (int)e;
 }
 
+static int64_t unused_pieces(int32_t B, int32_t table_width) {
+  return ((int64_t)table_width + kUnusedPiece - 1) / kUnusedPiece * B;
+}
 // whether a call runs in one launch
 static bool unused_small(int32_t B, int32_t num_pages, int32_t table_width, int32_t n_held) {
-  return num_pages <= kUnusedSmallPages && B <= kUnusedSmallRows && n_held <= kUnusedSmall &&
-         (int64_t)B * table_width <= kUnusedSmall;
+  return num_pages <= kUnusedSmallPages && B <= kUnusedSmallRows && n_held <= kUnusedSmallHeld &&
+         unused_pieces(B, table_width) <= kUnusedSmall;
 }
 
 extern "C" int htree_unused_pages_workspace_bytes(int32_t B, int32_t num_pages, int32_t table_width, int32_t n_held,
@@ -593,9 +606,9 @@ extern "C" int htree_unused_pages(int32_t B, int32_t page_size, int32_t num_page
     a.tiles = (int)(((int64_t)num_pages + kUnusedTile - 1) / kUnusedTile);
     a.flags = (uint8_t*)workspace;
     a.counts = (int32_t*)(a.flags + (int64_t)a.tiles * kUnusedTile);
-    const int64_t chunks = ((int64_t)table_width + kUnusedChunk - 1) / kUnusedChunk;
-    const int64_t blocks = (B * chunks + 3) / 4 + ((int64_t)n_held + 255) / 256;
-    if (blocks > 0x7fffffff) return HTREE_EUNSUPPORTED;
+    const int64_t pieces = unused_pieces(B, table_width);
+    const int64_t blocks = (pieces + 4 * kUnusedPieces - 1) / (4 * kUnusedPieces) + ((int64_t)n_held + 255) / 256;
+    if (pieces >= 0x7fffff00 || blocks > 0x7fffffff) return HTREE_EUNSUPPORTED;
     hipLaunchKernelGGL(unused_clear_kernel, dim3(a.tiles), dim3(256), 0, s, a.flags, (int64_t)a.tiles * kUnusedTile);
     if (blocks) hipLaunchKernelGGL(unused_mark_kernel, dim3((unsigned)blocks), dim3(256), 0, s, a);
     hipLaunchKernelGGL(unused_count_kernel, dim3(a.tiles), dim3(256), 0, s, a);

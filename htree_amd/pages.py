@@ -157,7 +157,9 @@ def fork_requests(block_table: torch.Tensor, lens: torch.Tensor, source: torch.T
     shared.  A partly filled last page stays with the first new request of
     its source; each further one gets a fresh page from the front of
     free_pages (int32 [F], as page_tables takes them), into which copy_pages
-    copies the page's tokens, before either request is appended to.
+    copies the page's tokens, before either request is appended to.  Requests
+    that share pages are not cut back into them: their lengths do not go below
+    what they were forked at.
 
     Returns Forked (`out`: written there; no overlap with the inputs).
     Entries behind a request's last page are -1, and so is a page that

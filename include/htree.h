@@ -473,7 +473,8 @@ int htree_unused_pages(int32_t B, int32_t page_size, int32_t num_pages, int32_t 
  * with pairs (d, d + D/2) as htree_forward rotates them.  Weights [D] are fp32
  * or of the inputs' type (w_dtype), NULL: ones; without positions and tables
  * (all NULL) nothing is rotated.  Rows whose position is outside the tables
- * are zero.  Everything is fp32, rounded once.  H or H_kv may be 0.
+ * are zero.  Everything is fp32, rounded once.  H or H_kv may be 0.  Outputs
+ * share no memory with the inputs.
  * HTREE_EUNSUPPORTED: D above 256 or not in whole 16-byte pieces, strides or
  * bases off 16 bytes, rows (H + H_kv) past 31 bits. */
 int htree_head_norm(int32_t dtype, int32_t w_dtype, int32_t rows, int32_t H, int32_t H_kv,

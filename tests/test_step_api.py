@@ -139,14 +139,14 @@ def test_unused_refusals():
         assert unused(**{name: None}) == N.HTREE_ENULL, name
     # small calls need no workspace
     need = lambda *a: size("htree_unused_pages_workspace_bytes", *a)
-    assert need(64, 1 << 18, 1024, 1 << 16) == (N.HTREE_OK, 0)
-    for many in ((64, (1 << 18) + 1, 1024, 0), (65, 100, 1024, 0), (257, 100, 1, 0), (1, 100, 1, (1 << 16) + 1)):
+    assert need(64, 1 << 18, 1024, 4096) == (N.HTREE_OK, 0)
+    for many in ((64, (1 << 18) + 1, 1024, 0), (65, 100, 1024, 0), (257, 100, 1, 0), (257, 100, 0, 0), (1, 100, 1, 4097)):
         rc, n = need(*many)
         assert rc == N.HTREE_OK and n > 0
         big = dict(B=many[0], pages=many[1], width=many[2], stride=many[2], n_held=many[3], out=at(400), count=at(500))
         assert unused(ws=at(600), n=n - 1, **big) == N.HTREE_EWORKSPACE
         assert unused(ws=None, n=n, **big) == N.HTREE_ENULL
-        assert unused(ws=at(1), n=n, **big) == N.HTREE_EOVERLAP and unused(ws=at(500), n=n, **big) == N.HTREE_EOVERLAP
+        assert unused(ws=at(2), n=n, **big) == N.HTREE_EOVERLAP and unused(ws=at(500), n=n, **big) == N.HTREE_EOVERLAP
     for name in ("out", "count"):
         for x in (1, 2, 3):
             assert unused(**{name: at(x)}) == N.HTREE_EOVERLAP
