@@ -252,29 +252,38 @@ struct Pieces {
 __device__ __forceinline__ uint32_t piece_count(const UnusedArgs& a) {
   return ((uint32_t)a.width + kUnusedPiece - 1) / kUnusedPiece * a.B;
 }
-// length(b): of request b
+// length(b): of request b.  False, and nothing is read, if none of them is live.
 template <typename L>
-__device__ __forceinline__ void load_pieces(const UnusedArgs& a, uint32_t p0, L length, Pieces* c) {
+__device__ __forceinline__ bool load_pieces(const UnusedArgs& a, uint32_t p0, L length, Pieces* c) {
   const int lane = threadIdx.x & 63;
   const uint32_t all = piece_count(a);
   uint32_t q = p0 / (uint32_t)a.B, b = p0 - q * a.B;
+  const int32_t* row[kUnusedPieces];
+  int first[kUnusedPieces], live[kUnusedPieces];
+  bool any = false;
 #pragma unroll
   for (int u = 0; u < kUnusedPieces; ++u) {
-    const int32_t* row = a.table + (int64_t)b * a.table_stride;
-    const int live = p0 + u < all ? live_pages(a, length((int)b)) : 0;
-    if (a.width < 4) {
-      c->x[u].v[0] = row[min(lane, a.width - 1)];
-      c->live[u] = live > 0;
-      c->lo[u] = 0, c->hi[u] = lane < live ? 1 : 0;
-    } else {
-      const int mine = (int)q * kUnusedPiece + lane * 4, at = min(mine, a.width - 4);
-      c->x[u] = *(const Entries*)(row + at);
-      c->live[u] = live > (int)q * kUnusedPiece;
-      c->lo[u] = mine - at, c->hi[u] = live - at;
-    }
+    row[u] = a.table + (int64_t)b * a.table_stride;
+    first[u] = (int)q * kUnusedPiece;
+    live[u] = p0 + u < all ? live_pages(a, length((int)b)) : 0;
+    c->live[u] = live[u] > first[u];
+    any |= c->live[u];
     // (past the last piece: that one again)
     if (p0 + u + 1 < all && ++b == (uint32_t)a.B) b = 0, ++q;
   }
+  if (!any) return false;
+#pragma unroll
+  for (int u = 0; u < kUnusedPieces; ++u) {
+    if (a.width < 4) {
+      c->x[u].v[0] = row[u][min(lane, a.width - 1)];
+      c->lo[u] = 0, c->hi[u] = lane < live[u] ? 1 : 0;
+    } else {
+      const int mine = first[u] + lane * 4, at = min(mine, a.width - 4);
+      c->x[u] = *(const Entries*)(row[u] + at);
+      c->lo[u] = mine - at, c->hi[u] = live[u] - at;
+    }
+  }
+  return true;
 }
 // f(page) for the pages that count
 template <typename F>
@@ -357,8 +366,7 @@ __global__ __launch_bounds__(1024) void unused_small_kernel(UnusedArgs a) {
   const uint32_t pieces = piece_count(a);
   for (uint32_t p = __builtin_amdgcn_readfirstlane(wv) * kUnusedPieces; p < pieces; p += 16 * kUnusedPieces) {
     Pieces c;
-    load_pieces(a, p, length, &c);
-    mark_pieces(a, c, mark);
+    if (load_pieces(a, p, length, &c)) mark_pieces(a, c, mark);
   }
   for (int i = tid; i < a.n_held; i += 1024)
     if ((uint32_t)a.held[i] < (uint32_t)a.num_pages) mark(a.held[i]);
@@ -396,8 +404,8 @@ __global__ __launch_bounds__(256) void unused_mark_kernel(UnusedArgs a) {
   const uint32_t p = (blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * kUnusedPieces;
   if (p >= pieces) return;
   Pieces c;
-  load_pieces(a, p, [&](int b) { return a.lens[b]; }, &c);
-  mark_pieces(a, c, [&](int page) { a.flags[page] = 1; });
+  if (load_pieces(a, p, [&](int b) { return a.lens[b]; }, &c))
+    mark_pieces(a, c, [&](int page) { a.flags[page] = 1; });
 }
 
 // bit i: page p0 + i is unused

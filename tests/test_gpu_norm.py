@@ -216,6 +216,24 @@ def test_same_every_run():
         assert all(torch.equal(x, y) for x, y in zip(r, runs[0]))
 
 
+def test_past_32_bits():
+    """More than 2^32 elements: the last rows are those of a call of their own."""
+    rows, H, D = 70000, 250, 256
+    q = torch.randn(1000, H, D, device=DEV).bfloat16().repeat(rows // 1000, 1, 1)
+    k, w = q[:, :1].contiguous(), torch.randn(D, device=DEV)
+    assert q.numel() > 2 ** 32
+    q[-7:].normal_()
+    pos = torch.arange(rows, device=DEV).to(torch.int32) % 500
+    cos, sin = htree_amd.rope_cache(D, 500, 10000.0, DEV)
+    q.requires_grad_()
+    out = htree_amd.head_norm(q, k, w, w, positions=pos, cos=cos, sin=sin)[0]
+    dq, = torch.autograd.grad(out, q, out.detach())
+    last = q.detach()[-7:].clone().requires_grad_()
+    want = htree_amd.head_norm(last, k[-7:], w, w, positions=pos[-7:].contiguous(), cos=cos, sin=sin)[0]
+    assert torch.equal(out[-7:], want)
+    assert torch.equal(dq[-7:], torch.autograd.grad(want, last, want.detach())[0])
+
+
 def test_empty():
     z = lambda *n: torch.zeros(n, device=DEV, requires_grad=True)
     w = z(64)

@@ -278,6 +278,17 @@ def test_strides_and_offsets(dtype):
     check(wide[:, 3:1006], None, tokens, starts, parents, u, d)
 
 
+def test_past_32_bits():
+    """Rows 2^30 entries apart: the last ones lie behind 2^32 of them."""
+    p, q, tokens, starts, parents, u, d = case([3, 6], 1003, "bfloat16", True, True, 6)
+    big = torch.empty(9, 1 << 30, dtype=torch.bfloat16, device=DEV)
+    wide_p, wide_q = big[:, 5:1008], big[:, 1 << 29:(1 << 29) + 1003]
+    wide_p.copy_(p), wide_q.copy_(q)
+    check(wide_p, wide_q, tokens, starts, parents, u, d)
+    check(wide_p, None, tokens, starts, parents, u, d)
+    check_greedy(wide_p, tokens, starts, parents)
+
+
 def test_starts_that_are_no_ranges_touch_nothing_outside():
     p, q, tokens, starts, parents, u, d = case([7, 5, 4], 100, "float32", True, True, 4)
     i32 = lambda x: torch.as_tensor(np.asarray(x, np.int32)).to(DEV)
