@@ -213,12 +213,15 @@ __global__ __launch_bounds__(256) void fork_requests_kernel(ForkArgs a) {
 struct UnusedArgs {
   const int32_t *table, *lens, *held;
   uint8_t* flags;   // [tiles * kUnusedTile] 1: held
-  int32_t* counts;  // [tiles] unused pages of a tile
+  int32_t* counts;  // [tiles] unused pages of a tile, nullptr: each block counts
   int32_t *pages, *count;
   int64_t table_stride;
   int32_t B, width, page_shift, num_pages, n_held, tiles;
 };
 constexpr int kUnusedTile = 4096;        // pages a block counts or lists: 16 a thread
+// Tiles that every block counts for itself: 5 of them 10.1 us (11.4 with a launch
+// that counts), 29 12.8 (12.0, and 2 us more of the host's time), 53 15.5 (12.7).
+constexpr int kUnusedCounted = 32;
 constexpr int kUnusedPiece = 256;        // entries of a row that a wave reads at once, 4 a lane,
 constexpr int kUnusedPieces = 4;         // of so many rows
 // Calls in one launch: pieces, requests and held pages at most, and pages, whose
@@ -431,10 +434,27 @@ __global__ __launch_bounds__(256) void unused_list_kernel(UnusedArgs a) {
   __shared__ int red[4];
   const uint32_t bits = unused_bits(a, (int64_t)blockIdx.x * kUnusedTile + threadIdx.x * 16);
   int before = 0, all = 0;
-  for (int t = threadIdx.x; t < a.tiles; t += 256) {
-    const int n = a.counts[t];
-    all += n;
-    if (t < (int)blockIdx.x) before += n;
+  if (a.counts) {
+    for (int t = threadIdx.x; t < a.tiles; t += 256) {
+      const int n = a.counts[t];
+      all += n;
+      if (t < (int)blockIdx.x) before += n;
+    }
+  } else {
+    // the held ones: their flags' bits, eight tiles in flight
+    for (int t0 = 0; t0 < a.tiles; t0 += 8) {
+      uint4 f[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        f[i] = *(const uint4*)(a.flags + (int64_t)min(t0 + i, a.tiles - 1) * kUnusedTile + threadIdx.x * 16);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int n = t0 + i < a.tiles ? __popc(f[i].x) + __popc(f[i].y) + __popc(f[i].z) + __popc(f[i].w) : 0;
+        all -= n;
+        if (t0 + i < (int)blockIdx.x) before -= n;
+      }
+    }
+    if (threadIdx.x == 0) all += a.num_pages, before += (int)blockIdx.x * kUnusedTile;
   }
   before = block_sum<4>(before, red);
   all = block_sum<4>(all, red);
@@ -619,7 +639,9 @@ extern "C" int htree_unused_pages(int32_t B, int32_t page_size, int32_t num_page
     if (pieces >= 0x7fffff00 || blocks > 0x7fffffff) return HTREE_EUNSUPPORTED;
     hipLaunchKernelGGL(unused_clear_kernel, dim3(a.tiles), dim3(256), 0, s, a.flags, (int64_t)a.tiles * kUnusedTile);
     if (blocks) hipLaunchKernelGGL(unused_mark_kernel, dim3((unsigned)blocks), dim3(256), 0, s, a);
-    hipLaunchKernelGGL(unused_count_kernel, dim3(a.tiles), dim3(256), 0, s, a);
+    // every block of few tiles counts their flags itself: a launch less
+    if (a.tiles <= kUnusedCounted) a.counts = nullptr;
+    else hipLaunchKernelGGL(unused_count_kernel, dim3(a.tiles), dim3(256), 0, s, a);
     hipLaunchKernelGGL(unused_list_kernel, dim3(a.tiles), dim3(256), 0, s, a);
   }
   const hipError_t e = hipGetLastError();

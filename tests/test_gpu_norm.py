@@ -145,6 +145,24 @@ def test_views_and_other_orders():
           gq[:, :, :1].expand(2, 33, 8, 64), gk[:1, :1, :1, :1].expand(2, 33, 2, 64))
 
 
+@pytest.mark.parametrize("dtype", list(DT))
+def test_weights_and_tables_from_anywhere(dtype):
+    """Weights and tables that begin at any element of a larger tensor."""
+    q, k, w, pos, cos, sin, gq, gk = data((50,), 6, 2, 64, dtype, dtype, True, 15)
+    w = [torch.cat([x[:n], x])[n:] for n, x in ((1, w[0]), (3, w[1]))]
+    assert w[0].is_contiguous() and w[0].data_ptr() % 4 != 0 or dtype == "float32"
+    cos, sin = torch.cat([cos.view(-1)[:1], cos.view(-1)])[1:].view_as(cos), torch.cat([sin.view(-1)[:3], sin.view(-1)])[3:].view_as(sin)
+    pos = torch.cat([pos[:1], pos])[1:]
+    plain = htree_amd.head_norm(q, k, *w, positions=pos, cos=cos, sin=sin)
+    leaves = [x.detach().requires_grad_() for x in (q, k, *w)]
+    out = htree_amd.head_norm(*leaves, positions=pos, cos=cos, sin=sin)
+    grads = torch.autograd.grad(out, leaves, (gq, gk))
+    same = [x.detach().clone().requires_grad_() for x in (q, k, *w)]
+    want = htree_amd.head_norm(*same, positions=pos.clone(), cos=cos.clone(), sin=sin.clone())
+    for x, y in zip((*out, *plain, *grads), (*want, *want, *torch.autograd.grad(want, same, (gq, gk)))):
+        assert torch.equal(x, y)
+
+
 def test_rows_without_a_position_are_zero():
     q, k, w, pos, cos, sin, gq, gk = data((9,), 4, 2, 64, "float32", "float32", True, 8)
     pos[::2] = torch.tensor([-1, 500, 2 ** 31 - 1, -2 ** 31, 499], dtype=torch.int32, device=DEV)
