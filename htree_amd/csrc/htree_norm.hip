@@ -330,6 +330,7 @@ extern "C" int htree_head_norm(int32_t dtype, int32_t w_dtype, int32_t rows, int
   a.side[1] = {(const char*)k, nullptr, (char*)k_out, k_weight, k_row * es, k_head * es, 0, 0, H_kv};
   a.positions = positions, a.cs = cos_table, a.sn = sin_table;
   a.items = (int64_t)rows * (H + H_kv);
+  if (a.items * L >= (int64_t)1 << 32) return HTREE_EUNSUPPORTED;  // threads of a grid
   a.rows = rows, a.D = D, a.rope_rows = rope_rows, a.w_f32 = w_dtype == HTREE_F32;
   a.eps = eps, a.inv_d = 1.f / D;
   hipStream_t s = (hipStream_t)stream;

@@ -9,6 +9,7 @@
 namespace htree {
 
 // ----------------------------------------------------------- moving tokens
+constexpr int kMoveMost = (1 << 24) - 1;  // blocks of 256 threads along a grid's first dimension
 constexpr int kMoveLayers = 64;  // layers of a launch: their pointers are its arguments
 // Layers and tokens that a thread reads before it writes the first.  Kept drafts
 // are few tokens of many layers, and to find them takes four loads one after
@@ -529,6 +530,7 @@ extern "C" int htree_copy_pages(const htree_cache* c, int32_t layers, void* cons
   const int rc = move_args(c, layers, k_layers, v_layers, &a.m);
   if (rc) return rc;
   if (n < 0) return HTREE_ESHAPE;
+  if (n > kMoveMost) return HTREE_EUNSUPPORTED;
   if (n == 0 || layers == 0) return HTREE_OK;
   if (!from || !to) return HTREE_ENULL;
   a.from = from, a.to = to, a.tokens = tokens, a.n = n;
@@ -636,7 +638,7 @@ extern "C" int htree_unused_pages(int32_t B, int32_t page_size, int32_t num_page
     a.counts = (int32_t*)(a.flags + (int64_t)a.tiles * kUnusedTile);
     const int64_t pieces = unused_pieces(B, table_width);
     const int64_t blocks = (pieces + 4 * kUnusedPieces - 1) / (4 * kUnusedPieces) + ((int64_t)n_held + 255) / 256;
-    if (pieces >= 0x7fffff00 || blocks > 0x7fffffff) return HTREE_EUNSUPPORTED;
+    if (pieces >= 0x7fffff00 || blocks > kMoveMost) return HTREE_EUNSUPPORTED;
     hipLaunchKernelGGL(unused_clear_kernel, dim3(a.tiles), dim3(256), 0, s, a.flags, (int64_t)a.tiles * kUnusedTile);
     if (blocks) hipLaunchKernelGGL(unused_mark_kernel, dim3((unsigned)blocks), dim3(256), 0, s, a);
     // every block of few tiles counts their flags itself: a launch less

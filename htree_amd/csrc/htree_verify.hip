@@ -615,7 +615,7 @@ static int verify_parts(int32_t B, int32_t V, bool drawn) {
 // 64 requests of 9 rows, 128000 16-bit entries (147 MB): 38 us at once, 67 one
 // after another; 256 of 13 rows, 32768 fp32 (436 MB): 80 and 67.
 static bool verify_all(int32_t dtype, int32_t rows, int32_t V) {
-  return (int64_t)rows * V * (dtype == HTREE_F32 ? 4 : 2) <= kVerifyAll;
+  return (int64_t)rows * V * (dtype == HTREE_F32 ? 4 : 2) <= kVerifyAll && rows < 1 << 21;  // (blocks of a grid)
 }
 
 }  // namespace htree

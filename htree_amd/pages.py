@@ -20,6 +20,7 @@ from .cache import INT32, MAX_REQUESTS, _describe, _ints, check_table, no_deriva
 
 Caches = Union[torch.Tensor, Sequence[torch.Tensor]]
 MAX_LAYERS = 65535
+MAX_COPIES = 1 << 24
 
 
 class Forked(NamedTuple):
@@ -127,7 +128,7 @@ def copy_pages(k_caches: Caches, v_caches: Caches, copy_from: torch.Tensor, copy
     c, layers, k_ptr, v_ptr, dev = _layers("copy_pages", k_caches, v_caches)
     assert copy_from.dim() == 1, "copy_from must be int32 [n]"
     n = copy_from.shape[0]
-    assert n < INT32, f"pages to copy must be below 2^31, got {n}"
+    assert n < MAX_COPIES, f"pages to copy must be less than {MAX_COPIES}, got {n}"
     _ints(copy_from, "copy_from", n, dev)
     _ints(copy_to, "copy_to", n, dev)
     if copy_tokens is not None:

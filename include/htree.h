@@ -452,7 +452,7 @@ int htree_fork_requests(int32_t B, int32_t N, int32_t page_size, int32_t num_pag
 
 /* The first tokens[i] tokens (NULL: all) of page from[i] to page to[i], in the
  * caches of `layers` layers.  Pages outside the cache: nothing.  No page of
- * `to` is in `from` too, nor twice in `to`. */
+ * `to` is in `from` too, nor twice in `to`.  n is below 2^24. */
 int htree_copy_pages(const htree_cache* c, int32_t layers, void* const* k_layers,
                      void* const* v_layers, int32_t n, const int32_t* from, const int32_t* to,
                      const int32_t* tokens, void* stream);
@@ -476,7 +476,8 @@ int htree_unused_pages(int32_t B, int32_t page_size, int32_t num_pages, int32_t 
  * are zero.  Everything is fp32, rounded once.  H or H_kv may be 0.  Outputs
  * share no memory with the inputs.
  * HTREE_EUNSUPPORTED: D above 256 or not in whole 16-byte pieces, strides or
- * bases off 16 bytes, rows (H + H_kv) past 31 bits. */
+ * bases off 16 bytes, rows (H + H_kv) past 31 bits or more than a grid holds
+ * (2^32 threads, up to 32 of them a head). */
 int htree_head_norm(int32_t dtype, int32_t w_dtype, int32_t rows, int32_t H, int32_t H_kv,
                     int32_t D, float eps, const void* q, int64_t q_row, int64_t q_head,
                     const void* k, int64_t k_row, int64_t k_head, const void* q_weight,

@@ -60,6 +60,7 @@ def test_verify_refusals():
     greedy = dict(u=None, d=None)
     assert need(2, 100, 0, 1) == (N.HTREE_OK, 24) and need(2, 1 << 20, 0, 1, rows=65) == (N.HTREE_OK, 0)
     assert need(2, 1 << 20, 0, 1, rows=128, dtype=1) == (N.HTREE_OK, 512)
+    assert need(2, 8, 0, 1, rows=1 << 21) == (N.HTREE_OK, 0)  # more blocks than a grid holds, at once
     assert verify(**greedy, q=at(20), q_row=100) == N.HTREE_ESHAPE and need(2, 100, 1, 1)[0] == N.HTREE_ESHAPE
     assert verify(**greedy, p=None, ws=at(9), n=24) == N.HTREE_ENULL
     assert verify(**greedy) == N.HTREE_ENULL and verify(**greedy, ws=at(9), n=23) == N.HTREE_EWORKSPACE
@@ -101,6 +102,7 @@ def test_moving_refusals():
         assert keep(**{name: None}) == N.HTREE_ENULL
     assert keep(B=0, slots=None) == N.HTREE_OK and keep(rows=0, slots=None) == N.HTREE_OK
     assert copy(n=-1) == N.HTREE_ESHAPE
+    assert copy(n=1 << 24) == N.HTREE_EUNSUPPORTED  # more blocks than a grid holds
     assert copy(frm=None) == N.HTREE_ENULL and copy(to=None) == N.HTREE_ENULL
     assert copy(n=0, frm=None) == N.HTREE_OK
 
@@ -185,6 +187,7 @@ def test_norm_refusals(f):
 
 
 def test_norm_backward_refusals():
+    assert norm(dtype=0, rows=1 << 22, H=32, D=256, qr=8192) == N.HTREE_EUNSUPPORTED  # more threads than a grid holds
     assert norm_bwd(dy=None) == N.HTREE_ENULL
     assert norm_bwd(ws=None) == N.HTREE_ENULL
     need = size("htree_head_norm_backward_workspace_bytes", 64)[1]
