@@ -77,7 +77,8 @@ def verify_drafts(target_probs: torch.Tensor, tokens: torch.Tensor, starts: torc
     Sums are 64-bit.  Entries that are no positive finite numbers count as
     zero, and so do uniforms and draws that are not positive.  A request
     without rows keeps 0 and has next token -1; without any mass (greedily: any
-    entry above -infinity) the next token is -1 too.  Of a request the first 1024 rows are looked at.
+    entry above -infinity) the next token is -1 too.  Of a request the first
+    MAX_DRAFT_ROWS rows are looked at.
 
     Returns Verified (`out`: written there; no overlap with the inputs).
     Nothing synchronises; the numbers are the same every run."""
