@@ -109,7 +109,9 @@ def verify_drafts(target_probs: torch.Tensor, tokens: torch.Tensor, starts: torc
     if parents is not None:
         _ints(parents, "parents", rows, dev)
     if out is None:
-        out = Verified(starts.new_empty(B), torch.empty_like(tokens, dtype=torch.int32), tokens.new_empty(B))
+        like = draws if draws is not None else starts[1:]
+        out = Verified(torch.empty_like(like, dtype=torch.int32), torch.empty_like(tokens, dtype=torch.int32),
+                       torch.empty_like(like, dtype=torch.int64))
     else:
         _ints(out.kept, "out.kept", B, dev)
         _ints(out.path, "out.path", rows, dev)

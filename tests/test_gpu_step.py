@@ -237,3 +237,39 @@ def test_on_another_stream():
     assert v.kept.tolist() == [1] and 0 <= int(v.next_tokens) < 50000
     r = x * (x.square().mean(-1, keepdim=True) + 1e-6).rsqrt() * w
     assert float((y - r).abs().max()) < 1e-4
+
+
+def test_two_streams_at_once():
+    """Calls that overlap, each with workspaces of its own: what they give is
+    what they give one after another."""
+    g = torch.Generator(device=DEV).manual_seed(9)
+    jobs = []
+    for i in range(2):
+        p, q = (torch.softmax(4 * torch.randn(24, 140001, generator=g, device=DEV), -1) for _ in range(2))
+        toks = torch.randint(140001, (24,), generator=g, device=DEV)
+        u, d = torch.rand(24, generator=g, device=DEV), torch.rand(4, generator=g, device=DEV)
+        table = torch.randint(300000, (600, 900), generator=g, device=DEV).int()
+        lens = torch.randint(900 * PAGE, (600,), generator=g, device=DEV).int()
+        x = [torch.randn(3000, h, 128, generator=g, device=DEV).bfloat16().requires_grad_() for h in (16, 2)]
+        w = [torch.randn(128, generator=g, device=DEV).requires_grad_() for _ in range(2)]
+        dy = [torch.randn(3000, h, 128, generator=g, device=DEV).bfloat16() for h in (16, 2)]
+        jobs.append((p, q, toks, u, d, table, lens, x, w, dy))
+
+    def run(p, q, toks, u, d, table, lens, x, w, dy):
+        out = [*htree_amd.verify_drafts(p, toks, i32([0, 6, 12, 18, 24]), u, d, draft_probs=q),
+               *htree_amd.verify_drafts(p, toks, i32([0, 6, 12, 18, 24])), *htree_amd.unused_pages(table, lens, PAGE, 300000)]
+        y = htree_amd.head_norm(*x, *w)
+        return out + [*y, *torch.autograd.grad(y, [*x, *w], dy)]
+
+    want = [run(*j) for j in jobs]
+    streams = [torch.cuda.Stream() for _ in jobs]
+    torch.cuda.synchronize()
+    for _ in range(4):
+        got = []
+        for s, j in zip(streams, jobs):
+            with torch.cuda.stream(s):
+                got.append([run(*j) for _ in range(3)])
+        torch.cuda.synchronize()
+        for runs, y in zip(got, want):
+            for r in runs:
+                assert all(torch.equal(a, b) for a, b in zip(r, y))
