@@ -194,7 +194,8 @@ def check_unused(table, lens, page, pages, held=None):
 
 @pytest.mark.parametrize("B,width,page,pages", [(1, 1, 16, 1), (3, 20, 16, 100), (7, 300, 64, 4096), (7, 300, 64, 4097),
                                                 (64, 1100, 16, 100000), (4096, 3, 16, 20000), (2, 40000, 16, 70001),
-                                                (300, 3000, 16, 9000), (0, 5, 16, 33), (4, 5, 1, 16), (5, 0, 16, 50), (300, 40, 16, 1 << 21)])
+                                                (300, 3000, 16, 9000), (20, 1000, 16, 262144), (3, 2000, 64, 250001), (256, 200, 16, 131073),
+                                                (0, 5, 16, 33), (4, 5, 1, 16), (5, 0, 16, 50), (300, 40, 16, 1 << 21)])
 def test_unused_pages(B, width, page, pages):
     for seed in range(2):
         g = np.random.default_rng(seed + width)
