@@ -224,7 +224,10 @@ constexpr int kUnusedTile = 4096;        // pages a block counts or lists: 16 a 
 // that counts), 29 12.8 (12.0, and 2 us more of the host's time), 53 15.5 (12.7).
 constexpr int kUnusedCounted = 32;
 constexpr int kUnusedPiece = 256;        // entries of a row that a wave reads at once, 4 a lane,
-constexpr int kUnusedPieces = 4;         // of so many rows
+// of so many rows: four in the one launch (64 requests of 1024 entries 13.1 us, with
+// two 13.5; 256 of 250 13.8 and 14.7), two in unused_mark_kernel (the call's launches
+// together, 512 requests of 256 11.8 us, with four 12.7; 300 of 63 9.3 and 10.0)
+constexpr int kUnusedPieces = 4, kUnusedMark = 2;
 // Calls in one launch: pieces, requests and held pages at most, and pages, whose
 // bits fill 32 KB of LDS.  Against the other form's four launches: 64 pieces 6.9
 // us (11.7), 128 9.2 (11.4), 256 12.4 to 14 (10 to 12.5, and 7 us more of the
@@ -241,32 +244,33 @@ __device__ __forceinline__ int live_pages(const UnusedArgs& a, int len) {
   return (int)min(table_pages(max(len, 0), a.page_shift), (int64_t)a.width);
 }
 
-// Four pieces of the table, from piece p0 on: piece p is the (p / B)-th 256
+// N pieces of the table, from piece p0 on: piece p is the (p / B)-th 256
 // entries of request p % B, so that first pieces, which have most of the live
 // entries, come first.  Reads that would pass a row's end start earlier; what the
 // lanes in front have is not marked again, 64 lanes would wait for one word: of a
 // lane's four entries those from `lo` to before `hi` count.  (Rows of less than
 // four entries: one a lane.)
+template <int N>
 struct Pieces {
-  Entries x[kUnusedPieces];
-  int lo[kUnusedPieces], hi[kUnusedPieces];
-  bool live[kUnusedPieces];  // any of the piece
+  Entries x[N];
+  int lo[N], hi[N];
+  bool live[N];  // any of the piece
 };
 // (less than 2^31 of them)
 __device__ __forceinline__ uint32_t piece_count(const UnusedArgs& a) {
   return ((uint32_t)a.width + kUnusedPiece - 1) / kUnusedPiece * a.B;
 }
 // length(b): of request b.  False, and nothing is read, if none of them is live.
-template <typename L>
-__device__ __forceinline__ bool load_pieces(const UnusedArgs& a, uint32_t p0, L length, Pieces* c) {
+template <int N, typename L>
+__device__ __forceinline__ bool load_pieces(const UnusedArgs& a, uint32_t p0, L length, Pieces<N>* c) {
   const int lane = threadIdx.x & 63;
   const uint32_t all = piece_count(a);
   uint32_t q = p0 / (uint32_t)a.B, b = p0 - q * a.B;
-  const int32_t* row[kUnusedPieces];
-  int first[kUnusedPieces], live[kUnusedPieces];
+  const int32_t* row[N];
+  int first[N], live[N];
   bool any = false;
 #pragma unroll
-  for (int u = 0; u < kUnusedPieces; ++u) {
+  for (int u = 0; u < N; ++u) {
     row[u] = a.table + (int64_t)b * a.table_stride;
     first[u] = (int)q * kUnusedPiece;
     live[u] = p0 + u < all ? live_pages(a, length((int)b)) : 0;
@@ -277,7 +281,7 @@ __device__ __forceinline__ bool load_pieces(const UnusedArgs& a, uint32_t p0, L 
   }
   if (!any) return false;
 #pragma unroll
-  for (int u = 0; u < kUnusedPieces; ++u) {
+  for (int u = 0; u < N; ++u) {
     if (a.width < 4) {
       c->x[u].v[0] = row[u][min(lane, a.width - 1)];
       c->lo[u] = 0, c->hi[u] = lane < live[u] ? 1 : 0;
@@ -290,10 +294,10 @@ __device__ __forceinline__ bool load_pieces(const UnusedArgs& a, uint32_t p0, L 
   return true;
 }
 // f(page) for the pages that count
-template <typename F>
-__device__ __forceinline__ void mark_pieces(const UnusedArgs& a, const Pieces& c, F f) {
+template <int N, typename F>
+__device__ __forceinline__ void mark_pieces(const UnusedArgs& a, const Pieces<N>& c, F f) {
 #pragma unroll
-  for (int u = 0; u < kUnusedPieces; ++u)
+  for (int u = 0; u < N; ++u)
     if (c.live[u])
 #pragma unroll
       for (int e = 0; e < 4; ++e)
@@ -369,7 +373,7 @@ __global__ __launch_bounds__(1024) void unused_small_kernel(UnusedArgs a) {
   auto length = [&](int b) { return __builtin_amdgcn_readfirstlane(lens[b]); };
   const uint32_t pieces = piece_count(a);
   for (uint32_t p = __builtin_amdgcn_readfirstlane(wv) * kUnusedPieces; p < pieces; p += 16 * kUnusedPieces) {
-    Pieces c;
+    Pieces<kUnusedPieces> c;
     if (load_pieces(a, p, length, &c)) mark_pieces(a, c, mark);
   }
   for (int i = tid; i < a.n_held; i += 1024)
@@ -393,21 +397,21 @@ __global__ __launch_bounds__(256) void unused_clear_kernel(uint8_t* flags, int64
   if (i < n) *(uint4*)(flags + i) = make_uint4(0, 0, 0, 0);
 }
 
-// A wave four pieces of the table (spread over the dies as pieces are numbered: a
+// A wave two pieces of the table (spread over the dies as pieces are numbered: a
 // die that had all the first ones took six times as long); the last blocks mark
 // the held pages.  Whoever holds a page writes the same 1: no atomics.
-// 1.3M entries, each a store to a line of its own, 12 us; all four launches 24.
+// 1.3M entries, each a store to a line of its own, 12 us; all four launches 20.
 __global__ __launch_bounds__(256) void unused_mark_kernel(UnusedArgs a) {
-  const uint32_t pieces = piece_count(a), blocks = (pieces + 4 * kUnusedPieces - 1) / (4 * kUnusedPieces);
+  const uint32_t pieces = piece_count(a), blocks = (pieces + 4 * kUnusedMark - 1) / (4 * kUnusedMark);
   if (blockIdx.x >= blocks) {
     const int64_t i = (int64_t)(blockIdx.x - blocks) * 256 + threadIdx.x;
     const int page = i < a.n_held ? cache_page(a.held[i], a.num_pages) : -1;
     if (page >= 0) a.flags[page] = 1;
     return;
   }
-  const uint32_t p = (blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * kUnusedPieces;
+  const uint32_t p = (blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * kUnusedMark;
   if (p >= pieces) return;
-  Pieces c;
+  Pieces<kUnusedMark> c;
   if (load_pieces(a, p, [&](int b) { return a.lens[b]; }, &c))
     mark_pieces(a, c, [&](int page) { a.flags[page] = 1; });
 }
@@ -637,7 +641,7 @@ extern "C" int htree_unused_pages(int32_t B, int32_t page_size, int32_t num_page
     a.flags = (uint8_t*)workspace;
     a.counts = (int32_t*)(a.flags + (int64_t)a.tiles * kUnusedTile);
     const int64_t pieces = unused_pieces(B, table_width);
-    const int64_t blocks = (pieces + 4 * kUnusedPieces - 1) / (4 * kUnusedPieces) + ((int64_t)n_held + 255) / 256;
+    const int64_t blocks = (pieces + 4 * kUnusedMark - 1) / (4 * kUnusedMark) + ((int64_t)n_held + 255) / 256;
     if (pieces >= 0x7fffff00 || blocks > kMoveMost) return HTREE_EUNSUPPORTED;
     hipLaunchKernelGGL(unused_clear_kernel, dim3(a.tiles), dim3(256), 0, s, a.flags, (int64_t)a.tiles * kUnusedTile);
     if (blocks) hipLaunchKernelGGL(unused_mark_kernel, dim3((unsigned)blocks), dim3(256), 0, s, a);
