@@ -396,12 +396,14 @@ __device__ __forceinline__ Request open_request(const VerifyArgs& a, int b, int 
   const int tid = threadIdx.x;
   const int s0 = min(max(a.starts[b], 0), a.rows), s1 = min(max(a.starts[b + 1], s0), a.rows);
   if (part == 0) {
-    for (int i = s0 + tid; i < s1; i += kVerifyThreads) a.path[i] = i == s0 ? 0 : -1;
+    // (unsigned: behind the last of 2^31 - 1 rows a signed one would begin again below zero)
+    const uint32_t first = s0, last = s1, rows = a.rows;
+    for (uint32_t i = first + tid; i < last; i += kVerifyThreads) a.path[i] = i == first ? 0 : -1;
     // rows of no request
     if (b == 0)
-      for (int i = tid; i < s0; i += kVerifyThreads) a.path[i] = -1;
+      for (uint32_t i = tid; i < first; i += kVerifyThreads) a.path[i] = -1;
     if (b == a.B - 1)
-      for (int i = s1 + tid; i < a.rows; i += kVerifyThreads) a.path[i] = -1;
+      for (uint32_t i = last + tid; i < rows; i += kVerifyThreads) a.path[i] = -1;
     if (s0 == s1 && tid == 0) {
       a.kept[b] = 0, a.next[b] = -1;
       if (a.parts > 1) a.ends[b].row = -1;
