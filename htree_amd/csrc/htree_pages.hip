@@ -109,12 +109,12 @@ __global__ __launch_bounds__(256) void keep_drafts_kernel(KeepArgs a) {
   const MoveColumn c = move_column(a.m, piece);
   const int64_t slots = (int64_t)a.m.num_pages << a.m.page_shift;
   const int64_t mask = ((int64_t)1 << a.m.page_shift) - 1;
-  for (int j0 = 0; j0 < kept; j0 += kKeepTokens) {
+  for (uint32_t j0 = 0; j0 < (uint32_t)max(kept, 0); j0 += kKeepTokens) {
     int64_t from[kKeepTokens], to[kKeepTokens];
     bool any = false;
 #pragma unroll
     for (int i = 0; i < kKeepTokens; ++i) {
-      const int j = j0 + i;
+      const int j = (int)j0 + i;
       from[i] = c.at, to[i] = -1;
       if (j >= kept) continue;
       const int p = a.path[s0 + j];
@@ -197,8 +197,8 @@ __global__ __launch_bounds__(256) void fork_requests_kernel(ForkArgs a) {
     const bool own = fresh[i + 1] > fresh[i];
     const int page = own && fresh[i] < a.n_free ? cache_page(a.free_pages[fresh[i]], a.num_pages) : -1;
     const int32_t* row = a.table + (int64_t)s * a.table_stride;
-    for (int j = tid; j < a.width; j += 256)
-      a.out_table[(int64_t)i * a.out_stride + j] = j >= live ? -1 : own && j == full ? page : row[j];
+    for (uint32_t j = tid; j < (uint32_t)a.width; j += 256)  // (a width below 2^31 and 256 pass it)
+      a.out_table[(int64_t)i * a.out_stride + j] = j >= live ? -1 : own && (int)j == full ? page : row[j];
     if (tid == 0) {
       a.out_lens[i] = len;
       const int old = own ? cache_page(row[full], a.num_pages) : -1;
