@@ -5,6 +5,7 @@
 #include "htree_cache_index.h"
 #include "htree_cache_scan.h"
 #include "htree_common.h"
+#include "htree_layers.h"
 
 namespace htree {
 
@@ -489,6 +490,21 @@ static int move_args(const htree_cache* c, int32_t layers, void* const* k, void*
   return HTREE_OK;
 }
 
+// HTREE_EOVERLAP where a piece of a layer is another's too, or a list's: blocks
+// would write what others read.
+template <int N>
+static int moves_apart(const htree_cache* c, const MoveArgs& m, int32_t layers, void* const* k, void* const* v,
+                       const Range (&lists)[N]) {
+  auto layer = [&](int64_t run, int64_t page, int64_t token, int64_t head) {
+    Runs r;
+    r.at = 0, r.run = run;
+    r.add(c->num_pages, page), r.add(c->page_size, token), r.add(c->H_kv, head);
+    return r;
+  };
+  return layers_apart(layer(m.k_pieces * 16, m.k_page, m.k_token, m.k_head),
+                      layer(m.v_pieces * 16, m.v_page, m.v_token, m.v_head), layers, k, v, lists, N);
+}
+
 // runs f(blocks in y) for 64 layers at a time, `by` of them a block
 template <typename F>
 static int by_layers(int32_t layers, void* const* k, void* const* v, int by, MoveArgs* m, F f) {
@@ -517,6 +533,8 @@ extern "C" int htree_keep_drafts(const htree_cache* c, int32_t layers, void* con
   if (B > kCacheMaxRequests) return HTREE_EUNSUPPORTED;
   if (B == 0 || rows == 0 || layers == 0) return HTREE_OK;
   if (!slots || !starts || !path || !kept) return HTREE_ENULL;
+  const Range lists[4] = {{slots, rows * 8ll}, {starts, (B + 1) * 4ll}, {path, rows * 4ll}, {kept, B * 4ll}};
+  if (const int shared = moves_apart(c, a.m, layers, k_layers, v_layers, lists)) return shared;
   a.slots = slots, a.starts = starts, a.path = path, a.kept = kept, a.rows = rows;
   const unsigned threads = a.m.pieces >= 256 ? 256 : (a.m.pieces + 63) / 64 * 64;
   const unsigned z = (a.m.pieces + threads - 1) / threads;
@@ -537,6 +555,8 @@ extern "C" int htree_copy_pages(const htree_cache* c, int32_t layers, void* cons
   if (n > kMoveMost) return HTREE_EUNSUPPORTED;
   if (n == 0 || layers == 0) return HTREE_OK;
   if (!from || !to) return HTREE_ENULL;
+  const Range lists[3] = {{from, n * 4ll}, {to, n * 4ll}, {tokens, tokens ? n * 4ll : 0}};
+  if (const int shared = moves_apart(c, a.m, layers, k_layers, v_layers, lists)) return shared;
   a.from = from, a.to = to, a.tokens = tokens, a.n = n;
   a.columns = a.m.pieces < 256 ? a.m.pieces : 256;
   // so many blocks that a thread reads its tokens at once, up to 16 a page

@@ -4,8 +4,9 @@ that no request holds, for the next step's page_tables.
 
 Caches are given for one layer, k_caches [pages, page_size, H_kv, K] as
 cache.py has it, or for all layers at once: one tensor [layers, pages, ...]
-or a sequence of a tensor each, alike in sizes and strides.  All layers move
-in one launch.  Nothing here synchronises."""
+or a sequence of a tensor each, alike in sizes and strides.  They may lie in one
+buffer, in any order, but no two entries in the same place.  All layers move in
+one launch.  Nothing here synchronises."""
 from __future__ import annotations
 
 import ctypes
@@ -21,6 +22,7 @@ from .cache import INT32, MAX_REQUESTS, _describe, _ints, check_table, no_deriva
 Caches = Union[torch.Tensor, Sequence[torch.Tensor]]
 MAX_LAYERS = 65535
 MAX_COPIES = 1 << 24
+_SHARED = "each layer's keys and values must have memory of their own, apart from the lists, and not be expanded"
 
 
 class Forked(NamedTuple):
@@ -115,6 +117,7 @@ def keep_drafts(k_caches: Caches, v_caches: Caches, slots: torch.Tensor, starts:
     rc = N.launch(N.lib().htree_keep_drafts, dev, c, layers, k_ptr.buffer_info()[0], v_ptr.buffer_info()[0], B, rows, slots.data_ptr(),
                   starts.data_ptr(), path.data_ptr(), kept.data_ptr())
     if rc:
+        assert rc != N.HTREE_EOVERLAP, _SHARED
         N.check(rc, "htree_keep_drafts")
 
 
@@ -136,6 +139,7 @@ def copy_pages(k_caches: Caches, v_caches: Caches, copy_from: torch.Tensor, copy
     rc = N.launch(N.lib().htree_copy_pages, dev, c, layers, k_ptr.buffer_info()[0], v_ptr.buffer_info()[0], n,
                   copy_from.data_ptr(), copy_to.data_ptr(), N.address(copy_tokens))
     if rc:
+        assert rc != N.HTREE_EOVERLAP, _SHARED
         N.check(rc, "htree_copy_pages")
 
 

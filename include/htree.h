@@ -425,7 +425,10 @@ int htree_verify_drafts(int32_t dtype, int32_t B, int32_t rows, int32_t V, const
  * the caches of `layers` layers (host arrays of device pointers; c describes
  * each): what is in slot slots[starts[b] + path[starts[b] + j]] goes to slot
  * slots[starts[b] + j], for j < kept[b].  path ascends (path[j] >= j); entries
- * that do not are left out, and so are slots outside the cache. */
+ * that do not are left out, and so are slots outside the cache.
+ * HTREE_EOVERLAP: two entries of the caches (of a layer, of two, of keys and
+ * values) share memory, or an entry and a list; gaps between entries may hold
+ * others. */
 int htree_keep_drafts(const htree_cache* c, int32_t layers, void* const* k_layers,
                       void* const* v_layers, int32_t B, int32_t rows, const int64_t* slots,
                       const int32_t* starts, const int32_t* path, const int32_t* kept,
@@ -452,7 +455,8 @@ int htree_fork_requests(int32_t B, int32_t N, int32_t page_size, int32_t num_pag
 
 /* The first tokens[i] tokens (NULL: all) of page from[i] to page to[i], in the
  * caches of `layers` layers.  Pages outside the cache: nothing.  No page of
- * `to` is in `from` too, nor twice in `to`.  n is below 2^24. */
+ * `to` is in `from` too, nor twice in `to`.  n is below 2^24.
+ * HTREE_EOVERLAP: as htree_keep_drafts. */
 int htree_copy_pages(const htree_cache* c, int32_t layers, void* const* k_layers,
                      void* const* v_layers, int32_t n, const int32_t* from, const int32_t* to,
                      const int32_t* tokens, void* stream);
