@@ -56,9 +56,10 @@ def verify_drafts(target_probs: torch.Tensor, tokens: torch.Tensor, starts: torc
     (float32, bfloat16 or float16; a row sums to one).  A kept row's drafts
     are tried in order, with T the target's probabilities there and S = 1:
       with draft_probs [rows, V], the drafter's probabilities after each row,
-        from which its drafts were drawn one by one: draft c of token x is
-        accepted if uniforms[c] S q(x) < T(x); a rejected one leaves
-        T = max(T - S q, 0) and S = sum T to the next;
+        from which its drafts were drawn independently, with replacement (one
+        token may come twice): draft c of token x is accepted if
+        uniforms[c] S q(x) < T(x); a rejected one leaves T = max(T - S q, 0)
+        and S = sum T to the next;
       without them (drafts that were not drawn, the likeliest for instance):
         accepted if uniforms[c] S < T(x); a rejected one leaves T(x) = 0, and
         S less what T(x) was.
