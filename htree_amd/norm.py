@@ -120,8 +120,9 @@ def head_norm(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tensor]
     (their squares are summed).  D is at most 256, in whole 16-byte pieces;
     inputs at other steps than 16 bytes are copied first, and so are those
     whose leading dims are no one step apart.  Rows times heads are below 2^31,
-    and times the lanes that a head takes (D / 8 of fp32, D / 16 else, the next
-    power of two) below 2^32.  Returns contiguous tensors.
+    and times the lanes that a head takes below 2^32: the least power of two of
+    at least D / 8 (fp32; D / 16 else), or D / 4 (D / 8) where half a head is no
+    whole 16-byte pieces.  Returns contiguous tensors.
 
     Gradients of q, k and the weights: dx = r (g - x r^2 mean(g x)) with g the
     output's gradient rotated back, times the weight; the weights' are summed

@@ -481,7 +481,8 @@ int htree_unused_pages(int32_t B, int32_t page_size, int32_t num_pages, int32_t 
  * share no memory with the inputs.
  * HTREE_EUNSUPPORTED: D above 256 or not in whole 16-byte pieces, strides or
  * bases off 16 bytes, rows (H + H_kv) past 31 bits or more than a grid holds
- * (2^32 threads, up to 32 of them a head). */
+ * (2^32 threads; a head takes the least power of two of at least D / 8, fp32, or
+ * D / 16; D / 4 or D / 8 where half a head is no whole 16-byte pieces). */
 int htree_head_norm(int32_t dtype, int32_t w_dtype, int32_t rows, int32_t H, int32_t H_kv,
                     int32_t D, float eps, const void* q, int64_t q_row, int64_t q_head,
                     const void* k, int64_t k_row, int64_t k_head, const void* q_weight,
