@@ -42,7 +42,9 @@ def verify_drafts(target_probs: torch.Tensor, tokens: torch.Tensor, starts: torc
                   draft_probs: Optional[torch.Tensor] = None, parents: Optional[torch.Tensor] = None,
                   out: Optional[Verified] = None) -> Verified:
     """Accepts or rejects drafted tokens so that what is kept is distributed
-    as the target's own tokens would be.
+    as the target's own tokens would be.  (Not so for siblings drawn without
+    replacement, each from what the ones before it left of draft_probs: those
+    are neither of the two kinds below.)
 
     Rows starts[b] .. starts[b + 1] - 1 (int32 [B + 1]) are request b's new
     tokens (tokens, int64 [rows]), as page_tables and draft_attention take

@@ -393,8 +393,9 @@ int htree_draft_attention(const htree_cache* c, int32_t B, int32_t rows, int32_t
  * smaller one of the request; other rows are never kept, nor is anything
  * drafted after them.  At a kept row its drafts are tried in order, T being
  * the target's probabilities there, S = 1:
- *   with draft_probs (each drawn from draft_probs' row on its own): accepted
- *     if uniforms[c] S q(token) < T(token), else T = max(T - S q, 0), S = sum T
+ *   with draft_probs (each drawn from draft_probs' row independently of its
+ *     siblings, so with replacement): accepted if
+ *     uniforms[c] S q(token) < T(token), else T = max(T - S q, 0), S = sum T
  *   without: accepted if uniforms[c] S < T(token), else T(token) = 0 and
  *     S -= T(token)
  * An accepted one is kept and the walk goes on there.  Where none is, the next
