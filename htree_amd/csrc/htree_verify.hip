@@ -6,7 +6,7 @@
 // (p at first) and S its sum (1 at first), child c of token x is accepted if
 // u_c S q(x) < T(x); a rejected one takes q's mass away, T <- max(T - S q, 0),
 // which is max(p - a q, 0) with a the sum of the S so far.  Without a drafter's
-// probabilities a draft is what it is, q = 1 at its token: accepted if
+// probabilities a draft, however it was chosen, has q = 1 at its token: accepted if
 // u_c S < p(x), a rejected one takes its token away.  The walk goes on at the
 // accepted child; where none is, the next token is drawn from T.
 //

@@ -42,9 +42,7 @@ def verify_drafts(target_probs: torch.Tensor, tokens: torch.Tensor, starts: torc
                   draft_probs: Optional[torch.Tensor] = None, parents: Optional[torch.Tensor] = None,
                   out: Optional[Verified] = None) -> Verified:
     """Accepts or rejects drafted tokens so that what is kept is distributed
-    as the target's own tokens would be.  (Not so for siblings drawn without
-    replacement, each from what the ones before it left of draft_probs: those
-    are neither of the two kinds below.)
+    as the target's own tokens would be.
 
     Rows starts[b] .. starts[b + 1] - 1 (int32 [B + 1]) are request b's new
     tokens (tokens, int64 [rows]), as page_tables and draft_attention take
@@ -62,9 +60,10 @@ def verify_drafts(target_probs: torch.Tensor, tokens: torch.Tensor, starts: torc
         token may come twice): draft c of token x is accepted if
         uniforms[c] S q(x) < T(x); a rejected one leaves T = max(T - S q, 0)
         and S = sum T to the next;
-      without them (drafts that were not drawn, the likeliest for instance):
-        accepted if uniforms[c] S < T(x); a rejected one leaves T(x) = 0, and
-        S less what T(x) was.
+      without them (drafts chosen in any way, the likeliest for instance or
+        siblings drawn without replacement, for which draft_probs would give
+        another distribution): accepted if uniforms[c] S < T(x); a rejected one
+        leaves T(x) = 0, and S less what T(x) was.
     An accepted draft is kept and its own drafts follow.  Where none is
     accepted, or there are none, the next token is drawn from T: the first
     whose cumulative T passes draws[b] sum T (if nothing is left of T, from

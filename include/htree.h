@@ -396,8 +396,8 @@ int htree_draft_attention(const htree_cache* c, int32_t B, int32_t rows, int32_t
  *   with draft_probs (each drawn from draft_probs' row independently of its
  *     siblings, so with replacement): accepted if
  *     uniforms[c] S q(token) < T(token), else T = max(T - S q, 0), S = sum T
- *   without: accepted if uniforms[c] S < T(token), else T(token) = 0 and
- *     S -= T(token)
+ *   without (drafts chosen in any way): accepted if uniforms[c] S < T(token),
+ *     else T(token) = 0 and S -= T(token)
  * An accepted one is kept and the walk goes on there.  Where none is, the next
  * token is the first whose cumulative T passes draws[b] sum T (T: the target's
  * probabilities if nothing is left of them).  Sums are fp64.  Entries that are
