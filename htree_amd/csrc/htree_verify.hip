@@ -28,8 +28,7 @@ constexpr int kVerifySteps = 4;      // steps in a range, at least; of 16-bit ty
 
 // Few requests over a large vocabulary: `parts` blocks share a request's sums.
 constexpr int kVerifyParts = 4;        // at most: their waves' sums fill a wave
-constexpr int kVerifySplit = 1 << 17;  // elements of a row of p (and q) from which on they do,
-constexpr int kVerifyPart = 1 << 14;   // and that a part has at least
+constexpr int kVerifySplit = 1 << 17;  // elements of a row of p (and q) from which on they do
 constexpr int kVerifyFull = 256;       // blocks that fill the GPU
 constexpr int64_t kVerifyAll = 1 << 28;  // bytes of a call whose rows are all searched, greedily
 
@@ -607,9 +606,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_greedy_kernel(VerifyArg
 static int verify_parts(int32_t B, int32_t V, bool drawn) {
   const int64_t all = (int64_t)V * (drawn ? 2 : 1);
   if (all < kVerifySplit || 2 * B > kVerifyFull) return 1;
-  int64_t parts = kVerifyFull / B;
-  if (parts > kVerifyParts) parts = kVerifyParts;
-  return (int)(all / kVerifyPart < parts ? all / kVerifyPart : parts);
+  return kVerifyFull / B < kVerifyParts ? kVerifyFull / B : kVerifyParts;
 }
 
 // Whether all rows are searched for their largest entry at once, or only those
