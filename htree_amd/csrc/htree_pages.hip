@@ -39,7 +39,7 @@ struct KeepArgs {
 struct CopyArgs {
   MoveArgs m;
   const int32_t *from, *to, *tokens;
-  int32_t n, columns, parts;  // pieces that a block takes, blocks that share a page's tokens
+  int32_t columns, parts;  // pieces that a block takes, blocks that share a page's tokens
 };
 
 // The column of a token's bytes that a thread owns: one 16-byte piece of a
@@ -557,7 +557,7 @@ extern "C" int htree_copy_pages(const htree_cache* c, int32_t layers, void* cons
   if (!from || !to) return HTREE_ENULL;
   const Range lists[3] = {{from, n * 4ll}, {to, n * 4ll}, {tokens, tokens ? n * 4ll : 0}};
   if (const int shared = moves_apart(c, a.m, layers, k_layers, v_layers, lists)) return shared;
-  a.from = from, a.to = to, a.tokens = tokens, a.n = n;
+  a.from = from, a.to = to, a.tokens = tokens;
   a.columns = a.m.pieces < 256 ? a.m.pieces : 256;
   // so many blocks that a thread reads its tokens at once, up to 16 a page
   const int once = kCopyTokens * (256 / a.columns), parts = (c->page_size + once - 1) / once;
