@@ -14,9 +14,10 @@ constexpr int kMoveMost = (1 << 24) - 1;  // blocks of 256 threads along a grid'
 constexpr int kMoveLayers = 64;  // layers of a launch: their pointers are its arguments
 // Layers and tokens that a thread reads before it writes the first.  Kept drafts
 // are few tokens of many layers, and to find them takes four loads one after
-// another: four layers at once 39.8 us for 256 requests and 32 layers, one 48.0.
-// Pages are many tokens, found at once: 192 of them in 16 layers one layer a
-// block 12.9 us, four 15.9.
+// another: four layers at once 39.6 us for 256 requests and 32 layers, one 47.8.
+// Pages are many tokens, found at once: 65 of them, 504 tokens in 16 layers, one
+// layer a block 8.5 us, four 8.9; in a list of 256 whose other entries copy
+// nothing 12.9 and 12.5.
 constexpr int kKeepLayers = 4, kKeepTokens = 4;
 constexpr int kCopyLayers = 1, kCopyTokens = 4;
 
@@ -130,9 +131,11 @@ __global__ __launch_bounds__(256) void keep_drafts_kernel(KeepArgs a) {
   }
 }
 
-// The first tokens[i] tokens of page from[i] to page to[i]: 192 pages of 8
-// tokens on average, 16 layers of 4 x 128 bf16, 13.7 us (33 MB); a page to seven
-// others, 16 layers 4.8 us, a launch and two loads one after the other.
+// The first tokens[i] tokens of page from[i] to page to[i]: 65 pages, 504 tokens
+// together, in 16 layers of 4 x 128 bf16 8.5 us (33 MB, 3.9 TB/s).  Entries that
+// copy nothing have blocks as well: 191 of them in the same list and it takes
+// 12.9, 256 of them alone 3.4.  A page to seven others, 16 layers 4.6 us, a launch
+// and two loads one after the other.
 __global__ __launch_bounds__(256) void copy_pages_kernel(CopyArgs a) {
   const int i = blockIdx.x;
   const int from = cache_page(a.from[i], a.m.num_pages), to = cache_page(a.to[i], a.m.num_pages);
@@ -221,8 +224,9 @@ struct UnusedArgs {
   int32_t B, width, page_shift, num_pages, n_held, tiles;
 };
 constexpr int kUnusedTile = 4096;        // pages a block counts or lists: 16 a thread
-// Tiles that every block counts for itself: 5 of them 10.1 us (11.4 with a launch
-// that counts), 29 12.8 (12.0, and 2 us more of the host's time), 53 15.5 (12.7).
+// Tiles that every block counts for itself: a call of 5 of them 9.3 us in a graph
+// (10.6 with a launch that counts), 28 12.2 (11.3), 53 14.5 (11.8); the launch
+// takes 3 us of the host's time, which bounds such calls outside a graph.
 constexpr int kUnusedCounted = 32;
 constexpr int kUnusedPiece = 256;        // entries of a row that a wave reads at once, 4 a lane,
 // of so many rows: four in the one launch (64 requests of 1024 entries 13.1 us, with
@@ -230,9 +234,12 @@ constexpr int kUnusedPiece = 256;        // entries of a row that a wave reads a
 // together, 512 requests of 256 11.8 us, with four 12.7; 300 of 63 9.3 and 10.0)
 constexpr int kUnusedPieces = 4, kUnusedMark = 2;
 // Calls in one launch: pieces, requests and held pages at most, and pages, whose
-// bits fill 32 KB of LDS.  Against the other form's four launches: 64 pieces 6.9
-// us (11.7), 128 9.2 (11.4), 256 12.4 to 14 (10 to 12.5, and 7 us more of the
-// host's time); 1024 38 (12.7).
+// bits fill 32 KB of LDS.  A call, and in brackets the other form's, three launches
+// at these sizes: outside a graph, where those are bound by the host, up to 128
+// pieces 9.2 to 9.5 us (15.5), 192 10.9 to 11.5 (15.5), 256 12.9 to 14.2 (15.4 to
+// 18.1); in a graph 32 pieces 6.7 (9.4), 64 7.1 (9.5), 128 8.9 to 9.5 (9.6), 192
+// 10.9 to 11.7 (10.2), 256 13.0 to 14.4 (9.2 to 12.0).  The limit is for calls
+// outside one.
 constexpr int kUnusedSmall = 256, kUnusedSmallRows = 256, kUnusedSmallHeld = 4096;
 constexpr int kUnusedSmallPages = 1 << 18;
 constexpr int kUnusedSmallTile = 8192;   // pages a block lists: 8 a thread
