@@ -485,7 +485,7 @@ const char* htree_strerror(int status) {
     case HTREE_ESCRATCH:
       return "backward needs more scratch than htree_backward_noalloc's device array "
              "(HTREE_NOALLOC_SCRATCH_BYTES) holds: use htree_backward with a workspace";
-    case HTREE_EOVERLAP: return "an input lies in memory that the call writes: in a cache's range, copy it first";
+    case HTREE_EOVERLAP: return "memory that the call writes is an input's too (in a cache's range: copy it first), another output's or another layer's";
     default: return status > 0 ? hipGetErrorString((hipError_t)status) : "unknown htree status";
   }
 }

@@ -56,8 +56,8 @@ enum htree_status {
   HTREE_EWORKSPACE = -5,   /* workspace too small */
   HTREE_ESCRATCH = -6,     /* htree_backward_noalloc: the problem's backward
                               needs more than HTREE_NOALLOC_SCRATCH_BYTES */
-  HTREE_EOVERLAP = -7      /* serving: an input shares memory with what the
-                              call writes */
+  HTREE_EOVERLAP = -7      /* serving: an input, or another output or layer,
+                              shares memory with what the call writes */
 };
 
 /* Size of the device array htree_backward_noalloc works in (one per GPU). */
